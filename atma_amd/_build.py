@@ -39,9 +39,14 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (set HIPCC)")
 
 
+def compile_command(src: Path) -> list:
+    """The hipcc line of one source, without its inputs and outputs."""
+    return [hipcc(), *COMMON_FLAGS, *DEVICE_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}"]
+
+
 def _compile(src: Path) -> Path:
     obj = OBJDIR / (src.stem + ".o")
-    cmd = [hipcc(), *COMMON_FLAGS, *DEVICE_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)]
+    cmd = [*compile_command(src), "-c", str(src), "-o", str(obj)]
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"compile failed: {src.name}\n{' '.join(cmd)}\n{proc.stdout}")

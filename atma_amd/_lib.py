@@ -5,6 +5,7 @@ torch is imported first on purpose: the library's HIP runtime dependency
 pointers and streams are shared with torch.
 """
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -80,6 +81,13 @@ SIGNATURES = {
     "atma_linear_tokens_chunks": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i32, _p]),
     "atma_residual_rms_norm": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64,
                                       _p, _p, _i64, _i64, _i64, _f32, _i32, _p]),
+    "atma_residual_rms_norm_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64,
+                                          _p, _p, _i64, _p, _i64, _i64, _i64, _f32, _i32, _p]),
+    "atma_quantize_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
+    "atma_quantize_weight_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
+    "atma_linear_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _i32, _p]),
+    "atma_linear_gated_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _p, _i64, _i64, _i64,
+                                     _i64, _p]),
     "atma_partial_sums": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_memory_gate_logits": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_polar_params_f32": (_i32, [_p] * 6 + [_i64, _i64, _i32, _p]),
@@ -181,6 +189,15 @@ def stream_handle(device) -> int:
     """The current stream of ``device``, without building a Stream object (5 us of host time a launch)."""
     index = device.index if isinstance(device, torch.device) else torch.device(device).index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device(device):
+    """The context of a launch on ``device``: makes it the current device where another one is."""
+    index = device.index
+    return _same_device if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def dtype_code(dtype) -> int:

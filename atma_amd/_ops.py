@@ -947,3 +947,144 @@ def canon_conv_bwd_op(gs: List[Tensor], xs: List[Tensor], ws: List[Tensor]) -> L
 @canon_conv_bwd_op.register_fake
 def _(gs, xs, ws):
     return [torch.empty_like(x) for x in xs] + [torch.empty_like(w) for w in ws]
+
+
+# --------------------------------------------------------------------------- 8-bit inference (kernel/fp8.py)
+FP8, FP8_SCALE, FP8_BLOCK = torch.float8_e4m3fn, torch.float8_e8m0fnu, 128
+
+
+def _fp8_blocks(n: int) -> int:
+    return (n + FP8_BLOCK - 1) // FP8_BLOCK
+
+
+def _fp8_pair(like: Tensor, rows: int, cols: int, scale_rows: int):
+    """Empty (data, scale); a row of scales starts at a multiple of 4 bytes, as the products read them."""
+    nb = _fp8_blocks(cols)
+    scale = like.new_empty((scale_rows, (nb + 3) // 4 * 4), dtype=FP8_SCALE)
+    return like.new_empty((rows, cols), dtype=FP8), scale[:, :nb]
+
+
+def _rows_apart(t: Tensor) -> Tensor:
+    """Rows that start at multiples of 16 bytes and do not overlap (those of an expanded tensor do)."""
+    return _rows16(t if t.shape[0] < 2 or t.stride(0) >= t.shape[1] else t.contiguous())
+
+
+def _fp8_scales(t: Tensor) -> Tensor:
+    """Rows of scales at multiples of 4 bytes."""
+    if t.stride(1) == 1 and t.data_ptr() % 4 == 0 and t.stride(0) % 4 == 0 and t.stride(0) >= t.shape[1]:
+        return t
+    held = t.new_empty((t.shape[0], (t.shape[1] + 3) // 4 * 4))
+    held[:, :t.shape[1]].copy_(t)
+    return held[:, :t.shape[1]]
+
+
+def _quantize_fp8(name, x, scale_rows):
+    _need_cuda(x)
+    with _lib.on_device(x.device):
+        x = _rows_apart(x)
+        data, scale = _fp8_pair(x, x.shape[0], x.shape[1], scale_rows)
+        rc = getattr(_lib.load(), "atma_" + name)(
+            x.data_ptr(), x.stride(0), data.data_ptr(), data.stride(0), scale.data_ptr(), scale.stride(0), x.shape[0],
+            x.shape[1], _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
+        _lib.check(rc, name)
+    return [data, scale]
+
+
+@_op("quantize_fp8", mutates_args=())
+def quantize_fp8_op(x: Tensor) -> List[Tensor]:
+    return _quantize_fp8("quantize_fp8", x, x.shape[0])
+
+
+@quantize_fp8_op.register_fake
+def _(x):
+    return list(_fp8_pair(x, x.shape[0], x.shape[1], x.shape[0]))
+
+
+@_op("quantize_weight_fp8", mutates_args=())
+def quantize_weight_fp8_op(weight: Tensor) -> List[Tensor]:
+    return _quantize_fp8("quantize_weight_fp8", weight, _fp8_blocks(weight.shape[0]))
+
+
+@quantize_weight_fp8_op.register_fake
+def _(weight):
+    return list(_fp8_pair(weight, weight.shape[0], weight.shape[1], _fp8_blocks(weight.shape[0])))
+
+
+@_op("residual_rms_norm_fp8", mutates_args=())
+def residual_rms_norm_fp8_op(y: Optional[Tensor], parts: Optional[Tensor], biases: List[Tensor], mu_x: Optional[Tensor],
+                             mu_w: Optional[Tensor], residual: Optional[Tensor], weight: Tensor, eps: float,
+                             keep: bool) -> List[Tensor]:
+    """[data, scale] and, with ``keep``, the new stream; exactly one of y (M, D) and parts (P, M, D)."""
+    src = y if parts is None else parts
+    _need_cuda(src, residual, weight, mu_x, mu_w, *biases)
+    M, D = src.shape[-2:]
+    with _lib.on_device(src.device):
+        y, residual = (None if t is None else _rows_apart(t) for t in (y, residual))
+        parts, mu_w = (None if t is None else _aligned16(t) for t in (parts, mu_w))
+        biases, weight = [_aligned16(b) for b in biases], _aligned16(weight)
+        if mu_x is not None and (mu_x.stride(1) != 1 or mu_x.stride(0) % 2 or mu_x.stride(0) < mu_x.shape[1]
+                                 or mu_x.data_ptr() % 4):
+            mu_x = _aligned16(mu_x)
+        data, scale = _fp8_pair(weight, M, D, M)
+        stream = weight.new_empty((M, D)) if keep else None
+        held = (ctypes.c_void_p * max(1, len(biases)))(*[b.data_ptr() for b in biases])
+        rc = _lib.load().atma_residual_rms_norm_fp8(
+            _lib.ptr(y), 0 if y is None else y.stride(0), _lib.ptr(parts), 0 if parts is None else parts.shape[0],
+            ctypes.addressof(held), len(biases), _lib.ptr(mu_x), 0 if mu_x is None else mu_x.stride(0), _lib.ptr(mu_w),
+            0 if mu_x is None else mu_x.shape[1], _lib.ptr(residual), 0 if residual is None else residual.stride(0),
+            _lib.ptr(stream), D, weight.data_ptr(), data.data_ptr(), D, scale.data_ptr(), scale.stride(0), M, D, eps,
+            _lib.dtype_code(weight.dtype), _lib.stream_handle(src.device))
+        _lib.check(rc, "residual_rms_norm_fp8")
+    return [data, scale, stream] if keep else [data, scale]
+
+
+@residual_rms_norm_fp8_op.register_fake
+def _(y, parts, biases, mu_x, mu_w, residual, weight, eps, keep):
+    M, D = (y if parts is None else parts).shape[-2:]
+    return list(_fp8_pair(weight, M, D, M)) + ([weight.new_empty((M, D))] if keep else [])
+
+
+@_op("linear_fp8", mutates_args=())
+def linear_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
+                  out_dtype: torch.dtype) -> Tensor:
+    _need_cuda(x, x_scale, weight, weight_scale, bias)
+    with _lib.on_device(x.device):
+        x, weight, x_scale, weight_scale = _rows_apart(x), _rows_apart(weight), _fp8_scales(x_scale), _fp8_scales(weight_scale)
+        bias = None if bias is None else bias.contiguous()
+        (M, K), N = x.shape, weight.shape[0]
+        out = torch.empty((M, N), device=x.device, dtype=out_dtype)
+        rc = _lib.load().atma_linear_fp8(
+            x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), weight.data_ptr(), weight.stride(0),
+            weight_scale.data_ptr(), weight_scale.stride(0), _lib.ptr(bias),
+            _lib.ATMA_F32 if bias is None else _lib.dtype_code(bias.dtype), out.data_ptr(), N, M, N, K,
+            _lib.dtype_code(out_dtype), _lib.stream_handle(x.device))
+        _lib.check(rc, "linear_fp8")
+    return out
+
+
+@linear_fp8_op.register_fake
+def _(x, x_scale, weight, weight_scale, bias, out_dtype):
+    return x.new_empty((x.shape[0], weight.shape[0]), dtype=out_dtype)
+
+
+@_op("linear_gated_fp8", mutates_args=())
+def linear_gated_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor,
+                        bias: Optional[Tensor]) -> List[Tensor]:
+    _need_cuda(x, x_scale, weight, weight_scale, bias)
+    with _lib.on_device(x.device):
+        x, weight, x_scale, weight_scale = _rows_apart(x), _rows_apart(weight), _fp8_scales(x_scale), _fp8_scales(weight_scale)
+        bias = None if bias is None else bias.contiguous()
+        (M, K), H = x.shape, weight.shape[0] // 2
+        data, scale = _fp8_pair(x, M, H, M)
+        rc = _lib.load().atma_linear_gated_fp8(
+            x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), weight.data_ptr(), weight.stride(0),
+            weight_scale.data_ptr(), weight_scale.stride(0), _lib.ptr(bias),
+            _lib.ATMA_F32 if bias is None else _lib.dtype_code(bias.dtype), data.data_ptr(), H, scale.data_ptr(),
+            scale.stride(0), M, H, K, _lib.stream_handle(x.device))
+        _lib.check(rc, "linear_gated_fp8")
+    return [data, scale]
+
+
+@linear_gated_fp8_op.register_fake
+def _(x, x_scale, weight, weight_scale, bias):
+    return list(_fp8_pair(x, x.shape[0], weight.shape[0] // 2, x.shape[0]))

@@ -10,6 +10,8 @@
 //    atma_partial_sums is the same sum without the norm: a layer called on its own writes its output in one launch where
 //    torch makes about nine (three biases and a low-rank term of 8, bf16: 65,536 x 1,024 92 us where torch takes 635, 2,999 x
 //    1,024 13 where it takes 83).
+//    residual_rms_norm_fp8 is the same launch with the norm in 8 bits (fp8.h), quantized from its fp32 values: a block of
+//    128 columns is the 16 lanes of a DPP row, so a scale costs four lane exchanges and the 16-bit norm is never written.
 //  * lfm2_conv_step: the LFM2 block's gated conv for one token, c * conv(b * x)
 //    (model/reference.py:31-48, inference/models/atma.py:625-673) from the rows of its
 //    in_proj output, state table advanced in place.
@@ -21,7 +23,7 @@
 //
 // All are latency-bound at decode sizes (a few KB per row); a row is one wave (64 lanes,
 // 8 contiguous 16-bit values per lane per pass), reductions stay inside the wave.
-#include "common.h"
+#include "fp8.h"
 #include "gated_delta.h"
 
 namespace atma {
@@ -55,8 +57,10 @@ struct ResNormArgs {
   void* res_out;  // new stream (may be null when res is null)
   int64_t ldro;
   const void* w;  // (D,) T RMSNorm gain
-  void* out;      // (M, D) T; null: no norm, the stream alone
+  void* out;      // (M, D) T, or e4m3fn (F8); null: no norm, the stream alone
   int64_t ldo;
+  uint8_t* scale;  // F8: (M, ceil(D / 128)) scales, row stride lds
+  int64_t lds;
   float eps;
   int M, D;
 };
@@ -77,7 +81,7 @@ __device__ __forceinline__ f32x4 ld4(const float* p) { return *(const f32x4*)p; 
 // biases, residual) before its first arithmetic, so a row costs one memory round trip per
 // pass.  MU: the low-rank term's width (0: none), a template so that its weights index
 // registers statically.
-template <typename T, int P, int MU, int RPW, bool PARTS>
+template <typename T, int P, int MU, int RPW, bool PARTS, bool F8>
 __global__ void __launch_bounds__(256) residual_rms_norm_kernel(ResNormArgs a) {
   const int lane = threadIdx.x & 63;
   const int m0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW;
@@ -193,29 +197,50 @@ __global__ void __launch_bounds__(256) residual_rms_norm_kernel(ResNormArgs a) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int c = (p * 64 + lane) * 8;
-      if (c >= a.D) continue;
+      if constexpr (!F8) {
+        if (c >= a.D) continue;
+      }
       float w8[8], o[8];
       unpack8<T>(wv[p], w8);
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = (s[p][e] * rstd) * w8[e];
-      store8((T*)a.out + (int64_t)m * a.ldo + c, o);
+      if constexpr (!F8) {
+        store8((T*)a.out + (int64_t)m * a.ldo + c, o);
+      } else {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_abs(o[e]));
+        const int code = fp8_scale_code(row16_max(c < a.D ? top : 0.f));
+        if (c >= a.D) continue;
+        const float inv = fp8_inv_scale(code);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] *= inv;
+        *(u32x2*)((uint8_t*)a.out + (int64_t)m * a.ldo + c) =
+            u32x2{fp8_pack4(o[0], o[1], o[2], o[3]), fp8_pack4(o[4], o[5], o[6], o[7])};
+        if ((lane & 15) == 0) a.scale[(int64_t)m * a.lds + c / kFp8Block] = (uint8_t)code;
+      }
     }
   }
 }
 
-template <typename T, int MU, int RPW, bool PARTS>
+template <typename T, int MU, int RPW, bool PARTS, bool F8>
 static void launch_res_norm_form(const ResNormArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.M + 4 * RPW - 1) / (4 * RPW))), block(256);
-  if (a.D <= 512) residual_rms_norm_kernel<T, 1, MU, RPW, PARTS><<<grid, block, 0, s>>>(a);
-  else if (a.D <= 1024) residual_rms_norm_kernel<T, 2, MU, RPW, PARTS><<<grid, block, 0, s>>>(a);
-  else if (a.D <= 2048) residual_rms_norm_kernel<T, 4, MU, RPW, PARTS><<<grid, block, 0, s>>>(a);
-  else residual_rms_norm_kernel<T, 8, MU, RPW, PARTS><<<grid, block, 0, s>>>(a);
+  if (a.D <= 512) residual_rms_norm_kernel<T, 1, MU, RPW, PARTS, F8><<<grid, block, 0, s>>>(a);
+  else if (a.D <= 1024) residual_rms_norm_kernel<T, 2, MU, RPW, PARTS, F8><<<grid, block, 0, s>>>(a);
+  else if (a.D <= 2048) residual_rms_norm_kernel<T, 4, MU, RPW, PARTS, F8><<<grid, block, 0, s>>>(a);
+  else residual_rms_norm_kernel<T, 8, MU, RPW, PARTS, F8><<<grid, block, 0, s>>>(a);
 }
 
 template <typename T, int MU, int RPW>
 static void launch_res_norm_rows(const ResNormArgs& a, hipStream_t s) {
-  if (a.y) launch_res_norm_form<T, MU, RPW, false>(a, s);
-  else launch_res_norm_form<T, MU, RPW, true>(a, s);
+  if (a.scale) {
+    if (a.y) launch_res_norm_form<T, MU, RPW, false, true>(a, s);
+    else launch_res_norm_form<T, MU, RPW, true, true>(a, s);
+  } else {
+    if (a.y) launch_res_norm_form<T, MU, RPW, false, false>(a, s);
+    else launch_res_norm_form<T, MU, RPW, true, false>(a, s);
+  }
 }
 
 // the low-rank form over many rows shares its weights across 8 rows per wave; few rows (the
@@ -358,11 +383,12 @@ __global__ void __launch_bounds__(64) global_decode_prep_kernel(GlobalPrepArgs a
 // ---------------------------------------------------------------------------- C ABI
 using namespace atma;
 
-// atma_residual_rms_norm (weight and out given) and atma_partial_sums (neither).
+// atma_residual_rms_norm (weight and out given), atma_residual_rms_norm_fp8 (and scale) and atma_partial_sums (none).
 static int res_norm(const char* what, const void* y, int64_t ldy, const float* parts, int64_t n_parts,
                     const void* const* bias, int64_t n_bias, const void* mu_x, int64_t ldmu, const void* mu_w,
                     int64_t mu_k, const void* res, int64_t ldr, void* res_out, int64_t ldro, const void* weight,
-                    void* out, int64_t ldo, int64_t M, int64_t D, float eps, int dtype, void* stream) {
+                    void* out, int64_t ldo, int64_t M, int64_t D, float eps, int dtype, void* stream,
+                    void* scale = nullptr, int64_t lds = 0) {
   if (dtype != ATMA_BF16 && dtype != ATMA_F16)
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: 16-bit only (dtype %d)", what, dtype);
   if (M < 0 || D < 8 || D % 8 || D > 4096 || M > 0x7fffffff)
@@ -400,6 +426,8 @@ static int res_norm(const char* what, const void* y, int64_t ldy, const float* p
   a.w = weight;
   a.out = out;
   a.ldo = ldo;
+  a.scale = (uint8_t*)scale;
+  a.lds = lds;
   a.eps = eps;
   a.M = (int)M;
   a.D = (int)D;
@@ -418,6 +446,20 @@ extern "C" int atma_residual_rms_norm(const void* y, int64_t ldy, const float* p
     return set_error(ATMA_ERR_INVALID, "residual_rms_norm: need weight, out and exactly one of y / parts");
   return res_norm("residual_rms_norm", y, ldy, parts, n_parts, bias, n_bias, mu_x, ldmu, mu_w, mu_k, res, ldr, res_out,
                   ldro, weight, out, ldo, M, D, eps, dtype, stream);
+}
+
+extern "C" int atma_residual_rms_norm_fp8(const void* y, int64_t ldy, const float* parts, int64_t n_parts,
+                                          const void* const* bias, int64_t n_bias, const void* mu_x, int64_t ldmu,
+                                          const void* mu_w, int64_t mu_k, const void* res, int64_t ldr, void* res_out,
+                                          int64_t ldro, const void* weight, void* out, int64_t ldo, void* scale,
+                                          int64_t lds, int64_t M, int64_t D, float eps, int dtype, void* stream) {
+  if (M > 0 && (dtype == ATMA_BF16 || dtype == ATMA_F16) && (!weight || !out || !scale))
+    return set_error(ATMA_ERR_INVALID, "residual_rms_norm_fp8: need weight, out, scale and exactly one of y / parts");
+  if (D % 16) return set_error(ATMA_ERR_INVALID, "residual_rms_norm_fp8: D must be a multiple of 16 (got %lld)", (long long)D);
+  if (M > 0 && lds < (D + kFp8Block - 1) / kFp8Block)
+    return set_error(ATMA_ERR_INVALID, "residual_rms_norm_fp8: rows of scales must hold %lld", (long long)((D + 127) / 128));
+  return res_norm("residual_rms_norm_fp8", y, ldy, parts, n_parts, bias, n_bias, mu_x, ldmu, mu_w, mu_k, res, ldr, res_out,
+                  ldro, weight, out, ldo, M, D, eps, dtype, stream, scale, lds);
 }
 
 extern "C" int atma_partial_sums(const void* y, int64_t ldy, const float* parts, int64_t n_parts,

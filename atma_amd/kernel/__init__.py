@@ -20,6 +20,8 @@ from .. import _lib
 _lib.load()   # raises HipLibraryMissing (ImportError) when the library is absent
 
 from .conv import causal_conv1d_decode_step  # noqa: E402
+from .fp8 import (linear_fp8, linear_gated_fp8, quantize_fp8, quantize_weight_fp8,  # noqa: E402
+                  residual_rms_norm_fp8)
 from .inference_ops import (linear_tokens, linear_tokens_supported, packed_causal_conv1d,  # noqa: E402
                             softcap_argmax, softcap_logits, squared_relu_gate)
 from .gated_delta import (StartSignal, chunk_gated_delta_rule, gated_delta_decode_step,  # noqa: E402
@@ -52,4 +54,9 @@ __all__ = [
     "softcap_logits",
     "softcap_argmax",
     "packed_causal_conv1d",
+    "quantize_fp8",
+    "quantize_weight_fp8",
+    "residual_rms_norm_fp8",
+    "linear_fp8",
+    "linear_gated_fp8",
 ]

@@ -1,0 +1,125 @@
+"""8-bit inference: quantizers, the residual norm with an 8-bit output, the block-scaled product and the MLP's gated first
+projection (C ABI ``atma_quantize_fp8``, ``atma_quantize_weight_fp8``, ``atma_residual_rms_norm_fp8``,
+``atma_linear_fp8``, ``atma_linear_gated_fp8``).
+
+An 8-bit tensor is a pair ``(data, scale)``: ``data`` float8_e4m3fn, ``scale`` float8_e8m0fnu (a power of two), one scale
+for each 128 values along a row (activations, ``scale`` (rows, ceil(K / 128))) or for each 128 x 128 block (weights, ``scale``
+(ceil(N / 128), ceil(K / 128))); its values are ``data * scale``.  The scale of a block is the smallest 2^e, e in
+[-126, 120], that brings its largest finite magnitude to 448 or less; values are rounded to nearest even, infinities and
+NaN are stored as NaN and leave the block's other values as they are.
+
+No reference counterparts: the served form of ``model/layers.py:19-31`` and ``model/reference.py:22-28`` with weights and
+activations in 8 bits.  Inference only (an input that requires a gradient is refused in grad mode), on the GPU, graph
+capturable; rows are any number, zero among them, K is a multiple of 16.
+"""
+
+import torch
+
+from .. import _ops
+from .decode_fusions import PartialSums
+
+_DT = (torch.bfloat16, torch.float16)
+_DT32 = (torch.bfloat16, torch.float16, torch.float32)
+FP8, FP8_SCALE, FP8_BLOCK = _ops.FP8, _ops.FP8_SCALE, _ops.FP8_BLOCK
+
+
+def _check(what, *ts):
+    """Every tensor of a call on one GPU, none of them waiting for a gradient."""
+    ts = [t for t in ts if t is not None]
+    if any(not t.is_cuda for t in ts):
+        raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
+    if any(t.device != ts[0].device for t in ts):
+        raise ValueError(f"{what}: every tensor must be on {ts[0].device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), or detach its inputs")
+
+
+def _matrix(what, name, t, dtypes):
+    if t.dim() != 2 or t.dtype not in dtypes:
+        raise ValueError(f"{what}: {name} must be a matrix of {', '.join(str(d)[6:] for d in dtypes)} "
+                         f"(got {tuple(t.shape)} {t.dtype})")
+    if t.shape[1] < 16 or t.shape[1] % 16:
+        raise ValueError(f"{what}: rows of {name} must be a multiple of 16 long (got {t.shape[1]})")
+
+
+def quantize_fp8(x):
+    """Rows to 8 bits: x (M, K) in fp32 or 16 bits, K a multiple of 16 -> (data (M, K), scale (M, ceil(K / 128)))."""
+    _matrix("quantize_fp8", "x", x, _DT32)
+    _check("quantize_fp8", x)
+    return tuple(_ops.run.quantize_fp8(x))
+
+
+def quantize_weight_fp8(weight):
+    """A weight matrix to 8 bits: (N, K) in fp32 or 16 bits, K a multiple of 16 -> (data (N, K), scale (ceil(N / 128),
+    ceil(K / 128))).  ``linear_gated_fp8`` takes the a and gate rows as one (2H, K) matrix, H a multiple of 128."""
+    _matrix("quantize_weight_fp8", "weight", weight, _DT32)
+    _check("quantize_weight_fp8", weight)
+    return tuple(_ops.run.quantize_weight_fp8(weight))
+
+
+def residual_rms_norm_fp8(branch, residual, weight, eps):
+    """``residual_rms_norm`` with its norm in 8 bits: ``s = residual + branch`` (rounded to the stream's type),
+    ``rms_norm(s) * weight`` quantized from its fp32 values.  ``branch``: (M, D) or ``PartialSums``; ``residual`` None starts
+    the stream with the branch; D a multiple of 16, at most 4,096.  Returns (data, scale, s)."""
+    what = "residual_rms_norm_fp8"
+    ps = branch if isinstance(branch, PartialSums) else None
+    y, parts = (branch, None) if ps is None else (ps.base, ps.parts)
+    src = y if parts is None else parts
+    dtype = branch.dtype
+    if src.dim() != (2 if parts is None else 3):
+        raise ValueError(f"{what}: the branch must be (M, D), partial sums (P, M, D)")
+    M, D = src.shape[-2:]
+    if dtype not in _DT or D % 16 or not 16 <= D <= 4096 or weight.shape != (D,) or weight.dtype != dtype:
+        raise ValueError(f"{what}: unsupported rows of {D} {dtype}, weight {tuple(weight.shape)} {weight.dtype}")
+    if src.dtype != (dtype if parts is None else torch.float32) or (parts is not None and not 1 <= parts.shape[0] <= 8):
+        raise ValueError(f"{what}: a branch in the stream's type or up to 8 fp32 partial sums")
+    if residual is not None and (residual.shape != (M, D) or residual.dtype != dtype):
+        raise ValueError(f"{what}: residual must match the branch")
+    biases = [] if ps is None else list(ps.biases)
+    mu_x, mu_w = (None, None) if ps is None else (ps.mu_x, ps.mu_w)
+    if len(biases) > 3 or any(b.shape != (D,) or b.dtype != dtype for b in biases):
+        raise ValueError(f"{what}: up to three biases ({D},) in the stream's type")
+    if mu_x is not None and (mu_x.dim() != 2 or mu_x.shape[1] not in (4, 8, 16) or mu_x.shape[0] != M
+                             or mu_w.shape != (D, mu_x.shape[1]) or mu_x.dtype != dtype or mu_w.dtype != dtype):
+        raise ValueError(f"{what}: the low-rank term takes mu_x (M, k) and mu_w (D, k), k 4, 8 or 16")
+    _check(what, src, residual, weight, mu_x, mu_w, *biases)
+    keep = residual is not None or ps is not None
+    out = _ops.run.residual_rms_norm_fp8(y, parts, biases, mu_x, mu_w, residual, weight, float(eps), keep)
+    return out[0], out[1], (out[2] if keep else branch)
+
+
+def _operands(what, x, x_scale, weight, weight_scale, bias, dtypes):
+    _matrix(what, "x", x, (FP8,))
+    _matrix(what, "weight", weight, (FP8,))
+    N, K = weight.shape
+    nb = _ops._fp8_blocks(K)
+    if x.shape[1] != K or N < 1:
+        raise ValueError(f"{what}: x (M, K) and weight (N, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
+    for name, t, rows in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, _ops._fp8_blocks(N))):
+        if t.dtype != FP8_SCALE or t.shape != (rows, nb):
+            raise ValueError(f"{what}: {name} must be ({rows}, {nb}) float8_e8m0fnu (got {tuple(t.shape)} {t.dtype})")
+    if bias is not None and (bias.shape != (N,) or bias.dtype not in dtypes):
+        raise ValueError(f"{what}: bias must be ({N},) of {', '.join(str(d)[6:] for d in dtypes)}")
+    _check(what, x, x_scale, weight, weight_scale, bias)
+
+
+def linear_fp8(x, x_scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
+    """``F.linear`` of 8-bit operands: x (M, K) with x_scale (M, ceil(K / 128)), weight (N, K) with weight_scale
+    (ceil(N / 128), ceil(K / 128)); bias (N,) in fp32 or 16 bits or None.  Sums in fp32, one rounding to ``out_dtype``
+    (bfloat16 or float16).  The matrix instructions add the products of eight neighbouring k with 14 bits below the largest
+    of them, 1.4e-5 of a result of normally distributed values.  Scales whose rows start at multiples of 4 bytes, as
+    ``quantize_fp8`` lays them, are read in place; others are copied."""
+    if out_dtype not in _DT:
+        raise ValueError(f"linear_fp8: out_dtype must be bfloat16 or float16 (got {out_dtype})")
+    _operands("linear_fp8", x, x_scale, weight, weight_scale, bias, _DT32)
+    return _ops.run.linear_fp8(x, x_scale, weight, weight_scale, bias, out_dtype)
+
+
+def linear_gated_fp8(x, x_scale, weight, weight_scale, bias=None):
+    """The MLP's first projection with its activation, 8 bits in and out: ``a, gate = linear(x, weight, bias).chunk(2, -1)``
+    as fp32 sums, ``gate * relu(a)^2`` quantized once.  Operands as ``linear_fp8``, weight (2H, K) with H a multiple of 128.
+    Returns (data (M, H), scale (M, H / 128))."""
+    if weight.dim() == 2 and (weight.shape[0] < 256 or weight.shape[0] % 256):
+        raise ValueError(f"linear_gated_fp8: weight (2H, K) with H a multiple of 128 (got {tuple(weight.shape)})")
+    _operands("linear_gated_fp8", x, x_scale, weight, weight_scale, bias, _DT32)
+    return tuple(_ops.run.linear_gated_fp8(x, x_scale, weight, weight_scale, bias))

@@ -604,6 +604,55 @@ int atma_residual_rms_norm(const void* y, int64_t ldy, const float* parts, int64
                            int64_t ldo, int64_t M, int64_t D, float eps, int dtype, void* stream);
 
 /*
+ * 8-bit inference (no reference counterparts).  An 8-bit tensor is float8_e4m3fn bytes with power-of-two scales, one
+ * byte each (float8_e8m0fnu: code c is 2^(c - 127)): a scale for each 128 consecutive values of a row (activations; the
+ * last block of a row may be shorter) or for each 128 x 128 block (weights).  The scale of a block is the smallest 2^e, e
+ * in [-126, 120], that brings its largest finite magnitude to 448 or less; values are divided by it and rounded to
+ * nearest even, infinities and NaN become NaN.  Row strides are in elements (bytes for values and scales).
+ */
+
+/*
+ * atma_residual_rms_norm with its norm in 8 bits: out (M, D) and scale (M, ceil(D / 128)) hold
+ * s * rsqrt(mean(s^2) + eps) * weight, quantized from fp32.  Arguments as there; D a multiple of 16; rows of out
+ * 8-byte aligned (ldo % 8 == 0, out 16-byte aligned).
+ */
+int atma_residual_rms_norm_fp8(const void* y, int64_t ldy, const float* parts, int64_t n_parts,
+                               const void* const* bias, int64_t n_bias, const void* mu_x, int64_t ldmu,
+                               const void* mu_w, int64_t mu_k, const void* res, int64_t ldr, void* res_out,
+                               int64_t ldro, const void* weight, void* out, int64_t ldo, void* scale, int64_t lds,
+                               int64_t M, int64_t D, float eps, int dtype, void* stream);
+
+/*
+ * Rows to 8 bits: x (M, K) in `dtype` to data (M, K) and scale (M, ceil(K / 128)).  K a multiple of 16; rows of x
+ * 16-byte aligned, of data 8-byte.
+ */
+int atma_quantize_fp8(const void* x, int64_t ldx, void* data, int64_t ldd, void* scale, int64_t lds, int64_t M,
+                      int64_t K, int dtype, void* stream);
+
+/* A weight matrix to 8 bits: w (N, K) to data (N, K) and scale (ceil(N / 128), ceil(K / 128)); alignment as above. */
+int atma_quantize_weight_fp8(const void* w, int64_t ldw, void* data, int64_t ldd, void* scale, int64_t lds, int64_t N,
+                             int64_t K, int dtype, void* stream);
+
+/*
+ * y[m, n] = round(sum_k x[m, k] w[n, k] + bias[n]) in `dtype` (16-bit) for 8-bit x (M, K) with scales xs (M, nb) and
+ * 8-bit w (N, K) with scales ws (ceil(N / 128), nb), nb = ceil(K / 128); bias (N,) in `bias_dtype` or NULL.  K a multiple
+ * of 16; rows of x and w 16-byte aligned, of xs and ws 4-byte (the bytes behind a row's last scale, up to the next
+ * multiple of 4, are read and not used); y 16-byte aligned where ldy % 8 == 0.
+ */
+int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw, const void* ws,
+                    int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, int64_t M, int64_t N,
+                    int64_t K, int dtype, void* stream);
+
+/*
+ * The MLP's first projection with its activation, 8 bits in and out (atma_linear_gated's shape: w (2H, K), the a rows,
+ * then the gate rows; bias (2H,) or NULL): y (M, H) with scales ys (M, H / 128) hold gate * relu(a)^2 for the fp32 sums
+ * a and gate, quantized once.  H a multiple of 128; x, xs, w, ws and K as atma_linear_fp8; rows of y 16-byte aligned.
+ */
+int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw,
+                          const void* ws, int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, void* ys,
+                          int64_t ldys, int64_t M, int64_t H, int64_t K, void* stream);
+
+/*
  * The LFM2 block's decode mixer (model/reference.py:31-48, inference/models/atma.py:
  * 625-673) as one call: with b, c, x the three D-wide thirds of each bcx row (in_proj's
  * output), out = c * conv(b * x), the depthwise conv of K taps (weight (D, K)) over the
