@@ -36,6 +36,7 @@ struct Fp8Args {
   int64_t ldw;
   const uint8_t* ws;  // (ceil(rows / 128), nk), row stride ldws
   int64_t ldws;
+  int64_t w_blocks;  // rows of ws
   const void* bias;  // (N,) or (2 N,), or null
   int bias_dtype;
   void* y;  // (M, N): T, or gated: e4m3fn
@@ -61,31 +62,36 @@ __device__ __forceinline__ float gate_act(float av, float gv) {
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
-// Chunk position of a tile's row in LDS: rows are 128 bytes, 8 chunks of 16, chunk c of row r at position c ^ f(r).  The
-// 16 lanes that read one chunk of 16 rows cover all banks when f takes 8 values over the rows of each parity: 16
-// consecutive token rows; weight rows 16 a + 4 t + b, a, b < 4 (the order below), or 8 a + 4 t + b.
-__device__ __forceinline__ int x_swizzle(int r) { return (r >> 1) & 7; }
-template <int G>
-__device__ __forceinline__ int w_swizzle(int r) {
-  if constexpr (G == 4) return ((r >> 1) & 1) | (((r >> 4) & 3) << 1);
-  else if constexpr (G == 2) return ((r >> 1) & 1) | (((r >> 3) & 3) << 1);
-  else return (r >> 1) & 7;
-}
+// A workgroup of four waves, WF x WM, owns BF weight rows x BM tokens, a wave TF x TM tiles of 32 x 32
+// (v_mfma_scale_f32_32x32x64_f8f6f4: two instructions for a block of 128 along K).  K runs in steps of 64 through a ring of
+// NS stages in LDS, filled NS - 1 steps ahead by direct copies; the workgroup is persistent and the ring runs on across its
+// tiles, so a tile's first copies fly during the last steps and the epilogue of the one before.  Everything else a tile
+// reads -- the scales of four blocks at a time, the bias -- comes through the same copies into small rings of their own:
+// the loop has no load into registers, whose wait would drain the ring.
+//
+// A step's rows are 64 bytes, four chunks of 16, chunk c of row r at position c ^ f(r): the 16 lanes that read one chunk of
+// 16 rows cover all banks when f takes four values over the rows of each residue mod 4.  The weights are the MFMA's rows,
+// in an order such that a lane's accumulators are 16 consecutive features of one token (row 8 q + 4 h + e is feature
+// 16 h + 4 q + e; lane half h holds the rows 4 h + e of each 8): outputs are stored straight from registers.
+__device__ __forceinline__ int x_swizzle(int r) { return (r >> 2) & 3; }
+__device__ __forceinline__ int w_swizzle(int r) { return ((r >> 2) & 1) | (((r >> 4) & 1) << 1); }
 
-// A workgroup of WF x WM waves owns BF weight rows x BM tokens and a wave TF x TM tiles of 16 x 16.  The weights are the
-// MFMA's rows: their order inside a wave's rows is chosen such that a lane's accumulators of G tiles are 4 G consecutive
-// features of one token (tile t's row 4 a + b is feature 4 G a + 4 t + b), stored straight from registers.
-template <typename T, int TF, int TM, int WF, int WM, bool GATED>
+template <int TF, int TM, int WF, int WM, int NS, bool GATED>
 struct Fp8Tile {
   static constexpr int NW = WF * WM;
-  static constexpr int BF = 16 * TF * WF, BM = 16 * TM * WM;
-  static constexpr int OF = GATED ? BF / 2 : BF;   // output features
-  static constexpr int TO = GATED ? TF / 2 : TF;   // tiles of output features a wave
-  static constexpr int G = TO < 4 ? TO : 4;
-  static constexpr int STAGE = (BF + BM) * kFp8Block;
-  static constexpr int WCOPY = BF / 8 / NW, XCOPY = BM / 8 / NW;  // copies a wave and step: 8 rows each
-  static_assert(BF % (8 * NW) == 0 && BM % (8 * NW) == 0 && (NW == 4 || NW == 8), "whole copies");
-  static_assert(!GATED || OF == kFp8Block, "a gated tile is one block of output features");
+  static constexpr int BF = 32 * TF * WF, BM = 32 * TM * WM;
+  static constexpr int OF = GATED ? BF / 2 : BF;  // output features
+  static constexpr int TO = GATED ? TF / 2 : TF;  // tiles of output features a wave
+  static constexpr int STAGE = (BF + BM) * 64;
+  static constexpr int WCOPY = BF / 16 / NW, XCOPY = BM / 16 / NW;  // copies a wave and step: 16 rows each
+  static constexpr int XS = BM > 64 ? BM : 64;                      // words of token scales
+  static constexpr int AUX = (NS - 1) / 2 + 2;  // scale groups and tiles that can be under way (two steps at least each)
+  static constexpr int LDS_AUX = NS * STAGE, LDS_BIAS = LDS_AUX + AUX * (XS + 64) * 4;
+  static constexpr int LDS_TOP = LDS_BIAS + AUX * 1024, LDS = LDS_TOP + (GATED ? WF * BM * 4 : 0);
+  static_assert(NW == 4 && BF % (16 * NW) == 0 && BF <= 256 && BM <= 256, "whole copies, a bias of 1 KiB");
+  static_assert(BM % (16 * NW) == 0 || BM == 32, "whole copies");
+  static_assert(!GATED || (OF == kFp8Block && TF == 2), "a gated tile is one block of output features");
+  static_assert((NS - 2) * (WCOPY + XCOPY + 1) < 64, "vmcnt counts to 63");
 };
 
 template <typename C>
@@ -99,223 +105,249 @@ __device__ __forceinline__ bool fp8_tile_at(const Fp8Args& a, int xcd, int u, in
   return true;
 }
 
-template <typename T, int TF, int TM, int WF, int WM, bool GATED>
-__global__ void __launch_bounds__(64 * WF * WM) fp8_tile_kernel(Fp8Args a) {
-  using C = Fp8Tile<T, TF, TM, WF, WM, GATED>;
-  constexpr int G = C::G, TO = C::TO;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * C::STAGE];
-  __shared__ float amax_part[GATED ? WF : 1][GATED ? C::BM : 1];
+template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
+__global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
+  using C = Fp8Tile<TF, TM, WF, WM, NS, GATED>;
+  constexpr int TO = C::TO;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave % WF, wm = wave / WF;
-  const int r = lane & 15, g = lane >> 4;
+  const int r = lane & 31, h = lane >> 5;
   const int xcd = blockIdx.x & 7, nper = gridDim.x >> 3;
+  const int steps = 2 * a.nk;
   int64_t m0, f0;
   int u = blockIdx.x >> 3;
   if (!fp8_tile_at<C>(a, xcd, u, m0, f0)) return;
 
-  // ---- copies: instruction i of a wave moves rows 8 (i NW + wave) .. + 7 of a tile; lane l writes row l / 8, position
-  // l % 8, and reads the chunk that belongs there; chunks past K (offset 2^31, past every tile) and rows past the end
-  // read as zeros
-  const int crow = lane >> 3, cpos = lane & 7;
-  auto row_of = [&](int i) { return 8 * (i * C::NW + wave) + crow; };
-  __amdgpu_buffer_rsrc_t xr, wr, gr;
+  // ---- the copies, NS - 1 steps ahead of the products.  Copy i of a wave moves rows 16 (i NW + wave) .. + 15: lane l
+  // writes row l / 4, position l % 4, and reads the chunk that belongs there; chunks past K (offset 2^31, past every tile)
+  // and rows past the end read as zeros
+  const uint32_t lds0 = lds_offset(lds);
+  const int crow = lane >> 2;
+  const int wk = 16 * ((lane & 3) ^ w_swizzle(16 * wave + crow)), xk = 16 * ((lane & 3) ^ x_swizzle(crow));
+  const uint32_t wv0 = (uint32_t)(16 * wave + crow) * (uint32_t)a.ldw, xv0 = (uint32_t)(16 * wave + crow) * (uint32_t)a.ldx;
+  const uint32_t wstep = 16u * C::NW * (uint32_t)a.ldw, xstep = 16u * C::NW * (uint32_t)a.ldx;
+  __amdgpu_buffer_rsrc_t xr, wr, gr, xsr, wsr;
+  int pu = u, pk = 0, pstage = 0, paux = 0, ptile = 0;
+  int64_t pf0 = 0;
+  bool pmore = true;
   auto aim = [&](int64_t tm0, int64_t tf0) {
-    xr = buffer_rsrc(a.x + tm0 * a.ldx, (uint32_t)(min((int64_t)C::BM, a.M - tm0) * a.ldx));
+    const int64_t rows = min((int64_t)C::BM, a.M - tm0);
+    xr = buffer_rsrc(a.x + tm0 * a.ldx, (uint32_t)(rows * a.ldx));
+    xsr = buffer_rsrc(a.xs + tm0 * a.ldxs, (uint32_t)(rows * a.ldxs));
     const uint32_t wb = (uint32_t)(min((int64_t)C::OF, a.N - tf0) * a.ldw);
     wr = buffer_rsrc(a.w + tf0 * a.ldw, wb);
     if constexpr (GATED) gr = buffer_rsrc(a.w + (a.N + tf0) * a.ldw, wb);
+    const int64_t b0 = tf0 / kFp8Block;
+    wsr = buffer_rsrc(a.ws + b0 * a.ldws, (uint32_t)((a.w_blocks - b0) * a.ldws));
+    pf0 = tf0;
   };
-  const uint32_t lds0 = lds_offset(lds);
-  auto issue = [&](int stage, int kb) {
-    const uint32_t d = lds0 + stage * C::STAGE + 1024 * wave;
+  auto issue = [&]() {
+    if (pk == 0 && a.bias && wave == C::NW - 2) {
+      // 256 biases (gated: 128 of a, 128 of gate), in words, to this tile's slot
+      const int size = a.bias_dtype == ATMA_F32 ? 4 : 2;
+      const int64_t total = (GATED ? 2 : 1) * a.N * size;
+      const __amdgpu_buffer_rsrc_t br = buffer_rsrc(a.bias, (uint32_t)((total + 3) & ~3ll));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int word = 64 * i + lane, f = word * 4 / size;  // the word's first feature in the tile
+        if (64 * i * 4 / size < 256) {
+          const int64_t n = pf0 + (GATED && f >= C::OF ? a.N + f - C::OF : f);
+          dma_buf4(br, n * size < total ? (uint32_t)(n * size) : 0xfffffffcu, 0u,
+                   lds + C::LDS_BIAS + 1024 * ptile + 256 * i);
+        }
+      }
+    }
+    if ((pk & 7) == 0) {
+      const uint32_t slot = lds0 + C::LDS_AUX + paux * (C::XS + 64) * 4;
+      const uint32_t k4 = (uint32_t)pk >> 1;
+      if (wave < C::XS / 64)
+        dma_buf4_at(xsr, (uint32_t)(64 * wave + lane) * (uint32_t)a.ldxs + k4, 0u, slot + 256 * wave);
+      if (wave == C::NW - 1) {
+        const uint32_t row = GATED ? (lane ? (uint32_t)(a.N / kFp8Block) : 0u) : (uint32_t)lane;
+        dma_buf4_at(wsr, lane < 2 ? row * (uint32_t)a.ldws + k4 : 0x80000000u, 0u, slot + 4 * C::XS);
+      }
+      paux = paux + 1 == C::AUX ? 0 : paux + 1;
+    }
+    const uint32_t d = lds0 + pstage * C::STAGE + 1024 * wave;
+    const int k = 64 * pk;
+    const uint32_t wv = k + wk < a.K ? wv0 + (uint32_t)(k + wk) : 0x80000000u;
+    const uint32_t xv = k + xk < a.K ? xv0 + (uint32_t)(k + xk) : 0x80000000u;
 #pragma unroll
     for (int i = 0; i < C::WCOPY; ++i) {
-      const int row = row_of(i);
-      const int k = kb * kFp8Block + 16 * (cpos ^ w_swizzle<G>(row));
-      const int half = GATED ? C::BF / 2 : C::BF;
-      const bool second = GATED && 8 * i * C::NW >= half;
-      const uint32_t v = k < a.K ? (uint32_t)(row - (second ? half : 0)) * (uint32_t)a.ldw + (uint32_t)k : 0x80000000u;
-      dma_buf16_at(second ? gr : wr, v, 0u, d + 1024 * C::NW * i);
+      constexpr int half = C::WCOPY / 2;  // gated: the first half of a wave's copies are a rows, the others gate rows
+      if (GATED && i >= half) dma_buf16_at(gr, wv + (i - half) * wstep, 0u, d + 1024 * C::NW * i);
+      else dma_buf16_at(wr, wv + i * wstep, 0u, d + 1024 * C::NW * i);
+    }
+    if constexpr (C::XCOPY == 0) {
+      if (wave < C::BM / 16) dma_buf16_at(xr, xv, 0u, d + C::BF * 64);
     }
 #pragma unroll
-    for (int i = 0; i < C::XCOPY; ++i) {
-      const int row = row_of(i);
-      const int k = kb * kFp8Block + 16 * (cpos ^ x_swizzle(row));
-      const uint32_t v = k < a.K ? (uint32_t)row * (uint32_t)a.ldx + (uint32_t)k : 0x80000000u;
-      dma_buf16_at(xr, v, 0u, d + C::BF * kFp8Block + 1024 * C::NW * i);
+    for (int i = 0; i < C::XCOPY; ++i) dma_buf16_at(xr, xv + i * xstep, 0u, d + C::BF * 64 + 1024 * C::NW * i);
+    pstage = pstage + 1 == NS ? 0 : pstage + 1;
+    if (++pk == steps) {
+      int64_t nm0, nf0;
+      pk = 0;
+      ptile = ptile + 1 == C::AUX ? 0 : ptile + 1;
+      pu += nper;
+      pmore = fp8_tile_at<C>(a, xcd, pu, nm0, nf0);
+      if (pmore) aim(nm0, nf0);
     }
-  };
-
-  // ---- scales of the wave's tokens and weight blocks, four steps a word
-  uint32_t xs_next[TM], ws_next[2];
-  const int wrow0 = 16 * TO * wf;  // the wave's first output feature in the tile
-  auto load_scales = [&](int64_t tm0, int64_t tf0, int kb) {
-#pragma unroll
-    for (int t = 0; t < TM; ++t) {
-      const int64_t m = min(tm0 + 16 * (TM * wm + t) + r, a.M - 1);
-      xs_next[t] = *(const uint32_t*)(a.xs + m * a.ldxs + kb);
-    }
-    const int64_t wb = min(tf0 + wrow0, a.N - 1) / kFp8Block;
-    ws_next[0] = *(const uint32_t*)(a.ws + wb * a.ldws + kb);
-    if constexpr (GATED) ws_next[1] = *(const uint32_t*)(a.ws + (a.N / kFp8Block + wb) * a.ldws + kb);
   };
 
   // ---- operand reads
-  uint32_t wofs[TF][2], xofs[2];
+  const int wrow0 = 32 * TO * wf;  // the wave's first output feature in the tile
+  const int wrow = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+  uint32_t wofs[2], xofs[2];
 #pragma unroll
-  for (int t = 0; t < TF; ++t) {
-    const int to = t % TO, grp = to / G;  // tile to of the a half or the gate half
-    const int row = (t / TO) * (C::BF / 2) + wrow0 + 16 * G * grp + 4 * G * (r >> 2) + 4 * (to % G) + (r & 3);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) wofs[t][h] = row * kFp8Block + 16 * ((g + 4 * h) ^ w_swizzle<G>(row));
+  for (int q = 0; q < 2; ++q) {
+    wofs[q] = (uint32_t)((wrow0 + wrow) * 64 + 16 * ((2 * h + q) ^ w_swizzle(wrow)));
+    xofs[q] = (uint32_t)(C::BF * 64 + (32 * TM * wm + r) * 64 + 16 * ((2 * h + q) ^ x_swizzle(r)));
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    xofs[h] = C::BF * kFp8Block + (16 * TM * wm + r) * kFp8Block + 16 * ((g + 4 * h) ^ x_swizzle(r));
 
-  f32x4 acc[TF][TM];
-  uint32_t xs_now[TM], ws_now[2];
-  int stage = 0;
+  f32x16 acc[TF][TM];
+  int stage = 0, aux = 0, tile = 0;
   aim(m0, f0);
-  load_scales(m0, f0, 0);
-  issue(0, 0);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (pmore) issue();
   while (true) {
+    const uint32_t* words = nullptr;
+    uint32_t xs[TM], ws[2];
+    for (int k = 0; k < steps; k += 2) {
 #pragma unroll
-    for (int t = 0; t < TF; ++t)
+      for (int s = 0; s < 2; ++s) {
+        // this step's copies have landed in every wave, and every wave is done with the stage before it
+        if (pmore) wait_vmcnt<(NS - 2) * (C::WCOPY + C::XCOPY)>();
+        else wait_vmcnt<0>();
+        lds_barrier();
+        if (pmore) issue();
+        if (s == 0) {
+          if (k == 0) {
 #pragma unroll
-      for (int j = 0; j < TM; ++j) acc[t][j] = f32x4{};
-    int64_t nm0 = 0, nf0 = 0;
-    bool more = false;
-    for (int kb = 0; kb < a.nk; ++kb) {
-      // the copies of this step have landed in every wave, and every wave is done with the other stage
-      wait_vmcnt<0>();
-      if ((kb & 3) == 0) {
+            for (int t = 0; t < TF; ++t) {
+              float b[16] = {};
+              const int f = wrow0 + 16 * h + (GATED ? t / TO * C::OF + 32 * (t % TO) : 32 * t);
+              if (a.bias) {
+                const uint8_t* slot = lds + C::LDS_BIAS + 1024 * tile;
+                if (a.bias_dtype == ATMA_F32) {
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-          xs_now[j] = xs_next[j];
-          asm volatile("" : "+v"(xs_now[j]));  // the compiler's own wait belongs here, before the next copies
+                  for (int e = 0; e < 16; e += 4) {
+                    const f32x4 v = *(const f32x4*)(slot + 4 * (f + e));
+                    b[e] = v[0], b[e + 1] = v[1], b[e + 2] = v[2], b[e + 3] = v[3];
+                  }
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 16; e += 8) {
+                    const u32x4 v = *(const u32x4*)(slot + 2 * (f + e));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                      b[e + i] = a.bias_dtype == ATMA_BF16 ? elem16<bf16>(v, i) : elem16<f16>(v, i);
+                  }
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < TM; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[t][j][e] = b[e];
+            }
+            tile = tile + 1 == C::AUX ? 0 : tile + 1;
+          }
+          if ((k & 7) == 0) {
+            words = (const uint32_t*)(lds + C::LDS_AUX + aux * (C::XS + 64) * 4);
+            aux = aux + 1 == C::AUX ? 0 : aux + 1;
+          }
+          const int sh = 4 * (k & 7);  // byte (k / 2) % 4
+#pragma unroll
+          for (int j = 0; j < TM; ++j) xs[j] = words[32 * (TM * wm + j) + r] >> sh;
+          ws[0] = words[C::XS + (GATED ? 0 : wrow0 / kFp8Block)] >> sh;
+          ws[1] = GATED ? words[C::XS + 1] >> sh : 0;
         }
-        ws_now[0] = ws_next[0];
-        ws_now[1] = GATED ? ws_next[1] : 0;
-        asm volatile("" : "+v"(ws_now[0]), "+v"(ws_now[1]));
-      }
-      lds_barrier();
-      if (kb + 1 < a.nk) {
-        if (((kb + 1) & 3) == 0) load_scales(m0, f0, kb + 1);
-        issue(stage ^ 1, kb + 1);
-      } else {
-        u += nper;
-        more = fp8_tile_at<C>(a, xcd, u, nm0, nf0);
-        if (more) {
-          aim(nm0, nf0);
-          load_scales(nm0, nf0, 0);
-          issue(stage ^ 1, 0);
-        }
-      }
-      const uint8_t* base = lds + stage * C::STAGE;
-      const int sh = 8 * (kb & 3);
-      Frag8 wv[TF];
-#pragma unroll
-      for (int t = 0; t < TF; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) wv[t].q[h] = *(const u32x4*)(base + wofs[t][h]);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        Frag8 xv;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) xv.q[h] = *(const u32x4*)(base + xofs[h] + 16 * j * kFp8Block);
-        const int xsc = (int)(xs_now[j] >> sh);
+        const uint8_t* base = lds + stage * C::STAGE;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        Frag8 wv[TF], xv[TM];
 #pragma unroll
         for (int t = 0; t < TF; ++t)
-          acc[t][j] = mfma_fp8(wv[t], xv, acc[t][j], (int)(ws_now[GATED ? t / TO : 0] >> sh), xsc);
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            wv[t].q[q] = *(const u32x4*)(base + wofs[q] + (GATED ? t / TO * (C::BF / 2) + 32 * (t % TO) : 32 * t) * 64);
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) xv[j].q[q] = *(const u32x4*)(base + xofs[q] + 32 * 64 * j);
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int t = 0; t < TF; ++t)
+            acc[t][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                wv[t].v, xv[j].v, acc[t][j], 0, 0, 0, (int)ws[GATED ? t / TO : 0], 0, (int)xs[j]);
       }
-      stage ^= 1;
     }
 
-    // ---- epilogue of tile (m0, f0): token 16 (TM wm + j) + r, features 4 G consecutive per group of tiles
+    // ---- epilogue of tile (m0, f0): token 32 (TM wm + j) + r, 16 consecutive features a tile
     if constexpr (!GATED) {
       const bool whole = f0 + C::OF <= a.N && a.ldy % 8 == 0;
 #pragma unroll
-      for (int grp = 0; grp < TO / G; ++grp) {
-        const int64_t n0 = f0 + wrow0 + 16 * G * grp + 4 * G * g;
-        float b[4 * G];
+      for (int j = 0; j < TM; ++j) {
+        const int64_t m = m0 + 32 * (TM * wm + j) + r;
+        if (m < a.M) {
 #pragma unroll
-        for (int e = 0; e < 4 * G; ++e) b[e] = n0 + e < a.N ? bias_at(a, n0 + e) : 0.f;
+          for (int t = 0; t < TF; ++t) {
+            const int64_t n0 = f0 + wrow0 + 32 * t + 16 * h;
+            T* y = (T*)a.y + m * a.ldy + n0;
+            const f32x16& v = acc[t][j];
+            if (whole) {
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-          const int64_t m = m0 + 16 * (TM * wm + j) + r;
-          if (m >= a.M) continue;
-          T* y = (T*)a.y + m * a.ldy + n0;
-          float v[4 * G];
+              for (int e = 0; e < 16; e += 8)
+                *(u32x4*)(y + e) = u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]),
+                                         pack2<T>(v[e + 4], v[e + 5]), pack2<T>(v[e + 6], v[e + 7])};
+            } else {
 #pragma unroll
-          for (int e = 0; e < 4 * G; ++e) v[e] = acc[grp * G + e / 4][j][e & 3] + b[e];
-          if (whole) {
-#pragma unroll
-            for (int e = 0; e < 4 * G; e += 8)
-              *(u32x4*)(y + e) = u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]),
-                                       pack2<T>(v[e + 4], v[e + 5]), pack2<T>(v[e + 6], v[e + 7])};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4 * G; ++e)
-              if (n0 + e < a.N) y[e] = from_f32<T>(v[e]);
+              for (int e = 0; e < 16; ++e)
+                if (n0 + e < a.N) y[e] = from_f32<T>(v[e]);
+            }
           }
         }
       }
     } else {
-      // the activations, in place of the a half's accumulators, and their largest magnitude over the wave's features
-      float top[TM] = {};
-#pragma unroll
-      for (int t = 0; t < TO; ++t) {
-        const int64_t n0 = f0 + wrow0 + 16 * G * (t / G) + 4 * G * g + 4 * (t % G);
-        float ba[4], bg[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ba[e] = bias_at(a, n0 + e), bg[e] = bias_at(a, a.N + n0 + e);
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float h = gate_act(acc[t][j][e] + ba[e], acc[TO + t][j][e] + bg[e]);
-            acc[t][j][e] = h;
-            top[j] = fmaxf(top[j], finite_abs(h));
-          }
-      }
+      // the activations in place of a's accumulators, their largest magnitude over the wave's features, then the tile's
+      float* part = (float*)(lds + C::LDS_TOP);
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        top[j] = fmaxf(top[j], wave_xor(top[j], 16));
-        top[j] = fmaxf(top[j], wave_xor(top[j], 32));
-        if (g == 0) amax_part[wf][16 * (TM * wm + j) + r] = top[j];
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float v = gate_act(acc[0][j][e], acc[1][j][e]);
+          acc[0][j][e] = v;
+          top = fmaxf(top, finite_abs(v));
+        }
+        top = fmaxf(top, wave_xor(top, 32));
+        if (h == 0) part[wf * C::BM + 32 * (TM * wm + j) + r] = top;
       }
       lds_barrier();
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const int row = 16 * (TM * wm + j) + r;
-        float t = amax_part[0][row];
+        const int row = 32 * (TM * wm + j) + r;
+        float top = part[row];
 #pragma unroll
-        for (int q = 1; q < WF; ++q) t = fmaxf(t, amax_part[q][row]);
-        const int code = fp8_scale_code(t);
+        for (int q = 1; q < WF; ++q) top = fmaxf(top, part[q * C::BM + row]);
+        const int code = fp8_scale_code(top);
         const float inv = fp8_inv_scale(code);
         const int64_t m = m0 + row;
-        if (m >= a.M) continue;
-        if (wf == 0 && g == 0) a.ys[m * a.ldys + f0 / kFp8Block] = (uint8_t)code;
+        if (m < a.M) {
+          if (wf == 0 && h == 0) a.ys[m * a.ldys + f0 / kFp8Block] = (uint8_t)code;
+          const f32x16& v = acc[0][j];
+          u32x4 o;
 #pragma unroll
-        for (int grp = 0; grp < TO / G; ++grp) {
-          uint32_t o[G];
-#pragma unroll
-          for (int t4 = 0; t4 < G; ++t4) {
-            const f32x4& h = acc[grp * G + t4][j];
-            o[t4] = fp8_pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-          }
-          uint8_t* y = (uint8_t*)a.y + m * a.ldy + f0 + wrow0 + 16 * G * grp + 4 * G * g;
-          if constexpr (G == 4) *(u32x4*)y = u32x4{o[0], o[1], o[2], o[3]};
-          else if constexpr (G == 2) *(u32x2*)y = u32x2{o[0], o[1]};
-          else *(uint32_t*)y = o[0];
+          for (int q = 0; q < 4; ++q)
+            o[q] = fp8_pack4(v[4 * q] * inv, v[4 * q + 1] * inv, v[4 * q + 2] * inv, v[4 * q + 3] * inv);
+          *(u32x4*)((uint8_t*)a.y + m * a.ldy + f0 + wrow0 + 16 * h) = o;
         }
       }
     }
-    if (!more) break;
-    m0 = nm0;
-    f0 = nf0;
+    u += nper;
+    if (!fp8_tile_at<C>(a, xcd, u, m0, f0)) break;
   }
 }
 
@@ -465,21 +497,21 @@ __global__ void __launch_bounds__(1024) fp8_few_gated_kernel(Fp8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-template <typename T, int TF, int TM, int WF, int WM, bool GATED>
+template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
 static void launch_tiles(Fp8Args a, hipStream_t s) {
-  using C = Fp8Tile<T, TF, TM, WF, WM, GATED>;
+  using C = Fp8Tile<TF, TM, WF, WM, NS, GATED>;
   a.m_tiles = (int)((a.M + C::BM - 1) / C::BM);
   a.f_tiles = (int)((a.N + C::OF - 1) / C::OF);
   const int64_t tiles = (int64_t)a.m_tiles * a.f_tiles;
   a.per_xcd = (int)((tiles + 7) / 8);
-  const int per_cu = 160 * 1024 / (2 * C::STAGE + 4096);  // workgroups that fit a CU's LDS
-  const int64_t wgs = std::min<int64_t>((int64_t)device_cu_count() / 8 * 8 * std::max(per_cu, 1), 8 * (int64_t)a.per_xcd);
-  fp8_tile_kernel<T, TF, TM, WF, WM, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
+  constexpr int per_cu = std::min(4, 160 * 1024 / C::LDS);  // workgroups that fit a CU's LDS
+  const int64_t wgs = std::min<int64_t>((int64_t)device_cu_count() / 8 * 8 * per_cu, 8 * (int64_t)a.per_xcd);
+  fp8_tile_kernel<T, TF, TM, WF, WM, NS, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
 }
 
 // Checks shared by the products; rows: weight rows (N, or 2 N gated)
 static int check_fp8(const char* what, const Fp8Args& a, int64_t rows) {
-  if (a.M < 0 || a.N < 1 || a.K < 16 || a.K % 16 || a.K > (1 << 22) || a.M > (1 << 30) || rows > (1 << 30))
+  if (a.M < 0 || a.N < 1 || a.K < 16 || a.K % 16 || a.K > (1 << 22) || a.M > (1 << 30) || rows > (1 << 28))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: unsupported shape M=%lld N=%lld K=%d (K a multiple of 16)", what,
                      (long long)a.M, (long long)a.N, a.K);
   if (a.M == 0) return ATMA_OK;
@@ -491,8 +523,9 @@ static int check_fp8(const char* what, const Fp8Args& a, int64_t rows) {
   // a tile's rows (at most 256) are addressed by 32-bit byte offsets
   if (a.ldx > (1 << 23) || a.ldw > (1 << 23))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: rows more than 8 MiB apart", what);
-  if (a.bias && (uintptr_t)a.bias % (size_t)std::max(dtype_size(a.bias_dtype), 1))
-    return set_error(ATMA_ERR_INVALID, "%s: unaligned bias", what);
+  if (a.ldxs > (1 << 20) || a.w_blocks * a.ldws >= (1ll << 31))
+    return set_error(ATMA_ERR_UNSUPPORTED, "%s: scales too far apart", what);
+  if (a.bias && (uintptr_t)a.bias % 4) return set_error(ATMA_ERR_INVALID, "%s: bias must be 4-byte aligned", what);
   if (a.bias && !dtype_size(a.bias_dtype))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: bias in fp32 or 16 bits (dtype %d)", what, a.bias_dtype);
   return ATMA_OK;
@@ -504,10 +537,12 @@ static void launch_linear(const Fp8Args& a, hipStream_t s) {
     fp8_few_kernel<T, 1, 1, 8><<<dim3((unsigned)((a.N + 15) / 16)), 512, 0, s>>>(a);
   } else if (a.M <= 32) {
     fp8_few_kernel<T, 2, 1, 8><<<dim3((unsigned)((a.N + 15) / 16)), 512, 0, s>>>(a);
-  } else if (((a.M + 255) / 256) * ((a.N + 255) / 256) >= device_cu_count()) {
-    launch_tiles<T, 4, 8, 4, 2, false>(a, s);
+  } else if (((a.M + 127) / 128) * ((a.N + 255) / 256) >= 2 * device_cu_count()) {
+    launch_tiles<T, 2, 4, 4, 1, 3, false>(a, s);
+  } else if (((a.M + 127) / 128) * ((a.N + 127) / 128) >= device_cu_count()) {
+    launch_tiles<T, 2, 2, 2, 2, 4, false>(a, s);
   } else {
-    launch_tiles<T, 4, 4, 2, 2, false>(a, s);
+    launch_tiles<T, 1, 1, 2, 2, 8, false>(a, s);
   }
 }
 
@@ -520,8 +555,8 @@ extern "C" int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64
   if (dtype != ATMA_BF16 && dtype != ATMA_F16)
     return set_error(ATMA_ERR_UNSUPPORTED, "linear_fp8: 16-bit output only (dtype %d)", dtype);
   if (K < 0 || K > (1 << 22)) return set_error(ATMA_ERR_UNSUPPORTED, "linear_fp8: K=%lld", (long long)K);
-  Fp8Args a{(const uint8_t*)x, ldx, (const uint8_t*)xs, ldxs, (const uint8_t*)w, ldw, (const uint8_t*)ws, ldws, bias,
-            bias_dtype, y, ldy, nullptr, 0, M, N, (int)K, (int)((K + kFp8Block - 1) / kFp8Block), 0, 0, 0};
+  Fp8Args a{(const uint8_t*)x, ldx, (const uint8_t*)xs, ldxs, (const uint8_t*)w, ldw, (const uint8_t*)ws, ldws,
+            (N + kFp8Block - 1) / kFp8Block, bias, bias_dtype, y, ldy, nullptr, 0, M, N, (int)K, (int)((K + kFp8Block - 1) / kFp8Block), 0, 0, 0};
   if (const int rc = check_fp8("linear_fp8", a, N)) return rc;
   if (M == 0) return ATMA_OK;
   if (ldy < N || (uintptr_t)y % 2 || (ldy % 8 == 0 && (uintptr_t)y % 16))
@@ -537,9 +572,9 @@ extern "C" int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs,
                                      void* stream) {
   using namespace atma;
   if (K < 0 || K > (1 << 22)) return set_error(ATMA_ERR_UNSUPPORTED, "linear_gated_fp8: K=%lld", (long long)K);
-  Fp8Args a{(const uint8_t*)x, ldx, (const uint8_t*)xs, ldxs, (const uint8_t*)w, ldw, (const uint8_t*)ws, ldws, bias,
-            bias_dtype, y, ldy, (uint8_t*)ys, ldys, M, H, (int)K, (int)((K + kFp8Block - 1) / kFp8Block), 0, 0, 0};
-  if (H < kFp8Block || H % kFp8Block || H > (1 << 29))
+  Fp8Args a{(const uint8_t*)x, ldx, (const uint8_t*)xs, ldxs, (const uint8_t*)w, ldw, (const uint8_t*)ws, ldws,
+            2 * H / kFp8Block, bias, bias_dtype, y, ldy, (uint8_t*)ys, ldys, M, H, (int)K, (int)((K + kFp8Block - 1) / kFp8Block), 0, 0, 0};
+  if (H < kFp8Block || H % kFp8Block || H > (1 << 27))
     return set_error(ATMA_ERR_UNSUPPORTED, "linear_gated_fp8: H must be a multiple of %d (got %lld)", kFp8Block,
                      (long long)H);
   if (const int rc = check_fp8("linear_gated_fp8", a, 2 * H)) return rc;
@@ -549,7 +584,8 @@ extern "C" int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs,
   hipStream_t s = (hipStream_t)stream;
   if (M <= 16) fp8_few_gated_kernel<1><<<dim3((unsigned)(H / kFp8Block)), 1024, 0, s>>>(a);
   else if (M <= 32) fp8_few_gated_kernel<2><<<dim3((unsigned)(H / kFp8Block)), 1024, 0, s>>>(a);
-  else if (((M + 255) / 256) * (H / kFp8Block) >= device_cu_count()) launch_tiles<bf16, 4, 8, 4, 2, true>(a, s);
-  else launch_tiles<bf16, 4, 4, 4, 1, true>(a, s);
+  else if (((M + 127) / 128) * (H / kFp8Block) >= 2 * device_cu_count()) launch_tiles<bf16, 2, 4, 4, 1, 3, true>(a, s);
+  else if (((M + 63) / 64) * (H / kFp8Block) >= device_cu_count()) launch_tiles<bf16, 2, 2, 4, 1, 3, true>(a, s);
+  else launch_tiles<bf16, 2, 1, 4, 1, 4, true>(a, s);
   return check_launch("linear_gated_fp8");
 }

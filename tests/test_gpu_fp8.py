@@ -189,7 +189,8 @@ def _near_product(y, exact, size):
 
 SHAPES = [(1, 1, 16), (1, 1024, 4096), (2, 7, 128), (16, 40, 144), (17, 129, 272), (31, 1001, 1024), (32, 128, 112),
           (33, 16, 128), (33, 129, 1040), (64, 256, 640), (100, 257, 2048), (129, 1000, 384), (257, 130, 1024),
-          (300, 512, 528), (700, 72, 896)]
+          (300, 512, 528), (700, 72, 896),
+          (2100, 2001, 528), (8200, 2104, 272), (4100, 4097, 80)]
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -207,7 +208,8 @@ def test_linear(dev, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("M,H,K", [(1, 128, 16), (1, 4096, 1024), (9, 256, 144), (16, 384, 1040), (32, 128, 2048),
-                                   (33, 128, 128), (64, 256, 272), (100, 640, 1024), (129, 128, 384), (300, 512, 640)])
+                                   (33, 128, 128), (64, 256, 272), (100, 640, 1024), (129, 128, 384), (300, 512, 640),
+                                   (2001, 1024, 272), (4201, 2048, 144)])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 def test_linear_gated(dev, M, H, K, bias):
     from atma_amd.kernel import linear_gated_fp8
