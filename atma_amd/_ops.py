@@ -950,18 +950,16 @@ def _(gs, xs, ws):
 
 
 # --------------------------------------------------------------------------- 8-bit inference (kernel/fp8.py)
+# Each op is a launch on operands as the kernels take them (``fp8_*``, which kernel/fp8.py calls by itself where nothing is
+# to dispatch or to copy) behind whatever copies bring them there.
 FP8, FP8_SCALE, FP8_BLOCK = torch.float8_e4m3fn, torch.float8_e8m0fnu, 128
-
-
-def _fp8_blocks(n: int) -> int:
-    return (n + FP8_BLOCK - 1) // FP8_BLOCK
 
 
 def _fp8_pair(like: Tensor, rows: int, cols: int, scale_rows: int):
     """Empty (data, scale); a row of scales starts at a multiple of 4 bytes, as the products read them."""
-    nb = _fp8_blocks(cols)
+    nb = (cols + 127) // 128
     scale = like.new_empty((scale_rows, (nb + 3) // 4 * 4), dtype=FP8_SCALE)
-    return like.new_empty((rows, cols), dtype=FP8), scale[:, :nb]
+    return like.new_empty((rows, cols), dtype=FP8), scale if nb % 4 == 0 else scale[:, :nb]
 
 
 def _rows_apart(t: Tensor) -> Tensor:
@@ -978,21 +976,27 @@ def _fp8_scales(t: Tensor) -> Tensor:
     return held[:, :t.shape[1]]
 
 
-def _quantize_fp8(name, x, scale_rows):
-    _need_cuda(x)
-    with _lib.on_device(x.device):
-        x = _rows_apart(x)
-        data, scale = _fp8_pair(x, x.shape[0], x.shape[1], scale_rows)
-        rc = getattr(_lib.load(), "atma_" + name)(
-            x.data_ptr(), x.stride(0), data.data_ptr(), data.stride(0), scale.data_ptr(), scale.stride(0), x.shape[0],
-            x.shape[1], _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
-        _lib.check(rc, name)
-    return [data, scale]
+def _bias4(t: Optional[Tensor]) -> Optional[Tensor]:
+    if t is None or (t.stride(0) == 1 and t.data_ptr() % 4 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def fp8_quantize(name: str, x: Tensor, scale_rows: int):
+    rows, cols = x.shape
+    data, scale = _fp8_pair(x, rows, cols, scale_rows)
+    rc = getattr(_lib.load(), name)(x.data_ptr(), x.stride(0), data.data_ptr(), cols, scale.data_ptr(), scale.stride(0), rows,
+                                    cols, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(x.device))
+    if rc:
+        _lib.check(rc, name[5:])
+    return data, scale
 
 
 @_op("quantize_fp8", mutates_args=())
 def quantize_fp8_op(x: Tensor) -> List[Tensor]:
-    return _quantize_fp8("quantize_fp8", x, x.shape[0])
+    _need_cuda(x)
+    with _lib.on_device(x.device):
+        return list(fp8_quantize("atma_quantize_fp8", _rows_apart(x), x.shape[0]))
 
 
 @quantize_fp8_op.register_fake
@@ -1002,12 +1006,33 @@ def _(x):
 
 @_op("quantize_weight_fp8", mutates_args=())
 def quantize_weight_fp8_op(weight: Tensor) -> List[Tensor]:
-    return _quantize_fp8("quantize_weight_fp8", weight, _fp8_blocks(weight.shape[0]))
+    _need_cuda(weight)
+    with _lib.on_device(weight.device):
+        return list(fp8_quantize("atma_quantize_weight_fp8", _rows_apart(weight), (weight.shape[0] + 127) // 128))
 
 
 @quantize_weight_fp8_op.register_fake
 def _(weight):
-    return list(_fp8_pair(weight, weight.shape[0], weight.shape[1], _fp8_blocks(weight.shape[0])))
+    return list(_fp8_pair(weight, weight.shape[0], weight.shape[1], (weight.shape[0] + 127) // 128))
+
+
+def fp8_norm(y, parts, biases, mu_x, mu_w, residual, weight, eps, keep):
+    M, D = y.shape if parts is None else parts.shape[1:]
+    data, scale = _fp8_pair(weight, M, D, M)
+    stream = weight.new_empty((M, D)) if keep else None
+    held = None
+    if biases:
+        held = (ctypes.c_void_p * len(biases))(*[b.data_ptr() for b in biases])
+    rc = _lib.load().atma_residual_rms_norm_fp8(
+        None if y is None else y.data_ptr(), 0 if y is None else y.stride(0), None if parts is None else parts.data_ptr(),
+        0 if parts is None else parts.shape[0], held, len(biases), _lib.ptr(mu_x), 0 if mu_x is None else mu_x.stride(0),
+        _lib.ptr(mu_w), 0 if mu_x is None else mu_x.shape[1], None if residual is None else residual.data_ptr(),
+        0 if residual is None else residual.stride(0), stream.data_ptr() if keep else None, D, weight.data_ptr(),
+        data.data_ptr(), D, scale.data_ptr(), scale.stride(0), M, D, eps, _lib.DTYPE_CODE[weight.dtype],
+        _lib.stream_handle(weight.device))
+    if rc:
+        _lib.check(rc, "residual_rms_norm_fp8")
+    return data, scale, stream
 
 
 @_op("residual_rms_norm_fp8", mutates_args=())
@@ -1015,27 +1040,15 @@ def residual_rms_norm_fp8_op(y: Optional[Tensor], parts: Optional[Tensor], biase
                              mu_w: Optional[Tensor], residual: Optional[Tensor], weight: Tensor, eps: float,
                              keep: bool) -> List[Tensor]:
     """[data, scale] and, with ``keep``, the new stream; exactly one of y (M, D) and parts (P, M, D)."""
-    src = y if parts is None else parts
-    _need_cuda(src, residual, weight, mu_x, mu_w, *biases)
-    M, D = src.shape[-2:]
-    with _lib.on_device(src.device):
+    _need_cuda(y, parts, residual, weight, mu_x, mu_w, *biases)
+    with _lib.on_device(weight.device):
         y, residual = (None if t is None else _rows_apart(t) for t in (y, residual))
         parts, mu_w = (None if t is None else _aligned16(t) for t in (parts, mu_w))
-        biases, weight = [_aligned16(b) for b in biases], _aligned16(weight)
         if mu_x is not None and (mu_x.stride(1) != 1 or mu_x.stride(0) % 2 or mu_x.stride(0) < mu_x.shape[1]
                                  or mu_x.data_ptr() % 4):
             mu_x = _aligned16(mu_x)
-        data, scale = _fp8_pair(weight, M, D, M)
-        stream = weight.new_empty((M, D)) if keep else None
-        held = (ctypes.c_void_p * max(1, len(biases)))(*[b.data_ptr() for b in biases])
-        rc = _lib.load().atma_residual_rms_norm_fp8(
-            _lib.ptr(y), 0 if y is None else y.stride(0), _lib.ptr(parts), 0 if parts is None else parts.shape[0],
-            ctypes.addressof(held), len(biases), _lib.ptr(mu_x), 0 if mu_x is None else mu_x.stride(0), _lib.ptr(mu_w),
-            0 if mu_x is None else mu_x.shape[1], _lib.ptr(residual), 0 if residual is None else residual.stride(0),
-            _lib.ptr(stream), D, weight.data_ptr(), data.data_ptr(), D, scale.data_ptr(), scale.stride(0), M, D, eps,
-            _lib.dtype_code(weight.dtype), _lib.stream_handle(src.device))
-        _lib.check(rc, "residual_rms_norm_fp8")
-    return [data, scale, stream] if keep else [data, scale]
+        out = fp8_norm(y, parts, [_aligned16(b) for b in biases], mu_x, mu_w, residual, _aligned16(weight), eps, keep)
+    return list(out) if keep else list(out[:2])
 
 
 @residual_rms_norm_fp8_op.register_fake
@@ -1044,22 +1057,26 @@ def _(y, parts, biases, mu_x, mu_w, residual, weight, eps, keep):
     return list(_fp8_pair(weight, M, D, M)) + ([weight.new_empty((M, D))] if keep else [])
 
 
+def fp8_linear(x, x_scale, weight, weight_scale, bias, out_dtype):
+    (M, K), N = x.shape, weight.shape[0]
+    out = x.new_empty((M, N), dtype=out_dtype)
+    rc = _lib.load().atma_linear_fp8(
+        x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), weight.data_ptr(), weight.stride(0),
+        weight_scale.data_ptr(), weight_scale.stride(0), None if bias is None else bias.data_ptr(),
+        0 if bias is None else _lib.DTYPE_CODE[bias.dtype], out.data_ptr(), N, M, N, K, _lib.DTYPE_CODE[out_dtype],
+        _lib.stream_handle(x.device))
+    if rc:
+        _lib.check(rc, "linear_fp8")
+    return out
+
+
 @_op("linear_fp8", mutates_args=())
 def linear_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
                   out_dtype: torch.dtype) -> Tensor:
     _need_cuda(x, x_scale, weight, weight_scale, bias)
     with _lib.on_device(x.device):
-        x, weight, x_scale, weight_scale = _rows_apart(x), _rows_apart(weight), _fp8_scales(x_scale), _fp8_scales(weight_scale)
-        bias = None if bias is None else bias.contiguous()
-        (M, K), N = x.shape, weight.shape[0]
-        out = torch.empty((M, N), device=x.device, dtype=out_dtype)
-        rc = _lib.load().atma_linear_fp8(
-            x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), weight.data_ptr(), weight.stride(0),
-            weight_scale.data_ptr(), weight_scale.stride(0), _lib.ptr(bias),
-            _lib.ATMA_F32 if bias is None else _lib.dtype_code(bias.dtype), out.data_ptr(), N, M, N, K,
-            _lib.dtype_code(out_dtype), _lib.stream_handle(x.device))
-        _lib.check(rc, "linear_fp8")
-    return out
+        return fp8_linear(_rows_apart(x), _fp8_scales(x_scale), _rows_apart(weight), _fp8_scales(weight_scale), _bias4(bias),
+                          out_dtype)
 
 
 @linear_fp8_op.register_fake
@@ -1067,22 +1084,26 @@ def _(x, x_scale, weight, weight_scale, bias, out_dtype):
     return x.new_empty((x.shape[0], weight.shape[0]), dtype=out_dtype)
 
 
+def fp8_linear_gated(x, x_scale, weight, weight_scale, bias):
+    (M, K), H = x.shape, weight.shape[0] // 2
+    data, scale = _fp8_pair(x, M, H, M)
+    rc = _lib.load().atma_linear_gated_fp8(
+        x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), weight.data_ptr(), weight.stride(0),
+        weight_scale.data_ptr(), weight_scale.stride(0), None if bias is None else bias.data_ptr(),
+        0 if bias is None else _lib.DTYPE_CODE[bias.dtype], data.data_ptr(), H, scale.data_ptr(), scale.stride(0), M, H, K,
+        _lib.stream_handle(x.device))
+    if rc:
+        _lib.check(rc, "linear_gated_fp8")
+    return data, scale
+
+
 @_op("linear_gated_fp8", mutates_args=())
 def linear_gated_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor,
                         bias: Optional[Tensor]) -> List[Tensor]:
     _need_cuda(x, x_scale, weight, weight_scale, bias)
     with _lib.on_device(x.device):
-        x, weight, x_scale, weight_scale = _rows_apart(x), _rows_apart(weight), _fp8_scales(x_scale), _fp8_scales(weight_scale)
-        bias = None if bias is None else bias.contiguous()
-        (M, K), H = x.shape, weight.shape[0] // 2
-        data, scale = _fp8_pair(x, M, H, M)
-        rc = _lib.load().atma_linear_gated_fp8(
-            x.data_ptr(), x.stride(0), x_scale.data_ptr(), x_scale.stride(0), weight.data_ptr(), weight.stride(0),
-            weight_scale.data_ptr(), weight_scale.stride(0), _lib.ptr(bias),
-            _lib.ATMA_F32 if bias is None else _lib.dtype_code(bias.dtype), data.data_ptr(), H, scale.data_ptr(),
-            scale.stride(0), M, H, K, _lib.stream_handle(x.device))
-        _lib.check(rc, "linear_gated_fp8")
-    return [data, scale]
+        return list(fp8_linear_gated(_rows_apart(x), _fp8_scales(x_scale), _rows_apart(weight), _fp8_scales(weight_scale),
+                                     _bias4(bias)))
 
 
 @linear_gated_fp8_op.register_fake

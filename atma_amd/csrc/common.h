@@ -175,12 +175,6 @@ __device__ __forceinline__ void dma_buf4(__amdgpu_buffer_rsrc_t r, uint32_t voff
                "{m0}"(__builtin_amdgcn_readfirstlane(off))
                : "memory");
 }
-__device__ __forceinline__ void dma_buf4_at(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff,
-                                            uint32_t lds_byte_offset) {
-  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff),
-               "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
-               : "memory");
-}
 __device__ __forceinline__ void buffer_store16(__amdgpu_buffer_rsrc_t r, uint32_t voff, u32x4 x) {
   __builtin_amdgcn_raw_buffer_store_b128(x, r, voff, 0, 0);
 }

@@ -23,6 +23,7 @@ __device__ __forceinline__ int fp8_scale_code(float amax) {
 __device__ __forceinline__ float fp8_inv_scale(int code) {
   return __builtin_bit_cast(float, (uint32_t)(254 - code) << 23);
 }
+__device__ __forceinline__ float fp8_scale(int code) { return __builtin_bit_cast(float, (uint32_t)code << 23); }
 // |x|, 0 where x is not finite
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
@@ -33,6 +34,14 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   v = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
   return (uint32_t)v;
+}
+// Four values divided by a power of two to e4m3fn (v_cvt_scalef32_pk_fp8_f32), rounded as above
+__device__ __forceinline__ uint32_t fp8_scaled4(float a, float b, float c, float d, float scale) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 v = {0, 0};
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, a, b, scale, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, v);
 }
 
 }  // namespace atma

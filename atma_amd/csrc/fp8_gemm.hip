@@ -16,16 +16,13 @@
 
 namespace atma {
 
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 union Frag8 {  // one operand: 32 values of a row
   i32x8 v;
   u32x4 q[2];
 };
-
-__device__ __forceinline__ f32x4 mfma_fp8(const Frag8& w, const Frag8& x, const f32x4& c, int ws, int xs) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, c, 0, 0, 0, ws, 0, xs);
-}
 
 struct Fp8Args {
   const uint8_t* x;  // (M, K), row stride ldx
@@ -55,47 +52,43 @@ __device__ __forceinline__ float bias_at(const Fp8Args& a, int64_t n) {
   return ((const float*)a.bias)[n];
 }
 
-// relu(a)^2 * gate in fp32 (NaN passes through, as torch's relu)
+// relu(a)^2 * gate in fp32 (v_maximum3_f32: NaN passes through, as torch's relu)
 __device__ __forceinline__ float gate_act(float av, float gv) {
-  const float pos = av < 0.f ? 0.f : av;
+  const float pos = __builtin_elementwise_maximum(av, 0.f);
   return gv * (pos * pos);
 }
 
-// ------------------------------------------------------------------------------------------------ tiles
-// A workgroup of four waves, WF x WM, owns BF weight rows x BM tokens, a wave TF x TM tiles of 32 x 32
-// (v_mfma_scale_f32_32x32x64_f8f6f4: two instructions for a block of 128 along K).  K runs in steps of 64 through a ring of
-// NS stages in LDS, filled NS - 1 steps ahead by direct copies; the workgroup is persistent and the ring runs on across its
-// tiles, so a tile's first copies fly during the last steps and the epilogue of the one before.  Everything else a tile
-// reads -- the scales of four blocks at a time, the bias -- comes through the same copies into small rings of their own:
-// the loop has no load into registers, whose wait would drain the ring.
-//
-// A step's rows are 64 bytes, four chunks of 16, chunk c of row r at position c ^ f(r): the 16 lanes that read one chunk of
-// 16 rows cover all banks when f takes four values over the rows of each residue mod 4.  The weights are the MFMA's rows,
-// in an order such that a lane's accumulators are 16 consecutive features of one token (row 8 q + 4 h + e is feature
-// 16 h + 4 q + e; lane half h holds the rows 4 h + e of each 8): outputs are stored straight from registers.
-__device__ __forceinline__ int x_swizzle(int r) { return (r >> 2) & 3; }
-__device__ __forceinline__ int w_swizzle(int r) { return ((r >> 2) & 1) | (((r >> 4) & 1) << 1); }
+// Rows of 128 bytes in LDS, eight chunks of 16, chunk c of row r at position c ^ f(r): the 16 lanes that read one chunk of
+// 16 rows cover all banks when f takes eight values over the rows of each parity (measured: no conflicts).  The weights are
+// the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token (row 8 q + 4 h + e
+// is feature 16 h + 4 q + e; lane half h holds the rows 4 h + e of each 8): outputs are stored straight from registers.
+__device__ __forceinline__ int x_swizzle(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int w_swizzle(int r) { return ((r >> 1) & 3) | (((r >> 4) & 1) << 2); }
 
-template <int TF, int TM, int WF, int WM, int NS, bool GATED>
-struct Fp8Tile {
-  static constexpr int NW = WF * WM;
-  static constexpr int BF = 32 * TF * WF, BM = 32 * TM * WM;
-  static constexpr int OF = GATED ? BF / 2 : BF;  // output features
-  static constexpr int TO = GATED ? TF / 2 : TF;  // tiles of output features a wave
-  static constexpr int STAGE = (BF + BM) * 64;
-  static constexpr int WCOPY = BF / 16 / NW, XCOPY = BM / 16 / NW;  // copies a wave and step: 16 rows each
-  static constexpr int XS = BM > 64 ? BM : 64;                      // words of token scales
-  static constexpr int AUX = (NS - 1) / 2 + 2;  // scale groups and tiles that can be under way (two steps at least each)
-  static constexpr int LDS_AUX = NS * STAGE, LDS_BIAS = LDS_AUX + AUX * (XS + 64) * 4;
-  static constexpr int LDS_TOP = LDS_BIAS + AUX * 1024, LDS = LDS_TOP + (GATED ? WF * BM * 4 : 0);
-  static_assert(NW == 4 && BF % (16 * NW) == 0 && BF <= 256 && BM <= 256, "whole copies, a bias of 1 KiB");
-  static_assert(BM % (16 * NW) == 0 || BM == 32, "whole copies");
-  static_assert(!GATED || (OF == kFp8Block && TF == 2), "a gated tile is one block of output features");
-  static_assert((NS - 2) * (WCOPY + XCOPY + 1) < 64, "vmcnt counts to 63");
-};
+// The kernel's arguments read again where they are needed: kept in scalar registers through the loop they would be spilled
+typedef const __attribute__((address_space(4))) Fp8Args* LateArgs;
+__device__ __forceinline__ LateArgs late_args() {
+  LateArgs p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
-template <typename C>
-__device__ __forceinline__ bool fp8_tile_at(const Fp8Args& a, int xcd, int u, int64_t& m0, int64_t& f0) {
+// The 4-byte copy where a descriptor may just have been read back from a vector register: five wait states before it
+__device__ __forceinline__ void dma_buf4_rare(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_byte_offset) {
+  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(r),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
+               : "memory");
+}
+// 4 bytes a lane from an address a lane to lds_byte_offset + 4 lane
+__device__ __forceinline__ void dma_load4_at(const void* p, uint32_t lds_byte_offset) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
+               : "memory");
+}
+
+// Tile u of an XCD: each owns a contiguous range, walked as groups of four token tiles x all feature tiles
+template <typename C, typename A>
+__device__ __forceinline__ bool fp8_tile_at(const A& a, int xcd, int u, int64_t& m0, int64_t& f0) {
   const int t = xcd * a.per_xcd + u;
   if (u >= a.per_xcd || t >= a.m_tiles * a.f_tiles) return false;
   const int grp = t / (4 * a.f_tiles), r = t - grp * 4 * a.f_tiles;
@@ -104,6 +97,41 @@ __device__ __forceinline__ bool fp8_tile_at(const Fp8Args& a, int xcd, int u, in
   f0 = (int64_t)(r / gm) * C::OF;
   return true;
 }
+
+__device__ __forceinline__ f32x4 mfma_fp8(const Frag8& w, const Frag8& x, const f32x4& c, int ws, int xs) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, c, 0, 0, 0, ws, 0, xs);
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+// A workgroup of WF x WM waves owns BF weight rows x BM tokens, a wave TF x TM tiles of 32 x 32
+// (v_mfma_scale_f32_32x32x64_f8f6f4: two instructions for a block of 128 along K).  K runs in blocks through a ring of NS
+// stages in LDS, filled by direct copies of whole 128-byte lines (a CU takes in 58 to 94 bytes a cycle that way, 29 to 54
+// in rows of 64 bytes: measured from L2 with four and eight waves).  While the products of one half of a block run from
+// registers, the operands of the next half are read from LDS, a token operand into the registers of the one just used,
+// the weights into a second set; in the second half the copies of block k + NS go into the stage just read.  The
+// workgroup is persistent and all of this runs on across its tiles: a tile's first copies fly and its first operands are
+// read during the last blocks of the one before.
+//
+// A block is straight code (the compiler gathers products behind any branch): copies behind the last tile go on, out of
+// range, and the scales of a block come with its copies.
+template <int TF, int TM, int WF, int WM, int NS_, bool GATED>
+struct Fp8Tile {
+  static constexpr int NW = WF * WM, NS = NS_;
+  static constexpr int BF = 32 * TF * WF, BM = 32 * TM * WM;
+  static constexpr int OF = GATED ? BF / 2 : BF;  // output features
+  static constexpr int TO = GATED ? TF / 2 : TF;  // tiles of output features a wave
+  static constexpr int STAGE = (BF + BM) * kFp8Block;
+  static constexpr int WCOPY = BF / 8 / NW, XCOPY = BM / 8 / NW, COPIES = WCOPY + XCOPY;  // a wave and block, 8 rows each
+  static constexpr int XW = BM / NW;     // token scales a wave copies
+  static constexpr int RING = NS + 2;    // blocks and tiles under way: copies run NS blocks ahead
+  static constexpr int SLOT = NW * 256;  // a block's scales
+  static constexpr int AUX = NS * STAGE, BIAS = AUX + RING * SLOT, TOP = BIAS + RING * 1024;
+  static constexpr int LDS = TOP + (GATED ? WF * BM * 4 : 0);
+  static_assert((NW == 4 || NW == 8) && BF % (8 * NW) == 0 && BM % (8 * NW) == 0 && BF <= 256 && XW <= 32,
+                "whole copies, a bias of 1 KiB");
+  static_assert(!GATED || (OF == kFp8Block && TF == 2), "a gated tile is one block of output features");
+  static_assert((NS - 2) * (COPIES + 1) < 63, "vmcnt counts to 63");
+};
 
 template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
 __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
@@ -114,188 +142,208 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave % WF, wm = wave / WF;
   const int r = lane & 31, h = lane >> 5;
-  const int xcd = blockIdx.x & 7, nper = gridDim.x >> 3;
-  const int steps = 2 * a.nk;
+  const int nk = a.nk;
   int64_t m0, f0;
   int u = blockIdx.x >> 3;
-  if (!fp8_tile_at<C>(a, xcd, u, m0, f0)) return;
+  if (!fp8_tile_at<C>(a, blockIdx.x & 7, u, m0, f0)) return;
 
-  // ---- the copies, NS - 1 steps ahead of the products.  Copy i of a wave moves rows 16 (i NW + wave) .. + 15: lane l
-  // writes row l / 4, position l % 4, and reads the chunk that belongs there; chunks past K (offset 2^31, past every tile)
-  // and rows past the end read as zeros
+  // ---- the copies, NS blocks ahead.  Copy i of a wave moves rows 8 (i NW + wave) .. + 7: lane l writes row l / 8,
+  // position l % 8, and reads the chunk that belongs there; out of range (chunks past K, rows past the end, everything
+  // behind the last tile) zeros are written
   const uint32_t lds0 = lds_offset(lds);
-  const int crow = lane >> 2;
-  const int wk = 16 * ((lane & 3) ^ w_swizzle(16 * wave + crow)), xk = 16 * ((lane & 3) ^ x_swizzle(crow));
-  const uint32_t wv0 = (uint32_t)(16 * wave + crow) * (uint32_t)a.ldw, xv0 = (uint32_t)(16 * wave + crow) * (uint32_t)a.ldx;
-  const uint32_t wstep = 16u * C::NW * (uint32_t)a.ldw, xstep = 16u * C::NW * (uint32_t)a.ldx;
-  __amdgpu_buffer_rsrc_t xr, wr, gr, xsr, wsr;
-  int pu = u, pk = 0, pstage = 0, paux = 0, ptile = 0;
-  int64_t pf0 = 0;
-  bool pmore = true;
+  const int crow = 8 * wave + (lane >> 3);
+  const int wk = 16 * ((lane & 7) ^ w_swizzle(crow)), xk = 16 * ((lane & 7) ^ x_swizzle(crow));
+  const uint32_t wv0 = (uint32_t)crow * (uint32_t)a.ldw + (uint32_t)wk, xv0 = (uint32_t)crow * (uint32_t)a.ldx + (uint32_t)xk;
+  const uint32_t wstep = 8u * C::NW * (uint32_t)a.ldw, xstep = 8u * C::NW * (uint32_t)a.ldx;
+  __amdgpu_buffer_rsrc_t xr, wr, gr;
+  const uint8_t* scales;  // a lane's row: lanes 0 .. XW - 1 token rows, 32 and 33 weight blocks, the others as lane 0
+  int pu = u, pk = 0, plimit = 0, ptile = 0, pslot = 0, pstage = 0;
   auto aim = [&](int64_t tm0, int64_t tf0) {
-    const int64_t rows = min((int64_t)C::BM, a.M - tm0);
-    xr = buffer_rsrc(a.x + tm0 * a.ldx, (uint32_t)(rows * a.ldx));
-    xsr = buffer_rsrc(a.xs + tm0 * a.ldxs, (uint32_t)(rows * a.ldxs));
-    const uint32_t wb = (uint32_t)(min((int64_t)C::OF, a.N - tf0) * a.ldw);
-    wr = buffer_rsrc(a.w + tf0 * a.ldw, wb);
-    if constexpr (GATED) gr = buffer_rsrc(a.w + (a.N + tf0) * a.ldw, wb);
+    LateArgs p = late_args();
+    const int64_t rows = min((int64_t)C::BM, p->M - tm0);
+    xr = buffer_rsrc(p->x + tm0 * p->ldx, (uint32_t)(rows * p->ldx));
+    const uint32_t wb = (uint32_t)(min((int64_t)C::OF, p->N - tf0) * p->ldw);
+    wr = buffer_rsrc(p->w + tf0 * p->ldw, wb);
+    if constexpr (GATED) gr = buffer_rsrc(p->w + (p->N + tf0) * p->ldw, wb);
+    const int64_t m = min(tm0 + C::XW * wave + (lane < C::XW ? lane : 0), p->M - 1);
     const int64_t b0 = tf0 / kFp8Block;
-    wsr = buffer_rsrc(a.ws + b0 * a.ldws, (uint32_t)((a.w_blocks - b0) * a.ldws));
-    pf0 = tf0;
+    const int64_t b = lane == 33 ? (GATED ? b0 + p->N / kFp8Block : min(b0 + 1, p->w_blocks - 1)) : b0;
+    scales = lane == 32 || lane == 33 ? p->ws + b * p->ldws : p->xs + m * p->ldxs;
+    plimit = p->K;
+    if (p->bias && wave == 2) {
+      // the tile's biases (gated: 128 of a, 128 of gate), in words, to its slot
+      const int size = p->bias_dtype == ATMA_F32 ? 4 : 2;
+      const int64_t total = (GATED ? 2 : 1) * p->N * size;
+      const __amdgpu_buffer_rsrc_t br = buffer_rsrc(p->bias, (uint32_t)((total + 3) & ~3ll));
+      for (int i = 0; i < size; ++i) {
+        const int f = (64 * i + lane) * 4 / size;  // the word's first feature in the tile
+        const int64_t n = tf0 + (GATED && f >= C::OF ? p->N + f - C::OF : f);
+        dma_buf4_rare(br, n * size < total ? (uint32_t)(n * size) : 0xfffffffcu,
+                      lds0 + C::BIAS + 1024 * ptile + 256 * i);
+      }
+    }
+    ptile = ptile + 1 == C::RING ? 0 : ptile + 1;
   };
-  auto issue = [&]() {
-    if (pk == 0 && a.bias && wave == C::NW - 2) {
-      // 256 biases (gated: 128 of a, 128 of gate), in words, to this tile's slot
-      const int size = a.bias_dtype == ATMA_F32 ? 4 : 2;
-      const int64_t total = (GATED ? 2 : 1) * a.N * size;
-      const __amdgpu_buffer_rsrc_t br = buffer_rsrc(a.bias, (uint32_t)((total + 3) & ~3ll));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int word = 64 * i + lane, f = word * 4 / size;  // the word's first feature in the tile
-        if (64 * i * 4 / size < 256) {
-          const int64_t n = pf0 + (GATED && f >= C::OF ? a.N + f - C::OF : f);
-          dma_buf4(br, n * size < total ? (uint32_t)(n * size) : 0xfffffffcu, 0u,
-                   lds + C::LDS_BIAS + 1024 * ptile + 256 * i);
-        }
-      }
-    }
-    if ((pk & 7) == 0) {
-      const uint32_t slot = lds0 + C::LDS_AUX + paux * (C::XS + 64) * 4;
-      const uint32_t k4 = (uint32_t)pk >> 1;
-      if (wave < C::XS / 64)
-        dma_buf4_at(xsr, (uint32_t)(64 * wave + lane) * (uint32_t)a.ldxs + k4, 0u, slot + 256 * wave);
-      if (wave == C::NW - 1) {
-        const uint32_t row = GATED ? (lane ? (uint32_t)(a.N / kFp8Block) : 0u) : (uint32_t)lane;
-        dma_buf4_at(wsr, lane < 2 ? row * (uint32_t)a.ldws + k4 : 0x80000000u, 0u, slot + 4 * C::XS);
-      }
-      paux = paux + 1 == C::AUX ? 0 : paux + 1;
-    }
-    const uint32_t d = lds0 + pstage * C::STAGE + 1024 * wave;
-    const int k = 64 * pk;
-    const uint32_t wv = k + wk < a.K ? wv0 + (uint32_t)(k + wk) : 0x80000000u;
-    const uint32_t xv = k + xk < a.K ? xv0 + (uint32_t)(k + xk) : 0x80000000u;
-#pragma unroll
-    for (int i = 0; i < C::WCOPY; ++i) {
-      constexpr int half = C::WCOPY / 2;  // gated: the first half of a wave's copies are a rows, the others gate rows
-      if (GATED && i >= half) dma_buf16_at(gr, wv + (i - half) * wstep, 0u, d + 1024 * C::NW * i);
-      else dma_buf16_at(wr, wv + i * wstep, 0u, d + 1024 * C::NW * i);
-    }
-    if constexpr (C::XCOPY == 0) {
-      if (wave < C::BM / 16) dma_buf16_at(xr, xv, 0u, d + C::BF * 64);
-    }
-#pragma unroll
-    for (int i = 0; i < C::XCOPY; ++i) dma_buf16_at(xr, xv + i * xstep, 0u, d + C::BF * 64 + 1024 * C::NW * i);
+  auto next_tile = [&]() {
+    int64_t nm0, nf0;
+    pk = 0;
+    pu += gridDim.x >> 3;
+    if (fp8_tile_at<C>(*late_args(), blockIdx.x & 7, pu, nm0, nf0)) aim(nm0, nf0);
+    else plimit = 0;
+  };
+  uint32_t pd, pwv, pxv;
+  auto copies_begin = [&]() {
+    dma_load4_at(scales + (plimit ? pk & ~3 : 0), lds0 + C::AUX + C::SLOT * pslot + 256 * wave);
+    pslot = pslot + 1 == C::RING ? 0 : pslot + 1;
+    pd = lds0 + pstage * C::STAGE + 1024 * wave;
     pstage = pstage + 1 == NS ? 0 : pstage + 1;
-    if (++pk == steps) {
-      int64_t nm0, nf0;
-      pk = 0;
-      ptile = ptile + 1 == C::AUX ? 0 : ptile + 1;
-      pu += nper;
-      pmore = fp8_tile_at<C>(a, xcd, pu, nm0, nf0);
-      if (pmore) aim(nm0, nf0);
-    }
+    const int k = kFp8Block * pk++;
+    pwv = k + wk < plimit ? wv0 + (uint32_t)k : 0x80000000u;
+    pxv = k + xk < plimit ? xv0 + (uint32_t)k : 0x80000000u;
+  };
+  auto copy = [&](int i) {
+    constexpr int half = C::WCOPY / 2;  // gated: the first half of a wave's copies are a rows, the others gate rows
+    if (i >= C::WCOPY) dma_buf16_at(xr, pxv + (i - C::WCOPY) * xstep, 0u, pd + C::BF * kFp8Block + 1024 * C::NW * (i - C::WCOPY));
+    else if (GATED && i >= half) dma_buf16_at(gr, pwv + (i - half) * wstep, 0u, pd + 1024 * C::NW * i);
+    else dma_buf16_at(wr, pwv + i * wstep, 0u, pd + 1024 * C::NW * i);
   };
 
-  // ---- operand reads
+  // ---- operand reads: half s of a block is the chunks 4 s .. 4 s + 3, lane half h takes two of them
   const int wrow0 = 32 * TO * wf;  // the wave's first output feature in the tile
   const int wrow = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
-  uint32_t wofs[2], xofs[2];
+  uint32_t wofs[2][2], xofs[2][2];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    wofs[q] = (uint32_t)((wrow0 + wrow) * 64 + 16 * ((2 * h + q) ^ w_swizzle(wrow)));
-    xofs[q] = (uint32_t)(C::BF * 64 + (32 * TM * wm + r) * 64 + 16 * ((2 * h + q) ^ x_swizzle(r)));
-  }
-
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      wofs[s][q] = (uint32_t)((wrow0 + wrow) * kFp8Block + 16 * ((4 * s + 2 * h + q) ^ w_swizzle(wrow)));
+      xofs[s][q] = (uint32_t)((C::BF + 32 * TM * wm + r) * kFp8Block + 16 * ((4 * s + 2 * h + q) ^ x_swizzle(r)));
+    }
+  auto wtile = [](int t) { return GATED ? t / TO * (C::BF / 2) + 32 * (t % TO) : 32 * t; };
   f32x16 acc[TF][TM];
-  int stage = 0, aux = 0, tile = 0;
-  aim(m0, f0);
+  Frag8 wv[2][TF], xv[TM];
+  uint32_t xw[TM], ww[2];
+  int stage = 0, slot = 0, tile = 0;  // what is read next
+  auto read_w = [&](const uint8_t* base, int s, int t) {
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (pmore) issue();
+    for (int q = 0; q < 2; ++q) wv[s][t].q[q] = *(const u32x4*)(base + wofs[s][q] + kFp8Block * wtile(t));
+  };
+  auto read_x = [&](const uint8_t* base, int s, int j) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) xv[j].q[q] = *(const u32x4*)(base + xofs[s][q] + kFp8Block * 32 * j);
+  };
+  auto read_scales = [&]() {
+    const uint8_t* p = lds + C::AUX + C::SLOT * slot;
+    slot = slot + 1 == C::RING ? 0 : slot + 1;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int row = 32 * (TM * wm + j) + r;
+      xw[j] = *(const uint32_t*)(p + 256 * (row / C::XW) + 4 * (row % C::XW));
+    }
+    const uint32_t* q = (const uint32_t*)(p + 256 * wave + 128);
+    ww[0] = q[GATED ? 0 : wrow0 / kFp8Block];
+    ww[1] = GATED ? q[1] : 0;
+  };
+
+  aim(m0, f0);
+#pragma unroll 1
+  for (int i = 0; i < NS; ++i) {
+    if (pk == nk) next_tile();
+    copies_begin();
+#pragma unroll
+    for (int c = 0; c < C::COPIES; ++c) copy(c);
+  }
+  wait_vmcnt<(NS - 1) * (C::COPIES + 1)>();
+  lds_barrier();
+#pragma unroll
+  for (int t = 0; t < TF; ++t) read_w(lds, 0, t);
+#pragma unroll
+  for (int j = 0; j < TM; ++j) read_x(lds, 0, j);
+  read_scales();
   while (true) {
-    const uint32_t* words = nullptr;
-    uint32_t xs[TM], ws[2];
-    for (int k = 0; k < steps; k += 2) {
+    // ---- the sums start from the bias
+#pragma unroll
+    for (int t = 0; t < TF; ++t) {
+      float b[16] = {};
+      const int f = wrow0 + 16 * h + (GATED ? t / TO * C::OF + 32 * (t % TO) : 32 * t);
+      LateArgs p = late_args();
+      if (p->bias) {
+        const uint8_t* at = lds + C::BIAS + 1024 * tile;
+        if (p->bias_dtype == ATMA_F32) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const f32x4 v = *(const f32x4*)(at + 4 * (f + e));
+            b[e] = v[0], b[e + 1] = v[1], b[e + 2] = v[2], b[e + 3] = v[3];
+          }
+        } else {
+          const bool bf = p->bias_dtype == ATMA_BF16;
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            const u32x4 v = *(const u32x4*)(at + 2 * (f + e));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[e + i] = bf ? elem16<bf16>(v, i) : elem16<f16>(v, i);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][j][e] = b[e];
+    }
+    tile = tile + 1 == C::RING ? 0 : tile + 1;
+
+    for (int kb = 0; kb < nk; ++kb) {
+      if (pk == nk) next_tile();
+      int xs[TM], ws[2];
+      const int sh = 8 * (kb & 3);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) xs[j] = (int)(xw[j] >> sh);
+      ws[0] = (int)(ww[0] >> sh);
+      ws[1] = (int)(ww[1] >> sh);
+      const uint8_t* base = lds + stage * C::STAGE;
+      stage = stage + 1 == NS ? 0 : stage + 1;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        // this step's copies have landed in every wave, and every wave is done with the stage before it
-        if (pmore) wait_vmcnt<(NS - 2) * (C::WCOPY + C::XCOPY)>();
-        else wait_vmcnt<0>();
-        lds_barrier();
-        if (pmore) issue();
-        if (s == 0) {
-          if (k == 0) {
-#pragma unroll
-            for (int t = 0; t < TF; ++t) {
-              float b[16] = {};
-              const int f = wrow0 + 16 * h + (GATED ? t / TO * C::OF + 32 * (t % TO) : 32 * t);
-              if (a.bias) {
-                const uint8_t* slot = lds + C::LDS_BIAS + 1024 * tile;
-                if (a.bias_dtype == ATMA_F32) {
-#pragma unroll
-                  for (int e = 0; e < 16; e += 4) {
-                    const f32x4 v = *(const f32x4*)(slot + 4 * (f + e));
-                    b[e] = v[0], b[e + 1] = v[1], b[e + 2] = v[2], b[e + 3] = v[3];
-                  }
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 16; e += 8) {
-                    const u32x4 v = *(const u32x4*)(slot + 2 * (f + e));
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                      b[e + i] = a.bias_dtype == ATMA_BF16 ? elem16<bf16>(v, i) : elem16<f16>(v, i);
-                  }
-                }
-              }
-#pragma unroll
-              for (int j = 0; j < TM; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[t][j][e] = b[e];
-            }
-            tile = tile + 1 == C::AUX ? 0 : tile + 1;
-          }
-          if ((k & 7) == 0) {
-            words = (const uint32_t*)(lds + C::LDS_AUX + aux * (C::XS + 64) * 4);
-            aux = aux + 1 == C::AUX ? 0 : aux + 1;
-          }
-          const int sh = 4 * (k & 7);  // byte (k / 2) % 4
-#pragma unroll
-          for (int j = 0; j < TM; ++j) xs[j] = words[32 * (TM * wm + j) + r] >> sh;
-          ws[0] = words[C::XS + (GATED ? 0 : wrow0 / kFp8Block)] >> sh;
-          ws[1] = GATED ? words[C::XS + 1] >> sh : 0;
+        if (s == 1) {
+          // the next block's copies have landed in every wave, and every wave has read this block
+          wait_vmcnt<(NS - 2) * (C::COPIES + 1)>();
+          lds_barrier();
+          base = lds + stage * C::STAGE;
+          copies_begin();
         }
-        const uint8_t* base = lds + stage * C::STAGE;
-        stage = stage + 1 == NS ? 0 : stage + 1;
-        Frag8 wv[TF], xv[TM];
 #pragma unroll
-        for (int t = 0; t < TF; ++t)
-#pragma unroll
-          for (int q = 0; q < 2; ++q)
-            wv[t].q[q] = *(const u32x4*)(base + wofs[q] + (GATED ? t / TO * (C::BF / 2) + 32 * (t % TO) : 32 * t) * 64);
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) xv[j].q[q] = *(const u32x4*)(base + xofs[q] + 32 * 64 * j);
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
+        for (int j = 0; j < TM; ++j) {
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int t = 0; t < TF; ++t)
             acc[t][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                wv[t].v, xv[j].v, acc[t][j], 0, 0, 0, (int)ws[GATED ? t / TO : 0], 0, (int)xs[j]);
+                wv[s][t].v, xv[j].v, acc[t][j], 0, 0, 0, ws[GATED ? t / TO : 0], 0, xs[j]);
+          // behind the products of token tile j: its operand of the next half, a share of the weights and copies
+          read_x(base, s ^ 1, j);
+#pragma unroll
+          for (int t = j * TF / TM; t < (j + 1) * TF / TM; ++t) read_w(base, s ^ 1, t);
+          if (s == 1) {
+#pragma unroll
+            for (int c = j * C::COPIES / TM; c < (j + 1) * C::COPIES / TM; ++c) copy(c);
+            if (j == TM - 1) read_scales();
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 
     // ---- epilogue of tile (m0, f0): token 32 (TM wm + j) + r, 16 consecutive features a tile
+    LateArgs p = late_args();
     if constexpr (!GATED) {
-      const bool whole = f0 + C::OF <= a.N && a.ldy % 8 == 0;
+      const bool whole = f0 + C::OF <= p->N && p->ldy % 8 == 0;
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         const int64_t m = m0 + 32 * (TM * wm + j) + r;
-        if (m < a.M) {
+        if (m < p->M) {
 #pragma unroll
           for (int t = 0; t < TF; ++t) {
             const int64_t n0 = f0 + wrow0 + 32 * t + 16 * h;
-            T* y = (T*)a.y + m * a.ldy + n0;
+            T* y = (T*)p->y + m * p->ldy + n0;
             const f32x16& v = acc[t][j];
             if (whole) {
 #pragma unroll
@@ -305,14 +353,14 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
             } else {
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                if (n0 + e < a.N) y[e] = from_f32<T>(v[e]);
+                if (n0 + e < p->N) y[e] = from_f32<T>(v[e]);
             }
           }
         }
       }
     } else {
-      // the activations in place of a's accumulators, their largest magnitude over the wave's features, then the tile's
-      float* part = (float*)(lds + C::LDS_TOP);
+      // the activations in place of a's sums, their largest magnitude over the wave's features, then over the tile's
+      float* part = (float*)(lds + C::TOP);
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         float top = 0.f;
@@ -320,7 +368,12 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
         for (int e = 0; e < 16; ++e) {
           const float v = gate_act(acc[0][j][e], acc[1][j][e]);
           acc[0][j][e] = v;
-          top = fmaxf(top, finite_abs(v));
+          top = fmaxf(top, fabsf(v));
+        }
+        if (top == __builtin_inff()) {  // (NaN does not enter the maximum; infinities must not)
+          top = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, finite_abs(acc[0][j][e]));
         }
         top = fmaxf(top, wave_xor(top, 32));
         if (h == 0) part[wf * C::BM + 32 * (TM * wm + j) + r] = top;
@@ -333,22 +386,23 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
         for (int q = 1; q < WF; ++q) top = fmaxf(top, part[q * C::BM + row]);
         const int code = fp8_scale_code(top);
-        const float inv = fp8_inv_scale(code);
+        const float scale = fp8_scale(code);
         const int64_t m = m0 + row;
-        if (m < a.M) {
-          if (wf == 0 && h == 0) a.ys[m * a.ldys + f0 / kFp8Block] = (uint8_t)code;
+        if (m < p->M) {
+          if (wf == 0 && h == 0) p->ys[m * p->ldys + f0 / kFp8Block] = (uint8_t)code;
           const f32x16& v = acc[0][j];
           u32x4 o;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            o[q] = fp8_pack4(v[4 * q] * inv, v[4 * q + 1] * inv, v[4 * q + 2] * inv, v[4 * q + 3] * inv);
-          *(u32x4*)((uint8_t*)a.y + m * a.ldy + f0 + wrow0 + 16 * h) = o;
+            o[q] = fp8_scaled4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], scale);
+          *(u32x4*)((uint8_t*)p->y + m * p->ldy + f0 + wrow0 + 16 * h) = o;
         }
       }
     }
-    u += nper;
-    if (!fp8_tile_at<C>(a, xcd, u, m0, f0)) break;
+    u += gridDim.x >> 3;
+    if (!fp8_tile_at<C>(*late_args(), blockIdx.x & 7, u, m0, f0)) break;
   }
+  wait_vmcnt<0>();  // no copy outlives its workgroup's LDS
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -412,90 +466,6 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   }
 }
 
-// The gated form: a workgroup of 16 waves owns one block of 128 output features; wave w takes their tile w % 8 (its a and
-// gate rows) and the blocks of K of parity w / 8.
-template <int MT>
-__global__ void __launch_bounds__(1024) fp8_few_gated_kernel(Fp8Args a) {
-  __shared__ f32x4 red[8][2][MT][64];
-  __shared__ float top[8][16 * MT];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int tile = wave & 7, part = wave >> 3;
-  const int r = lane & 15, g = lane >> 4;
-  const int64_t f0 = (int64_t)blockIdx.x * kFp8Block;
-  const uint8_t* wp[2];
-  const uint8_t* wsp[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    wp[t] = a.w + (t * a.N + f0 + 16 * tile + r) * a.ldw;
-    wsp[t] = a.ws + (t * a.N + f0) / kFp8Block * a.ldws;
-  }
-  const uint8_t* xp[MT];
-  const uint8_t* xsp[MT];
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int64_t m = min((int64_t)(16 * j + r), a.M - 1);
-    xp[j] = a.x + m * a.ldx;
-    xsp[j] = a.xs + m * a.ldxs;
-  }
-  f32x4 acc[2][MT] = {};
-  for (int kb = part; kb < a.nk; kb += 2) {
-    Frag8 wv[2], xv[MT];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = kb * kFp8Block + 32 * g + 16 * h;
-      const bool in = k < a.K;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) wv[t].q[h] = in ? *(const u32x4*)(wp[t] + k) : u32x4{};
-#pragma unroll
-      for (int j = 0; j < MT; ++j) xv[j].q[h] = in ? *(const u32x4*)(xp[j] + k) : u32x4{};
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) acc[t][j] = mfma_fp8(wv[t], xv[j], acc[t][j], wsp[t][kb], xsp[j][kb]);
-  }
-  if (part == 1) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int j = 0; j < MT; ++j) red[tile][t][j][lane] = acc[t][j];
-  }
-  __syncthreads();
-  const int64_t n0 = f0 + 16 * tile + 4 * g;
-  if (part == 0) {
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const f32x4 sa = acc[0][j] + red[tile][0][j][lane], sg = acc[1][j] + red[tile][1][j][lane];
-      float m = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float h = gate_act(sa[e] + bias_at(a, n0 + e), sg[e] + bias_at(a, a.N + n0 + e));
-        acc[0][j][e] = h;
-        m = fmaxf(m, finite_abs(h));
-      }
-      m = fmaxf(m, wave_xor(m, 16));
-      m = fmaxf(m, wave_xor(m, 32));
-      if (g == 0) top[tile][16 * j + r] = m;
-    }
-  }
-  __syncthreads();
-  if (part == 0) {
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int64_t m = 16 * j + r;
-      if (m >= a.M) continue;
-      float t = 0.f;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) t = fmaxf(t, top[q][16 * j + r]);
-      const int code = fp8_scale_code(t);
-      const float inv = fp8_inv_scale(code);
-      const f32x4& h = acc[0][j];
-      *(uint32_t*)((uint8_t*)a.y + m * a.ldy + n0) = fp8_pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-      if (tile == 0 && g == 0) a.ys[m * a.ldys + f0 / kFp8Block] = (uint8_t)code;
-    }
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ host
 template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
 static void launch_tiles(Fp8Args a, hipStream_t s) {
@@ -533,16 +503,17 @@ static int check_fp8(const char* what, const Fp8Args& a, int64_t rows) {
 
 template <typename T>
 static void launch_linear(const Fp8Args& a, hipStream_t s) {
+  const int64_t cus = device_cu_count();
   if (a.M <= 16) {
     fp8_few_kernel<T, 1, 1, 8><<<dim3((unsigned)((a.N + 15) / 16)), 512, 0, s>>>(a);
   } else if (a.M <= 32) {
     fp8_few_kernel<T, 2, 1, 8><<<dim3((unsigned)((a.N + 15) / 16)), 512, 0, s>>>(a);
-  } else if (((a.M + 127) / 128) * ((a.N + 255) / 256) >= 2 * device_cu_count()) {
-    launch_tiles<T, 2, 4, 4, 1, 3, false>(a, s);
-  } else if (((a.M + 127) / 128) * ((a.N + 127) / 128) >= device_cu_count()) {
-    launch_tiles<T, 2, 2, 2, 2, 4, false>(a, s);
+  } else if (((a.M + 255) / 256) * ((a.N + 255) / 256) >= cus) {
+    launch_tiles<T, 2, 4, 4, 2, 2, false>(a, s);
+  } else if (((a.M + 127) / 128) * ((a.N + 127) / 128) >= cus / 2) {
+    launch_tiles<T, 2, 2, 2, 2, 2, false>(a, s);
   } else {
-    launch_tiles<T, 1, 1, 2, 2, 8, false>(a, s);
+    launch_tiles<T, 1, 1, 2, 2, 4, false>(a, s);
   }
 }
 
@@ -582,10 +553,7 @@ extern "C" int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs,
   if (!ys || (uintptr_t)y % 16 || ldy % 16 || ldy < H || ldys < H / kFp8Block)
     return set_error(ATMA_ERR_INVALID, "linear_gated_fp8: rows of y must be 16-byte aligned and at least H long");
   hipStream_t s = (hipStream_t)stream;
-  if (M <= 16) fp8_few_gated_kernel<1><<<dim3((unsigned)(H / kFp8Block)), 1024, 0, s>>>(a);
-  else if (M <= 32) fp8_few_gated_kernel<2><<<dim3((unsigned)(H / kFp8Block)), 1024, 0, s>>>(a);
-  else if (((M + 127) / 128) * (H / kFp8Block) >= 2 * device_cu_count()) launch_tiles<bf16, 2, 4, 4, 1, 3, true>(a, s);
-  else if (((M + 63) / 64) * (H / kFp8Block) >= device_cu_count()) launch_tiles<bf16, 2, 2, 4, 1, 3, true>(a, s);
-  else launch_tiles<bf16, 2, 1, 4, 1, 4, true>(a, s);
+  if (((M + 255) / 256) * (H / kFp8Block) >= device_cu_count()) launch_tiles<bf16, 2, 4, 4, 2, 2, true>(a, s);
+  else launch_tiles<bf16, 2, 2, 4, 1, 3, true>(a, s);
   return check_launch("linear_gated_fp8");
 }

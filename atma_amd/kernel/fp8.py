@@ -23,29 +23,48 @@ _DT32 = (torch.bfloat16, torch.float16, torch.float32)
 FP8, FP8_SCALE, FP8_BLOCK = _ops.FP8, _ops.FP8_SCALE, _ops.FP8_BLOCK
 
 
-def _check(what, *ts):
-    """Every tensor of a call on one GPU, none of them waiting for a gradient."""
-    ts = [t for t in ts if t is not None]
-    if any(not t.is_cuda for t in ts):
-        raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
-    if any(t.device != ts[0].device for t in ts):
-        raise ValueError(f"{what}: every tensor must be on {ts[0].device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), or detach its inputs")
+def _placed(what, *ts):
+    """Every tensor of a call on one GPU, none of them waiting for a gradient.  Returns whether the call may go straight to
+    its launch: that GPU is the current one and nothing watches, transforms or overrides the call."""
+    device, grad, plain = ts[0].get_device(), torch.is_grad_enabled(), True
+    for t in ts:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
+        if at != device:
+            raise ValueError(f"{what}: every tensor must be on one GPU")
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), or detach its inputs")
+        if type(t) not in _ops._PLAIN:
+            plain = False
+    return (plain and device == torch.cuda.current_device() and not _ops.watched()
+            and not torch._C._len_torch_function_stack())
+
+
+def _dtypes(dtypes):
+    return ", ".join(str(d)[6:] for d in dtypes)
 
 
 def _matrix(what, name, t, dtypes):
     if t.dim() != 2 or t.dtype not in dtypes:
-        raise ValueError(f"{what}: {name} must be a matrix of {', '.join(str(d)[6:] for d in dtypes)} "
-                         f"(got {tuple(t.shape)} {t.dtype})")
+        raise ValueError(f"{what}: {name} must be a matrix of {_dtypes(dtypes)} (got {tuple(t.shape)} {t.dtype})")
     if t.shape[1] < 16 or t.shape[1] % 16:
         raise ValueError(f"{what}: rows of {name} must be a multiple of 16 long (got {t.shape[1]})")
+
+
+def _aligned_rows(t):
+    """Rows at multiples of 16 bytes that do not overlap."""
+    row, one = t.stride()
+    return one == 1 and not (t.data_ptr() | row * t.element_size()) & 15 and row >= t.shape[1]
 
 
 def quantize_fp8(x):
     """Rows to 8 bits: x (M, K) in fp32 or 16 bits, K a multiple of 16 -> (data (M, K), scale (M, ceil(K / 128)))."""
     _matrix("quantize_fp8", "x", x, _DT32)
-    _check("quantize_fp8", x)
+    if _placed("quantize_fp8", x) and _aligned_rows(x):
+        return _ops.fp8_quantize("atma_quantize_fp8", x, x.shape[0])
     return tuple(_ops.run.quantize_fp8(x))
 
 
@@ -53,7 +72,8 @@ def quantize_weight_fp8(weight):
     """A weight matrix to 8 bits: (N, K) in fp32 or 16 bits, K a multiple of 16 -> (data (N, K), scale (ceil(N / 128),
     ceil(K / 128))).  ``linear_gated_fp8`` takes the a and gate rows as one (2H, K) matrix, H a multiple of 128."""
     _matrix("quantize_weight_fp8", "weight", weight, _DT32)
-    _check("quantize_weight_fp8", weight)
+    if _placed("quantize_weight_fp8", weight) and _aligned_rows(weight):
+        return _ops.fp8_quantize("atma_quantize_weight_fp8", weight, (weight.shape[0] + 127) // 128)
     return tuple(_ops.run.quantize_weight_fp8(weight))
 
 
@@ -62,45 +82,56 @@ def residual_rms_norm_fp8(branch, residual, weight, eps):
     ``rms_norm(s) * weight`` quantized from its fp32 values.  ``branch``: (M, D) or ``PartialSums``; ``residual`` None starts
     the stream with the branch; D a multiple of 16, at most 4,096.  Returns (data, scale, s)."""
     what = "residual_rms_norm_fp8"
-    ps = branch if isinstance(branch, PartialSums) else None
-    y, parts = (branch, None) if ps is None else (ps.base, ps.parts)
-    src = y if parts is None else parts
-    dtype = branch.dtype
+    if isinstance(branch, PartialSums):
+        y, parts, biases, mu_x, mu_w = branch.base, branch.parts, list(branch.biases), branch.mu_x, branch.mu_w
+    else:
+        y, parts, biases, mu_x, mu_w = branch, None, [], None, None
+    src, dtype = (y if parts is None else parts), branch.dtype
     if src.dim() != (2 if parts is None else 3):
         raise ValueError(f"{what}: the branch must be (M, D), partial sums (P, M, D)")
-    M, D = src.shape[-2:]
+    M, D = shape = src.shape[-2:]
     if dtype not in _DT or D % 16 or not 16 <= D <= 4096 or weight.shape != (D,) or weight.dtype != dtype:
         raise ValueError(f"{what}: unsupported rows of {D} {dtype}, weight {tuple(weight.shape)} {weight.dtype}")
     if src.dtype != (dtype if parts is None else torch.float32) or (parts is not None and not 1 <= parts.shape[0] <= 8):
         raise ValueError(f"{what}: a branch in the stream's type or up to 8 fp32 partial sums")
-    if residual is not None and (residual.shape != (M, D) or residual.dtype != dtype):
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype):
         raise ValueError(f"{what}: residual must match the branch")
-    biases = [] if ps is None else list(ps.biases)
-    mu_x, mu_w = (None, None) if ps is None else (ps.mu_x, ps.mu_w)
     if len(biases) > 3 or any(b.shape != (D,) or b.dtype != dtype for b in biases):
         raise ValueError(f"{what}: up to three biases ({D},) in the stream's type")
     if mu_x is not None and (mu_x.dim() != 2 or mu_x.shape[1] not in (4, 8, 16) or mu_x.shape[0] != M
                              or mu_w.shape != (D, mu_x.shape[1]) or mu_x.dtype != dtype or mu_w.dtype != dtype):
         raise ValueError(f"{what}: the low-rank term takes mu_x (M, k) and mu_w (D, k), k 4, 8 or 16")
-    _check(what, src, residual, weight, mu_x, mu_w, *biases)
-    keep = residual is not None or ps is not None
-    out = _ops.run.residual_rms_norm_fp8(y, parts, biases, mu_x, mu_w, residual, weight, float(eps), keep)
+    keep = residual is not None or src is not branch
+    straight = _placed(what, src, residual, weight, mu_x, mu_w, *biases)
+    if straight and mu_x is None and not weight.data_ptr() & 15 and weight.is_contiguous()             and (_aligned_rows(y) if parts is None else parts.is_contiguous() and not parts.data_ptr() & 15)             and (residual is None or _aligned_rows(residual))             and all(b.stride(0) == 1 and not b.data_ptr() & 15 for b in biases):
+        out = _ops.fp8_norm(y, parts, biases, None, None, residual, weight, float(eps), keep)
+    else:
+        out = _ops.run.residual_rms_norm_fp8(y, parts, biases, mu_x, mu_w, residual, weight, float(eps), keep)
     return out[0], out[1], (out[2] if keep else branch)
 
 
-def _operands(what, x, x_scale, weight, weight_scale, bias, dtypes):
+def _operands(what, x, x_scale, weight, weight_scale, bias):
+    """Checks a product's operands; returns whether it may go straight to its launch (``_placed``, and nothing to copy)."""
     _matrix(what, "x", x, (FP8,))
     _matrix(what, "weight", weight, (FP8,))
-    N, K = weight.shape
-    nb = _ops._fp8_blocks(K)
-    if x.shape[1] != K or N < 1:
+    (M, K), (N, Kw) = x.shape, weight.shape
+    nb = (K + 127) // 128
+    if K != Kw or N < 1:
         raise ValueError(f"{what}: x (M, K) and weight (N, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
-    for name, t, rows in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, _ops._fp8_blocks(N))):
-        if t.dtype != FP8_SCALE or t.shape != (rows, nb):
-            raise ValueError(f"{what}: {name} must be ({rows}, {nb}) float8_e8m0fnu (got {tuple(t.shape)} {t.dtype})")
-    if bias is not None and (bias.shape != (N,) or bias.dtype not in dtypes):
-        raise ValueError(f"{what}: bias must be ({N},) of {', '.join(str(d)[6:] for d in dtypes)}")
-    _check(what, x, x_scale, weight, weight_scale, bias)
+    if x_scale.dtype != FP8_SCALE or x_scale.shape != (M, nb):
+        raise ValueError(f"{what}: x_scale must be ({M}, {nb}) float8_e8m0fnu (got {tuple(x_scale.shape)} {x_scale.dtype})")
+    if weight_scale.dtype != FP8_SCALE or weight_scale.shape != ((N + 127) // 128, nb):
+        raise ValueError(f"{what}: weight_scale must be ({(N + 127) // 128}, {nb}) float8_e8m0fnu "
+                         f"(got {tuple(weight_scale.shape)} {weight_scale.dtype})")
+    if bias is not None and (bias.shape != (N,) or bias.dtype not in _DT32):
+        raise ValueError(f"{what}: bias must be ({N},) of {_dtypes(_DT32)}")
+    if not _placed(what, x, x_scale, weight, weight_scale, bias):
+        return False
+    (ldx, ix), (ldw, iw), (lxs, ixs), (lws, iws) = x.stride(), weight.stride(), x_scale.stride(), weight_scale.stride()
+    return (ix == iw == ixs == iws == 1 and ldx >= K and ldw >= K and lxs >= nb and lws >= nb
+            and not (x.data_ptr() | weight.data_ptr() | ldx | ldw) & 15
+            and not (x_scale.data_ptr() | weight_scale.data_ptr() | lxs | lws) & 3
+            and (bias is None or (bias.stride(0) == 1 and not bias.data_ptr() & 3)))
 
 
 def linear_fp8(x, x_scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
@@ -111,7 +142,8 @@ def linear_fp8(x, x_scale, weight, weight_scale, bias=None, out_dtype=torch.bflo
     ``quantize_fp8`` lays them, are read in place; others are copied."""
     if out_dtype not in _DT:
         raise ValueError(f"linear_fp8: out_dtype must be bfloat16 or float16 (got {out_dtype})")
-    _operands("linear_fp8", x, x_scale, weight, weight_scale, bias, _DT32)
+    if _operands("linear_fp8", x, x_scale, weight, weight_scale, bias):
+        return _ops.fp8_linear(x, x_scale, weight, weight_scale, bias, out_dtype)
     return _ops.run.linear_fp8(x, x_scale, weight, weight_scale, bias, out_dtype)
 
 
@@ -119,7 +151,8 @@ def linear_gated_fp8(x, x_scale, weight, weight_scale, bias=None):
     """The MLP's first projection with its activation, 8 bits in and out: ``a, gate = linear(x, weight, bias).chunk(2, -1)``
     as fp32 sums, ``gate * relu(a)^2`` quantized once.  Operands as ``linear_fp8``, weight (2H, K) with H a multiple of 128.
     Returns (data (M, H), scale (M, H / 128))."""
-    if weight.dim() == 2 and (weight.shape[0] < 256 or weight.shape[0] % 256):
+    if weight.dim() == 2 and weight.shape[0] % 256:
         raise ValueError(f"linear_gated_fp8: weight (2H, K) with H a multiple of 128 (got {tuple(weight.shape)})")
-    _operands("linear_gated_fp8", x, x_scale, weight, weight_scale, bias, _DT32)
+    if _operands("linear_gated_fp8", x, x_scale, weight, weight_scale, bias):
+        return _ops.fp8_linear_gated(x, x_scale, weight, weight_scale, bias)
     return tuple(_ops.run.linear_gated_fp8(x, x_scale, weight, weight_scale, bias))
