@@ -9,13 +9,13 @@
 // of the result for normally distributed values: far below the rounding to a 16-bit output, and the reason why there is
 // no fp32 output.  The order of k inside a block is free (one scale covers it), so a lane takes whichever 16-byte pieces
 // load best, the same ones of x and w.
+#include <math.h>
+
 #include <algorithm>
-#include <type_traits>
 
 #include "fp8.h"
 
 namespace atma {
-
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -407,8 +407,8 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 
 // ------------------------------------------------------------------------------------------------ few rows
 // At most 16 MT tokens: a stream of the weights.  A workgroup of NW waves owns FT tiles of 16 weight rows and its waves
-// take the blocks of K in turn; operands come straight from memory in the MFMA's layout (32 bytes of a row a lane) and the
-// waves' sums are joined through LDS in a fixed order.
+// take the blocks of K in turn, two under way at a time; operands come straight from memory in the MFMA's layout (the four
+// lanes of a row take 64 consecutive bytes a load) and the waves' sums are joined through LDS in a fixed order.
 template <typename T, int MT, int FT, int NW>
 __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   __shared__ f32x4 red[NW][FT][MT][64];
@@ -419,50 +419,71 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   const uint8_t* xp[MT];
   const uint8_t* xsp[MT];
 #pragma unroll
-  for (int t = 0; t < FT; ++t) wp[t] = a.w + min(f0 + 16 * t + r, a.N - 1) * a.ldw;
+  for (int t = 0; t < FT; ++t) wp[t] = a.w + min(f0 + 16 * t + r, a.N - 1) * a.ldw + 16 * g;
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int64_t m = min((int64_t)(16 * j + r), a.M - 1);
-    xp[j] = a.x + m * a.ldx;
+    xp[j] = a.x + m * a.ldx + 16 * g;
     xsp[j] = a.xs + m * a.ldxs;
   }
   const uint8_t* wsp = a.ws + f0 / kFp8Block * a.ldws;
   f32x4 acc[FT][MT] = {};
-  for (int kb = wave; kb < a.nk; kb += NW) {
-    Frag8 wv[FT], xv[MT];
-    int xsc[MT];
+  for (int kb = wave; kb < a.nk; kb += 2 * NW) {
+    Frag8 wv[2][FT], xv[2][MT];
+    int xsc[2][MT], wsc[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = kb * kFp8Block + 32 * g + 16 * h;
-      const bool in = k < a.K;
+    for (int b = 0; b < 2; ++b) {
+      const int kk = kb + b * NW;
+      const int k = kk * kFp8Block;
 #pragma unroll
-      for (int t = 0; t < FT; ++t) wv[t].q[h] = in ? *(const u32x4*)(wp[t] + k) : u32x4{};
+      for (int q = 0; q < 2; ++q) {
+        const bool in = k + 64 * q + 16 * g < a.K;  // (K < 2^23: no overflow in the block behind the last)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) xv[j].q[h] = in ? *(const u32x4*)(xp[j] + k) : u32x4{};
+        for (int t = 0; t < FT; ++t) wv[b][t].q[q] = in ? *(const u32x4*)(wp[t] + k + 64 * q) : u32x4{};
+#pragma unroll
+        for (int j = 0; j < MT; ++j) xv[b][j].q[q] = in ? *(const u32x4*)(xp[j] + k + 64 * q) : u32x4{};
+      }
+      const int ks = min(kk, a.nk - 1);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) xsc[b][j] = xsp[j][ks];
+      wsc[b] = wsp[ks];
     }
 #pragma unroll
-    for (int j = 0; j < MT; ++j) xsc[j] = xsp[j][kb];
-    const int wsc = wsp[kb];
+    for (int b = 0; b < 2; ++b) {
+      if (kb + b * NW < a.nk) {
 #pragma unroll
-    for (int t = 0; t < FT; ++t)
+        for (int t = 0; t < FT; ++t)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[t][j] = mfma_fp8(wv[t], xv[j], acc[t][j], wsc, xsc[j]);
+          for (int j = 0; j < MT; ++j) acc[t][j] = mfma_fp8(wv[b][t], xv[b][j], acc[t][j], wsc[b], xsc[b][j]);
+      }
+    }
   }
 #pragma unroll
   for (int t = 0; t < FT; ++t)
 #pragma unroll
     for (int j = 0; j < MT; ++j) red[wave][t][j][lane] = acc[t][j];
   __syncthreads();
-  for (int i = wave; i < FT * MT; i += NW) {
+#pragma unroll
+  for (int i0 = 0; i0 < FT * MT; i0 += NW) {
+    const int i = i0 + wave;
+    if (i >= FT * MT) break;
     const int t = i / MT, j = i % MT;
     f32x4 s = red[0][t][j][lane];
+#pragma unroll
     for (int q = 1; q < NW; ++q) s += red[q][t][j][lane];
     const int64_t n0 = f0 + 16 * t + 4 * g, m = 16 * j + r;
     if (m >= a.M) continue;
     T* y = (T*)a.y + m * a.ldy + n0;
+    float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n0 + e < a.N) y[e] = from_f32<T>(s[e] + bias_at(a, n0 + e));
+    for (int e = 0; e < 4; ++e) v[e] = s[e] + (n0 + e < a.N ? bias_at(a, n0 + e) : 0.f);
+    if (n0 + 4 <= a.N && a.ldy % 8 == 0) {
+      *(u32x2*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n0 + e < a.N) y[e] = from_f32<T>(v[e]);
+    }
   }
 }
 
@@ -501,19 +522,68 @@ static int check_fp8(const char* what, const Fp8Args& a, int64_t rows) {
   return ATMA_OK;
 }
 
+// What a tile shape costs: us a tile to begin and end it, and us a block of K, where few CUs work (latency) and where all do.
+// Fitted to 30 shapes of 64 to 4,096 rows, 300 to 8,192 features and K 512 to 4,096, which it orders as measured but for
+// differences under 10% (us: 1,000 x 1,024 -> 4,096 17.1 / 10.1 / 12.6 / 13.0 for 256 x 256, 128 x 128, 64 x 128 and 64 x 64,
+// 4,000 x 512 -> 8,192 30 / 33 / 52 / 54, 64 x 4,096 -> 1,024 37 / 17.5 / 14.5 / 12.5; gated 777 x 1,024 -> 4,096 17.7 / 11.6 /
+// 15.6 for 256, 128 and 64 tokens, 5,000 x 4,096 -> 1,024 47 / 60 / 59, 64 x 1,024 -> 4,096 15.0 / 9.6 / 8.2).
+struct TileCost {
+  int features, tokens;
+  float tile, few, all;
+};
+
+static int cheapest(const Fp8Args& a, const TileCost* c, int n) {
+  const float cus = (float)device_cu_count();
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const int64_t tiles = ((a.M + c[i].tokens - 1) / c[i].tokens) * ((a.N + c[i].features - 1) / c[i].features);
+    const float fill = (float)tiles / cus;
+    float t;
+    if (fill <= 1.f) t = c[i].tile + (float)a.nk * (c[i].few + (c[i].all - c[i].few) * fill);
+    else t = ceilf(fill) * (c[i].tile + (float)a.nk * c[i].all);
+    if (i == 0 || t < least) best = i, least = t;
+  }
+  return best;
+}
+
+template <typename T, int MT, int FT, int NW>
+static void launch_few(const Fp8Args& a, hipStream_t s) {
+  fp8_few_kernel<T, MT, FT, NW><<<dim3((unsigned)((a.N + 16 * FT - 1) / (16 * FT))), dim3(64 * NW), 0, s>>>(a);
+}
+
 template <typename T>
 static void launch_linear(const Fp8Args& a, hipStream_t s) {
   const int64_t cus = device_cu_count();
-  if (a.M <= 16) {
-    fp8_few_kernel<T, 1, 1, 8><<<dim3((unsigned)((a.N + 15) / 16)), 512, 0, s>>>(a);
-  } else if (a.M <= 32) {
-    fp8_few_kernel<T, 2, 1, 8><<<dim3((unsigned)((a.N + 15) / 16)), 512, 0, s>>>(a);
-  } else if (((a.M + 255) / 256) * ((a.N + 255) / 256) >= cus) {
-    launch_tiles<T, 2, 4, 4, 2, 2, false>(a, s);
-  } else if (((a.M + 127) / 128) * ((a.N + 127) / 128) >= cus / 2) {
-    launch_tiles<T, 2, 2, 2, 2, 2, false>(a, s);
-  } else {
-    launch_tiles<T, 1, 1, 2, 2, 4, false>(a, s);
+  if (a.M <= 32 && a.N < 48 * cus) {
+    // two tiles of features share each activation load where that leaves work for every CU
+    const bool two = a.N >= 24 * cus;
+    if (a.M <= 16 && two) launch_few<T, 1, 2, 8>(a, s);
+    else if (a.M <= 16) launch_few<T, 1, 1, 8>(a, s);
+    else if (two) launch_few<T, 2, 2, 8>(a, s);
+    else launch_few<T, 2, 1, 8>(a, s);
+    return;
+  }
+  static constexpr TileCost kTiles[4] = {{256, 256, 5.5f, 1.15f, 1.72f},
+                                         {128, 128, 1.2f, 0.50f, 0.72f},
+                                         {64, 128, 1.3f, 0.36f, 0.42f},
+                                         {64, 64, 0.7f, 0.32f, 0.30f}};
+  switch (cheapest(a, kTiles, 4)) {
+    case 0: launch_tiles<T, 2, 4, 4, 2, 2, false>(a, s); break;
+    case 1: launch_tiles<T, 2, 2, 2, 2, 2, false>(a, s); break;
+    case 2: launch_tiles<T, 1, 2, 2, 2, 3, false>(a, s); break;
+    default: launch_tiles<T, 1, 1, 2, 2, 4, false>(a, s); break;
+  }
+}
+
+static void launch_gated(const Fp8Args& a, hipStream_t s) {
+  static constexpr TileCost kTiles[3] = {{128, 256, 5.0f, 1.00f, 1.60f},
+                                         {128, 128, 1.7f, 0.70f, 0.98f},
+                                         {128, 64, 1.3f, 0.53f, 0.63f}};
+  switch (cheapest(a, kTiles, 3)) {
+    case 0: launch_tiles<bf16, 2, 4, 4, 2, 2, true>(a, s); break;
+    case 1: launch_tiles<bf16, 2, 2, 4, 2, 2, true>(a, s); break;
+    default: launch_tiles<bf16, 2, 1, 4, 2, 3, true>(a, s); break;
   }
 }
 
@@ -552,8 +622,6 @@ extern "C" int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs,
   if (M == 0) return ATMA_OK;
   if (!ys || (uintptr_t)y % 16 || ldy % 16 || ldy < H || ldys < H / kFp8Block)
     return set_error(ATMA_ERR_INVALID, "linear_gated_fp8: rows of y must be 16-byte aligned and at least H long");
-  hipStream_t s = (hipStream_t)stream;
-  if (((M + 255) / 256) * (H / kFp8Block) >= device_cu_count()) launch_tiles<bf16, 2, 4, 4, 2, 2, true>(a, s);
-  else launch_tiles<bf16, 2, 2, 4, 1, 3, true>(a, s);
+  launch_gated(a, (hipStream_t)stream);
   return check_launch("linear_gated_fp8");
 }

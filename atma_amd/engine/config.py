@@ -51,6 +51,7 @@ class Config:
     max_num_batched_tokens: int = 16384 * 8
     max_model_len: int = 4096
     enforce_eager: bool = False
+    fp8_mlp: bool = False                   # serve the MLPs in 8 bits (e4m3, block scales); 16-bit models only
     strict_weights: bool = False
     eos: int = 50256
     num_kvcache_blocks: int = -1            # -1: enough for max_num_seqs x max_model_len, within memory

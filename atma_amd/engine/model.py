@@ -24,8 +24,10 @@ from ..kernel import causal_conv1d_decode_step, packed_causal_conv1d, softcap_ar
 from ..kernel.decode_fusions import (PartialSums, lfm2_conv_step, linear_tokens_conv, linear_tokens_conv_supported,
                                      residual_rms_norm_supported)
 from ..kernel.layer_fusions import lfm2_conv_packed
+from ..kernel.train_glue import plain_module
 from ..layers.attention import Attention
-from ..layers.global_attention import MLP, GlobalLayerCache, Linear, PolarAttention, RMSNorm, decode_rows
+from ..layers.global_attention import (MLP, Fp8MLP, GlobalLayerCache, Linear, PolarAttention, RMSNorm,
+                                       decode_rows)
 from .config import AtmaConfig
 from .context import get_context
 
@@ -165,8 +167,11 @@ class AtmaDecoderBlock(nn.Module):
         and the stream before it go in, each add is fused with the norm after it
         (``RMSNorm.add_norm``), and this block's MLP output comes out unadded -- the
         additions are the eager block's, in the same dtype, so the stream's values are
-        unchanged.  Returns (mlp branch, stream)."""
+        unchanged.  Returns (mlp branch, stream).  An MLP in 8 bits takes its rows quantized by the norm before it."""
         h, residual = self.norm1.add_norm(branch, residual)
+        if plain_module(self.mlp, Fp8MLP) and plain_module(self.norm2, RMSNorm):
+            data, scale, residual = self.norm2.add_norm_fp8(self.attn(h, defer=True), residual)
+            return self.mlp.forward_fp8(data, scale, residual.dtype), residual
         h, residual = self.norm2.add_norm(self.attn(h, defer=True), residual)
         return self.mlp(h, defer=True), residual
 
@@ -212,6 +217,13 @@ class Atma(nn.Module):
         if logits.dtype in (torch.bfloat16, torch.float16):
             return softcap_argmax(logits, ids_out)
         return softcap_logits(logits), None
+
+    def quantize_mlps(self):
+        """Replace every block's MLP by its 8-bit form (``Fp8MLP``), for inference; the weights must be on the GPU."""
+        for block in self.blocks:
+            if not isinstance(block.mlp, Fp8MLP):
+                block.mlp = Fp8MLP(block.mlp)
+        return self
 
     def init_weights(self, std=0.02, seed=0):
         """Every parameter N(0, std) from ``seed`` (the random-init convention of the

@@ -54,7 +54,11 @@ class ModelRunner:
                 load_model(model, config.model, strict=config.strict_weights)
             else:
                 model.init_weights(config.init_std, config.seed)
+        if config.fp8_mlp and hf.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"Config.fp8_mlp serves 16-bit models (got {hf.dtype})")
         self.model = model.to(self.device, hf.dtype).eval()
+        if config.fp8_mlp:
+            self.model.quantize_mlps()
         self.sampler = Sampler()
         self.last_logits = None
         self.allocate_conv_state_tables()

@@ -50,6 +50,8 @@ from ..kernel.decode_fusions import (PartialSums, chunk_width, global_decode_gat
                                      linear_tokens_chunks, linear_tokens_gated, linear_tokens_multi,
                                      linear_tokens_multi_supported,
                                      residual_rms_norm, residual_rms_norm_supported)
+from ..kernel.fp8 import (FP8, FP8_SCALE, linear_fp8, linear_gated_fp8, quantize_fp8, quantize_weight_fp8,
+                          residual_rms_norm_fp8)
 from ..kernel.gated_delta import gated_delta_prefill, gated_delta_prefill_supported
 from ..kernel.inference_ops import (linear_tokens, linear_tokens_supported, packed_causal_conv1d,
                                      squared_relu_gate)
@@ -709,6 +711,11 @@ class RMSNorm(nn.Module):
         s = branch if residual is None else residual + branch
         return self(s), s
 
+    def add_norm_fp8(self, branch, residual):
+        """``add_norm`` with the norm in 8 bits, in one launch (``residual_rms_norm_fp8``): returns (data, scale, s).
+        16-bit GPU rows outside autograd, a multiple of 16 and at most 4,096 wide."""
+        return residual_rms_norm_fp8(branch, residual, self.weight.detach().to(branch.dtype), self.eps)
+
 
 class MLP(nn.Module):
     """Squared-ReLU gated MLP (``model/layers.py:19-31``)."""
@@ -750,6 +757,35 @@ class MLP(nn.Module):
             h = squared_relu_gate(a.reshape(-1, a.shape[-1]), gate.reshape(-1, gate.shape[-1]))
             return self.proj(h.view(*lead, -1))
         return self.proj(gate * a.relu().square())
+
+
+class Fp8MLP(nn.Module):
+    """``MLP`` for inference with its weights and the activations it multiplies in 8 bits (``kernel/fp8``): two block-scaled
+    products, the activation formed and quantized in the first one's epilogue.  Made from an ``MLP`` on the GPU; the weights
+    are held as bytes (a module's ``half()`` or ``to(dtype)`` leaves them alone), half of the 16-bit MLP's memory.  The
+    output is in the 16-bit type of the activations."""
+
+    def __init__(self, mlp):
+        super().__init__()
+        with torch.no_grad():
+            for name, linear in (("fc", mlp.fc), ("proj", mlp.proj)):
+                data, scale = quantize_weight_fp8(linear.weight)
+                self.register_buffer(name + "_weight", data.view(torch.uint8))
+                self.register_buffer(name + "_scale", scale.view(torch.uint8))
+                self.register_buffer(name + "_bias", None if linear.bias is None else linear.bias.detach().clone())
+
+    def forward(self, x, defer=False):
+        """x (..., dim) in 16 bits on the GPU.  ``defer`` is ``MLP``'s; the output is always summed."""
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"Fp8MLP takes 16-bit activations (got {x.dtype})")
+        data, scale = quantize_fp8(x.reshape(-1, x.shape[-1]))
+        return self.forward_fp8(data, scale, x.dtype).view(x.shape)
+
+    def forward_fp8(self, data, scale, dtype):
+        """The MLP of quantized rows (``RMSNorm.add_norm_fp8``): (rows, dim) in ``dtype``."""
+        h, h_scale = linear_gated_fp8(data, scale, self.fc_weight.view(FP8), self.fc_scale.view(FP8_SCALE), self.fc_bias)
+        return linear_fp8(h, h_scale, self.proj_weight.view(FP8), self.proj_scale.view(FP8_SCALE), self.proj_bias,
+                          out_dtype=dtype)
 
 
 class GlobalBlock(nn.Module):

@@ -61,6 +61,16 @@ def test_refusals():
         linear_gated_fp8(_x(4, 144), _s(4, 2), _x(128, 144), _s(1, 2))
 
 
+def test_modules_refuse_the_cpu_and_fp32():
+    from atma_amd.engine import Config
+    from atma_amd.layers.global_attention import MLP, Fp8MLP, RMSNorm
+    with pytest.raises(RuntimeError, match="GPU only"):
+        Fp8MLP(MLP(64))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+        RMSNorm(64).add_norm_fp8(torch.zeros(2, 64, dtype=torch.bfloat16), None)
+    assert Config().fp8_mlp is False
+
+
 def test_entry_points_validate_without_launch():
     lib, null = _lib.load(), None
     ptr = ctypes.cast(ctypes.create_string_buffer(256), ctypes.c_void_p)

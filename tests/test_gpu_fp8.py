@@ -190,7 +190,10 @@ def _near_product(y, exact, size):
 SHAPES = [(1, 1, 16), (1, 1024, 4096), (2, 7, 128), (16, 40, 144), (17, 129, 272), (31, 1001, 1024), (32, 128, 112),
           (33, 16, 128), (33, 129, 1040), (64, 256, 640), (100, 257, 2048), (129, 1000, 384), (257, 130, 1024),
           (300, 512, 528), (700, 72, 896),
-          (2100, 2001, 528), (8200, 2104, 272), (4100, 4097, 80)]
+          # more than one tile of features a workgroup for few rows, and tiles for them; each tile shape, one and two
+          # tiles a workgroup, one block of K
+          (9, 6200, 144), (20, 6150, 272), (5, 12300, 128), (2000, 1000, 528), (2100, 2001, 528), (4000, 4001, 272),
+          (8100, 4090, 272), (4100, 4097, 80)]
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -209,7 +212,8 @@ def test_linear(dev, M, N, K, dtype):
 
 @pytest.mark.parametrize("M,H,K", [(1, 128, 16), (1, 4096, 1024), (9, 256, 144), (16, 384, 1040), (32, 128, 2048),
                                    (33, 128, 128), (64, 256, 272), (100, 640, 1024), (129, 128, 384), (300, 512, 640),
-                                   (2001, 1024, 272), (4201, 2048, 144)])
+                                   (2001, 1024, 272), (770, 4096, 144), (4201, 2048, 144), (4090, 2048, 912),
+                                   (8190, 2048, 912)])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 def test_linear_gated(dev, M, H, K, bias):
     from atma_amd.kernel import linear_gated_fp8
@@ -380,3 +384,93 @@ def test_same_bits_every_time_and_in_every_batch(dev):
     first = _chain(branch, res, w, fc, proj)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, _chain(branch, res, w, fc, proj)))
+
+
+# ------------------------------------------------------------------------------------------------ the MLP and the engine
+def _mlp(dev, dim, dtype=torch.bfloat16, seed=0):
+    from atma_amd.layers.global_attention import MLP
+    torch.manual_seed(seed)
+    return MLP(dim).to(dtype).to(dev)
+
+
+def _exact_mlp(m, h):
+    a, _ = O.linear(h, O.values(m.fc_weight.view(torch.float8_e4m3fn), m.fc_scale.view(torch.float8_e8m0fnu), 128), m.fc_bias.cpu())
+    y, _ = O.linear(O.gated(a), O.values(m.proj_weight.view(torch.float8_e4m3fn), m.proj_scale.view(torch.float8_e8m0fnu), 128),
+                    m.proj_bias.cpu())
+    return y
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_mlp_module(dev, dtype):
+    """``Fp8MLP`` of rows and of batches, against float64 of its 8-bit weights (two roundings of activations to 8 bits, the
+    first one doubled by the square, 0.026 rms each); ``half()`` leaves the weights alone; grad mode without leaves works,
+    with one is refused."""
+    from atma_amd.layers.global_attention import Fp8MLP
+    m = Fp8MLP(_mlp(dev, 256, dtype))
+    assert m.fc_weight.dtype == torch.uint8 and m.half().fc_weight.dtype == torch.uint8
+    m = Fp8MLP(_mlp(dev, 256, dtype))
+    x = torch.randn(3, 50, 256, generator=_g(1)).to(dtype)
+    y = m(x.to(dev))
+    assert y.shape == x.shape and y.dtype == dtype
+    exact = _exact_mlp(m, x.double().view(-1, 256))
+    assert ((y.cpu().double().view(-1, 256) - exact).norm() / exact.norm()).item() <= 4 * 0.026
+    assert torch.equal(m(x[1].to(dev)), y[1]) and torch.equal(m(x.to(dev), defer=True), y)
+    with pytest.raises(ValueError):
+        m(x.to(dev).float())
+    with pytest.raises(RuntimeError, match="inference"):
+        m(x.to(dev).requires_grad_())
+
+
+def test_block_stream_takes_the_fused_norm(dev):
+    """The decoder block's stream route quantizes in the norm; a hook on the MLP, which it would not call, sends it through
+    the modules, whose norm is rounded to 16 bits on the way."""
+    from atma_amd.engine.model import Atma
+    from atma_amd.engine import AtmaConfig
+    hf = AtmaConfig(vocab_size=64, num_hidden_layers=1, hidden_size=256, head_dim=64)
+    block = Atma(hf).init_weights(0.05, 1).to(dev, torch.bfloat16).quantize_mlps().blocks[0]
+    with torch.no_grad():
+        block.norm1.weight.fill_(1), block.norm2.weight.fill_(1)
+    block.attn = torch.nn.Identity()
+    block.attn.forward = lambda h, defer=False: h
+    x, res = (torch.randn(9, 256, generator=_g(i)).bfloat16().to(dev) for i in (1, 2))
+    with torch.no_grad():
+        y, s = block.forward_stream(x, res)
+        h, s1 = block.norm1.add_norm(x, res)
+        data, scale, s2 = block.norm2.add_norm_fp8(h, s1)
+        assert torch.equal(s, s2) and torch.equal(y, block.mlp.forward_fp8(data, scale, torch.bfloat16))
+        calls = []
+        handle = block.mlp.register_forward_hook(lambda *a: calls.append(1))
+        y2, s3 = block.forward_stream(x, res)
+        handle.remove()
+        assert calls == [1] and torch.equal(s3, s2)
+        exact = _exact_mlp(block.mlp, O.residual_norm(s2.cpu(), None, torch.ones(256), 1e-6, torch.bfloat16)[0])
+        for out in (y, y2):
+            assert ((out.cpu().double() - exact).norm() / exact.norm()).item() <= 4 * 0.026
+
+
+def test_engine_with_8_bit_mlps(dev):
+    """A greedy generation with ``Config.fp8_mlp``: every prefill and decode step near the whole-model oracle on the 8-bit
+    weights' values.  Each of the four blocks' MLP branches is off by 4 * 0.026 of itself at most (above) and no larger than
+    the stream it joins, coherently 4 * 0.104 in all, and the 16-bit route adds 5e-2.  Captured decode equals eager."""
+    from atma_amd.engine import Config, LLMEngine
+    from oracle import model as OM
+    from tests.test_gpu_engine import _drive, _model, _prompts
+    runs = []
+    for eager in (True, False):
+        hf, model, sd = _model(torch.bfloat16)
+        cfg = Config(kvcache_block_size=16, max_num_seqs=4, max_num_batched_tokens=4096, max_model_len=160,
+                     num_kvcache_blocks=64, enforce_eager=eager, hf_config=hf, fp8_mlp=True)
+        engine = LLMEngine(cfg, model=model)
+        runs.append(_drive(engine, _prompts([17, 40, 129], 2), new_tokens=4)[1])
+        engine.exit()
+    for a, b in zip(*runs):
+        assert a[3] == b[3] and torch.equal(a[2], b[2])
+    for i, b in enumerate(model.blocks):
+        for n in ("fc", "proj"):
+            sd[f"blocks.{i}.mlp.{n}.weight"] = O.values(getattr(b.mlp, n + "_weight").view(torch.float8_e4m3fn),
+                                                       getattr(b.mlp, n + "_scale").view(torch.float8_e8m0fnu), 128)
+    kw = dict(num_layers=hf.num_hidden_layers, H=hf.num_attention_heads, Hkv=hf.num_key_value_heads, dk=hf.head_dim)
+    for is_prefill, hist, logits, _ in runs[0]:
+        for row, h in enumerate(hist):
+            ref = OM.atma_logits(sd, torch.tensor(h)[None], **kw)[0, -1]
+            assert ((logits[row].double() - ref).norm() / ref.norm()).item() <= 4 * 0.104 + 5e-2, (is_prefill, len(h))
