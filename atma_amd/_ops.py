@@ -956,10 +956,8 @@ FP8, FP8_SCALE, FP8_BLOCK = torch.float8_e4m3fn, torch.float8_e8m0fnu, 128
 
 
 def _fp8_pair(like: Tensor, rows: int, cols: int, scale_rows: int):
-    """Empty (data, scale); a row of scales starts at a multiple of 4 bytes, as the products read them."""
-    nb = (cols + 127) // 128
-    scale = like.new_empty((scale_rows, (nb + 3) // 4 * 4), dtype=FP8_SCALE)
-    return like.new_empty((rows, cols), dtype=FP8), scale if nb % 4 == 0 else scale[:, :nb]
+    """Empty (data, scale)."""
+    return (like.new_empty((rows, cols), dtype=FP8), like.new_empty((scale_rows, (cols + 127) // 128), dtype=FP8_SCALE))
 
 
 def _rows_apart(t: Tensor) -> Tensor:
@@ -968,12 +966,7 @@ def _rows_apart(t: Tensor) -> Tensor:
 
 
 def _fp8_scales(t: Tensor) -> Tensor:
-    """Rows of scales at multiples of 4 bytes."""
-    if t.stride(1) == 1 and t.data_ptr() % 4 == 0 and t.stride(0) % 4 == 0 and t.stride(0) >= t.shape[1]:
-        return t
-    held = t.new_empty((t.shape[0], (t.shape[1] + 3) // 4 * 4))
-    held[:, :t.shape[1]].copy_(t)
-    return held[:, :t.shape[1]]
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _bias4(t: Optional[Tensor]) -> Optional[Tensor]:

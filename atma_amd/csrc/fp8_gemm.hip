@@ -27,7 +27,7 @@ union Frag8 {  // one operand: 32 values of a row
 struct Fp8Args {
   const uint8_t* x;  // (M, K), row stride ldx
   int64_t ldx;
-  const uint8_t* xs;  // (M, nk), row stride ldxs, a multiple of 4
+  const uint8_t* xs;  // (M, nk), row stride ldxs
   int64_t ldxs;
   const uint8_t* w;  // (N, K) or, gated, (2 N, K): the a rows, then the gate rows
   int64_t ldw;
@@ -79,9 +79,9 @@ __device__ __forceinline__ void dma_buf4_rare(__amdgpu_buffer_rsrc_t r, uint32_t
                "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
                : "memory");
 }
-// 4 bytes a lane from an address a lane to lds_byte_offset + 4 lane
-__device__ __forceinline__ void dma_load4_at(const void* p, uint32_t lds_byte_offset) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p),
+// A byte a lane, from an address a lane, to the word at lds_byte_offset + 4 lane
+__device__ __forceinline__ void dma_load1_at(const void* p, uint32_t lds_byte_offset) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(p),
                "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
                : "memory");
 }
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
   };
   uint32_t pd, pwv, pxv;
   auto copies_begin = [&]() {
-    dma_load4_at(scales + (plimit ? pk & ~3 : 0), lds0 + C::AUX + C::SLOT * pslot + 256 * wave);
+    dma_load1_at(scales + (plimit ? pk : 0), lds0 + C::AUX + C::SLOT * pslot + 256 * wave);
     pslot = pslot + 1 == C::RING ? 0 : pslot + 1;
     pd = lds0 + pstage * C::STAGE + 1024 * wave;
     pstage = pstage + 1 == NS ? 0 : pstage + 1;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
   auto wtile = [](int t) { return GATED ? t / TO * (C::BF / 2) + 32 * (t % TO) : 32 * t; };
   f32x16 acc[TF][TM];
   Frag8 wv[2][TF], xv[TM];
-  uint32_t xw[TM], ww[2];
+  int xs[TM], ws[2];
   int stage = 0, slot = 0, tile = 0;  // what is read next
   auto read_w = [&](const uint8_t* base, int s, int t) {
 #pragma unroll
@@ -238,11 +238,11 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
       const int row = 32 * (TM * wm + j) + r;
-      xw[j] = *(const uint32_t*)(p + 256 * (row / C::XW) + 4 * (row % C::XW));
+      xs[j] = *(const int*)(p + 256 * (row / C::XW) + 4 * (row % C::XW));
     }
-    const uint32_t* q = (const uint32_t*)(p + 256 * wave + 128);
-    ww[0] = q[GATED ? 0 : wrow0 / kFp8Block];
-    ww[1] = GATED ? q[1] : 0;
+    const int* q = (const int*)(p + 256 * wave + 128);
+    ws[0] = q[GATED ? 0 : wrow0 / kFp8Block];
+    ws[1] = GATED ? q[1] : 0;
   };
 
   aim(m0, f0);
@@ -294,12 +294,6 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 
     for (int kb = 0; kb < nk; ++kb) {
       if (pk == nk) next_tile();
-      int xs[TM], ws[2];
-      const int sh = 8 * (kb & 3);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) xs[j] = (int)(xw[j] >> sh);
-      ws[0] = (int)(ww[0] >> sh);
-      ws[1] = (int)(ww[1] >> sh);
       const uint8_t* base = lds + stage * C::STAGE;
       stage = stage + 1 == NS ? 0 : stage + 1;
 #pragma unroll
@@ -509,13 +503,10 @@ static int check_fp8(const char* what, const Fp8Args& a, int64_t rows) {
   if (!a.x || !a.xs || !a.w || !a.ws || !a.y) return set_error(ATMA_ERR_INVALID, "%s: null pointer", what);
   if ((uintptr_t)a.x % 16 || a.ldx % 16 || a.ldx < a.K || (uintptr_t)a.w % 16 || a.ldw % 16 || a.ldw < a.K)
     return set_error(ATMA_ERR_INVALID, "%s: rows of x and w must be 16-byte aligned and at least K long", what);
-  if ((uintptr_t)a.xs % 4 || a.ldxs % 4 || a.ldxs < a.nk || (uintptr_t)a.ws % 4 || a.ldws % 4 || a.ldws < a.nk)
-    return set_error(ATMA_ERR_INVALID, "%s: rows of scales must be 4-byte aligned and hold %d", what, a.nk);
+  if (a.ldxs < 0 || a.ldws < 0) return set_error(ATMA_ERR_INVALID, "%s: negative stride of scales", what);
   // a tile's rows (at most 256) are addressed by 32-bit byte offsets
   if (a.ldx > (1 << 23) || a.ldw > (1 << 23))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: rows more than 8 MiB apart", what);
-  if (a.ldxs > (1 << 20) || a.w_blocks * a.ldws >= (1ll << 31))
-    return set_error(ATMA_ERR_UNSUPPORTED, "%s: scales too far apart", what);
   if (a.bias && (uintptr_t)a.bias % 4) return set_error(ATMA_ERR_INVALID, "%s: bias must be 4-byte aligned", what);
   if (a.bias && !dtype_size(a.bias_dtype))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: bias in fp32 or 16 bits (dtype %d)", what, a.bias_dtype);

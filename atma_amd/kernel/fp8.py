@@ -127,10 +127,9 @@ def _operands(what, x, x_scale, weight, weight_scale, bias):
         raise ValueError(f"{what}: bias must be ({N},) of {_dtypes(_DT32)}")
     if not _placed(what, x, x_scale, weight, weight_scale, bias):
         return False
-    (ldx, ix), (ldw, iw), (lxs, ixs), (lws, iws) = x.stride(), weight.stride(), x_scale.stride(), weight_scale.stride()
-    return (ix == iw == ixs == iws == 1 and ldx >= K and ldw >= K and lxs >= nb and lws >= nb
+    (ldx, ix), (ldw, iw) = x.stride(), weight.stride()
+    return (ix == iw == x_scale.stride(1) == weight_scale.stride(1) == 1 and ldx >= K and ldw >= K
             and not (x.data_ptr() | weight.data_ptr() | ldx | ldw) & 15
-            and not (x_scale.data_ptr() | weight_scale.data_ptr() | lxs | lws) & 3
             and (bias is None or (bias.stride(0) == 1 and not bias.data_ptr() & 3)))
 
 
@@ -138,8 +137,7 @@ def linear_fp8(x, x_scale, weight, weight_scale, bias=None, out_dtype=torch.bflo
     """``F.linear`` of 8-bit operands: x (M, K) with x_scale (M, ceil(K / 128)), weight (N, K) with weight_scale
     (ceil(N / 128), ceil(K / 128)); bias (N,) in fp32 or 16 bits or None.  Sums in fp32, one rounding to ``out_dtype``
     (bfloat16 or float16).  The matrix instructions add the products of eight neighbouring k with 14 bits below the largest
-    of them, 1.4e-5 of a result of normally distributed values.  Scales whose rows start at multiples of 4 bytes, as
-    ``quantize_fp8`` lays them, are read in place; others are copied."""
+    of them, 1.4e-5 of a result of normally distributed values."""
     if out_dtype not in _DT:
         raise ValueError(f"linear_fp8: out_dtype must be bfloat16 or float16 (got {out_dtype})")
     if _operands("linear_fp8", x, x_scale, weight, weight_scale, bias):

@@ -105,7 +105,7 @@ def test_entry_points_validate_without_launch():
         assert f(K=136) == 2 and f(K=0) == 2 and f(K=1 << 23) == 2 and f(M=-1) == 2 and f(M=1 << 40) == 2
         assert f(ldx=1 << 24) == 2 and f(bias=ptr, bt=9) == 2
         for bad in (dict(x=null), dict(xs=null), dict(w=null), dict(ws=null), dict(y=null), dict(x=odd), dict(w=odd),
-                    dict(ldx=128), dict(ldw=152), dict(ldxs=1), dict(ldxs=6), dict(ldws=2), dict(ldy=128),
+                    dict(ldx=128), dict(ldw=152), dict(ldxs=-1), dict(ldws=-1), dict(ldy=128),
                     dict(bias=ctypes.c_void_p(ptr.value + 2))):
             assert f(**bad) == 1, bad
     assert linear(dt=F32) == 2 and linear(N=0) == 2
@@ -117,6 +117,6 @@ def test_copies_have_their_wait_states(tmp_path):
     proc = subprocess.run([*_build.compile_command(src), "--cuda-device-only", "-S", str(src), "-o", str(out)],
                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     assert proc.returncode == 0, proc.stdout[-2000:]
-    # the scales' copy, 4 bytes from an address a lane, has the 16-byte form's operands: m0 and vector registers
-    found, copies = check_assembly(out.read_text().replace("global_load_lds_dword ", "global_load_lds_dwordx4 "))
+    # the scales' copy, a byte from an address a lane, has the 16-byte form's operands: m0 and vector registers
+    found, copies = check_assembly(out.read_text().replace("global_load_lds_ubyte ", "global_load_lds_dwordx4 "))
     assert found == [] and copies > 0, "\n".join(found[:20])
