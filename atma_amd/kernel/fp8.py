@@ -21,26 +21,26 @@ from .decode_fusions import PartialSums
 _DT = (torch.bfloat16, torch.float16)
 _DT32 = (torch.bfloat16, torch.float16, torch.float32)
 FP8, FP8_SCALE, FP8_BLOCK = _ops.FP8, _ops.FP8_SCALE, _ops.FP8_BLOCK
+_Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
+_grad_enabled, _function_modes = torch.is_grad_enabled, torch._C._len_torch_function_stack
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
 def _placed(what, *ts):
     """Every tensor of a call on one GPU, none of them waiting for a gradient.  Returns whether the call may go straight to
     its launch: that GPU is the current one and nothing watches, transforms or overrides the call."""
-    device, grad, plain = ts[0].get_device(), torch.is_grad_enabled(), True
+    device, grad, plain = ts[0].get_device(), _grad_enabled(), True
     for t in ts:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
-            raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
-        if at != device:
-            raise ValueError(f"{what}: every tensor must be on one GPU")
-        if grad and t.requires_grad:
-            raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), or detach its inputs")
-        if type(t) not in _ops._PLAIN:
-            plain = False
-    return (plain and device == torch.cuda.current_device() and not _ops.watched()
-            and not torch._C._len_torch_function_stack())
+        if t is not None:
+            if t.get_device() != device or device < 0:
+                if t.get_device() < 0 or device < 0:
+                    raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
+                raise ValueError(f"{what}: every tensor must be on one GPU")
+            if grad and t.requires_grad:
+                raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), or detach its inputs")
+            if type(t) is not _Tensor and type(t) is not _Parameter:
+                plain = False
+    return plain and device == _current_device() and not _ops.watched() and not _function_modes()
 
 
 def _dtypes(dtypes):
@@ -112,8 +112,10 @@ def residual_rms_norm_fp8(branch, residual, weight, eps):
 
 def _operands(what, x, x_scale, weight, weight_scale, bias):
     """Checks a product's operands; returns whether it may go straight to its launch (``_placed``, and nothing to copy)."""
-    _matrix(what, "x", x, (FP8,))
-    _matrix(what, "weight", weight, (FP8,))
+    if x.dim() != 2 or x.dtype is not FP8 or x.shape[1] % 16 or x.shape[1] < 16:
+        _matrix(what, "x", x, (FP8,))
+    if weight.dim() != 2 or weight.dtype is not FP8:
+        _matrix(what, "weight", weight, (FP8,))
     (M, K), (N, Kw) = x.shape, weight.shape
     nb = (K + 127) // 128
     if K != Kw or N < 1:
