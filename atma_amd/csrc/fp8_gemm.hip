@@ -126,7 +126,8 @@ struct Fp8Tile {
   static constexpr int RING = NS + 2;    // blocks and tiles under way: copies run NS blocks ahead
   static constexpr int SLOT = NW * 256;  // a block's scales
   static constexpr int AUX = NS * STAGE, BIAS = AUX + RING * SLOT, TOP = BIAS + RING * 1024;
-  static constexpr int LDS = TOP + (GATED ? WF * BM * 4 : 0);
+  static constexpr bool TURNED = !GATED && NW == 8;  // outputs leave through LDS, where there is room
+  static constexpr int TURN = TOP, LDS = TOP + (GATED ? WF * BM * 4 : TURNED ? 2048 * NW : 0);
   static_assert((NW == 4 || NW == 8) && BF % (8 * NW) == 0 && BM % (8 * NW) == 0 && BF <= 256 && XW <= 32,
                 "whole copies, a bias of 1 KiB");
   static_assert(!GATED || (OF == kFp8Block && TF == 2), "a gated tile is one block of output features");
@@ -330,24 +331,62 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
     LateArgs p = late_args();
     if constexpr (!GATED) {
       const bool whole = f0 + C::OF <= p->N && p->ldy % 8 == 0;
+      if constexpr (C::TURNED) {
+        // through LDS, a wave its own 2 KiB: 32 tokens x 32 features at a time turn from a token a lane to 64-byte pieces, four
+        // lanes each (chunk c of row r at position c ^ (r / 4) % 4): a CU alone stores 80 bytes a cycle so, 28 as they lie
+        // (65,536 x 1,024 -> 8,192 630 to 605 us, 4,096 x 1,024 -> 4,096 23.4 to 21.8)
+        uint8_t* turn = lds + C::TURN + 2048 * wave;
+        const int64_t ldy = p->ldy, N = p->N, M = p->M;
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        const int64_t m = m0 + 32 * (TM * wm + j) + r;
-        if (m < p->M) {
+        for (int j = 0; j < TM; ++j) {
 #pragma unroll
           for (int t = 0; t < TF; ++t) {
-            const int64_t n0 = f0 + wrow0 + 32 * t + 16 * h;
-            T* y = (T*)p->y + m * p->ldy + n0;
             const f32x16& v = acc[t][j];
-            if (whole) {
+            wave_sync();
 #pragma unroll
-              for (int e = 0; e < 16; e += 8)
-                *(u32x4*)(y + e) = u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]),
-                                         pack2<T>(v[e + 4], v[e + 5]), pack2<T>(v[e + 6], v[e + 7])};
-            } else {
+            for (int e = 0; e < 16; e += 8)
+              *(u32x4*)(turn + 64 * r + 16 * ((2 * h + e / 8) ^ ((r >> 2) & 3))) =
+                  u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]), pack2<T>(v[e + 4], v[e + 5]),
+                        pack2<T>(v[e + 6], v[e + 7])};
+            wave_sync();
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (n0 + e < p->N) y[e] = from_f32<T>(v[e]);
+            for (int i = 0; i < 2; ++i) {
+              const int row = 16 * i + (lane >> 2);
+              const u32x4 o = *(const u32x4*)(turn + 64 * row + 16 * ((lane & 3) ^ ((row >> 2) & 3)));
+              const int64_t m = m0 + 32 * (TM * wm + j) + row, n0 = f0 + wrow0 + 32 * t + 8 * (lane & 3);
+              T* y = (T*)p->y + m * ldy + n0;
+              if (m < M) {
+                if (whole) {
+                  *(u32x4*)y = o;
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    if (n0 + e < N) y[e] = __builtin_bit_cast(T, (uint16_t)(o[e >> 1] >> (16 * (e & 1))));
+                }
+              }
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          const int64_t m = m0 + 32 * (TM * wm + j) + r;
+          if (m < p->M) {
+#pragma unroll
+            for (int t = 0; t < TF; ++t) {
+              const int64_t n0 = f0 + wrow0 + 32 * t + 16 * h;
+              T* y = (T*)p->y + m * p->ldy + n0;
+              const f32x16& v = acc[t][j];
+              if (whole) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 8)
+                  *(u32x4*)(y + e) = u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]),
+                                           pack2<T>(v[e + 4], v[e + 5]), pack2<T>(v[e + 6], v[e + 7])};
+              } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  if (n0 + e < p->N) y[e] = from_f32<T>(v[e]);
+              }
             }
           }
         }
