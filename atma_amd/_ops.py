@@ -962,7 +962,7 @@ def _fp8_pair(like: Tensor, rows: int, cols: int, scale_rows: int):
 
 def _rows_apart(t: Tensor) -> Tensor:
     """Rows that start at multiples of 16 bytes and do not overlap (those of an expanded tensor do)."""
-    return _rows16(t if t.shape[0] < 2 or t.stride(0) >= t.shape[1] else t.contiguous())
+    return _rows16(t if t.stride(0) >= t.shape[1] else t.clone(memory_format=torch.contiguous_format))
 
 
 def _fp8_scales(t: Tensor) -> Tensor:

@@ -3,6 +3,8 @@
 //
 // Both read each value once, keep it in registers through the reduction of its block's largest magnitude and write one
 // byte for it, so they are bound by memory: 3 bytes a 16-bit value, 5 a 32-bit one.
+#include <algorithm>
+
 #include "fp8.h"
 
 namespace atma {
@@ -37,22 +39,23 @@ struct QuantArgs {
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t m = item / a.groups;
-  if (m >= a.M) return;
-  const int c = (int)(item - m * a.groups) * 512 + lane * 8;
-  float v[8] = {};
-  if (c < a.K) load8f<T>((const T*)a.x + m * a.ldx + c, v);
-  float amax = 0.f;
+  for (int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);; item += (int64_t)gridDim.x * 4) {
+    const int64_t m = item / a.groups;
+    if (m >= a.M) return;
+    const int c = (int)(item - m * a.groups) * 512 + lane * 8;
+    float v[8] = {};
+    if (c < a.K) load8f<T>((const T*)a.x + m * a.ldx + c, v);
+    float amax = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(v[e]));
-  const int code = fp8_scale_code(row16_max(amax));
-  if (c >= a.K) return;
-  const float inv = fp8_inv_scale(code);
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(v[e]));
+    const int code = fp8_scale_code(row16_max(amax));
+    if (c >= a.K) continue;
+    const float inv = fp8_inv_scale(code);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] *= inv;
-  *(u32x2*)(a.data + m * a.ldd + c) = u32x2{fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7])};
-  if ((lane & 15) == 0) a.scale[m * a.lds + c / kFp8Block] = (uint8_t)code;
+    for (int e = 0; e < 8; ++e) v[e] *= inv;
+    *(u32x2*)(a.data + m * a.ldd + c) = u32x2{fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7])};
+    if ((lane & 15) == 0) a.scale[m * a.lds + c / kFp8Block] = (uint8_t)code;
+  }
 }
 
 // A workgroup takes one 128 x 128 block: thread t the 8 columns 8 (t % 16) of rows t / 16, + 16, ...
@@ -108,13 +111,13 @@ static int quantize(const char* what, bool weight, const void* x, int64_t ldx, v
       const int64_t mb = (M + kFp8Block - 1) / kFp8Block;
       quantize_weight_kernel<T><<<dim3((unsigned)nb, (unsigned)mb), 256, 0, s>>>(a);
     } else {
-      quantize_rows_kernel<T><<<dim3((unsigned)((M * a.groups + 3) / 4)), 256, 0, s>>>(a);
+      // a wave for each 512 columns; rows past a million workgroups share them
+      const int64_t wgs = std::min<int64_t>((M * a.groups + 3) / 4, 1 << 20);
+      quantize_rows_kernel<T><<<dim3((unsigned)wgs), 256, 0, s>>>(a);
     }
   };
   if (weight && (M + kFp8Block - 1) / kFp8Block > 65535)
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: at most %d rows", what, 65535 * kFp8Block);
-  if (!weight && (M * a.groups + 3) / 4 > 0x7fffffff)
-    return set_error(ATMA_ERR_UNSUPPORTED, "%s: too many values", what);
   if (dtype == ATMA_BF16) launch(bf16{});
   else if (dtype == ATMA_F16) launch(f16{});
   else launch(float{});

@@ -40,7 +40,7 @@ def _placed(what, *ts):
                 raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), or detach its inputs")
             if type(t) is not _Tensor and type(t) is not _Parameter:
                 plain = False
-    return plain and device == _current_device() and not _ops.watched() and not _function_modes()
+    return plain and not _ops.watched() and not _function_modes() and device == _current_device()
 
 
 def _dtypes(dtypes):

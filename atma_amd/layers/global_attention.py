@@ -767,6 +767,8 @@ class Fp8MLP(nn.Module):
 
     def __init__(self, mlp):
         super().__init__()
+        if mlp.fc.weight.shape[0] % 256 or mlp.fc.weight.shape[1] % 16:
+            raise ValueError(f"Fp8MLP: hidden sizes are multiples of 128, the width of 16 (got {tuple(mlp.fc.weight.shape)})")
         with torch.no_grad():
             for name, linear in (("fc", mlp.fc), ("proj", mlp.proj)):
                 data, scale = quantize_weight_fp8(linear.weight)

@@ -66,6 +66,8 @@ def test_modules_refuse_the_cpu_and_fp32():
     from atma_amd.layers.global_attention import MLP, Fp8MLP, RMSNorm
     with pytest.raises(RuntimeError, match="GPU only"):
         Fp8MLP(MLP(64))
+    with pytest.raises(ValueError, match="multiples of 128"):
+        Fp8MLP(MLP(48))
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
         RMSNorm(64).add_norm_fp8(torch.zeros(2, 64, dtype=torch.bfloat16), None)
     assert Config().fp8_mlp is False

@@ -153,9 +153,10 @@ def test_residual_norm_partial_sums(dev, rows, parts, mu, dtype):
     mx, mw = (torch.randn(rows, mu, generator=g).to(dtype).to(dev), torch.randn(D, mu, generator=g).to(dtype).to(dev)) if mu \
         else (None, None)
     ps = PartialSums(p, b, mu_x=mx, mu_w=mw, dtype=dtype)
-    data, scale, stream = residual_rms_norm_fp8(ps, res, w, 1e-6)
-    assert torch.equal(stream, residual_rms_norm(ps, res, w, 1e-6)[1])
-    _near_quantized(data, scale, O.residual_norm(stream.cpu(), None, w.cpu(), 1e-6, dtype)[0])
+    for r in (res, None):   # joining a stream, starting one
+        data, scale, stream = residual_rms_norm_fp8(ps, r, w, 1e-6)
+        assert torch.equal(stream, residual_rms_norm(ps, r, w, 1e-6)[1])
+        _near_quantized(data, scale, O.residual_norm(stream.cpu(), None, w.cpu(), 1e-6, dtype)[0])
 
 
 def test_residual_norm_strided_and_empty(dev):
@@ -288,6 +289,41 @@ def test_products_at_other_layouts(dev, M):
     assert torch.equal(one, one[:1].expand_as(one))
 
 
+def test_one_row_at_any_stride(dev):
+    """A single row whose row stride says nothing (expanded, shorter than the row): x, weight, residual, quantizer input."""
+    from atma_amd.kernel import linear_fp8, quantize_fp8, quantize_weight_fp8, residual_rms_norm_fp8
+    x, xs, w, ws, _, _ = _operands(dev, 1, 1, 144, 3)
+    want = linear_fp8(x, xs, w, ws)
+    for stride in (0, 1, 16):
+        one = lambda t: t.as_strided(t.shape, (stride, 1))   # noqa: E731
+        assert torch.equal(linear_fp8(one(x), one(xs), one(w), one(ws)), want)
+        v = _rows(1, 144, 5, torch.bfloat16).to(dev)
+        for f in (quantize_fp8, quantize_weight_fp8):
+            assert torch.equal(f(one(v))[0].view(torch.uint8), f(v)[0].view(torch.uint8))
+        g = torch.ones(144, dtype=torch.bfloat16, device=dev)
+        assert torch.equal(residual_rms_norm_fp8(one(v), one(v), g, 1e-6)[2], residual_rms_norm_fp8(v, v, g, 1e-6)[2])
+
+
+@pytest.mark.parametrize("M", [3, 50, 300])
+def test_products_with_a_bias_anywhere(dev, M):
+    """A bias at an odd offset, with a stride, expanded: equal to the call on a fresh copy."""
+    from atma_amd.kernel import linear_fp8, linear_gated_fp8
+    x, xs, w, ws, _, _ = _operands(dev, M, 256, 144, 4)
+    held = torch.randn(600, generator=_g(1)).bfloat16().to(dev)
+    for b in (held[1:257], held[3:515:2], held[7].expand(256)):
+        assert torch.equal(linear_fp8(x, xs, w, ws, b), linear_fp8(x, xs, w, ws, b.clone()))
+        for p, q in zip(linear_gated_fp8(x, xs, w, ws, b), linear_gated_fp8(x, xs, w, ws, b.clone())):
+            assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
+    for bad in (float("-inf"), float("nan")):   # a pruned feature (0 after the activation), a lost one
+        b = torch.zeros(256)
+        b[5] = bad
+        data, scale = linear_gated_fp8(x, xs, w, ws, b.to(dev))
+        d = data.cpu().float()
+        clean = linear_gated_fp8(x, xs, w, ws, torch.zeros(256, device=dev))
+        assert (d[:, 5] == 0).all() if bad == float("-inf") else torch.isnan(d[:, 5]).all()
+        assert not torch.isnan(torch.cat([d[:, :5], d[:, 6:]], 1)).any() and scale.shape == clean[1].shape
+
+
 def test_products_of_no_rows(dev):
     from atma_amd.kernel import linear_fp8, linear_gated_fp8
     x, xs, w, ws, _, _ = _operands(dev, 4, 256, 128, 1)
@@ -378,7 +414,36 @@ def test_chain_captured_and_on_another_stream(dev):
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
 
 
-def test_same_bits_every_time_and_in_every_batch(dev):
+@pytest.mark.parametrize("rows", [5, 200])
+def test_chain_compiles_as_one_graph(dev, rows):
+    branch, res, w, fc, proj = _chain_operands(dev, rows, 5)
+    want = _chain(branch, res, w, fc, proj)
+    compiled = torch.compile(_chain, fullgraph=True, backend="aot_eager")
+    with torch.no_grad():
+        got = compiled(branch, res, w, fc, proj)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_calls_under_modes_and_subclasses_are_dispatched(dev):
+    """What watches torch calls sees the operators; a subclass is not launched past."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    branch, res, w, fc, proj = _chain_operands(dev, 5, 5)
+    want = _chain(branch, res, w, fc, proj)
+    with Watch():
+        got = _chain(branch, res, w, fc, proj)
+    for name in ("residual_rms_norm_fp8", "linear_gated_fp8", "linear_fp8"):
+        assert any(f"atma_hip.{name}" in s for s in seen)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_same_bits_every_time(dev):
     """Nothing depends on the order in which workgroups run: calls repeat bit for bit."""
     branch, res, w, fc, proj = _chain_operands(dev, 300, 7)
     first = _chain(branch, res, w, fc, proj)
