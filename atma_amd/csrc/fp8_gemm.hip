@@ -439,58 +439,73 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// At most 16 MT tokens: a stream of the weights.  A workgroup of NW waves owns FT tiles of 16 weight rows and its waves
-// take the blocks of K in turn, two under way at a time; operands come straight from memory in the MFMA's layout (the four
-// lanes of a row take 64 consecutive bytes a load) and the waves' sums are joined through LDS in a fixed order.
-template <typename T, int MT, int FT, int NW>
+// Few rows: latency, not bandwidth.  A workgroup owns FT tiles of 16 features x MT tiles of 16 tokens and its NW waves take the
+// blocks of K in turn, so a chain of K is NW times shorter; their sums are joined through LDS in a fixed order.  Each wave
+// has a ring of its own of NS blocks, filled by direct copies of whole 128-byte lines, and waits for nothing but its own
+// copies.  (Operands read from memory in the MFMA's layout, 16 rows to an instruction, come in at 11 bytes a cycle and CU, at
+// 17 with the halves of odd rows swapped; copied this way at 38: 64 x 16,384 -> 1,024 30.7, 20.6 and 10.5 us.)  Four waves of
+// two blocks measured best: more CU-wide copies in flight or more waves leave fewer workgroups a CU (32 x 1,024 -> 1,024,
+// 8 waves 3.7 us, 4 waves of four blocks 3.6, of two 3.2).
+template <typename T, int MT, int FT, int NW, int NS>
 __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
-  __shared__ f32x4 red[NW][FT][MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int ROWS = 16 * (FT + MT), STAGE = ROWS * kFp8Block + 256, COPIES = ROWS / 8;
+  static_assert(FT * MT * 1024 <= NS * STAGE && 16 * MT < 64 && kFp8Block % (16 * FT) == 0,
+                "the sums fit the ring, a lane is left for the weights' scale, one block of weight rows");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * NS * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int64_t f0 = (int64_t)blockIdx.x * 16 * FT;
-  const uint8_t* wp[FT];
-  const uint8_t* xp[MT];
-  const uint8_t* xsp[MT];
+  const int64_t f0 = (int64_t)blockIdx.x * 16 * FT, m0 = (int64_t)blockIdx.y * 16 * MT;
+  const __amdgpu_buffer_rsrc_t wr = buffer_rsrc(a.w + f0 * a.ldw, (uint32_t)(min((int64_t)16 * FT, a.N - f0) * a.ldw));
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc(a.x + m0 * a.ldx, (uint32_t)(min((int64_t)16 * MT, a.M - m0) * a.ldx));
+  // copy i of a block moves rows 8 i .. 8 i + 7, lane l the chunk that belongs at position l % 8 of row 8 i + l / 8
+  const int crow = lane >> 3, chunk = 16 * ((lane & 7) ^ (crow >> 1));
+  const uint32_t wv0 = (uint32_t)crow * (uint32_t)a.ldw, xv0 = (uint32_t)crow * (uint32_t)a.ldx;
+  const uint8_t* scales = lane < 16 * MT ? a.xs + min(m0 + lane, a.M - 1) * a.ldxs : a.ws + f0 / kFp8Block * a.ldws;
+  uint8_t* ring = lds + wave * NS * STAGE;
+  const uint32_t ring0 = lds_offset(ring);
+  auto copies = [&](int kk, int slot) {
+    const uint32_t d = ring0 + slot * STAGE;
+    dma_load1_at(scales + min(kk, a.nk - 1), d + ROWS * kFp8Block);
 #pragma unroll
-  for (int t = 0; t < FT; ++t) wp[t] = a.w + min(f0 + 16 * t + r, a.N - 1) * a.ldw + 16 * g;
+    for (int i = 0; i < COPIES; ++i) {
+      const int k = kk * kFp8Block + (chunk ^ (i % 2 * 64));  // (K <= 2^22: no overflow in the blocks behind the last)
+      const bool w = i < 2 * FT;
+      const uint32_t at = w ? wv0 + 8u * i * (uint32_t)a.ldw : xv0 + 8u * (i - 2 * FT) * (uint32_t)a.ldx;
+      dma_buf16_at(w ? wr : xr, k < a.K ? at + (uint32_t)k : 0x80000000u, 0u, d + 1024 * i);
+    }
+  };
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int64_t m = min((int64_t)(16 * j + r), a.M - 1);
-    xp[j] = a.x + m * a.ldx + 16 * g;
-    xsp[j] = a.xs + m * a.ldxs;
-  }
-  const uint8_t* wsp = a.ws + f0 / kFp8Block * a.ldws;
+  for (int i = 0; i < NS; ++i) copies(wave + i * NW, i);
   f32x4 acc[FT][MT] = {};
-  for (int kb = wave; kb < a.nk; kb += 2 * NW) {
-    Frag8 wv[2][FT], xv[2][MT];
-    int xsc[2][MT], wsc[2];
+  int slot = 0;
+  for (int kk = wave; kk < a.nk; kk += NW) {
+    wait_vmcnt<(NS - 1) * (COPIES + 1)>();
+    const uint8_t* base = ring + slot * STAGE;
+    Frag8 wv[FT], xv[MT];
+    int xsc[MT];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int kk = kb + b * NW;
-      const int k = kk * kFp8Block;
+    for (int q = 0; q < 2; ++q) {
+      const int at = r * kFp8Block + 16 * ((4 * q + g) ^ x_swizzle(r));
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const bool in = k + 64 * q + 16 * g < a.K;  // (K < 2^23: no overflow in the block behind the last)
+      for (int t = 0; t < FT; ++t) wv[t].q[q] = *(const u32x4*)(base + 2048 * t + at);
 #pragma unroll
-        for (int t = 0; t < FT; ++t) wv[b][t].q[q] = in ? *(const u32x4*)(wp[t] + k + 64 * q) : u32x4{};
-#pragma unroll
-        for (int j = 0; j < MT; ++j) xv[b][j].q[q] = in ? *(const u32x4*)(xp[j] + k + 64 * q) : u32x4{};
-      }
-      const int ks = min(kk, a.nk - 1);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) xsc[b][j] = xsp[j][ks];
-      wsc[b] = wsp[ks];
+      for (int j = 0; j < MT; ++j) xv[j].q[q] = *(const u32x4*)(base + 2048 * (FT + j) + at);
     }
+    const int* sc = (const int*)(base + ROWS * kFp8Block);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if (kb + b * NW < a.nk) {
+    for (int j = 0; j < MT; ++j) xsc[j] = sc[16 * j + r];
+    const int wsc = sc[16 * MT];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the copies that overwrite them start
+    copies(kk + NS * NW, slot);
+    slot = slot + 1 == NS ? 0 : slot + 1;
 #pragma unroll
-        for (int t = 0; t < FT; ++t)
+    for (int t = 0; t < FT; ++t)
 #pragma unroll
-          for (int j = 0; j < MT; ++j) acc[t][j] = mfma_fp8(wv[b][t], xv[b][j], acc[t][j], wsc[b], xsc[b][j]);
-      }
-    }
+      for (int j = 0; j < MT; ++j) acc[t][j] = mfma_fp8(wv[t], xv[j], acc[t][j], wsc, xsc[j]);
   }
+  wait_vmcnt<0>();
+  __syncthreads();  // every wave's copies, those behind the last block too, are done: the ring is free
+  auto red = (f32x4(*)[FT][MT][64])lds;
 #pragma unroll
   for (int t = 0; t < FT; ++t)
 #pragma unroll
@@ -504,7 +519,7 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
     f32x4 s = red[0][t][j][lane];
 #pragma unroll
     for (int q = 1; q < NW; ++q) s += red[q][t][j][lane];
-    const int64_t n0 = f0 + 16 * t + 4 * g, m = 16 * j + r;
+    const int64_t n0 = f0 + 16 * t + 4 * g, m = m0 + 16 * j + r;
     if (m >= a.M) continue;
     T* y = (T*)a.y + m * a.ldy + n0;
     float v[4];
@@ -577,23 +592,25 @@ static int cheapest(const Fp8Args& a, const TileCost* c, int n) {
   return best;
 }
 
-template <typename T, int MT, int FT, int NW>
+template <typename T, int MT, int FT, int NW = 4, int NS = 2>
 static void launch_few(const Fp8Args& a, hipStream_t s) {
-  fp8_few_kernel<T, MT, FT, NW><<<dim3((unsigned)((a.N + 16 * FT - 1) / (16 * FT))), dim3(64 * NW), 0, s>>>(a);
+  const dim3 grid((unsigned)((a.N + 16 * FT - 1) / (16 * FT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+  fp8_few_kernel<T, MT, FT, NW, NS><<<grid, dim3(64 * NW), 0, s>>>(a);
 }
 
 template <typename T>
 static void launch_linear(const Fp8Args& a, hipStream_t s) {
   const int64_t cus = device_cu_count();
-  if (a.M <= 32 && a.N < 48 * cus) {
-    // two tiles of features share each activation load where that leaves work for every CU
-    const bool two = a.N >= 24 * cus;
-    if (a.M <= 16 && two) launch_few<T, 1, 2, 8>(a, s);
-    else if (a.M <= 16) launch_few<T, 1, 1, 8>(a, s);
-    else if (two) launch_few<T, 2, 2, 8>(a, s);
-    else launch_few<T, 2, 1, 8>(a, s);
-    return;
-  }
+  // Few rows, while the split over K is what fills the card (us, split kernel / tiles; x = rows x K -> features).  Features in
+  // sixteens up to a workgroup a CU, above it in two sixteens that share the tokens (64 x 1,024 -> 1,024 3.3 and 3.7, 32 x 1,024
+  // -> 8,192 4.4 and 3.8), and no split past these borders: 64 x 4,096 -> 1,024 4.8 / 12.1, 64 x 1,024 -> 8,192 5.2 / 5.8, 256 x
+  // 1,024 -> 4,096 8.8 / 6.1; 16 x 1,024 -> 24,576 5.3 / 6.7, 32 x 1,024 -> 24,576 7.3 / 6.9; weights that no L2 holds for the
+  // second group of tokens, 64 x 8,192 -> 8,192, 27.2 / 21.5.
+  const int64_t groups = (a.M + 31) / 32, narrow = groups * ((a.N + 15) / 16), wide = groups * ((a.N + 31) / 32);
+  const int tokens = a.M <= 16 ? 16 : 32;
+  if (narrow <= cus) return tokens == 16 ? launch_few<T, 1, 1>(a, s) : launch_few<T, 2, 1>(a, s);
+  if (tokens == 16 && wide <= 3 * cus) return launch_few<T, 1, 2>(a, s);
+  if (a.M <= 32 ? 2 * wide <= 3 * cus : wide <= 2 * cus && a.N * a.K <= (32 << 20)) return launch_few<T, 2, 2>(a, s);
   static constexpr TileCost kTiles[4] = {{256, 256, 5.5f, 1.15f, 1.72f},
                                          {128, 128, 1.2f, 0.50f, 0.72f},
                                          {64, 128, 1.3f, 0.36f, 0.42f},

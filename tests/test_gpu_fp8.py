@@ -194,7 +194,11 @@ SHAPES = [(1, 1, 16), (1, 1024, 4096), (2, 7, 128), (16, 40, 144), (17, 129, 272
           # more than one tile of features a workgroup for few rows, and tiles for them; each tile shape, one and two
           # tiles a workgroup, one block of K
           (9, 6200, 144), (20, 6150, 272), (5, 12300, 128), (2000, 1000, 528), (2100, 2001, 528), (4000, 4001, 272),
-          (8100, 4090, 272), (4100, 4097, 80)]
+          (8100, 4090, 272), (4100, 4097, 80),
+          # few rows in groups of 32: features in sixteens and in two sixteens, long K, waves without a block, the last
+          # group of one token, past the split's borders
+          (64, 1024, 4096), (250, 500, 1552), (97, 2500, 272), (65, 8190, 144), (129, 1001, 16), (33, 40, 8208),
+          (30, 12288, 400), (16, 24570, 144), (15, 24577, 144), (65, 8193, 144)]
 
 
 @pytest.mark.parametrize("dtype", DT)
