@@ -456,6 +456,8 @@ extern "C" int atma_residual_rms_norm_fp8(const void* y, int64_t ldy, const floa
   if (M > 0 && (dtype == ATMA_BF16 || dtype == ATMA_F16) && (!weight || !out || !scale))
     return set_error(ATMA_ERR_INVALID, "residual_rms_norm_fp8: need weight, out, scale and exactly one of y / parts");
   if (D % 16) return set_error(ATMA_ERR_INVALID, "residual_rms_norm_fp8: D must be a multiple of 16 (got %lld)", (long long)D);
+  if (M > (1 << 25))  // a workgroup of 256 for four rows: a launch holds fewer than 2^32 threads
+    return set_error(ATMA_ERR_UNSUPPORTED, "residual_rms_norm_fp8: at most %d rows (got %lld)", 1 << 25, (long long)M);
   if (M > 0 && lds < (D + kFp8Block - 1) / kFp8Block)
     return set_error(ATMA_ERR_INVALID, "residual_rms_norm_fp8: rows of scales must hold %lld", (long long)((D + 127) / 128));
   return res_norm("residual_rms_norm_fp8", y, ldy, parts, n_parts, bias, n_bias, mu_x, ldmu, mu_w, mu_k, res, ldr, res_out,

@@ -2,9 +2,9 @@
 // a row and w (N, K) with a scale for each 128 x 128 block (fp8.h), and the MLP's first projection with its activation
 // formed from the fp32 sums, h = gate * relu(a)^2, and quantized in the epilogue.  No reference counterpart.
 //
-// Products: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction for each block of 128 along K.  Its scale operands carry
-// the blocks' power-of-two scales (lane l: row l % 16), so the accumulator holds scaled sums from the first product on and
-// no partial sum is ever rescaled.  Accumulators are fp32; inside the instruction the products of eight neighbouring k
+// Products: v_mfma_scale_f32_32x32x64_f8f6f4, two for each block of 128 along K (few rows: 16x16x128, one).  Its scale
+// operands carry the blocks' power-of-two scales, a lane its row's, so the accumulator holds scaled sums from the first product
+// on and no partial sum is ever rescaled.  Accumulators are fp32; inside the instruction the products of eight neighbouring k
 // are aligned to the largest of them and keep about 14 bits below it (measured: 2^2 beside 2^16 is lost), which is 1.4e-5
 // of the result for normally distributed values: far below the rounding to a 16-bit output, and the reason why there is
 // no fp32 output.  The order of k inside a block is free (one scale covers it), so a lane takes whichever 16-byte pieces

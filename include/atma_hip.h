@@ -614,7 +614,7 @@ int atma_residual_rms_norm(const void* y, int64_t ldy, const float* parts, int64
 /*
  * atma_residual_rms_norm with its norm in 8 bits: out (M, D) and scale (M, ceil(D / 128)) hold
  * s * rsqrt(mean(s^2) + eps) * weight, quantized from fp32.  Arguments as there; D a multiple of 16; rows of out
- * 8-byte aligned (ldo % 8 == 0, out 16-byte aligned).
+ * 8-byte aligned (ldo % 8 == 0, out 16-byte aligned); at most 2^25 rows.
  */
 int atma_residual_rms_norm_fp8(const void* y, int64_t ldy, const float* parts, int64_t n_parts,
                                const void* const* bias, int64_t n_bias, const void* mu_x, int64_t ldmu,
@@ -629,7 +629,8 @@ int atma_residual_rms_norm_fp8(const void* y, int64_t ldy, const float* parts, i
 int atma_quantize_fp8(const void* x, int64_t ldx, void* data, int64_t ldd, void* scale, int64_t lds, int64_t M,
                       int64_t K, int dtype, void* stream);
 
-/* A weight matrix to 8 bits: w (N, K) to data (N, K) and scale (ceil(N / 128), ceil(K / 128)); alignment as above. */
+/* A weight matrix to 8 bits: w (N, K) to data (N, K) and scale (ceil(N / 128), ceil(K / 128)); alignment as above; at
+ * most 65,535 blocks of rows. */
 int atma_quantize_weight_fp8(const void* w, int64_t ldw, void* data, int64_t ldd, void* scale, int64_t lds, int64_t N,
                              int64_t K, int dtype, void* stream);
 

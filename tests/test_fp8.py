@@ -93,6 +93,8 @@ def test_entry_points_validate_without_launch():
     assert lib.atma_residual_rms_norm_fp8(*n, ptr, 0, 2, 64, 1e-6, BF16, null) == 1
     assert lib.atma_residual_rms_norm_fp8(*n, ptr, 4, 2, 24, 1e-6, BF16, null) == 1
     assert lib.atma_residual_rms_norm_fp8(*n, ptr, 4, 2, 64, 1e-6, F32, null) == 2
+    assert lib.atma_residual_rms_norm_fp8(*n, ptr, 4, (1 << 25) + 1, 64, 1e-6, BF16, null) == 2
+    assert lib.atma_quantize_weight_fp8(ptr, 256, ptr, 256, ptr, 2, 65536 * 128, 256, BF16, null) == 2
 
     def linear(x=ptr, ldx=144, xs=ptr, ldxs=4, w=ptr, ldw=144, ws=ptr, ldws=4, bias=null, bt=F32, y=ptr, ldy=256, M=4, N=256,
                K=144, dt=BF16):

@@ -293,6 +293,22 @@ def test_products_at_other_layouts(dev, M):
     assert torch.equal(one, one[:1].expand_as(one))
 
 
+def test_quantize_more_rows_than_a_launch_holds(dev):
+    """67 million short rows: the rows at the seam of two launches and the last ones as in a call of their own."""
+    from atma_amd.kernel import quantize_fp8
+    M, seam = 67_108_900, 4 * (2 ** 24 - 1)
+    x = torch.zeros(M, 16, dtype=torch.bfloat16, device=dev)
+    parts = [slice(0, 7), slice(seam - 5, seam + 9), slice(M - 30, M)]
+    for i, p in enumerate(parts):
+        x[p] = _rows(p.stop - p.start, 16, i, torch.bfloat16).to(dev)
+    data, scale = quantize_fp8(x)
+    for p in parts:
+        d, s = quantize_fp8(x[p].clone())
+        assert torch.equal(data[p].view(torch.uint8), d.view(torch.uint8))
+        assert torch.equal(scale[p].view(torch.uint8), s.view(torch.uint8))
+    assert (scale.view(torch.uint8)[10:seam - 10] == 1).all()
+
+
 def test_one_row_at_any_stride(dev):
     """A single row whose row stride says nothing (expanded, shorter than the row): x, weight, residual, quantizer input."""
     from atma_amd.kernel import linear_fp8, quantize_fp8, quantize_weight_fp8, residual_rms_norm_fp8
