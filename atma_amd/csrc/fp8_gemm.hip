@@ -45,11 +45,24 @@ struct Fp8Args {
   int m_tiles, f_tiles, per_xcd;
 };
 
-__device__ __forceinline__ float bias_at(const Fp8Args& a, int64_t n) {
+// The biases of features n .. n + 3 as the words that hold them, read without a branch (nothing waits for them here) and
+// converted where they are added; features past the last of `rows` read as the last
+struct BiasWords {
+  uint32_t w[4];
+};
+__device__ __forceinline__ BiasWords bias_load(const Fp8Args& a, int64_t n, int64_t rows) {
+  const uint8_t* p = (const uint8_t*)(a.bias ? a.bias : a.w);
+  const int size = a.bias_dtype == ATMA_F32 ? 4 : 2;
+  BiasWords b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b.w[e] = *(const uint32_t*)(p + ((min(n + e, rows - 1) * size) & ~3ll));
+  return b;
+}
+__device__ __forceinline__ float bias_value(const Fp8Args& a, const BiasWords& b, int64_t n, int e) {
   if (!a.bias) return 0.f;
-  if (a.bias_dtype == ATMA_BF16) return to_f32(((const bf16*)a.bias)[n]);
-  if (a.bias_dtype == ATMA_F16) return to_f32(((const f16*)a.bias)[n]);
-  return ((const float*)a.bias)[n];
+  if (a.bias_dtype == ATMA_F32) return __builtin_bit_cast(float, b.w[e]);
+  const uint16_t v = (uint16_t)(b.w[e] >> (16 * ((n + e) & 1)));
+  return a.bias_dtype == ATMA_BF16 ? to_f32(__builtin_bit_cast(bf16, v)) : to_f32(__builtin_bit_cast(f16, v));
 }
 
 // relu(a)^2 * gate in fp32 (v_maximum3_f32: NaN passes through, as torch's relu)
@@ -442,14 +455,14 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 // Few rows: latency, not bandwidth.  A workgroup owns FT tiles of 16 features x MT tiles of 16 tokens and its NW waves take the
 // blocks of K in turn, so a chain of K is NW times shorter; their sums are joined through LDS in a fixed order.  Each wave
 // has a ring of its own of NS blocks, filled by direct copies of whole 128-byte lines, and waits for nothing but its own
-// copies.  (Operands read from memory in the MFMA's layout, 16 rows to an instruction, come in at 11 bytes a cycle and CU, at
-// 17 with the halves of odd rows swapped; copied this way at 38: 64 x 16,384 -> 1,024 30.7, 20.6 and 10.5 us.)  Four waves of
-// two blocks measured best: more CU-wide copies in flight or more waves leave fewer workgroups a CU (32 x 1,024 -> 1,024,
-// 8 waves 3.7 us, 4 waves of four blocks 3.6, of two 3.2).
+// copies.  Operands read from memory in the MFMA's layout, 16 rows to an instruction, come in at 28 GB/s a CU, at 46 with
+// the halves of odd rows swapped, copied this way at 104 (64 x 16,384 -> 1,024 30.7, 20.6 and 10.5 us).  The bias is read
+// ahead of the sums (0.25 to 0.3 us).  Four waves of two blocks measured best: more waves or more copies in flight leave fewer
+// workgroups a CU (32 x 1,024 -> 1,024, 8 waves 3.7 us, 4 waves of four blocks 3.6, of two 3.2).
 template <typename T, int MT, int FT, int NW, int NS>
 __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   constexpr int ROWS = 16 * (FT + MT), STAGE = ROWS * kFp8Block + 256, COPIES = ROWS / 8;
-  static_assert(FT * MT * 1024 <= NS * STAGE && 16 * MT < 64 && kFp8Block % (16 * FT) == 0,
+  static_assert(FT * MT <= NW && FT * MT * 1024 <= NS * STAGE && 16 * MT < 64 && kFp8Block % (16 * FT) == 0,
                 "the sums fit the ring, a lane is left for the weights' scale, one block of weight rows");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * NS * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -476,6 +489,10 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   };
 #pragma unroll
   for (int i = 0; i < NS; ++i) copies(wave + i * NW, i);
+  // the output tile that the wave joins
+  const int ot = wave / MT, oj = wave % MT;
+  const int64_t n0 = f0 + 16 * ot + 4 * g, m = m0 + 16 * oj + r;
+  const BiasWords bias = bias_load(a, n0, a.N);
   f32x4 acc[FT][MT] = {};
   int slot = 0;
   for (int kk = wave; kk < a.nk; kk += NW) {
@@ -511,28 +528,110 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) red[wave][t][j][lane] = acc[t][j];
   __syncthreads();
+  if (wave >= FT * MT || m >= a.M) return;
+  f32x4 s = red[0][ot][oj][lane];
 #pragma unroll
-  for (int i0 = 0; i0 < FT * MT; i0 += NW) {
-    const int i = i0 + wave;
-    if (i >= FT * MT) break;
-    const int t = i / MT, j = i % MT;
-    f32x4 s = red[0][t][j][lane];
+  for (int q = 1; q < NW; ++q) s += red[q][ot][oj][lane];
+  T* y = (T*)a.y + m * a.ldy + n0;
+  float v[4];
 #pragma unroll
-    for (int q = 1; q < NW; ++q) s += red[q][t][j][lane];
-    const int64_t n0 = f0 + 16 * t + 4 * g, m = m0 + 16 * j + r;
-    if (m >= a.M) continue;
-    T* y = (T*)a.y + m * a.ldy + n0;
-    float v[4];
+  for (int e = 0; e < 4; ++e) v[e] = s[e] + bias_value(a, bias, n0, e);
+  if (n0 + 4 <= a.N && a.ldy % 8 == 0) {
+    *(u32x2*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+  } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = s[e] + (n0 + e < a.N ? bias_at(a, n0 + e) : 0.f);
-    if (n0 + 4 <= a.N && a.ldy % 8 == 0) {
-      *(u32x2*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
-    } else {
+    for (int e = 0; e < 4; ++e)
+      if (n0 + e < a.N) y[e] = from_f32<T>(v[e]);
+  }
+}
+
+// Few rows of the gated form: a workgroup owns one block of 128 output features, whose scale stays inside, x 16 tokens.  Each of
+// its eight waves has 16 features, the a rows and the gate rows, all of K through a ring of the wave's own; the tokens come in
+// once, all of K, before the first block.  Bound by the 32 KiB of weights a block that one CU takes in (0.25 us: 62 bytes a
+// cycle) behind 3.2 us of launch, first copies and epilogue: us for 16 x 1,024 -> 4,096 and 16 x 4,096 -> 1,024, the 64-token
+// tile 7.8 and 18.3, tokens in each wave's ring 6.9 and 17.0, this 5.4 and 11.2 (5.8 and 11.6 with the bias read at the end).
+constexpr int kGatedFewBlocks = 36;  // of K, that LDS holds
+__global__ void __launch_bounds__(512) fp8_gated_few_kernel(Fp8Args a) {
+  constexpr int NS = 2, STAGE = 32 * kFp8Block, XB = 16 * kFp8Block + 256;  // a block of tokens, then its scales in words
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * NS * STAGE + kGatedFewBlocks * XB];
+  __shared__ float part[8][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int64_t f0 = (int64_t)blockIdx.x * kFp8Block, m0 = (int64_t)blockIdx.y * 16, fb = blockIdx.x;
+  const uint32_t wb = (uint32_t)(kFp8Block * a.ldw);
+  const __amdgpu_buffer_rsrc_t ar = buffer_rsrc(a.w + f0 * a.ldw, wb), gr = buffer_rsrc(a.w + (a.N + f0) * a.ldw, wb);
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc(a.x + m0 * a.ldx, (uint32_t)(min((int64_t)16, a.M - m0) * a.ldx));
+  // copies move 8 rows of 128 bytes as in fp8_few_kernel
+  const int crow = lane >> 3, chunk = 16 * ((lane & 7) ^ (crow >> 1));
+  const uint32_t wv0 = (uint32_t)(16 * wave + crow) * (uint32_t)a.ldw, xv0 = (uint32_t)crow * (uint32_t)a.ldx;
+  const uint8_t* xs = lds + 8 * NS * STAGE;
+  const uint32_t xs0 = lds_offset(xs);
+  const uint8_t* scales = lane < 32 ? a.xs + min(m0 + r, a.M - 1) * a.ldxs
+                                    : a.ws + (lane == 33 ? fb + a.N / kFp8Block : fb) * a.ldws;
+  for (int kk = wave; kk < a.nk; kk += 8) {
+    const uint32_t d = xs0 + kk * XB;
+    dma_load1_at(scales + kk, d + 16 * kFp8Block);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n0 + e < a.N) y[e] = from_f32<T>(v[e]);
+    for (int i = 0; i < 2; ++i) {
+      const int k = kk * kFp8Block + (chunk ^ (64 * i));
+      dma_buf16_at(xr, k < a.K ? xv0 + 8u * i * (uint32_t)a.ldx + (uint32_t)k : 0x80000000u, 0u, d + 1024 * i);
     }
   }
+  const uint8_t* ring = lds + wave * NS * STAGE;
+  const uint32_t ring0 = lds_offset(ring);
+  auto copies = [&](int kk, int slot) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = kk * kFp8Block + (chunk ^ (i % 2 * 64));
+      dma_buf16_at(i < 2 ? ar : gr, k < a.K ? wv0 + 8u * (i % 2) * (uint32_t)a.ldw + (uint32_t)k : 0x80000000u, 0u,
+                   ring0 + slot * STAGE + 1024 * i);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NS; ++i) copies(i, i);
+  wait_vmcnt<4 * NS>();
+  lds_barrier();  // the tokens are there, from every wave
+  const int64_t n0 = f0 + 16 * wave + 4 * g, m = m0 + r;
+  const BiasWords ba = bias_load(a, n0, 2 * a.N), bg = bias_load(a, a.N + n0, 2 * a.N);
+  f32x4 acc[2] = {};
+  int slot = 0;
+  for (int kk = 0; kk < a.nk; ++kk) {
+    wait_vmcnt<4 * (NS - 1)>();
+    const uint8_t *wp = ring + slot * STAGE, *xp = xs + kk * XB;
+    Frag8 wv[2], xv;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int at = r * kFp8Block + 16 * ((4 * q + g) ^ x_swizzle(r));
+#pragma unroll
+      for (int t = 0; t < 2; ++t) wv[t].q[q] = *(const u32x4*)(wp + 2048 * t + at);
+      xv.q[q] = *(const u32x4*)(xp + at);
+    }
+    const int* sc = (const int*)(xp + 16 * kFp8Block);
+    const int xsc = sc[r], wsc[2] = {sc[32], sc[33]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the copies that overwrite them start
+    copies(kk + NS, slot);
+    slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) acc[t] = mfma_fp8(wv[t], xv, acc[t], wsc[t], xsc);
+  }
+  wait_vmcnt<0>();  // no copy outlives its workgroup's LDS
+  f32x4 h;
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = gate_act(acc[0][e] + bias_value(a, ba, n0, e), acc[1][e] + bias_value(a, bg, n0, e));
+    top = fmaxf(top, finite_abs(h[e]));
+  }
+  top = fmaxf(top, wave_xor(top, 16));
+  top = fmaxf(top, wave_xor(top, 32));
+  if (g == 0) part[wave][r] = top;
+  lds_barrier();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) top = fmaxf(top, part[q][r]);
+  const int code = fp8_scale_code(top);
+  if (m >= a.M) return;
+  if (wave == 0 && g == 0) a.ys[m * a.ldys + fb] = (uint8_t)code;
+  *(uint32_t*)((uint8_t*)a.y + m * a.ldy + n0) = fp8_scaled4(h[0], h[1], h[2], h[3], fp8_scale(code));
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -601,7 +700,7 @@ static void launch_few(const Fp8Args& a, hipStream_t s) {
 template <typename T>
 static void launch_linear(const Fp8Args& a, hipStream_t s) {
   const int64_t cus = device_cu_count();
-  // Few rows, while the split over K is what fills the card (us, split kernel / tiles; x = rows x K -> features).  Features in
+  // Few rows, while the split over K is what fills the card (us, split kernel / tiles, without bias; rows x K -> features).  Features in
   // sixteens up to a workgroup a CU, above it in two sixteens that share the tokens (64 x 1,024 -> 1,024 3.3 and 3.7, 32 x 1,024
   // -> 8,192 4.4 and 3.8), and no split past these borders: 64 x 4,096 -> 1,024 4.8 / 12.1, 64 x 1,024 -> 8,192 5.2 / 5.8, 256 x
   // 1,024 -> 4,096 8.8 / 6.1; 16 x 1,024 -> 24,576 5.3 / 6.7, 32 x 1,024 -> 24,576 7.3 / 6.9; weights that no L2 holds for the
@@ -624,6 +723,13 @@ static void launch_linear(const Fp8Args& a, hipStream_t s) {
 }
 
 static void launch_gated(const Fp8Args& a, hipStream_t s) {
+  // Few rows: while a workgroup for every 16 tokens leaves none without a CU (us, split kernel / tiles; H 4,096, K 1,024: 128
+  // rows 5.9 / 8.2, 256 rows, two a CU, 10.3 / 8.3; H 8,192, K 4,096, 64 rows 15.7 / 20.2) and LDS holds their K
+  const int64_t blocks = a.N / kFp8Block, groups = (a.M + 15) / 16;
+  if (blocks * groups <= device_cu_count() && a.nk <= kGatedFewBlocks) {
+    fp8_gated_few_kernel<<<dim3((unsigned)blocks, (unsigned)groups), dim3(512), 0, s>>>(a);
+    return;
+  }
   static constexpr TileCost kTiles[3] = {{128, 256, 5.0f, 1.00f, 1.60f},
                                          {128, 128, 1.7f, 0.70f, 0.98f},
                                          {128, 64, 1.3f, 0.53f, 0.63f}};

@@ -218,7 +218,11 @@ def test_linear(dev, M, N, K, dtype):
 @pytest.mark.parametrize("M,H,K", [(1, 128, 16), (1, 4096, 1024), (9, 256, 144), (16, 384, 1040), (32, 128, 2048),
                                    (33, 128, 128), (64, 256, 272), (100, 640, 1024), (129, 128, 384), (300, 512, 640),
                                    (2001, 1024, 272), (770, 4096, 144), (4201, 2048, 144), (4090, 2048, 912),
-                                   (8190, 2048, 912)])
+                                   (8190, 2048, 912),
+                                   # few rows: all of K in LDS and one block more, the last group of one token, the
+                                   # largest grid and past it
+                                   (3, 256, 4608), (17, 256, 4624), (128, 4096, 80), (129, 4096, 80), (500, 1024, 272),
+                                   (1, 32896, 144)])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 def test_linear_gated(dev, M, H, K, bias):
     from atma_amd.kernel import linear_gated_fp8
