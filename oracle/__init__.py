@@ -12,7 +12,9 @@ algorithm of the four hot-path operations the HIP library implements:
 * the paged KV write ``store_kvcache`` -- ``oracle.kvcache``;
 * one global block (Polar + memory + MLP) for the CPU baseline -- ``oracle.block``;
 * the inference fusions (``squared_relu_gate``, ``softcap_logits``,
-  ``packed_causal_conv1d``) -- ``oracle.inference_ops``.
+  ``packed_causal_conv1d``) -- ``oracle.inference_ops``;
+* the 8-bit format, its quantizers, norm and products (no reference counterpart) --
+  ``oracle.fp8``.
 
 Every function cites the reference file:line it follows (paths relative to the
 akbar2habibullah/atma repository root).
