@@ -65,6 +65,21 @@ __device__ __forceinline__ float bias_value(const Fp8Args& a, const BiasWords& b
   return a.bias_dtype == ATMA_BF16 ? to_f32(__builtin_bit_cast(bf16, v)) : to_f32(__builtin_bit_cast(f16, v));
 }
 
+// Outputs n0 .. n0 + 7 of a row that ends at N.  Rows of odd widths start at any element: the vector stores take any address
+// (elements one by one cost 184 us instead of 109 at 28,106 x 1,712 -> 1,557); whole: the
+// tile has every feature
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+__device__ __forceinline__ void store_out8(uint16_t* y, const u32x4& o, bool whole, int64_t n0, int64_t N) {
+  if (whole || n0 + 8 <= N) {
+    *(u32x4_any*)y = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n0 + e < N) y[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
 // relu(a)^2 * gate in fp32 (v_maximum3_f32: NaN passes through, as torch's relu)
 __device__ __forceinline__ float gate_act(float av, float gv) {
   const float pos = __builtin_elementwise_maximum(av, 0.f);
@@ -343,7 +358,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
     // ---- epilogue of tile (m0, f0): token 32 (TM wm + j) + r, 16 consecutive features a tile
     LateArgs p = late_args();
     if constexpr (!GATED) {
-      const bool whole = f0 + C::OF <= p->N && p->ldy % 8 == 0;
+      const bool whole = f0 + C::OF <= p->N;  // every feature of the tile
       if constexpr (C::TURNED) {
         // through LDS, a wave its own 2 KiB: 32 tokens x 32 features at a time turn from a token a lane to 64-byte pieces, four
         // lanes each (chunk c of row r at position c ^ (r / 4) % 4): a CU alone stores 80 bytes a cycle so, 28 as they lie
@@ -367,16 +382,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
               const int row = 16 * i + (lane >> 2);
               const u32x4 o = *(const u32x4*)(turn + 64 * row + 16 * ((lane & 3) ^ ((row >> 2) & 3)));
               const int64_t m = m0 + 32 * (TM * wm + j) + row, n0 = f0 + wrow0 + 32 * t + 8 * (lane & 3);
-              T* y = (T*)p->y + m * ldy + n0;
-              if (m < M) {
-                if (whole) {
-                  *(u32x4*)y = o;
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 8; ++e)
-                    if (n0 + e < N) y[e] = __builtin_bit_cast(T, (uint16_t)(o[e >> 1] >> (16 * (e & 1))));
-                }
-              }
+              if (m < M) store_out8((uint16_t*)p->y + m * ldy + n0, o, whole, n0, N);
             }
           }
         }
@@ -388,18 +394,13 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
 #pragma unroll
             for (int t = 0; t < TF; ++t) {
               const int64_t n0 = f0 + wrow0 + 32 * t + 16 * h;
-              T* y = (T*)p->y + m * p->ldy + n0;
               const f32x16& v = acc[t][j];
-              if (whole) {
 #pragma unroll
-                for (int e = 0; e < 16; e += 8)
-                  *(u32x4*)(y + e) = u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]),
-                                           pack2<T>(v[e + 4], v[e + 5]), pack2<T>(v[e + 6], v[e + 7])};
-              } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  if (n0 + e < p->N) y[e] = from_f32<T>(v[e]);
-              }
+              for (int e = 0; e < 16; e += 8)
+                store_out8((uint16_t*)p->y + m * p->ldy + n0 + e,
+                           u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]), pack2<T>(v[e + 4], v[e + 5]),
+                                 pack2<T>(v[e + 6], v[e + 7])},
+                           whole, n0 + e, p->N);
             }
           }
         }
@@ -536,8 +537,8 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = s[e] + bias_value(a, bias, n0, e);
-  if (n0 + 4 <= a.N && a.ldy % 8 == 0) {
-    *(u32x2*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+  if (n0 + 4 <= a.N) {
+    *(u32x2_any*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
