@@ -169,7 +169,8 @@ class AtmaDecoderBlock(nn.Module):
         additions are the eager block's, in the same dtype, so the stream's values are
         unchanged.  Returns (mlp branch, stream).  An MLP in 8 bits takes its rows quantized by the norm before it."""
         h, residual = self.norm1.add_norm(branch, residual)
-        if plain_module(self.mlp, Fp8MLP) and plain_module(self.norm2, RMSNorm):
+        if (plain_module(self.mlp, Fp8MLP) and plain_module(self.norm2, RMSNorm)
+                and self.norm2.weight.shape[0] <= 4096):  # the fused norm's widest row
             data, scale, residual = self.norm2.add_norm_fp8(self.attn(h, defer=True), residual)
             return self.mlp.forward_fp8(data, scale, residual.dtype), residual
         h, residual = self.norm2.add_norm(self.attn(h, defer=True), residual)

@@ -103,7 +103,10 @@ def residual_rms_norm_fp8(branch, residual, weight, eps):
         raise ValueError(f"{what}: the low-rank term takes mu_x (M, k) and mu_w (D, k), k 4, 8 or 16")
     keep = residual is not None or src is not branch
     straight = _placed(what, src, residual, weight, mu_x, mu_w, *biases)
-    if straight and mu_x is None and not weight.data_ptr() & 15 and weight.is_contiguous()             and (_aligned_rows(y) if parts is None else parts.is_contiguous() and not parts.data_ptr() & 15)             and (residual is None or _aligned_rows(residual))             and all(b.stride(0) == 1 and not b.data_ptr() & 15 for b in biases):
+    if (straight and mu_x is None and not weight.data_ptr() & 15 and weight.is_contiguous()
+            and (_aligned_rows(y) if parts is None else parts.is_contiguous() and not parts.data_ptr() & 15)
+            and (residual is None or _aligned_rows(residual))
+            and all(b.stride(0) == 1 and not b.data_ptr() & 15 for b in biases)):
         out = _ops.fp8_norm(y, parts, biases, None, None, residual, weight, float(eps), keep)
     else:
         out = _ops.run.residual_rms_norm_fp8(y, parts, biases, mu_x, mu_w, residual, weight, float(eps), keep)

@@ -537,6 +537,25 @@ def test_block_stream_takes_the_fused_norm(dev):
             assert ((out.cpu().double() - exact).norm() / exact.norm()).item() <= 4 * 0.026
 
 
+def test_block_wider_than_the_fused_norm(dev):
+    """Rows of more than 4,096 are normed by the module and quantized by the MLP."""
+    from atma_amd.engine import AtmaConfig
+    from atma_amd.engine.model import AtmaDecoderBlock
+    from atma_amd.layers.global_attention import Fp8MLP
+    D = 4160
+    with torch.device(dev), torch.no_grad():
+        block = AtmaDecoderBlock(0, AtmaConfig(vocab_size=64, num_hidden_layers=1, hidden_size=D, head_dim=64)).bfloat16()
+        block.mlp = Fp8MLP(block.mlp)
+        block.norm1.weight.fill_(1), block.norm2.weight.fill_(1)
+        block.attn = torch.nn.Identity()
+        block.attn.forward = lambda h, defer=False: h
+        x, res = (torch.randn(5, D, generator=_g(i), device="cpu").bfloat16().to(dev) for i in (1, 2))
+        y, s = block.forward_stream(x, res)
+        h, s1 = block.norm1.add_norm(x, res)
+        h, s2 = block.norm2.add_norm(h, s1)
+        assert torch.equal(s, s2) and torch.equal(y, block.mlp(h))
+
+
 def test_engine_with_8_bit_mlps(dev):
     """A greedy generation with ``Config.fp8_mlp``: every prefill and decode step near the whole-model oracle on the 8-bit
     weights' values.  Each of the four blocks' MLP branches is off by 4 * 0.026 of itself at most (above) and no larger than
