@@ -965,6 +965,14 @@ def _rows_apart(t: Tensor) -> Tensor:
     return _rows16(t if t.stride(0) >= t.shape[1] else t.clone(memory_format=torch.contiguous_format))
 
 
+FP8_PITCH = 1 << 23   # the products address the rows of a tile by 32-bit offsets: the furthest apart that rows may start
+
+
+def _rows_near(t: Tensor) -> Tensor:
+    """``_rows_apart`` for the products' x and weight: rows that start further than ``FP8_PITCH`` apart are copied."""
+    return _rows_apart(t if t.stride(0) <= FP8_PITCH else t.clone(memory_format=torch.contiguous_format))
+
+
 def _fp8_scales(t: Tensor) -> Tensor:
     return t if t.stride(1) == 1 else t.contiguous()
 
@@ -1068,7 +1076,7 @@ def linear_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tens
                   out_dtype: torch.dtype) -> Tensor:
     _need_cuda(x, x_scale, weight, weight_scale, bias)
     with _lib.on_device(x.device):
-        return fp8_linear(_rows_apart(x), _fp8_scales(x_scale), _rows_apart(weight), _fp8_scales(weight_scale), _bias4(bias),
+        return fp8_linear(_rows_near(x), _fp8_scales(x_scale), _rows_near(weight), _fp8_scales(weight_scale), _bias4(bias),
                           out_dtype)
 
 
@@ -1095,7 +1103,7 @@ def linear_gated_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale
                         bias: Optional[Tensor]) -> List[Tensor]:
     _need_cuda(x, x_scale, weight, weight_scale, bias)
     with _lib.on_device(x.device):
-        return list(fp8_linear_gated(_rows_apart(x), _fp8_scales(x_scale), _rows_apart(weight), _fp8_scales(weight_scale),
+        return list(fp8_linear_gated(_rows_near(x), _fp8_scales(x_scale), _rows_near(weight), _fp8_scales(weight_scale),
                                      _bias4(bias)))
 
 

@@ -648,13 +648,15 @@ static void launch_tiles(Fp8Args a, hipStream_t s) {
   fp8_tile_kernel<T, TF, TM, WF, WM, NS, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
 }
 
-// Checks shared by the products; rows: weight rows (N, or 2 N gated)
-static int check_fp8(const char* what, const Fp8Args& a, int64_t rows) {
+// Checks shared by the products; rows: weight rows (N, or 2 N gated).  The stride of a single row means nothing: K stands for it
+static int check_fp8(const char* what, Fp8Args& a, int64_t rows) {
   if (a.M < 0 || a.N < 1 || a.K < 16 || a.K % 16 || a.K > (1 << 22) || a.M > (1 << 30) || rows > (1 << 28))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: unsupported shape M=%lld N=%lld K=%d (K a multiple of 16)", what,
                      (long long)a.M, (long long)a.N, a.K);
   if (a.M == 0) return ATMA_OK;
   if (!a.x || !a.xs || !a.w || !a.ws || !a.y) return set_error(ATMA_ERR_INVALID, "%s: null pointer", what);
+  if (a.M == 1) a.ldx = a.K;
+  if (rows == 1) a.ldw = a.K;
   if ((uintptr_t)a.x % 16 || a.ldx % 16 || a.ldx < a.K || (uintptr_t)a.w % 16 || a.ldw % 16 || a.ldw < a.K)
     return set_error(ATMA_ERR_INVALID, "%s: rows of x and w must be 16-byte aligned and at least K long", what);
   if (a.ldxs < 0 || a.ldws < 0) return set_error(ATMA_ERR_INVALID, "%s: negative stride of scales", what);

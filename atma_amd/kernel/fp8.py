@@ -21,6 +21,7 @@ from .decode_fusions import PartialSums
 _DT = (torch.bfloat16, torch.float16)
 _DT32 = (torch.bfloat16, torch.float16, torch.float32)
 FP8, FP8_SCALE, FP8_BLOCK = _ops.FP8, _ops.FP8_SCALE, _ops.FP8_BLOCK
+_PITCH = _ops.FP8_PITCH
 _Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
 _grad_enabled, _function_modes = torch.is_grad_enabled, torch._C._len_torch_function_stack
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
@@ -133,7 +134,7 @@ def _operands(what, x, x_scale, weight, weight_scale, bias):
     if not _placed(what, x, x_scale, weight, weight_scale, bias):
         return False
     (ldx, ix), (ldw, iw) = x.stride(), weight.stride()
-    return (ix == iw == x_scale.stride(1) == weight_scale.stride(1) == 1 and ldx >= K and ldw >= K
+    return (ix == iw == x_scale.stride(1) == weight_scale.stride(1) == 1 and K <= ldx <= _PITCH and K <= ldw <= _PITCH
             and not (x.data_ptr() | weight.data_ptr() | ldx | ldw) & 15
             and (bias is None or (bias.stride(0) == 1 and not bias.data_ptr() & 3)))
 

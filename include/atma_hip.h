@@ -637,8 +637,9 @@ int atma_quantize_weight_fp8(const void* w, int64_t ldw, void* data, int64_t ldd
 /*
  * y[m, n] = round(sum_k x[m, k] w[n, k] + bias[n]) in `dtype` (16-bit) for 8-bit x (M, K) with scales xs (M, nb) and
  * 8-bit w (N, K) with scales ws (ceil(N / 128), nb), nb = ceil(K / 128); bias (N,) in `bias_dtype` or NULL.  K a multiple
- * of 16; rows of x and w 16-byte aligned, scales anywhere; bias 4-byte aligned and read in words of 4 bytes (the one that
- * holds its last value is read whole); y 16-byte aligned where ldy % 8 == 0.
+ * of 16, at most 2^22; M at most 2^30, N at most 2^28.  Rows of x and w 16-byte aligned and at most 8 MiB apart (the stride
+ * of a single row is not used), scales anywhere; bias 4-byte aligned and read in words of 4 bytes (the one that holds its
+ * last value is read whole); y 16-byte aligned where ldy % 8 == 0.
  */
 int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw, const void* ws,
                     int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, int64_t M, int64_t N,
@@ -647,7 +648,8 @@ int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, co
 /*
  * The MLP's first projection with its activation, 8 bits in and out (atma_linear_gated's shape: w (2H, K), the a rows,
  * then the gate rows; bias (2H,) or NULL): y (M, H) with scales ys (M, H / 128) hold gate * relu(a)^2 for the fp32 sums
- * a and gate, quantized once.  H a multiple of 128; x, xs, w, ws and K as atma_linear_fp8; rows of y 16-byte aligned.
+ * a and gate, quantized once.  H a multiple of 128, at most 2^27; x, xs, w, ws, M and K as atma_linear_fp8; rows of y
+ * 16-byte aligned.
  */
 int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw,
                           const void* ws, int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, void* ys,
