@@ -220,10 +220,13 @@ class Atma(nn.Module):
         return softcap_logits(logits), None
 
     def quantize_mlps(self):
-        """Replace every block's MLP by its 8-bit form (``Fp8MLP``), for inference; the weights must be on the GPU."""
-        for block in self.blocks:
-            if not isinstance(block.mlp, Fp8MLP):
-                block.mlp = Fp8MLP(block.mlp)
+        """Replace every block's MLP by its 8-bit form (``Fp8MLP``), for inference; the weights must be on the GPU.  An MLP
+        that ``Fp8MLP`` does not stand for (changed, or of unsuited widths) is refused before any is replaced."""
+        blocks = [block for block in self.blocks if not isinstance(block.mlp, Fp8MLP)]
+        for block in blocks:
+            Fp8MLP.check(block.mlp)
+        for block in blocks:
+            block.mlp = Fp8MLP(block.mlp)
         return self
 
     def init_weights(self, std=0.02, seed=0):

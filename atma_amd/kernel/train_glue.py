@@ -21,14 +21,15 @@ _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _any_global_hook = torch.nn.modules.module._has_any_global_hook
 
 
-def plain_module(m, cls):
+def plain_module(m, cls, every=True):
     """``m`` is a ``cls`` itself (no subclass, no parametrisation, no ``forward`` of its own) and nothing hooks into its
-    calls, or into every module's: a fused call may stand in for it."""
+    calls, or into every module's: a fused call may stand in for it.  ``every`` False: hooks on every module do not matter,
+    since another module takes its place and they see that one's calls."""
     if type(m) is not cls:
         return False
     own = m.__dict__
     return not (own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"] or own["_backward_pre_hooks"]
-                or "forward" in own or _any_global_hook())
+                or "forward" in own or (every and _any_global_hook()))
 
 
 def train_glue_served(x, *params):

@@ -765,10 +765,23 @@ class Fp8MLP(nn.Module):
     are held as bytes (a module's ``half()`` or ``to(dtype)`` leaves them alone), half of the 16-bit MLP's memory.  The
     output is in the 16-bit type of the activations."""
 
-    def __init__(self, mlp):
-        super().__init__()
+    @staticmethod
+    def check(mlp):
+        """Raises where ``mlp`` has no 8-bit form: unsuited widths, or more to it than its weights and biases (a subclass,
+        a ``forward``, hook or parametrisation of its own, on the MLP or one of its projections)."""
+        if not plain_module(mlp, MLP, every=False):
+            raise ValueError("Fp8MLP is made from an MLP without hooks, parametrisations or a forward of its own "
+                             f"(got {type(mlp).__name__})")
+        for name, linear in (("fc", mlp.fc), ("proj", mlp.proj)):
+            if not any(plain_module(linear, cls, every=False) for cls in (Linear, nn.Linear)):
+                raise ValueError("Fp8MLP is made from plain Linear projections, without hooks, parametrisations or a forward "
+                                 f"of their own (got {type(linear).__name__} for {name})")
         if mlp.fc.weight.shape[0] % 256 or mlp.fc.weight.shape[1] % 16:
             raise ValueError(f"Fp8MLP: hidden sizes are multiples of 128, the width of 16 (got {tuple(mlp.fc.weight.shape)})")
+
+    def __init__(self, mlp):
+        super().__init__()
+        self.check(mlp)
         with torch.no_grad():
             for name, linear in (("fc", mlp.fc), ("proj", mlp.proj)):
                 data, scale = quantize_weight_fp8(linear.weight)
