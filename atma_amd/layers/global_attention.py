@@ -782,6 +782,7 @@ class Fp8MLP(nn.Module):
     def __init__(self, mlp):
         super().__init__()
         self.check(mlp)
+        self.train(mlp.training)
         with torch.no_grad():
             for name, linear in (("fc", mlp.fc), ("proj", mlp.proj)):
                 data, scale = quantize_weight_fp8(linear.weight)

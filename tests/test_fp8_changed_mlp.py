@@ -97,3 +97,11 @@ def test_nothing_is_replaced_beside_a_refused_mlp(monkeypatch):
     handle.remove()
     model.quantize_mlps()
     assert made == before and all(type(b.mlp) is Stand for b in model.blocks)
+
+
+@pytest.mark.parametrize("training", [True, False])
+def test_mode_is_kept(monkeypatch, training):
+    """A model in ``eval()`` stays in it."""
+    from atma_amd.layers import global_attention as G
+    monkeypatch.setattr(G, "quantize_weight_fp8", lambda w: (w.detach().byte(), w.detach().byte()))
+    assert Fp8MLP(MLP(32).train(training)).training is training
