@@ -45,24 +45,31 @@ struct Fp8Args {
   int m_tiles, f_tiles, per_xcd;
 };
 
-// The biases of features n .. n + 3 as the words that hold them, read without a branch (nothing waits for them here) and
-// converted where they are added; features past the last of `rows` read as the last
-struct BiasWords {
+// The biases of features n .. n + 3 as their bits, in loads of their own size (nothing behind the last of `rows` is read;
+// features past it read as the last), converted where they are added: nothing waits for them here
+struct BiasBits {
   uint32_t w[4];
+  uint16_t v[4];
 };
-__device__ __forceinline__ BiasWords bias_load(const Fp8Args& a, int64_t n, int64_t rows) {
-  const uint8_t* p = (const uint8_t*)(a.bias ? a.bias : a.w);
-  const int size = a.bias_dtype == ATMA_F32 ? 4 : 2;
-  BiasWords b;
+__device__ __forceinline__ BiasBits bias_load(const Fp8Args& a, int64_t n, int64_t rows) {
+  const void* p = a.bias ? a.bias : a.w;
+  BiasBits b;
+  if (a.bias_dtype == ATMA_F32) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) b.w[e] = *(const uint32_t*)(p + ((min(n + e, rows - 1) * size) & ~3ll));
+    for (int e = 0; e < 4; ++e) b.w[e] = ((const uint32_t*)p)[min(n + e, rows - 1)];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b.v[e] = ((const uint16_t*)p)[min(n + e, rows - 1)];
+  }
   return b;
 }
-__device__ __forceinline__ float bias_value(const Fp8Args& a, const BiasWords& b, int64_t n, int e) {
-  if (!a.bias) return 0.f;
-  if (a.bias_dtype == ATMA_F32) return __builtin_bit_cast(float, b.w[e]);
-  const uint16_t v = (uint16_t)(b.w[e] >> (16 * ((n + e) & 1)));
-  return a.bias_dtype == ATMA_BF16 ? to_f32(__builtin_bit_cast(bf16, v)) : to_f32(__builtin_bit_cast(f16, v));
+__device__ __forceinline__ float bias_f32(int dtype, uint32_t bits) {
+  if (dtype == ATMA_F32) return __builtin_bit_cast(float, bits);
+  const uint16_t v = (uint16_t)bits;
+  return dtype == ATMA_BF16 ? to_f32(__builtin_bit_cast(bf16, v)) : to_f32(__builtin_bit_cast(f16, v));
+}
+__device__ __forceinline__ float bias_value(const Fp8Args& a, const BiasBits& b, int e) {
+  return a.bias ? bias_f32(a.bias_dtype, a.bias_dtype == ATMA_F32 ? b.w[e] : b.v[e]) : 0.f;
 }
 
 // Outputs n0 .. n0 + 7 of a row that ends at N.  Rows of odd widths start at any element: the vector stores take any address
@@ -200,14 +207,14 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
     scales = lane == 32 || lane == 33 ? p->ws + b * p->ldws : p->xs + m * p->ldxs;
     plimit = p->K;
     if (p->bias && wave == 2) {
-      // the tile's biases (gated: 128 of a, 128 of gate), in words, to its slot
+      // the tile's biases (gated: 128 of a, 128 of gate), in whole words, to its slot
       const int size = p->bias_dtype == ATMA_F32 ? 4 : 2;
       const int64_t total = (GATED ? 2 : 1) * p->N * size;
-      const __amdgpu_buffer_rsrc_t br = buffer_rsrc(p->bias, (uint32_t)((total + 3) & ~3ll));
+      const __amdgpu_buffer_rsrc_t br = buffer_rsrc(p->bias, (uint32_t)total);
       for (int i = 0; i < size; ++i) {
         const int f = (64 * i + lane) * 4 / size;  // the word's first feature in the tile
         const int64_t n = tf0 + (GATED && f >= C::OF ? p->N + f - C::OF : f);
-        dma_buf4_rare(br, n * size < total ? (uint32_t)(n * size) : 0xfffffffcu,
+        dma_buf4_rare(br, n * size + 4 <= total ? (uint32_t)(n * size) : 0xfffffffcu,
                       lds0 + C::BIAS + 1024 * ptile + 256 * i);
       }
     }
@@ -291,6 +298,14 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
   read_scales();
   while (true) {
     // ---- the sums start from the bias
+    if constexpr (!GATED) {
+      // the last of an odd number in 16 bits is half a word, which no copy brings: every wave puts it beside the others
+      LateArgs p = late_args();
+      if (p->bias && p->bias_dtype != ATMA_F32 && p->N % 2 && f0 + C::OF >= p->N) {
+        *(uint16_t*)(lds + C::BIAS + 1024 * tile + 2 * (int)(p->N - 1 - f0)) = ((const uint16_t*)p->bias)[p->N - 1];
+        wave_sync();
+      }
+    }
 #pragma unroll
     for (int t = 0; t < TF; ++t) {
       float b[16] = {};
@@ -493,7 +508,7 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   // the output tile that the wave joins
   const int ot = wave / MT, oj = wave % MT;
   const int64_t n0 = f0 + 16 * ot + 4 * g, m = m0 + 16 * oj + r;
-  const BiasWords bias = bias_load(a, n0, a.N);
+  const BiasBits bias = bias_load(a, n0, a.N);
   f32x4 acc[FT][MT] = {};
   int slot = 0;
   for (int kk = wave; kk < a.nk; kk += NW) {
@@ -536,7 +551,7 @@ __global__ void __launch_bounds__(64 * NW) fp8_few_kernel(Fp8Args a) {
   T* y = (T*)a.y + m * a.ldy + n0;
   float v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = s[e] + bias_value(a, bias, n0, e);
+  for (int e = 0; e < 4; ++e) v[e] = s[e] + bias_value(a, bias, e);
   if (n0 + 4 <= a.N) {
     *(u32x2_any*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
   } else {
@@ -593,7 +608,7 @@ __global__ void __launch_bounds__(512) fp8_gated_few_kernel(Fp8Args a) {
   wait_vmcnt<4 * NS>();
   lds_barrier();  // the tokens are there, from every wave
   const int64_t n0 = f0 + 16 * wave + 4 * g, m = m0 + r;
-  const BiasWords ba = bias_load(a, n0, 2 * a.N), bg = bias_load(a, a.N + n0, 2 * a.N);
+  const BiasBits ba = bias_load(a, n0, 2 * a.N), bg = bias_load(a, a.N + n0, 2 * a.N);
   f32x4 acc[2] = {};
   int slot = 0;
   for (int kk = 0; kk < a.nk; ++kk) {
@@ -620,7 +635,7 @@ __global__ void __launch_bounds__(512) fp8_gated_few_kernel(Fp8Args a) {
   float top = 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    h[e] = gate_act(acc[0][e] + bias_value(a, ba, n0, e), acc[1][e] + bias_value(a, bg, n0, e));
+    h[e] = gate_act(acc[0][e] + bias_value(a, ba, e), acc[1][e] + bias_value(a, bg, e));
     top = fmaxf(top, finite_abs(h[e]));
   }
   top = fmaxf(top, wave_xor(top, 16));
