@@ -88,6 +88,8 @@ SIGNATURES = {
     "atma_linear_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _i32, _p]),
     "atma_linear_gated_fp8": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _p, _i64, _i64, _i64,
                                      _i64, _p]),
+    "atma_linear_fp8_form": (_i32, [_i64, _i64, _i64]),
+    "atma_linear_gated_fp8_form": (_i32, [_i64, _i64, _i64]),
     "atma_partial_sums": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_memory_gate_logits": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_polar_params_f32": (_i32, [_p] * 6 + [_i64, _i64, _i32, _p]),

@@ -715,8 +715,11 @@ static void launch_few(const Fp8Args& a, hipStream_t s) {
   fp8_few_kernel<T, MT, FT, NW, NS><<<grid, dim3(64 * NW), 0, s>>>(a);
 }
 
-template <typename T>
-static void launch_linear(const Fp8Args& a, hipStream_t s) {
+// The kernels of a product, in the order of the codes that atma_linear_fp8_form and atma_linear_gated_fp8_form return
+enum LinearForm { kFew16x16, kFew32x16, kFew16x32, kFew32x32, kTile256x256, kTile128x128, kTile64x128, kTile64x64 };
+enum GatedForm { kGatedFew, kGatedTile256, kGatedTile128, kGatedTile64 };
+
+static int linear_form(const Fp8Args& a) {
   const int64_t cus = device_cu_count();
   // Few rows, while the split over K is what fills the card (us, split kernel / tiles, without bias; rows x K -> features).  Features in
   // sixteens up to a workgroup a CU, above it in two sixteens that share the tokens (64 x 1,024 -> 1,024 3.3 and 3.7, 32 x 1,024
@@ -725,37 +728,61 @@ static void launch_linear(const Fp8Args& a, hipStream_t s) {
   // second group of tokens, 64 x 8,192 -> 8,192, 27.2 / 21.5.
   const int64_t groups = (a.M + 31) / 32, narrow = groups * ((a.N + 15) / 16), wide = groups * ((a.N + 31) / 32);
   const int tokens = a.M <= 16 ? 16 : 32;
-  if (narrow <= cus) return tokens == 16 ? launch_few<T, 1, 1>(a, s) : launch_few<T, 2, 1>(a, s);
-  if (tokens == 16 && wide <= 3 * cus) return launch_few<T, 1, 2>(a, s);
-  if (a.M <= 32 ? 2 * wide <= 3 * cus : wide <= 2 * cus && a.N * a.K <= (32 << 20)) return launch_few<T, 2, 2>(a, s);
+  if (narrow <= cus) return tokens == 16 ? kFew16x16 : kFew32x16;
+  if (tokens == 16 && wide <= 3 * cus) return kFew16x32;
+  if (a.M <= 32 ? 2 * wide <= 3 * cus : wide <= 2 * cus && a.N * a.K <= (32 << 20)) return kFew32x32;
   static constexpr TileCost kTiles[4] = {{256, 256, 5.5f, 1.15f, 1.72f},
                                          {128, 128, 1.2f, 0.50f, 0.72f},
                                          {64, 128, 1.3f, 0.36f, 0.42f},
                                          {64, 64, 0.7f, 0.32f, 0.30f}};
-  switch (cheapest(a, kTiles, 4)) {
-    case 0: launch_tiles<T, 2, 4, 4, 2, 2, false>(a, s); break;
-    case 1: launch_tiles<T, 2, 2, 2, 2, 2, false>(a, s); break;
-    case 2: launch_tiles<T, 1, 2, 2, 2, 3, false>(a, s); break;
+  return kTile256x256 + cheapest(a, kTiles, 4);
+}
+
+template <typename T>
+static void launch_linear(const Fp8Args& a, hipStream_t s) {
+  switch (linear_form(a)) {
+    case kFew16x16: launch_few<T, 1, 1>(a, s); break;
+    case kFew32x16: launch_few<T, 2, 1>(a, s); break;
+    case kFew16x32: launch_few<T, 1, 2>(a, s); break;
+    case kFew32x32: launch_few<T, 2, 2>(a, s); break;
+    case kTile256x256: launch_tiles<T, 2, 4, 4, 2, 2, false>(a, s); break;
+    case kTile128x128: launch_tiles<T, 2, 2, 2, 2, 2, false>(a, s); break;
+    case kTile64x128: launch_tiles<T, 1, 2, 2, 2, 3, false>(a, s); break;
     default: launch_tiles<T, 1, 1, 2, 2, 4, false>(a, s); break;
   }
 }
 
-static void launch_gated(const Fp8Args& a, hipStream_t s) {
+static int gated_form(const Fp8Args& a) {
   // Few rows: while a workgroup for every 16 tokens leaves none without a CU (us, split kernel / tiles; H 4,096, K 1,024: 128
   // rows 5.9 / 8.2, 256 rows, two a CU, 10.3 / 8.3; H 8,192, K 4,096, 64 rows 15.7 / 20.2) and LDS holds their K
   const int64_t blocks = a.N / kFp8Block, groups = (a.M + 15) / 16;
-  if (blocks * groups <= device_cu_count() && a.nk <= kGatedFewBlocks) {
-    fp8_gated_few_kernel<<<dim3((unsigned)blocks, (unsigned)groups), dim3(512), 0, s>>>(a);
-    return;
-  }
+  if (blocks * groups <= device_cu_count() && a.nk <= kGatedFewBlocks) return kGatedFew;
   static constexpr TileCost kTiles[3] = {{128, 256, 5.0f, 1.00f, 1.60f},
                                          {128, 128, 1.7f, 0.70f, 0.98f},
                                          {128, 64, 1.3f, 0.53f, 0.63f}};
-  switch (cheapest(a, kTiles, 3)) {
-    case 0: launch_tiles<bf16, 2, 4, 4, 2, 2, true>(a, s); break;
-    case 1: launch_tiles<bf16, 2, 2, 4, 2, 2, true>(a, s); break;
+  return kGatedTile256 + cheapest(a, kTiles, 3);
+}
+
+static void launch_gated(const Fp8Args& a, hipStream_t s) {
+  switch (gated_form(a)) {
+    case kGatedFew:
+      fp8_gated_few_kernel<<<dim3((unsigned)(a.N / kFp8Block), (unsigned)((a.M + 15) / 16)), dim3(512), 0, s>>>(a);
+      break;
+    case kGatedTile256: launch_tiles<bf16, 2, 4, 4, 2, 2, true>(a, s); break;
+    case kGatedTile128: launch_tiles<bf16, 2, 2, 4, 2, 2, true>(a, s); break;
     default: launch_tiles<bf16, 2, 1, 4, 2, 3, true>(a, s); break;
   }
+}
+
+// A product's sizes alone, within the limits of check_fp8; K 0 where they are not
+static Fp8Args fp8_sizes(int64_t M, int64_t N, int64_t K) {
+  Fp8Args a{};
+  if (M < 1 || N < 1 || K < 16 || K % 16 || K > (1 << 22) || M > (1 << 30) || N > (1 << 28)) return a;
+  a.M = M;
+  a.N = N;
+  a.K = (int)K;
+  a.nk = (int)((K + kFp8Block - 1) / kFp8Block);
+  return a;
 }
 
 }  // namespace atma
@@ -795,4 +822,14 @@ extern "C" int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs,
     return set_error(ATMA_ERR_INVALID, "linear_gated_fp8: rows of y must be 16-byte aligned and at least H long");
   launch_gated(a, (hipStream_t)stream);
   return check_launch("linear_gated_fp8");
+}
+
+extern "C" int atma_linear_fp8_form(int64_t M, int64_t N, int64_t K) {
+  const atma::Fp8Args a = atma::fp8_sizes(M, N, K);
+  return a.K ? atma::linear_form(a) : -1;
+}
+
+extern "C" int atma_linear_gated_fp8_form(int64_t M, int64_t H, int64_t K) {
+  const atma::Fp8Args a = atma::fp8_sizes(M, H, K);
+  return a.K && H % atma::kFp8Block == 0 && H <= (1 << 27) ? atma::gated_form(a) : -1;
 }

@@ -655,6 +655,14 @@ int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs, int64_t ld
                           int64_t ldys, int64_t M, int64_t H, int64_t K, void* stream);
 
 /*
+ * Which kernel a call of these sizes takes on the current device, -1 where they are not served.  atma_linear_fp8: 0 to 3 the
+ * few-row kernel of 16 x 16, 32 x 16, 16 x 32 and 32 x 32 tokens x features, 4 to 7 tiles of 256 x 256, 128 x 128, 64 x 128 and
+ * 64 x 64 features x tokens.  atma_linear_gated_fp8: 0 the few-row kernel, 1 to 3 tiles of 256, 128 and 64 tokens.
+ */
+int atma_linear_fp8_form(int64_t M, int64_t N, int64_t K);
+int atma_linear_gated_fp8_form(int64_t M, int64_t H, int64_t K);
+
+/*
  * The LFM2 block's decode mixer (model/reference.py:31-48, inference/models/atma.py:
  * 625-673) as one call: with b, c, x the three D-wide thirds of each bcx row (in_proj's
  * output), out = c * conv(b * x), the depthwise conv of K taps (weight (D, K)) over the
