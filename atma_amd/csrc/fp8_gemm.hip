@@ -798,8 +798,8 @@ extern "C" int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64
             (N + kFp8Block - 1) / kFp8Block, bias, bias_dtype, y, ldy, nullptr, 0, M, N, (int)K, (int)((K + kFp8Block - 1) / kFp8Block), 0, 0, 0};
   if (const int rc = check_fp8("linear_fp8", a, N)) return rc;
   if (M == 0) return ATMA_OK;
-  if (ldy < N || (uintptr_t)y % 2 || (ldy % 8 == 0 && (uintptr_t)y % 16))
-    return set_error(ATMA_ERR_INVALID, "linear_fp8: rows of y must be at least N long, 16-byte aligned where ldy %% 8 == 0");
+  if (ldy < N || (uintptr_t)y % 2)
+    return set_error(ATMA_ERR_INVALID, "linear_fp8: rows of y must be at least N long, at an address of their type");
   if (dtype == ATMA_BF16) launch_linear<bf16>(a, (hipStream_t)stream);
   else launch_linear<f16>(a, (hipStream_t)stream);
   return check_launch("linear_fp8");

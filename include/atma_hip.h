@@ -638,7 +638,7 @@ int atma_quantize_weight_fp8(const void* w, int64_t ldw, void* data, int64_t ldd
  * y[m, n] = round(sum_k x[m, k] w[n, k] + bias[n]) in `dtype` (16-bit) for 8-bit x (M, K) with scales xs (M, nb) and
  * 8-bit w (N, K) with scales ws (ceil(N / 128), nb), nb = ceil(K / 128); bias (N,) in `bias_dtype` or NULL.  K a multiple
  * of 16, at most 2^22; M at most 2^30, N at most 2^28.  Rows of x and w 16-byte aligned and at most 8 MiB apart (the stride
- * of a single row is not used), scales anywhere; bias 4-byte aligned; y 16-byte aligned where ldy % 8 == 0.
+ * of a single row is not used), scales anywhere; bias 4-byte aligned; rows of y anywhere.
  */
 int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw, const void* ws,
                     int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, int64_t M, int64_t N,

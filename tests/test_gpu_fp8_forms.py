@@ -341,3 +341,23 @@ def test_captured_repeated_and_on_another_stream(dev, gated, form, M, N, K):
         eager = call(*inputs[i])
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want[i])) and all(torch.equal(p, q) for p, q in zip(eager, want[i]))
+
+
+# ------------------------------------------------------------------------------------------------ the C ABI's outputs
+@pytest.mark.parametrize("form,M,N,K", SMALL)
+def test_linear_stores_rows_anywhere(dev, form, M, N, K):
+    """y at any element and any stride from N on, multiples of 8 among them; what lies between its rows stays as it was."""
+    from atma_amd import _lib
+    from atma_amd.kernel import linear_fp8
+    _form(form, M, N, K)
+    x, xs, w, ws = _operands(dev, M, N, K, 4)
+    want = linear_fp8(x, xs, w, ws)
+    for off, ldy in ((1, (N + 7) // 8 * 8), (3, (N + 7) // 8 * 8 + 8), (0, N), (7, N + 1), (4, (N + 15) // 8 * 8)):
+        held = torch.full((off + M * ldy + 8,), 7.0, dtype=torch.bfloat16, device=dev)
+        y = held[off:off + M * ldy].view(M, ldy)
+        rc = _lib.load().atma_linear_fp8(
+            x.data_ptr(), x.stride(0), xs.data_ptr(), xs.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(), ws.stride(0),
+            None, 0, y.data_ptr(), ldy, M, N, K, 1, _lib.stream_handle(dev))
+        assert rc == 0, _lib.load().atma_last_error()
+        assert torch.equal(y[:, :N], want)
+        assert (y[:, N:] == 7).all() and (held[:off] == 7).all() and (held[off + M * ldy:] == 7).all()
