@@ -666,8 +666,8 @@ static void launch_tiles(Fp8Args a, hipStream_t s) {
 // Checks shared by the products; rows: weight rows (N, or 2 N gated).  The stride of a single row means nothing: K stands for it
 static int check_fp8(const char* what, Fp8Args& a, int64_t rows) {
   if (a.M < 0 || a.N < 1 || a.K < 16 || a.K % 16 || a.K > (1 << 22) || a.M > (1 << 30) || rows > (1 << 28))
-    return set_error(ATMA_ERR_UNSUPPORTED, "%s: unsupported shape M=%lld N=%lld K=%d (K a multiple of 16)", what,
-                     (long long)a.M, (long long)a.N, a.K);
+    return set_error(ATMA_ERR_UNSUPPORTED, "%s: unsupported shape M=%lld N=%lld K=%d (K a multiple of 16 up to 2^22, M up to 2^30, "
+                     "weight rows up to 2^28)", what, (long long)a.M, (long long)a.N, a.K);
   if (a.M == 0) return ATMA_OK;
   if (!a.x || !a.xs || !a.w || !a.ws || !a.y) return set_error(ATMA_ERR_INVALID, "%s: null pointer", what);
   if (a.M == 1) a.ldx = a.K;

@@ -97,8 +97,8 @@ static int quantize(const char* what, bool weight, const void* x, int64_t ldx, v
   const int size = dtype_size(dtype);
   if (!size) return set_error(ATMA_ERR_UNSUPPORTED, "%s: fp32 or 16-bit input (dtype %d)", what, dtype);
   if (M < 0 || K < 16 || K % 16 || K > (1 << 24) || M > 0x7fffffff)
-    return set_error(ATMA_ERR_UNSUPPORTED, "%s: K must be a multiple of 16 (M=%lld K=%lld)", what, (long long)M,
-                     (long long)K);
+    return set_error(ATMA_ERR_UNSUPPORTED, "%s: K must be a multiple of 16 up to 2^24, M below 2^31 (M=%lld K=%lld)", what,
+                     (long long)M, (long long)K);
   if (M == 0) return ATMA_OK;
   if (!x || !data || !scale) return set_error(ATMA_ERR_INVALID, "%s: null pointer", what);
   const int64_t nb = (K + kFp8Block - 1) / kFp8Block;

@@ -623,14 +623,14 @@ int atma_residual_rms_norm_fp8(const void* y, int64_t ldy, const float* parts, i
                                int64_t M, int64_t D, float eps, int dtype, void* stream);
 
 /*
- * Rows to 8 bits: x (M, K) in `dtype` to data (M, K) and scale (M, ceil(K / 128)).  K a multiple of 16; rows of x
- * 16-byte aligned, of data 8-byte.
+ * Rows to 8 bits: x (M, K) in `dtype` to data (M, K) and scale (M, ceil(K / 128)).  K a multiple of 16, at most 2^24, M
+ * below 2^31; rows of x 16-byte aligned, of data 8-byte.
  */
 int atma_quantize_fp8(const void* x, int64_t ldx, void* data, int64_t ldd, void* scale, int64_t lds, int64_t M,
                       int64_t K, int dtype, void* stream);
 
-/* A weight matrix to 8 bits: w (N, K) to data (N, K) and scale (ceil(N / 128), ceil(K / 128)); alignment as above; at
- * most 65,535 blocks of rows. */
+/* A weight matrix to 8 bits: w (N, K) to data (N, K) and scale (ceil(N / 128), ceil(K / 128)); K and alignment
+ * as above; at most 65,535 blocks of rows. */
 int atma_quantize_weight_fp8(const void* w, int64_t ldw, void* data, int64_t ldd, void* scale, int64_t lds, int64_t N,
                              int64_t K, int dtype, void* stream);
 
@@ -639,6 +639,8 @@ int atma_quantize_weight_fp8(const void* w, int64_t ldw, void* data, int64_t ldd
  * 8-bit w (N, K) with scales ws (ceil(N / 128), nb), nb = ceil(K / 128); bias (N,) in `bias_dtype` or NULL.  K a multiple
  * of 16, at most 2^22; M at most 2^30, N at most 2^28.  Rows of x and w 16-byte aligned and at most 8 MiB apart (the stride
  * of a single row is not used), scales anywhere; bias 4-byte aligned; rows of y anywhere.
+ * Sums are fp32, but the matrix instruction adds the products of eight neighbouring k with 14 bits below the largest of
+ * them: 1.4e-5 of a result of normally distributed values.
  */
 int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw, const void* ws,
                     int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, int64_t M, int64_t N,
@@ -647,8 +649,9 @@ int atma_linear_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, co
 /*
  * The MLP's first projection with its activation, 8 bits in and out (atma_linear_gated's shape: w (2H, K), the a rows,
  * then the gate rows; bias (2H,) or NULL): y (M, H) with scales ys (M, H / 128) hold gate * relu(a)^2 for the fp32 sums
- * a and gate, quantized once.  H a multiple of 128, at most 2^27; x, xs, w, ws, M and K as atma_linear_fp8; rows of y
- * 16-byte aligned.
+ * a and gate, quantized once.  H a multiple of 128, at most 2^27; x, xs, w, ws, M and K as atma_linear_fp8, the sums' precision
+ * too: a value within it of a rounding border goes to either side of it (0.1% of normally distributed ones), and so does the
+ * scale of a block whose largest value lies that close to a power of two times 448 (4 in 10^5).  Rows of y 16-byte aligned.
  */
 int atma_linear_gated_fp8(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* w, int64_t ldw,
                           const void* ws, int64_t ldws, const void* bias, int bias_dtype, void* y, int64_t ldy, void* ys,
