@@ -790,6 +790,13 @@ class Fp8MLP(nn.Module):
                 self.register_buffer(name + "_scale", scale.view(torch.uint8))
                 self.register_buffer(name + "_bias", None if linear.bias is None else linear.bias.detach().clone())
 
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        """The 8-bit form's own state loads.  That of an ``MLP`` is an error also where missing and unexpected names are
+        none (``strict=False``): it would leave the weights as they were."""
+        if prefix + "fc.weight" in state_dict or prefix + "proj.weight" in state_dict:
+            args[-1].append(f"{prefix[:-1] or 'Fp8MLP'} holds its weights in 8 bits: load an MLP's before it is replaced")
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
     def forward(self, x, defer=False):
         """x (..., dim) in 16 bits on the GPU.  ``defer`` is ``MLP``'s; the output is always summed."""
         if x.dtype not in (torch.bfloat16, torch.float16):
