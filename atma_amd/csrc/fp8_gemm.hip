@@ -298,14 +298,6 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
   read_scales();
   while (true) {
     // ---- the sums start from the bias
-    if constexpr (!GATED) {
-      // the last of an odd number in 16 bits is half a word, which no copy brings: every wave puts it beside the others
-      LateArgs p = late_args();
-      if (p->bias && p->bias_dtype != ATMA_F32 && p->N % 2 && f0 + C::OF >= p->N) {
-        *(uint16_t*)(lds + C::BIAS + 1024 * tile + 2 * (int)(p->N - 1 - f0)) = ((const uint16_t*)p->bias)[p->N - 1];
-        wave_sync();
-      }
-    }
 #pragma unroll
     for (int t = 0; t < TF; ++t) {
       float b[16] = {};
@@ -320,6 +312,11 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
             b[e] = v[0], b[e + 1] = v[1], b[e + 2] = v[2], b[e + 3] = v[3];
           }
         } else {
+          if (!GATED && t == 0 && p->N % 2 && f0 + C::OF >= p->N) {
+            // the last of an odd number is half a word, which no copy brings: every wave puts it beside the others
+            *(uint16_t*)(lds + C::BIAS + 1024 * tile + 2 * (int)(p->N - 1 - f0)) = ((const uint16_t*)p->bias)[p->N - 1];
+            wave_sync();
+          }
           const bool bf = p->bias_dtype == ATMA_BF16;
 #pragma unroll
           for (int e = 0; e < 16; e += 8) {
