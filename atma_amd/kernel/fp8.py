@@ -100,7 +100,7 @@ def residual_rms_norm_fp8(branch, residual, weight, eps):
         raise ValueError(f"{what}: residual must match the branch")
     if len(biases) > 3 or any(b.shape != (D,) or b.dtype != dtype for b in biases):
         raise ValueError(f"{what}: up to three biases ({D},) in the stream's type")
-    if mu_x is not None and (mu_x.dim() != 2 or mu_x.shape[1] not in (4, 8, 16) or mu_x.shape[0] != M
+    if mu_x is not None and (mu_w is None or mu_x.dim() != 2 or mu_x.shape[1] not in (4, 8, 16) or mu_x.shape[0] != M
                              or mu_w.shape != (D, mu_x.shape[1]) or mu_x.dtype != dtype or mu_w.dtype != dtype):
         raise ValueError(f"{what}: the low-rank term takes mu_x (M, k) and mu_w (D, k), k 4, 8 or 16")
     keep = residual is not None or src is not branch
