@@ -1110,3 +1110,141 @@ def linear_gated_fp8_op(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale
 @linear_gated_fp8_op.register_fake
 def _(x, x_scale, weight, weight_scale, bias):
     return list(_fp8_pair(x, x.shape[0], weight.shape[0] // 2, x.shape[0]))
+
+
+# --------------------------------------------------------------------------- 4-bit weights (kernel/fp4.py)
+# As the 8-bit operators: a launch on operands as the kernels take them, behind whatever copies bring them there.
+FP4_GROUP = 32
+
+
+def _near(t: Tensor, pitch: int) -> Tensor:
+    """``_rows_apart`` with rows at most ``pitch`` elements apart."""
+    return _rows_apart(t if t.stride(0) <= pitch else t.clone(memory_format=torch.contiguous_format))
+
+
+def _row_bytes(t: Tensor) -> Tensor:
+    """A matrix of bytes with unit inner stride and rows in order."""
+    return t if t.stride(1) == 1 and t.stride(0) >= 0 else t.contiguous()
+
+
+def _vector(t: Optional[Tensor]) -> Optional[Tensor]:
+    return t if t is None or t.stride(0) == 1 else t.contiguous()
+
+
+def fp4_quantize(weight):
+    N, K = weight.shape
+    data = weight.new_empty((N, K // 2), dtype=torch.uint8)
+    scale = weight.new_empty((N, K // FP4_GROUP), dtype=FP8_SCALE)
+    rc = _lib.load().atma_quantize_weight_fp4(weight.data_ptr(), weight.stride(0), data.data_ptr(), K // 2, scale.data_ptr(),
+                                              K // FP4_GROUP, N, K, _lib.DTYPE_CODE[weight.dtype],
+                                              _lib.stream_handle(weight.device))
+    if rc:
+        _lib.check(rc, "quantize_weight_fp4")
+    return data, scale
+
+
+@_op("quantize_weight_fp4", mutates_args=())
+def quantize_weight_fp4_op(weight: Tensor) -> List[Tensor]:
+    _need_cuda(weight)
+    with _lib.on_device(weight.device):
+        return list(fp4_quantize(_rows_apart(weight)))
+
+
+@quantize_weight_fp4_op.register_fake
+def _(weight):
+    N, K = weight.shape
+    return [weight.new_empty((N, K // 2), dtype=torch.uint8), weight.new_empty((N, K // FP4_GROUP), dtype=FP8_SCALE)]
+
+
+def fp4_dequantize(data, scale, dtype):
+    N, K = data.shape[0], 2 * data.shape[1]
+    out = data.new_empty((N, K), dtype=dtype)
+    rc = _lib.load().atma_dequantize_weight_fp4(data.data_ptr(), data.stride(0), scale.data_ptr(), scale.stride(0),
+                                                out.data_ptr(), K, N, K, _lib.DTYPE_CODE[dtype],
+                                                _lib.stream_handle(data.device))
+    if rc:
+        _lib.check(rc, "dequantize_weight_fp4")
+    return out
+
+
+@_op("dequantize_weight_fp4", mutates_args=())
+def dequantize_weight_fp4_op(data: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
+    _need_cuda(data, scale)
+    with _lib.on_device(data.device):
+        return fp4_dequantize(_rows_apart(data), scale if scale.stride(1) == 1 and scale.stride(0) >= scale.shape[1]
+                              else scale.clone(memory_format=torch.contiguous_format), dtype)
+
+
+@dequantize_weight_fp4_op.register_fake
+def _(data, scale, dtype):
+    return data.new_empty((data.shape[0], 2 * data.shape[1]), dtype=dtype)
+
+
+FP4_PITCH = (1 << 22, 1 << 23)   # elements between rows of x, bytes between rows of the weights: what the products address
+
+
+def fp4_linear(x, data, scale, bias, gated):
+    (M, K), N = x.shape, data.shape[0] // (2 if gated else 1)
+    out = x.new_empty((M, N))
+    lib = _lib.load()
+    rc = (lib.atma_linear_gated_fp4 if gated else lib.atma_linear_fp4)(
+        x.data_ptr(), x.stride(0), data.data_ptr(), data.stride(0), scale.data_ptr(), scale.stride(0),
+        None if bias is None else bias.data_ptr(), 0 if bias is None else _lib.DTYPE_CODE[bias.dtype], out.data_ptr(), N,
+        M, N, K, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(x.device))
+    if rc:
+        _lib.check(rc, "linear_gated_fp4" if gated else "linear_fp4")
+    return out
+
+
+def _linear_fp4(x, data, scale, bias, gated):
+    _need_cuda(x, data, scale, bias)
+    with _lib.on_device(x.device):
+        return fp4_linear(_near(x, FP4_PITCH[0]), _near(data, FP4_PITCH[1]), _row_bytes(scale), _vector(bias), gated)
+
+
+@_op("linear_fp4", mutates_args=())
+def linear_fp4_op(x: Tensor, data: Tensor, scale: Tensor, bias: Optional[Tensor]) -> Tensor:
+    return _linear_fp4(x, data, scale, bias, False)
+
+
+@linear_fp4_op.register_fake
+def _(x, data, scale, bias):
+    return x.new_empty((x.shape[0], data.shape[0]))
+
+
+@_op("linear_gated_fp4", mutates_args=())
+def linear_gated_fp4_op(x: Tensor, data: Tensor, scale: Tensor, bias: Optional[Tensor]) -> Tensor:
+    return _linear_fp4(x, data, scale, bias, True)
+
+
+@linear_gated_fp4_op.register_fake
+def _(x, data, scale, bias):
+    return x.new_empty((x.shape[0], data.shape[0] // 2))
+
+
+# --------------------------------------------------------------------------- sampling (kernel/sampling.py)
+def sample_into(ids, logits, uniform, temperature, t0, top_k, k0, top_p, p0, min_p, m0):
+    rows, V = logits.shape
+    rc = _lib.load().atma_sample_tokens(
+        logits.data_ptr(), logits.stride(0), uniform.data_ptr(), _lib.ptr(temperature), t0, _lib.ptr(top_k), k0,
+        _lib.ptr(top_p), p0, _lib.ptr(min_p), m0, ids.data_ptr(), rows, V, _lib.DTYPE_CODE[logits.dtype],
+        _lib.stream_handle(logits.device))
+    if rc:
+        _lib.check(rc, "sample_tokens")
+    return ids
+
+
+@_op("sample_tokens", mutates_args=())
+def sample_tokens_op(logits: Tensor, uniform: Tensor, temperature: Optional[Tensor], t0: float, top_k: Optional[Tensor],
+                     k0: int, top_p: Optional[Tensor], p0: float, min_p: Optional[Tensor], m0: float) -> Tensor:
+    _need_cuda(logits, uniform, temperature, top_k, top_p, min_p)
+    if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        logits = logits.clone(memory_format=torch.contiguous_format)
+    with _lib.on_device(logits.device):
+        return sample_into(logits.new_empty((logits.shape[0],), dtype=torch.int64), logits, _vector(uniform),
+                           _vector(temperature), t0, _vector(top_k), k0, _vector(top_p), p0, _vector(min_p), m0)
+
+
+@sample_tokens_op.register_fake
+def _(logits, uniform, temperature, t0, top_k, k0, top_p, p0, min_p, m0):
+    return logits.new_empty((logits.shape[0],), dtype=torch.int64)

@@ -20,6 +20,7 @@ from .. import _lib
 _lib.load()   # raises HipLibraryMissing (ImportError) when the library is absent
 
 from .conv import causal_conv1d_decode_step  # noqa: E402
+from .fp4 import (dequantize_weight_fp4, linear_fp4, linear_gated_fp4, quantize_weight_fp4)  # noqa: E402
 from .fp8 import (linear_fp8, linear_gated_fp8, quantize_fp8, quantize_weight_fp8,  # noqa: E402
                   residual_rms_norm_fp8)
 from .inference_ops import (linear_tokens, linear_tokens_supported, packed_causal_conv1d,  # noqa: E402
@@ -28,6 +29,7 @@ from .gated_delta import (StartSignal, chunk_gated_delta_rule, gated_delta_decod
                           gated_delta_gates, recurrence_pays_to_overlap)
 from .polar import (global_decode_step, global_decode_step_supported, polar_attention_decode,  # noqa: E402
                     polar_attention_fwd, polar_attention_packed_fwd)
+from .sampling import sample_tokens  # noqa: E402
 from .polar_train import polar_attention  # noqa: E402
 
 HAS_HIP = torch.cuda.is_available()
@@ -59,4 +61,9 @@ __all__ = [
     "residual_rms_norm_fp8",
     "linear_fp8",
     "linear_gated_fp8",
+    "quantize_weight_fp4",
+    "dequantize_weight_fp4",
+    "linear_fp4",
+    "linear_gated_fp4",
+    "sample_tokens",
 ]

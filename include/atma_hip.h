@@ -666,6 +666,58 @@ int atma_linear_fp8_form(int64_t M, int64_t N, int64_t K);
 int atma_linear_gated_fp8_form(int64_t M, int64_t H, int64_t K);
 
 /*
+ * 4-bit weights for inference (no reference counterparts).  A 4-bit weight matrix (N, K) is bytes of two float4 e2m1 values (0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, codes 0 to 7 and 8 to 15; the even k in the low half), (N, K / 2), with a
+ * power-of-two scale for each group of 32 values of a row, one byte each (float8_e8m0fnu: code c is 2^(c - 127), 255 makes
+ * the group NaN), (N, K / 32).  K is a multiple of 32.  Row strides are in elements (bytes for values and scales).
+ */
+
+/*
+ * A weight matrix to 4 bits: w (N, K) in `dtype`.  The scale of a group is the smallest 2^e, e in [-125, 125], that brings its
+ * largest magnitude to 7 or less; values are divided by it and rounded to nearest even, above 6 to 6.  A group that holds
+ * an infinity or NaN gets code 255.  K at most 2^24, N below 2^31; rows of w 16-byte aligned, of data 4-byte.
+ */
+int atma_quantize_weight_fp4(const void* w, int64_t ldw, void* data, int64_t ldd, void* scale, int64_t lds, int64_t N,
+                             int64_t K, int dtype, void* stream);
+
+/* The values that a 4-bit weight matrix stands for, rounded to `dtype`; sizes and alignment as above. */
+int atma_dequantize_weight_fp4(const void* data, int64_t ldd, const void* scale, int64_t lds, void* w, int64_t ldw,
+                               int64_t N, int64_t K, int dtype, void* stream);
+
+/*
+ * y[m, n] = round(sum_k x[m, k] w[n, k] + bias[n]) in `dtype` (16-bit) for x (M, K) in `dtype` and 4-bit w (N, K) with scales
+ * ws (N, K / 32); bias (N,) in `bias_dtype` or NULL.  The weights enter the product in `dtype`: exact in bf16; in fp16 what
+ * lies below 2^-14 in multiples of 2^-24 and 65,520 or more as an infinity.  Sums are fp32.  K at most 2^22; M at most 2^30, N
+ * at most 2^28.  Rows of x and w 16-byte aligned and at most 8 MiB apart (the stride of a single row is not used), scales,
+ * bias and rows of y at any element.
+ */
+int atma_linear_fp4(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* ws, int64_t ldws, const void* bias,
+                    int bias_dtype, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
+
+/*
+ * The MLP's first projection with its activation (atma_linear_gated's shape: w (2H, K), the a rows, then the gate rows; bias
+ * (2H,) or NULL): y (M, H) = round(gate * relu(a)^2) of the fp32 sums a and gate.  H at most 2^27, the rest as
+ * atma_linear_fp4.
+ */
+int atma_linear_gated_fp4(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* ws, int64_t ldws,
+                          const void* bias, int bias_dtype, void* y, int64_t ldy, int64_t M, int64_t H, int64_t K, int dtype,
+                          void* stream);
+
+/*
+ * Next tokens from logits (rows, V), row stride ld: ids[r] for temperature[r] (or t0 for every row where the pointer is NULL;
+ * the filters likewise).  A temperature that is not above 0 takes the largest logit, the lowest index among equal ones;
+ * so does a row that holds a NaN, its first one.  Else w_i = exp((x_i - max x) / temperature), 1 for every largest logit (also
+ * where that is infinite), and in the order of falling logits, equal ones by index, are kept: the first top_k tokens (all
+ * where it is not in [1, V)), of these those before which less than top_p of their weight lies (all where it is not below 1;
+ * the first always), of these those with w_i >= min_p (all where it is not above 0; 1 and more: the largest).  ids[r] is the first index
+ * at which the sum of kept weights, in index order, exceeds uniform[r] (taken into [0, 1 - 2^-24], NaN as 0) times
+ * their whole sum.  Weights are held in multiples of 2^-43.  V from 1 to 2^20.
+ */
+int atma_sample_tokens(const void* logits, int64_t ld, const float* uniform, const float* temperature, float t0,
+                       const int32_t* top_k, int k0, const float* top_p, float p0, const float* min_p, float m0,
+                       int64_t* ids, int64_t rows, int64_t V, int dtype, void* stream);
+
+/*
  * The LFM2 block's decode mixer (model/reference.py:31-48, inference/models/atma.py:
  * 625-673) as one call: with b, c, x the three D-wide thirds of each bcx row (in_proj's
  * output), out = c * conv(b * x), the depthwise conv of K taps (weight (D, K)) over the
