@@ -1,10 +1,18 @@
 // Products with 4-bit weights: y[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]) for 16-bit x (M, K) and w (N, K) in the format of
 // fp4.h, and the MLP's first projection with its activation, gate * relu(a)^2 of the fp32 sums.  No reference counterpart.
+//
+// The weights become the matrix instructions' 16-bit operands in registers, one instruction for two of them, scale included
+// (fp4_unpack8), so what is read from memory and LDS for them stays at 4.25 bits.  The order of k within an instruction is
+// free as long as both operands follow it: a lane takes 16 bytes of a weight row, one group of 32 with its one scale, and the
+// same 32 k of a token, four 16-byte pieces.
 #include <algorithm>
 
 #include "fp4.h"
+#include "gemm_tiles.h"
 
 namespace atma {
+
+constexpr int kFp4Block = 64;  // of K, a stage of the tiles' ring: 128 bytes of a token's row, 32 of a weight's
 
 struct Fp4Args {
   const void* x;  // (M, K), row stride ldx
@@ -18,20 +26,270 @@ struct Fp4Args {
   void* y;  // (M, N), row stride ldy
   int64_t ldy;
   int64_t M, N;
-  int K;
+  int K, nk;  // nk: blocks of K
+  int m_tiles, f_tiles, per_xcd;
 };
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  Pack8 pa, pb;
+  pa.u = a;
+  pb.u = b;
+  if constexpr (__is_same(T, bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa.b, pb.b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(pa.h, pb.h, c, 0, 0, 0);
+}
+
+// The kernel's arguments read again where they are needed: kept in scalar registers through the loop they would be spilled
+typedef const __attribute__((address_space(4))) Fp4Args* LateArgs4;
+__device__ __forceinline__ LateArgs4 late_args4() {
+  LateArgs4 p = (LateArgs4)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+// A workgroup of WF x WM waves owns BF weight rows x BM tokens, a wave TF x TM tiles of 32 x 32.  K runs in blocks of 64 through a
+// ring of NS stages in LDS, filled by direct copies.  A block is four steps of 16 k a lane half: while the products of a
+// step run from registers, the tokens of the next step are read, each into the registers of the one just used, and the
+// next step's weights converted into a second set; in the last step the next block's weights are read, still packed, and
+// the copies of block k + NS go into the stage just read.  The workgroup is persistent and all of this runs on across its
+// tiles: a tile's first copies fly and its first operands are read during the last blocks of the one before.
+//
+// The weights are the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token
+// (row 8 q + 4 h + e is feature 16 h + 4 q + e).  Their rows are 32 bytes in LDS, chunk c of row r at position
+// c ^ (r / 16) % 2: the 16 lanes that read one chunk of 16 such rows cover all banks.
+template <int TF, int TM, int WF, int WM, int NS_, bool GATED>
+struct Fp4Tile {
+  static constexpr int NW = WF * WM, NS = NS_;
+  static constexpr int BF = 32 * TF * WF, BM = 32 * TM * WM;
+  static constexpr int OF = GATED ? BF / 2 : BF;  // output features
+  static constexpr int TO = GATED ? TF / 2 : TF;  // tiles of output features a wave
+  static constexpr int W = BM * 128, STAGE = W + BF * 32;
+  static constexpr int XCOPY = BM / 8 / NW, COPIES = XCOPY + 1;  // a wave and block: 8 token rows each, 32 weight rows
+  static constexpr int RING = NS + 2;    // blocks and tiles under way: copies run NS blocks ahead
+  static constexpr int SLOT = NW * 256;  // a block's scales, in words: two a weight row
+  static constexpr int AUX = NS * STAGE, BIAS = AUX + RING * SLOT, TURN = BIAS + RING * 1024, LDS = TURN + 2048 * NW;
+  static_assert(BF == 32 * NW && BM % (8 * NW) == 0 && BF <= 256 && NW > 2, "whole copies, a bias of 1 KiB, copied by wave 2");
+  static_assert(!GATED || TF % 2 == 0, "a gated wave has its features' a and gate rows");
+  static_assert(NS >= 3 && (NS - 2) * (COPIES + 1) < 63, "vmcnt counts to 63");
+};
+
+template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
+__global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
+  using C = Fp4Tile<TF, TM, WF, WM, NS, GATED>;
+  constexpr int TO = C::TO;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wf = wave % WF, wm = wave / WF;
+  const int r = lane & 31, h = lane >> 5;
+  const int nk = a.nk;
+  int64_t m0, f0;
+  int u = blockIdx.x >> 3;
+  if (!gemm_tile_at<C>(a, blockIdx.x & 7, u, m0, f0)) return;
+
+  // ---- the copies, NS blocks ahead.  Token copy i of a wave moves rows 8 (i NW + wave) .. + 7, lane l the chunk that belongs
+  // at position l % 8 of row l / 8; the weights' copy rows 32 wave .. + 31, lane l the chunk of position l % 2 of row l / 2;
+  // the scales' copy the same rows' codes, lane l group l % 2 of row l / 2.  Out of range (chunks past K, rows past the
+  // end, everything behind the last tile) zeros are written; scales past K or the last row are the last ones
+  const uint32_t lds0 = lds_offset(lds);
+  const int crow = 8 * wave + (lane >> 3);
+  const int xk = 16 * ((lane & 7) ^ x_swizzle(crow));  // bytes into the row
+  const uint32_t xv0 = (uint32_t)crow * (uint32_t)(2 * a.ldx) + (uint32_t)xk, xstep = 8u * C::NW * (uint32_t)(2 * a.ldx);
+  const int wk = 16 * ((lane & 1) ^ (lane >> 5));
+  constexpr int half = C::NW / 2;  // gated: the first half of the waves copy a rows, the others gate rows
+  const int wbase = 32 * (GATED ? wave % half : wave);
+  const uint32_t wv0 = (uint32_t)(wbase + (lane >> 1)) * (uint32_t)a.ldw + (uint32_t)wk;
+  __amdgpu_buffer_rsrc_t xr, wr;
+  const uint8_t* scales;  // the first code of a lane's weight row
+  int pu = u, pk = 0, plimit = 0, ptile = 0, pslot = 0, pstage = 0;
+  auto aim = [&](int64_t tm0, int64_t tf0) {
+    LateArgs4 p = late_args4();
+    const int64_t rows = min((int64_t)C::BM, p->M - tm0);
+    xr = buffer_rsrc((const uint16_t*)p->x + tm0 * p->ldx, (uint32_t)(rows * 2 * p->ldx));
+    const int64_t n0 = GATED && wave >= half ? p->N + tf0 : tf0;
+    wr = buffer_rsrc(p->w + n0 * p->ldw, (uint32_t)(min((int64_t)C::OF, p->N - tf0) * p->ldw));
+    const int64_t last = (GATED && wave >= half ? 2 : 1) * p->N - 1;
+    scales = p->ws + min(n0 + wbase + (lane >> 1), last) * p->ldws;
+    plimit = p->K;
+    if (p->bias && wave == 2) {
+      // the tile's biases (gated: those of a, then of gate), a word each, to its slot
+      const bool wide = p->bias_dtype == ATMA_F32;
+      for (int i = 0; i < C::BF / 64; ++i) {
+        const int f = 64 * i + lane;
+        const int64_t n = min(GATED && f >= C::OF ? p->N + tf0 + f - C::OF : tf0 + f, (GATED ? 2 : 1) * p->N - 1);
+        const uint32_t at = lds0 + C::BIAS + 1024 * ptile + 256 * i;
+        if (wide) dma_load4_at((const uint32_t*)p->bias + n, at);
+        else dma_load2_at((const uint16_t*)p->bias + n, at);
+      }
+    }
+    ptile = ptile + 1 == C::RING ? 0 : ptile + 1;
+  };
+  auto next_tile = [&]() {
+    int64_t nm0, nf0;
+    pk = 0;
+    pu += gridDim.x >> 3;
+    if (gemm_tile_at<C>(*late_args4(), blockIdx.x & 7, pu, nm0, nf0)) aim(nm0, nf0);
+    else plimit = 0;
+  };
+  uint32_t pd, pxv, pwv;
+  auto copies_begin = [&]() {
+    dma_load1_at(scales + max(0, min(2 * pk + (lane & 1), plimit / kFp4Group - 1)), lds0 + C::AUX + C::SLOT * pslot + 256 * wave);
+    pslot = pslot + 1 == C::RING ? 0 : pslot + 1;
+    pd = lds0 + pstage * C::STAGE + 1024 * wave;
+    pstage = pstage + 1 == NS ? 0 : pstage + 1;
+    const int k = kFp4Block * pk++;
+    pxv = k + xk / 2 < plimit ? xv0 + 2u * (uint32_t)k : 0x80000000u;
+    pwv = k + 2 * wk < plimit ? wv0 + (uint32_t)k / 2 : 0x80000000u;
+  };
+  auto copy = [&](int i) {
+    if (i < C::XCOPY) dma_buf16_at(xr, pxv + i * xstep, 0u, pd + 1024 * C::NW * i);
+    else dma_buf16_at(wr, pwv, 0u, pd + C::W);
+  };
+
+  // ---- operand reads
+  const int wrow0 = 32 * TO * wf;  // the wave's first output feature in the tile
+  const int wrow = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+  auto wtile = [](int t) { return GATED ? t / TO * (C::BF / 2) + 32 * (t % TO) : 32 * t; };
+  const uint32_t wofs = (uint32_t)(C::W + (wrow0 + wrow) * 32 + 16 * (h ^ ((r >> 2) & 1)));
+  const uint32_t sofs = (uint32_t)(C::AUX + 8 * (wrow0 + wrow) + 4 * h);
+  uint32_t xofs[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) xofs[j] = (uint32_t)((32 * TM * wm + r) * 128 + 16 * ((4 * h + j) ^ x_swizzle(r)));
+  f32x16 acc[TF][TM];
+  u32x4 raw[TF], wv[2][TF], xv[TM];
+  uint32_t code[TF];
+  int stage = 0, slot = 0, tile = 0;  // what is read next
+  auto read_w = [&](const uint8_t* base, int t) {
+    raw[t] = *(const u32x4*)(base + wofs + 32 * wtile(t));
+    code[t] = *(const uint32_t*)(lds + sofs + C::SLOT * slot + 8 * wtile(t));
+  };
+  auto convert = [&](int s, int j, int t) { wv[s][t] = fp4_unpack8<T>(raw[t][j], __builtin_bit_cast(float, code[t] << 23)); };
+  auto read_x = [&](const uint8_t* base, int j, int t) { xv[t] = *(const u32x4*)(base + xofs[j] + 4096 * t); };
+
+  aim(m0, f0);
+#pragma unroll 1
+  for (int i = 0; i < NS; ++i) {
+    if (pk == nk) next_tile();
+    copies_begin();
+#pragma unroll
+    for (int c = 0; c < C::COPIES; ++c) copy(c);
+  }
+  wait_vmcnt<(NS - 1) * (C::COPIES + 1)>();
+  lds_barrier();
+#pragma unroll
+  for (int t = 0; t < TF; ++t) read_w(lds, t);
+#pragma unroll
+  for (int t = 0; t < TM; ++t) read_x(lds, 0, t);
+#pragma unroll
+  for (int t = 0; t < TF; ++t) convert(0, 0, t);
+  slot = 1;
+  while (true) {
+    // ---- the sums start from the bias
+#pragma unroll
+    for (int t = 0; t < TF; ++t) {
+      float b[16] = {};
+      const int f = wrow0 + 16 * h + (GATED ? t / TO * C::OF + 32 * (t % TO) : 32 * t);
+      LateArgs4 p = late_args4();
+      if (p->bias) {
+        const uint8_t* at = lds + C::BIAS + 1024 * tile;
+        const int dtype = p->bias_dtype;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const u32x4 v = *(const u32x4*)(at + 4 * (f + e));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[e + i] = bias_f32(dtype, v[i]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][j][e] = b[e];
+    }
+    tile = tile + 1 == C::RING ? 0 : tile + 1;
+
+    for (int kb = 0; kb < nk; ++kb) {
+      if (pk == nk) next_tile();
+      const uint8_t* base = lds + stage * C::STAGE;
+      stage = stage + 1 == NS ? 0 : stage + 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j == 3) {
+          // the next block's copies have landed in every wave, and every wave has read this block
+          wait_vmcnt<(NS - 2) * (C::COPIES + 1)>();
+          lds_barrier();
+          base = lds + stage * C::STAGE;
+          copies_begin();
+        }
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int t = 0; t < TF; ++t) acc[t][m] = mfma32<T>(wv[j & 1][t], xv[m], acc[t][m]);
+          // behind the products of token tile m: its operand of the next step, a share of the weights and copies
+          if (j == 3 && m == 0) {
+#pragma unroll
+            for (int t = 0; t < TF; ++t) read_w(base, t);
+            slot = slot + 1 == C::RING ? 0 : slot + 1;
+          }
+          read_x(base, (j + 1) & 3, m);
+          if (j == 3) {
+#pragma unroll
+            for (int c = m * C::COPIES / TM; c < (m + 1) * C::COPIES / TM; ++c) copy(c);
+          }
+          // (the last step's first half waits for the next block's weights)
+          const int from = j == 3 ? max(0, 2 * m - TM) : m, share = j == 3 && TM > 1 ? 2 : 1;
+          if (j != 3 || TM == 1 || 2 * m >= TM) {
+#pragma unroll
+            for (int t = 0; t < TF; ++t)
+              if (t >= from * TF / TM && t < (from + share) * TF / TM) convert((j + 1) & 1, (j + 1) & 3, t);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+
+    // ---- epilogue of tile (m0, f0): token 32 (TM wm + j) + r, 16 consecutive features a tile.  Through LDS, a wave its own 2 KiB:
+    // 32 tokens x 32 features at a time turn from a token a lane to 64-byte pieces, four lanes each (chunk c of row r at position
+    // c ^ (r / 4) % 4)
+    LateArgs4 p = late_args4();
+    const bool whole = f0 + C::OF <= p->N;  // every feature of the tile
+    uint8_t* turn = lds + C::TURN + 2048 * wave;
+    const int64_t ldy = p->ldy, N = p->N, M = p->M;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+      for (int t = 0; t < TO; ++t) {
+        f32x16 v = acc[t][j];
+        if constexpr (GATED) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = gate_act(v[e], acc[TO + t][j][e]);
+        }
+        wave_sync();
+#pragma unroll
+        for (int e = 0; e < 16; e += 8)
+          *(u32x4*)(turn + 64 * r + 16 * ((2 * h + e / 8) ^ ((r >> 2) & 3))) =
+              u32x4{pack2<T>(v[e], v[e + 1]), pack2<T>(v[e + 2], v[e + 3]), pack2<T>(v[e + 4], v[e + 5]),
+                    pack2<T>(v[e + 6], v[e + 7])};
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 16 * i + (lane >> 2);
+          const u32x4 o = *(const u32x4*)(turn + 64 * row + 16 * ((lane & 3) ^ ((row >> 2) & 3)));
+          const int64_t m = m0 + 32 * (TM * wm + j) + row, n0 = f0 + wrow0 + 32 * t + 8 * (lane & 3);
+          if (m < M) store_out8((uint16_t*)p->y + m * ldy + n0, o, whole, n0, N);
+        }
+      }
+    }
+    u += gridDim.x >> 3;
+    if (!gemm_tile_at<C>(*late_args4(), blockIdx.x & 7, u, m0, f0)) break;
+  }
+  wait_vmcnt<0>();  // no copy outlives its workgroup's LDS
+}
 
 __device__ __forceinline__ float fp4_bias(const Fp4Args& a, int64_t n) {
   if (!a.bias) return 0.f;
-  if (a.bias_dtype == ATMA_F32) return ((const float*)a.bias)[n];
-  if (a.bias_dtype == ATMA_BF16) return to_f32(((const bf16*)a.bias)[n]);
-  return to_f32(((const f16*)a.bias)[n]);
-}
-
-// gate * relu(a)^2 in fp32 (v_maximum3_f32: NaN passes through, as torch's relu)
-__device__ __forceinline__ float fp4_gate(float av, float gv) {
-  const float pos = __builtin_elementwise_maximum(av, 0.f);
-  return gv * (pos * pos);
+  return bias_f32(a.bias_dtype, a.bias_dtype == ATMA_F32 ? ((const uint32_t*)a.bias)[n] : ((const uint16_t*)a.bias)[n]);
 }
 
 // A wave owns 16 features x 16 tokens; lane (r, g) holds row r of both operands, k = 8 g .. + 7 of each 32
@@ -57,9 +315,21 @@ __global__ void __launch_bounds__(64) fp4_kernel(Fp4Args a) {
     const int64_t n = f0 + 4 * g + e;
     if (n >= a.N) break;
     float v = acc[0][e] + fp4_bias(a, n);
-    if constexpr (GATED) v = fp4_gate(v, acc[1][e] + fp4_bias(a, a.N + n));
+    if constexpr (GATED) v = gate_act(v, acc[1][e] + fp4_bias(a, a.N + n));
     ((T*)a.y)[m * a.ldy + n] = from_f32<T>(v);
   }
+}
+
+template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
+static void launch_tiles4(Fp4Args a, hipStream_t s) {
+  using C = Fp4Tile<TF, TM, WF, WM, NS, GATED>;
+  a.m_tiles = (int)((a.M + C::BM - 1) / C::BM);
+  a.f_tiles = (int)((a.N + C::OF - 1) / C::OF);
+  const int64_t tiles = (int64_t)a.m_tiles * a.f_tiles;
+  a.per_xcd = (int)((tiles + 7) / 8);
+  constexpr int per_cu = 160 * 1024 / C::LDS;
+  const int64_t wgs = std::min<int64_t>((int64_t)device_cu_count() / 8 * 8 * per_cu, 8 * (int64_t)a.per_xcd);
+  fp4_tile_kernel<T, TF, TM, WF, WM, NS, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
 }
 
 static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dtype, void* stream) {
@@ -83,22 +353,33 @@ static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dt
   if (a.bias && !dtype_size(a.bias_dtype))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: bias in fp32 or 16 bits (dtype %d)", what, a.bias_dtype);
   if (a.bias && (uintptr_t)a.bias % dtype_size(a.bias_dtype)) return set_error(ATMA_ERR_INVALID, "%s: misaligned bias", what);
-  const int64_t tokens = (a.M + 15) / 16;
-  const int64_t most = 65535;
-  for (int64_t t = 0; t < tokens; t += most) {
-    Fp4Args p = a;
-    p.M = std::min(most * 16, a.M - t * 16);
-    p.x = (const char*)a.x + t * 16 * a.ldx * 2;
-    p.y = (char*)a.y + t * 16 * a.ldy * 2;
-    const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((p.M + 15) / 16));
-    auto launch = [&](auto zero) {
-      using T = decltype(zero);
-      if (gated) fp4_kernel<T, true><<<grid, 64, 0, (hipStream_t)stream>>>(p);
-      else fp4_kernel<T, false><<<grid, 64, 0, (hipStream_t)stream>>>(p);
-    };
-    if (dtype == ATMA_BF16) launch(bf16{});
-    else launch(f16{});
-  }
+  if (a.ldy < a.N) return set_error(ATMA_ERR_INVALID, "%s: rows of y must be at least N long", what);
+  a.nk = (a.K + kFp4Block - 1) / kFp4Block;
+  hipStream_t st = (hipStream_t)stream;
+  auto launch = [&](auto zero) {
+    using T = decltype(zero);
+    if (a.M <= 32) {
+      const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 15) / 16));
+      if (gated) fp4_kernel<T, true><<<grid, 64, 0, st>>>(a);
+      else fp4_kernel<T, false><<<grid, 64, 0, st>>>(a);
+    } else if (gated) {
+      static constexpr TileCost kTiles[3] = {{128, 256, 5.f, 1.15f, 1.72f}, {64, 128, 1.5f, 0.6f, 0.86f}, {64, 64, 1.f, 0.4f, 0.5f}};
+      switch (cheapest_tile(a.M, a.N, a.nk, kTiles, 3)) {
+        case 0: launch_tiles4<T, 2, 4, 4, 2, 3, true>(a, st); break;
+        case 1: launch_tiles4<T, 2, 2, 2, 2, 3, true>(a, st); break;
+        default: launch_tiles4<T, 2, 1, 2, 2, 4, true>(a, st); break;
+      }
+    } else {
+      static constexpr TileCost kTiles[3] = {{256, 256, 5.f, 1.15f, 1.72f}, {128, 128, 1.5f, 0.6f, 0.86f}, {128, 64, 1.f, 0.4f, 0.5f}};
+      switch (cheapest_tile(a.M, a.N, a.nk, kTiles, 3)) {
+        case 0: launch_tiles4<T, 2, 4, 4, 2, 3, false>(a, st); break;
+        case 1: launch_tiles4<T, 2, 2, 2, 2, 3, false>(a, st); break;
+        default: launch_tiles4<T, 2, 1, 2, 2, 4, false>(a, st); break;
+      }
+    }
+  };
+  if (dtype == ATMA_BF16) launch(bf16{});
+  else launch(f16{});
   return check_launch(what);
 }
 

@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "fp8.h"
+#include "gemm_tiles.h"
 
 namespace atma {
 
@@ -63,34 +64,8 @@ __device__ __forceinline__ BiasBits bias_load(const Fp8Args& a, int64_t n, int64
   }
   return b;
 }
-__device__ __forceinline__ float bias_f32(int dtype, uint32_t bits) {
-  if (dtype == ATMA_F32) return __builtin_bit_cast(float, bits);
-  const uint16_t v = (uint16_t)bits;
-  return dtype == ATMA_BF16 ? to_f32(__builtin_bit_cast(bf16, v)) : to_f32(__builtin_bit_cast(f16, v));
-}
 __device__ __forceinline__ float bias_value(const Fp8Args& a, const BiasBits& b, int e) {
   return a.bias ? bias_f32(a.bias_dtype, a.bias_dtype == ATMA_F32 ? b.w[e] : b.v[e]) : 0.f;
-}
-
-// Outputs n0 .. n0 + 7 of a row that ends at N.  Rows of odd widths start at any element: the vector stores take any address
-// (elements one by one cost 184 us instead of 109 at 28,106 x 1,712 -> 1,557); whole: the
-// tile has every feature
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
-typedef u32x2 u32x2_any __attribute__((aligned(2)));
-__device__ __forceinline__ void store_out8(uint16_t* y, const u32x4& o, bool whole, int64_t n0, int64_t N) {
-  if (whole || n0 + 8 <= N) {
-    *(u32x4_any*)y = o;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (n0 + e < N) y[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
-  }
-}
-
-// relu(a)^2 * gate in fp32 (v_maximum3_f32: NaN passes through, as torch's relu)
-__device__ __forceinline__ float gate_act(float av, float gv) {
-  const float pos = __builtin_elementwise_maximum(av, 0.f);
-  return gv * (pos * pos);
 }
 
 // Rows of 128 bytes in LDS, eight chunks of 16, chunk c of row r at position c ^ f(r): the 16 lanes that read one chunk of
@@ -98,7 +73,6 @@ __device__ __forceinline__ float gate_act(float av, float gv) {
 // cycles are conflicts; tiles of 16 tokens a wave lose 5% to their scales, which lie 256 bytes apart).  The weights are
 // the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token (row 8 q + 4 h + e
 // is feature 16 h + 4 q + e; lane half h holds the rows 4 h + e of each 8): outputs are stored straight from registers.
-__device__ __forceinline__ int x_swizzle(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int w_swizzle(int r) { return ((r >> 1) & 3) | (((r >> 4) & 1) << 2); }
 
 // The kernel's arguments read again where they are needed: kept in scalar registers through the loop they would be spilled
@@ -107,31 +81,6 @@ __device__ __forceinline__ LateArgs late_args() {
   LateArgs p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
   return p;
-}
-
-// The 4-byte copy where a descriptor may just have been read back from a vector register: five wait states before it
-__device__ __forceinline__ void dma_buf4_rare(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_byte_offset) {
-  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(r),
-               "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
-               : "memory");
-}
-// A byte a lane, from an address a lane, to the word at lds_byte_offset + 4 lane
-__device__ __forceinline__ void dma_load1_at(const void* p, uint32_t lds_byte_offset) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(p),
-               "{m0}"(__builtin_amdgcn_readfirstlane(lds_byte_offset))
-               : "memory");
-}
-
-// Tile u of an XCD: each owns a contiguous range, walked as groups of four token tiles x all feature tiles
-template <typename C, typename A>
-__device__ __forceinline__ bool fp8_tile_at(const A& a, int xcd, int u, int64_t& m0, int64_t& f0) {
-  const int t = xcd * a.per_xcd + u;
-  if (u >= a.per_xcd || t >= a.m_tiles * a.f_tiles) return false;
-  const int grp = t / (4 * a.f_tiles), r = t - grp * 4 * a.f_tiles;
-  const int gm = min(4, a.m_tiles - 4 * grp);
-  m0 = (int64_t)(4 * grp + r % gm) * C::BM;
-  f0 = (int64_t)(r / gm) * C::OF;
-  return true;
 }
 
 __device__ __forceinline__ f32x4 mfma_fp8(const Frag8& w, const Frag8& x, const f32x4& c, int ws, int xs) {
@@ -182,7 +131,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
   const int nk = a.nk;
   int64_t m0, f0;
   int u = blockIdx.x >> 3;
-  if (!fp8_tile_at<C>(a, blockIdx.x & 7, u, m0, f0)) return;
+  if (!gemm_tile_at<C>(a, blockIdx.x & 7, u, m0, f0)) return;
 
   // ---- the copies, NS blocks ahead.  Copy i of a wave moves rows 8 (i NW + wave) .. + 7: lane l writes row l / 8,
   // position l % 8, and reads the chunk that belongs there; out of range (chunks past K, rows past the end, everything
@@ -225,7 +174,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
     int64_t nm0, nf0;
     pk = 0;
     pu += gridDim.x >> 3;
-    if (fp8_tile_at<C>(*late_args(), blockIdx.x & 7, pu, nm0, nf0)) aim(nm0, nf0);
+    if (gemm_tile_at<C>(*late_args(), blockIdx.x & 7, pu, nm0, nf0)) aim(nm0, nf0);
     else plimit = 0;
   };
   uint32_t pd, pwv, pxv;
@@ -460,7 +409,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp8_tile_kernel(Fp8Args a) {
       }
     }
     u += gridDim.x >> 3;
-    if (!fp8_tile_at<C>(*late_args(), blockIdx.x & 7, u, m0, f0)) break;
+    if (!gemm_tile_at<C>(*late_args(), blockIdx.x & 7, u, m0, f0)) break;
   }
   wait_vmcnt<0>();  // no copy outlives its workgroup's LDS
 }
@@ -683,36 +632,16 @@ static int check_fp8(const char* what, Fp8Args& a, int64_t rows) {
   return ATMA_OK;
 }
 
-// What a tile shape costs: us a tile to begin and end it, and us a block of K, where few CUs work (latency) and where all do.
-// Fitted to 30 shapes of 64 to 4,096 rows, 300 to 8,192 features and K 512 to 4,096, which it orders as measured but for
-// differences under 10% (us: 1,000 x 1,024 -> 4,096 17.1 / 10.1 / 12.6 / 13.0 for 256 x 256, 128 x 128, 64 x 128 and 64 x 64,
-// 4,000 x 512 -> 8,192 30 / 33 / 52 / 54, 64 x 4,096 -> 1,024 37 / 17.5 / 14.5 / 12.5; gated 777 x 1,024 -> 4,096 17.7 / 11.6 /
-// 15.6 for 256, 128 and 64 tokens, 5,000 x 4,096 -> 1,024 47 / 60 / 59, 64 x 1,024 -> 4,096 15.0 / 9.6 / 8.2).
-struct TileCost {
-  int features, tokens;
-  float tile, few, all;
-};
-
-static int cheapest(const Fp8Args& a, const TileCost* c, int n) {
-  const float cus = (float)device_cu_count();
-  int best = 0;
-  float least = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const int64_t tiles = ((a.M + c[i].tokens - 1) / c[i].tokens) * ((a.N + c[i].features - 1) / c[i].features);
-    const float fill = (float)tiles / cus;
-    float t;
-    if (fill <= 1.f) t = c[i].tile + (float)a.nk * (c[i].few + (c[i].all - c[i].few) * fill);
-    else t = ceilf(fill) * (c[i].tile + (float)a.nk * c[i].all);
-    if (i == 0 || t < least) best = i, least = t;
-  }
-  return best;
-}
-
 template <typename T, int MT, int FT, int NW = 4, int NS = 2>
 static void launch_few(const Fp8Args& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.N + 16 * FT - 1) / (16 * FT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
   fp8_few_kernel<T, MT, FT, NW, NS><<<grid, dim3(64 * NW), 0, s>>>(a);
 }
+
+// The tiles' costs (TileCost), here and for the gated form, were fitted to 30 shapes of 64 to 4,096 rows, 300 to 8,192 features
+// and K 512 to 4,096, which they order as measured but for differences under 10% (us: 1,000 x 1,024 -> 4,096 17.1 / 10.1 / 12.6 / 13.0 for 256 x 256, 128 x 128, 64 x 128 and 64 x 64,
+// 4,000 x 512 -> 8,192 30 / 33 / 52 / 54, 64 x 4,096 -> 1,024 37 / 17.5 / 14.5 / 12.5; gated 777 x 1,024 -> 4,096 17.7 / 11.6 /
+// 15.6 for 256, 128 and 64 tokens, 5,000 x 4,096 -> 1,024 47 / 60 / 59, 64 x 1,024 -> 4,096 15.0 / 9.6 / 8.2).
 
 // The kernels of a product, in the order of the codes that atma_linear_fp8_form and atma_linear_gated_fp8_form return
 enum LinearForm { kFew16x16, kFew32x16, kFew16x32, kFew32x32, kTile256x256, kTile128x128, kTile64x128, kTile64x64 };
@@ -734,7 +663,7 @@ static int linear_form(const Fp8Args& a) {
                                          {128, 128, 1.2f, 0.50f, 0.72f},
                                          {64, 128, 1.3f, 0.36f, 0.42f},
                                          {64, 64, 0.7f, 0.32f, 0.30f}};
-  return kTile256x256 + cheapest(a, kTiles, 4);
+  return kTile256x256 + cheapest_tile(a.M, a.N, a.nk, kTiles, 4);
 }
 
 template <typename T>
@@ -759,7 +688,7 @@ static int gated_form(const Fp8Args& a) {
   static constexpr TileCost kTiles[3] = {{128, 256, 5.0f, 1.00f, 1.60f},
                                          {128, 128, 1.7f, 0.70f, 0.98f},
                                          {128, 64, 1.3f, 0.53f, 0.63f}};
-  return kGatedTile256 + cheapest(a, kTiles, 3);
+  return kGatedTile256 + cheapest_tile(a.M, a.N, a.nk, kTiles, 3);
 }
 
 static void launch_gated(const Fp8Args& a, hipStream_t s) {

@@ -1,12 +1,14 @@
 """The 4-bit weights where no GPU is needed: refusals, at the Python entry points and at the C ABI, and the oracle's own rules."""
 
 import ctypes
+import subprocess
 
 import pytest
 import torch
 
-from atma_amd import _lib
+from atma_amd import _build, _lib
 from oracle import fp4 as O
+from tests.test_copy_hazards import check_assembly
 
 E8 = torch.float8_e8m0fnu
 BF = torch.bfloat16
@@ -89,9 +91,23 @@ def test_c_refusals():
         assert linear(**{name: None}) == [1, 1]
     assert linear(x=at + 2) == [1, 1] and linear(ldx=68) == [1, 1] and linear(ldx=56) == [1, 1]
     assert linear(w=at + 8) == [1, 1] and linear(ldw=40) == [1, 1] and linear(ldw=16) == [1, 1] and linear(ldws=-1) == [1, 1]
+    assert linear(ldy=15) == [1, 1]
     assert linear(ldx=(1 << 22) + 8) == [2, 2] and linear(ldw=(1 << 23) + 16) == [2, 2]
     assert linear(bias=at, bias_dtype=9) == [2, 2] and linear(bias=at + 1) == [1, 1]
     assert linear(M=0, x=None) == [0, 0]
+
+
+def test_copies_have_their_wait_states(tmp_path):
+    src, out = _build.CSRC / "fp4_gemm.hip", tmp_path / "out.s"
+    proc = subprocess.run([*_build.compile_command(src), "--cuda-device-only", "-S", str(src), "-o", str(out)],
+                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert proc.returncode == 0, proc.stdout[-2000:]
+    # the copies of a byte, two and four from an address a lane have the 16-byte form's operands: m0 and vector registers
+    text = out.read_text()
+    for form in ("ubyte", "ushort", "dword"):
+        text = text.replace(f"global_load_lds_{form} ", "global_load_lds_dwordx4 ")
+    found, copies = check_assembly(text)
+    assert found == [] and copies > 0, "\n".join(found[:20])
 
 
 def test_oracle_rounds_to_the_nearest():
