@@ -50,10 +50,16 @@ __device__ __forceinline__ LateArgs4 late_args4() {
 // ------------------------------------------------------------------------------------------------ tiles
 // A workgroup of WF x WM waves owns BF weight rows x BM tokens, a wave TF x TM tiles of 32 x 32.  K runs in blocks of 64 through a
 // ring of NS stages in LDS, filled by direct copies.  A block is four steps of 16 k a lane half: while the products of a
-// step run from registers, the tokens of the next step are read, each into the registers of the one just used, and the
-// next step's weights converted into a second set; in the last step the next block's weights are read, still packed, and
-// the copies of block k + NS go into the stage just read.  The workgroup is persistent and all of this runs on across its
-// tiles: a tile's first copies fly and its first operands are read during the last blocks of the one before.
+// step run from registers, the operands of the next one are read into a second set, the weights converted.  Before the last step
+// the waves meet: the next block has landed, this one's stage is free, and the copies of block k + NS go there over the next
+// four steps.  The workgroup is persistent and all of this runs on across its tiles: a tile's first copies fly and its
+// first operands are read during the last blocks of the one before.
+//
+// A block of 256 x 256 takes 2,760 cycles, 2,048 of them products: two waves share a SIMD, and while one runs its steps
+// at 1.1 to 1.3 times the time of their products, what both lose lies behind the barrier.  Measured without gain: products ahead
+// of the reads in each step, a higher priority for the products, the weights' conversion behind the last step's products,
+// 128 x 64 tiles a wave instead of 64 x 128 (twice the conversions, two thirds of the reads).  65,536 x 4,096 -> 1,024 430 us, where the
+// library's 16-bit product takes 356.
 //
 // The weights are the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token
 // (row 8 q + 4 h + e is feature 16 h + 4 q + e).  Their rows are 32 bytes in LDS, chunk c of row r at position
@@ -65,13 +71,14 @@ struct Fp4Tile {
   static constexpr int OF = GATED ? BF / 2 : BF;  // output features
   static constexpr int TO = GATED ? TF / 2 : TF;  // tiles of output features a wave
   static constexpr int W = BM * 128, STAGE = W + BF * 32;
-  static constexpr int XCOPY = BM / 8 / NW, COPIES = XCOPY + 1;  // a wave and block: 8 token rows each, 32 weight rows
+  static constexpr int COPIES = 2 + BM / 8 / NW;  // a wave and block: scales, 32 weight rows, 8 token rows each
+  static constexpr int FIRST = COPIES / 4;        // of them in the last step of a block
   static constexpr int RING = NS + 2;    // blocks and tiles under way: copies run NS blocks ahead
   static constexpr int SLOT = NW * 256;  // a block's scales, in words: two a weight row
   static constexpr int AUX = NS * STAGE, BIAS = AUX + RING * SLOT, TURN = BIAS + RING * 1024, LDS = TURN + 2048 * NW;
   static_assert(BF == 32 * NW && BM % (8 * NW) == 0 && BF <= 256 && NW > 2, "whole copies, a bias of 1 KiB, copied by wave 2");
   static_assert(!GATED || TF % 2 == 0, "a gated wave has its features' a and gate rows");
-  static_assert(NS >= 3 && (NS - 2) * (COPIES + 1) < 63, "vmcnt counts to 63");
+  static_assert(NS >= 3 && (NS - 1) * COPIES < 63, "vmcnt counts to 63");
 };
 
 template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
@@ -133,8 +140,12 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
     else plimit = 0;
   };
   uint32_t pd, pxv, pwv;
+  uint32_t ps;
+  const uint8_t* pscale;
   auto copies_begin = [&]() {
-    dma_load1_at(scales + max(0, min(2 * pk + (lane & 1), plimit / kFp4Group - 1)), lds0 + C::AUX + C::SLOT * pslot + 256 * wave);
+    if (pk == nk) next_tile();
+    pscale = scales + max(0, min(2 * pk + (lane & 1), plimit / kFp4Group - 1));
+    ps = lds0 + C::AUX + C::SLOT * pslot + 256 * wave;
     pslot = pslot + 1 == C::RING ? 0 : pslot + 1;
     pd = lds0 + pstage * C::STAGE + 1024 * wave;
     pstage = pstage + 1 == NS ? 0 : pstage + 1;
@@ -143,8 +154,9 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
     pwv = k + 2 * wk < plimit ? wv0 + (uint32_t)k / 2 : 0x80000000u;
   };
   auto copy = [&](int i) {
-    if (i < C::XCOPY) dma_buf16_at(xr, pxv + i * xstep, 0u, pd + 1024 * C::NW * i);
-    else dma_buf16_at(wr, pwv, 0u, pd + C::W);
+    if (i == 0) dma_load1_at(pscale, ps);
+    else if (i == 1) dma_buf16_at(wr, pwv, 0u, pd + C::W);
+    else dma_buf16_at(xr, pxv + (i - 2) * xstep, 0u, pd + 1024 * C::NW * (i - 2));
   };
 
   // ---- operand reads
@@ -157,25 +169,30 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) xofs[j] = (uint32_t)((32 * TM * wm + r) * 128 + 16 * ((4 * h + j) ^ x_swizzle(r)));
   f32x16 acc[TF][TM];
-  u32x4 raw[TF], wv[2][TF], xv[TM];
+  u32x4 raw[TF], wv[2][TF], xv[2][TM];
   uint32_t code[TF];
   int stage = 0, slot = 0, tile = 0;  // what is read next
   auto read_w = [&](const uint8_t* base, int t) {
     raw[t] = *(const u32x4*)(base + wofs + 32 * wtile(t));
     code[t] = *(const uint32_t*)(lds + sofs + C::SLOT * slot + 8 * wtile(t));
   };
-  auto convert = [&](int s, int j, int t) { wv[s][t] = fp4_unpack8<T>(raw[t][j], __builtin_bit_cast(float, code[t] << 23)); };
-  auto read_x = [&](const uint8_t* base, int j, int t) { xv[t] = *(const u32x4*)(base + xofs[j] + 4096 * t); };
+  auto convert = [&](int s, int j, int t) {
+    wv[s][t] = fp4_unpack8<T>(raw[t][j], __builtin_bit_cast(float, code[t] << 23));
+    asm volatile("" : "+v"(wv[s][t]));  // here, not where it is used
+  };
+  auto read_x = [&](const uint8_t* base, int j, int t) { xv[j & 1][t] = *(const u32x4*)(base + xofs[j] + 4096 * t); };
 
   aim(m0, f0);
 #pragma unroll 1
-  for (int i = 0; i < NS; ++i) {
-    if (pk == nk) next_tile();
+  for (int i = 0; i < NS - 1; ++i) {
     copies_begin();
 #pragma unroll
     for (int c = 0; c < C::COPIES; ++c) copy(c);
   }
-  wait_vmcnt<(NS - 1) * (C::COPIES + 1)>();
+  copies_begin();
+#pragma unroll
+  for (int c = 0; c < C::FIRST; ++c) copy(c);
+  wait_vmcnt<(NS - 2) * C::COPIES + C::FIRST>();
   lds_barrier();
 #pragma unroll
   for (int t = 0; t < TF; ++t) read_w(lds, t);
@@ -209,34 +226,32 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
     tile = tile + 1 == C::RING ? 0 : tile + 1;
 
     for (int kb = 0; kb < nk; ++kb) {
-      if (pk == nk) next_tile();
       const uint8_t* base = lds + stage * C::STAGE;
       stage = stage + 1 == NS ? 0 : stage + 1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (j == 3) {
           // the next block's copies have landed in every wave, and every wave has read this block
-          wait_vmcnt<(NS - 2) * (C::COPIES + 1)>();
+          wait_vmcnt<(NS - 2) * C::COPIES>();
           lds_barrier();
           base = lds + stage * C::STAGE;
-          copies_begin();
         }
 #pragma unroll
         for (int m = 0; m < TM; ++m) {
           __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int t = 0; t < TF; ++t) acc[t][m] = mfma32<T>(wv[j & 1][t], xv[m], acc[t][m]);
-          // behind the products of token tile m: its operand of the next step, a share of the weights and copies
+          // ahead of the products of token tile m: a share of the next step's operands, all of them in the first half of the step
           if (j == 3 && m == 0) {
 #pragma unroll
             for (int t = 0; t < TF; ++t) read_w(base, t);
             slot = slot + 1 == C::RING ? 0 : slot + 1;
           }
-          read_x(base, (j + 1) & 3, m);
-          if (j == 3) {
 #pragma unroll
-            for (int c = m * C::COPIES / TM; c < (m + 1) * C::COPIES / TM; ++c) copy(c);
-          }
+          for (int t = 2 * m; t < min(2 * m + 2, TM); ++t) read_x(base, (j + 1) & 3, t);
+#pragma unroll
+          for (int t = 0; t < TF; ++t) acc[t][m] = mfma32<T>(wv[j & 1][t], xv[j & 1][m], acc[t][m]);
+          const int q = (j + 1) & 3, c0 = q * C::COPIES / 4, c1 = (q + 1) * C::COPIES / 4;  // this step's copies
+#pragma unroll
+          for (int c = c0 + m * (c1 - c0) / TM; c < c0 + (m + 1) * (c1 - c0) / TM; ++c) copy(c);
           // (the last step's first half waits for the next block's weights)
           const int from = j == 3 ? max(0, 2 * m - TM) : m, share = j == 3 && TM > 1 ? 2 : 1;
           if (j != 3 || TM == 1 || 2 * m >= TM) {
@@ -245,6 +260,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
               if (t >= from * TF / TM && t < (from + share) * TF / TM) convert((j + 1) & 1, (j + 1) & 3, t);
           }
         }
+        if (j == 2) copies_begin();  // (the addresses: nothing keeps the products behind the barrier waiting)
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -292,32 +308,196 @@ __device__ __forceinline__ float fp4_bias(const Fp4Args& a, int64_t n) {
   return bias_f32(a.bias_dtype, a.bias_dtype == ATMA_F32 ? ((const uint32_t*)a.bias)[n] : ((const uint16_t*)a.bias)[n]);
 }
 
-// A wave owns 16 features x 16 tokens; lane (r, g) holds row r of both operands, k = 8 g .. + 7 of each 32
-template <typename T, bool GATED>
-__global__ void __launch_bounds__(64) fp4_kernel(Fp4Args a) {
-  const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-  const int64_t f0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
-  const T* x = (const T*)a.x + min(m0 + r, a.M - 1) * a.ldx + 8 * g;
-  f32x4 acc[GATED ? 2 : 1] = {};
-  for (int kb = 0; kb < a.K; kb += 32) {
-    const u32x4 xv = *(const u32x4*)(x + kb);
+// ------------------------------------------------------------------------------------------------ few rows
+// Up to 16 MT tokens at a time: latency and the stream of weights.  A wave owns FT tiles of 16 features (gated: 16 a rows and the
+// gate rows of the same features), or one of `splits` shares of their K, whose sums are joined through LDS in a fixed order.
+// It has a ring of its own of NS blocks of 256 k, filled by direct copies of whole 128-byte lines of the weights, and waits
+// for nothing but its own copies.  The tokens lie in LDS, all of K, copied once (RING: where they do not fit, a
+// block of them comes with each block of weights).  A workgroup walks over its tiles, and the ring runs on across them.
+//
+// v_mfma_f32_16x16x32: lane (r, g) takes chunks g and g + 4 of a weight row's eight, one group of 32 k each with its scale, and
+// the same k of token r.  Chunk c of a weight row lies at position c ^ (r / 2) % 8, chunk c of a token's row at c ^ r % 16.
+constexpr int kFewBlock = 256;
+constexpr int kFewTokens = 64 * 1024;  // LDS for the tokens
+
+struct Fp4FewArgs {
+  Fp4Args a;
+  int tiles, log_splits;  // tiles of 16 FT weight rows (gated: of 16 features); splits of K, a power of two up to the blocks of K
+};
+
+template <int MT, int FT, int NW, bool RING>
+struct Fp4Few {
+  static constexpr int NS = RING ? 2 : 4;
+  static constexpr int WCOPY = 2 * FT, XCOPY = RING ? 8 * MT : 0, COPIES = 2 * WCOPY + XCOPY;
+  static constexpr int X = FT * (2048 + 512), STAGE = X + 1024 * XCOPY;
+  static constexpr int TOKENS = NW * NS * STAGE, RED = TOKENS + (RING ? 0 : kFewTokens), LDS = RED + NW * FT * MT * 1024;
+};
+
+template <typename T, int MT, int FT, int NW, bool RING, bool GATED>
+__global__ void __launch_bounds__(64 * NW) fp4_few_kernel(Fp4FewArgs f) {
+  using C = Fp4Few<MT, FT, NW, RING>;
+  constexpr int NS = C::NS, OT = GATED ? 1 : FT;  // tiles of output features
+  const Fp4Args& a = f.a;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int ls = f.log_splits, splits = 1 << ls, share = wave & (splits - 1), nk = a.nk;
+  const int64_t m0 = (int64_t)blockIdx.y * 16 * MT;
+  const int rows = (int)min((int64_t)16 * MT, a.M - m0);
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc((const uint16_t*)a.x + m0 * a.ldx, (uint32_t)(rows * 2 * a.ldx));
+  const uint32_t ring0 = lds_offset(lds) + wave * NS * C::STAGE;
+  auto tile_of = [&](int it) { return ((it << (31 - __builtin_clz(NW) - ls)) + (wave >> ls)) * (int)gridDim.x + (int)blockIdx.x; };
+
+  // ---- the weights' copies.  Copy i of a block moves rows 8 i .. + 7, lane l the chunk that belongs at position l % 8 of row
+  // l / 8; the scales' copies the same rows' codes, lane l group l % 8.  Chunks past K, rows past the end and tiles past the last
+  // one are zeros, scales there the nearest ones
+  const int crow = lane >> 3;
+  __amdgpu_buffer_rsrc_t wr[2];
+  const uint8_t* codes[2 * FT];
+  int pit = 0, pkb = share, plimit = 0;
+  auto aim = [&]() {
+    const int tile = tile_of(pit);
+    plimit = tile < f.tiles ? a.K : 0;
+    const int64_t n0 = min((int64_t)tile * 16 * OT, a.N - 1);
+    wr[0] = buffer_rsrc(a.w + n0 * a.ldw, (uint32_t)(min((int64_t)16 * OT, a.N - n0) * a.ldw));
+    if constexpr (GATED) wr[1] = buffer_rsrc(a.w + (a.N + n0) * a.ldw, (uint32_t)(min((int64_t)16, a.N - n0) * a.ldw));
 #pragma unroll
-    for (int t = 0; t < (GATED ? 2 : 1); ++t) {
-      const int64_t n = min(f0 + r, a.N - 1) + t * a.N;
-      const uint32_t w = *(const uint32_t*)(a.w + n * a.ldw + kb / 2 + 4 * g);
-      acc[t] = mfma16x16x32<T>(fp4_unpack8<T>(w, fp4_scale(a.ws[n * a.ldws + kb / kFp4Group])), xv, acc[t]);
+    for (int i = 0; i < 2 * FT; ++i) {
+      const int64_t n = GATED && i >= 2 ? a.N + min(n0 + 8 * (i - 2) + crow, a.N - 1) : min(n0 + 8 * i + crow, a.N - 1);
+      codes[i] = a.ws + n * a.ldws;
+    }
+  };
+  auto copies = [&](int slot) {
+    const uint32_t d = ring0 + slot * C::STAGE;
+    const int k0 = kFewBlock * pkb, group = min(8 * pkb + (lane & 7), a.K / kFp4Group - 1);
+#pragma unroll
+    for (int i = 0; i < 2 * FT; ++i) {
+      const int row = 8 * i + crow, at = GATED ? row & 15 : row;
+      const int chunk = (lane & 7) ^ x_swizzle(row);
+      const uint32_t v = (uint32_t)at * (uint32_t)a.ldw + 128u * (uint32_t)pkb + 16u * (uint32_t)chunk;
+      dma_buf16_at(wr[GATED ? i / 2 : 0], k0 + 32 * chunk < plimit ? v : 0x80000000u, 0u, d + 1024 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * FT; ++i) dma_load1_at(codes[i] + group, d + FT * 2048 + 256 * i);
+    if constexpr (RING) {
+      // two token rows of 512 bytes a copy
+#pragma unroll
+      for (int i = 0; i < C::XCOPY; ++i) {
+        const int row = 2 * i + (lane >> 5), chunk = (lane & 31) ^ (row & 15);
+        const uint32_t v = (uint32_t)row * (uint32_t)(2 * a.ldx) + 512u * (uint32_t)pkb + 16u * (uint32_t)chunk;
+        dma_buf16_at(xr, k0 + 8 * chunk < plimit ? v : 0x80000000u, 0u, d + C::X + 1024 * i);
+      }
+    }
+    pkb += splits;
+    if (pkb >= nk) {
+      pkb = share;
+      ++pit;
+      aim();
+    }
+  };
+  if constexpr (!RING) {
+    // chunk i of the tokens' rows, 32 nk chunks each
+    const int per = 32 * nk, total = rows * per;
+    for (int i0 = 64 * wave; i0 < total; i0 += 64 * NW) {
+      const int i = i0 + lane, row = i / per, at = i - row * per, chunk = at ^ (row & 15);
+      dma_buf16_at(xr, row < rows && 8 * chunk < a.K ? (uint32_t)row * (uint32_t)(2 * a.ldx) + 16u * (uint32_t)chunk : 0x80000000u,
+                   0u, lds_offset(lds) + C::TOKENS + 16 * i0);
     }
   }
-  const int64_t m = m0 + r;
-  if (m >= a.M) return;
+  aim();
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t n = f0 + 4 * g + e;
-    if (n >= a.N) break;
-    float v = acc[0][e] + fp4_bias(a, n);
-    if constexpr (GATED) v = gate_act(v, acc[1][e] + fp4_bias(a, a.N + n));
-    ((T*)a.y)[m * a.ldy + n] = from_f32<T>(v);
+  for (int i = 0; i < NS; ++i) copies(i);
+  if constexpr (!RING) {
+    wait_vmcnt<NS * C::COPIES>();
+    lds_barrier();  // the tokens are there, from every wave
   }
+
+  int slot = 0;
+  for (int it = 0;; ++it) {
+    const int tile = tile_of(it);
+    if (splits == 1 ? tile >= f.tiles : tile_of(it) - (wave >> ls) * (int)gridDim.x >= f.tiles) break;  // (the same for every wave that joins)
+    const int64_t n0 = (int64_t)tile * 16 * OT + 4 * g;
+    f32x4 acc[FT][MT] = {};
+    for (int kb = share; kb < nk; kb += splits) {
+      wait_vmcnt<(NS - 1) * C::COPIES>();
+      const uint8_t* base = lds + wave * NS * C::STAGE + slot * C::STAGE;
+      u32x4 raw[2][FT], xv[2][MT][4];
+      uint32_t code[2][FT];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int t = 0; t < FT; ++t) {
+          raw[q][t] = *(const u32x4*)(base + 2048 * t + 128 * r + 16 * ((4 * q + g) ^ x_swizzle(r)));
+          code[q][t] = *(const uint32_t*)(base + FT * 2048 + 512 * t + 32 * r + 4 * (4 * q + g));
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          const int row = RING ? 16 * j + r : min(16 * j + r, rows - 1);
+          const uint8_t* xp = RING ? base + C::X + 512 * row : lds + C::TOKENS + 512 * (row * nk + kb);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) xv[q][j][e] = *(const u32x4*)(xp + 16 * ((16 * q + 4 * g + e) ^ (row & 15)));
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the copies that overwrite them start
+      copies(slot);
+      slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int t = 0; t < FT; ++t) {
+          const float scale = __builtin_bit_cast(float, code[q][t] << 23);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const u32x4 wv = fp4_unpack8<T>(raw[q][t][e], scale);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[t][j] = mfma16x16x32<T>(wv, xv[q][j][e], acc[t][j]);
+          }
+        }
+    }
+    if (splits > 1) {
+      auto red = (f32x4(*)[FT][MT][64])(lds + C::RED);
+#pragma unroll
+      for (int t = 0; t < FT; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) red[wave][t][j][lane] = acc[t][j];
+      lds_barrier();
+    }
+    // every share stores some of the outputs
+#pragma unroll
+    for (int o = 0; o < OT * MT; ++o) {
+      if ((o & (splits - 1)) != share) continue;
+      const int t = o / MT, j = o % MT;
+      f32x4 v = acc[t][j], gate = acc[FT - 1][j];
+      if (splits > 1) {
+        auto red = (const f32x4(*)[FT][MT][64])(lds + C::RED);
+        const int first = wave & ~(splits - 1);
+        v = red[first][t][j][lane];
+        gate = red[first][FT - 1][j][lane];
+        for (int q = 1; q < splits; ++q) {
+          v += red[first + q][t][j][lane];
+          if constexpr (GATED) gate += red[first + q][FT - 1][j][lane];
+        }
+      }
+      const int64_t m = m0 + 16 * j + r, n = n0 + 16 * t;
+      if (16 * j + r >= rows || n >= a.N) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t ne = min(n + e, a.N - 1);
+        v[e] += fp4_bias(a, ne);
+        if constexpr (GATED) v[e] = gate_act(v[e], gate[e] + fp4_bias(a, a.N + ne));
+      }
+      T* y = (T*)a.y + m * a.ldy + n;
+      if (n + 4 <= a.N) {
+        *(u32x2_any*)y = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < a.N) y[e] = from_f32<T>(v[e]);
+      }
+    }
+    if (splits > 1) lds_barrier();  // the sums are read before the next tile's are written
+  }
+  wait_vmcnt<0>();  // no copy outlives its workgroup's LDS
 }
 
 template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
@@ -330,6 +510,34 @@ static void launch_tiles4(Fp4Args a, hipStream_t s) {
   constexpr int per_cu = 160 * 1024 / C::LDS;
   const int64_t wgs = std::min<int64_t>((int64_t)device_cu_count() / 8 * 8 * per_cu, 8 * (int64_t)a.per_xcd);
   fp4_tile_kernel<T, TF, TM, WF, WM, NS, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
+}
+
+template <typename T, int MT, int FT, int NW, bool RING, bool GATED>
+static void launch_few4(const Fp4Args& a, hipStream_t s) {
+  using C = Fp4Few<MT, FT, NW, RING>;
+  Fp4FewArgs f{a, (int)((a.N + 16 * (GATED ? 1 : FT) - 1) / (16 * (GATED ? 1 : FT))), 0};
+  f.a.nk = (a.K + kFewBlock - 1) / kFewBlock;
+  const int cus = device_cu_count(), groups = (int)((a.M + 16 * MT - 1) / (16 * MT));
+  // K is split among a workgroup's waves while every workgroup still finds a CU
+  while ((2 << f.log_splits) <= std::min(NW, f.a.nk) && (int64_t)f.tiles * groups * (2 << f.log_splits) <= (int64_t)cus * NW)
+    ++f.log_splits;
+  const int at_once = NW >> f.log_splits;  // tiles of a workgroup
+  const int wgs = std::min((f.tiles + at_once - 1) / at_once, std::max(1, cus * (160 * 1024 / C::LDS) / groups));
+  fp4_few_kernel<T, MT, FT, NW, RING, GATED><<<dim3((unsigned)wgs, (unsigned)groups), dim3(64 * NW), 0, s>>>(f);
+}
+
+template <typename T, bool GATED>
+static void launch_rows4(const Fp4Args& a, hipStream_t s) {
+  constexpr int FT = GATED ? 2 : 1, NW = GATED ? 4 : 8;
+  const int64_t per = (a.K + kFewBlock - 1) / kFewBlock * 512;  // LDS for a token
+  if (std::min<int64_t>(a.M, 16) * per > kFewTokens) {
+    if (GATED || a.M <= 16) launch_few4<T, 1, FT, 4, true, GATED>(a, s);
+    else launch_few4<T, 2, 1, 4, true, false>(a, s);
+  } else if (a.M <= 16 || std::min<int64_t>(a.M, 32) * per > kFewTokens) {
+    launch_few4<T, 1, FT, NW, false, GATED>(a, s);
+  } else {
+    launch_few4<T, 2, FT, NW, false, GATED>(a, s);
+  }
 }
 
 static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dtype, void* stream) {
@@ -359,9 +567,8 @@ static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dt
   auto launch = [&](auto zero) {
     using T = decltype(zero);
     if (a.M <= 32) {
-      const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 15) / 16));
-      if (gated) fp4_kernel<T, true><<<grid, 64, 0, st>>>(a);
-      else fp4_kernel<T, false><<<grid, 64, 0, st>>>(a);
+      if (gated) launch_rows4<T, true>(a, st);
+      else launch_rows4<T, false>(a, st);
     } else if (gated) {
       static constexpr TileCost kTiles[3] = {{128, 256, 5.f, 1.15f, 1.72f}, {64, 128, 1.5f, 0.6f, 0.86f}, {64, 64, 1.f, 0.4f, 0.5f}};
       switch (cheapest_tile(a.M, a.N, a.nk, kTiles, 3)) {
