@@ -81,11 +81,12 @@ def test_all_filters(dev, V, dtype):
         _check(dev, logits, u, t, *sel, doubtful=1)
 
 
+@pytest.mark.parametrize("V", [3000, 20000])
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
-def test_many_equal_logits(dev, dtype):
+def test_many_equal_logits(dev, dtype, V):
     """Borders inside runs of equal logits: the lowest indices are kept."""
     g = torch.Generator().manual_seed(1)
-    V, rows = 3000, 16
+    rows = 16
     logits = torch.randint(-3, 3, (rows, V), generator=g).to(dtype)
     logits[3] = 1.5
     u = [(r + 0.5) / rows for r in range(rows)]
@@ -94,6 +95,20 @@ def test_many_equal_logits(dev, dtype):
     p = [(r + 0.37) / rows for r in range(rows)]
     _check(dev, logits, u, [0.8] * rows, None, p, doubtful=1)
     _check(dev, logits, u, [0.8] * rows, k, p, doubtful=1)
+
+
+@pytest.mark.parametrize("V", [2000, 30000])
+def test_logits_close_together_and_far_apart(dev, V):
+    """Ranges of logits from far below a temperature to far above it, and rows of which a few tokens have all the weight."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(12, V, generator=g) * torch.tensor([1e-6, 1e-4, 1e-2, 0.1, 1.0, 10.0, 100.0, 1e4, 1e20, 3.0, 3.0, 3.0])[:, None]
+    x[9, 10:] = -math.inf
+    x[10, 5:] -= 200
+    x[11, 2000 // 2:] = x[11, 0]
+    u = [(r + 0.4) / 12 for r in range(12)]
+    for k, p in ((None, None), ([40] * 12, None), (None, [0.9] * 12), ([300] * 12, [0.8] * 12)):
+        _check(dev, x, u, [1.0] * 12, k, p, doubtful=1)
+        _check(dev, x.to(HF), u, [0.7] * 12, k, p, [0.05] * 12, doubtful=1)
 
 
 def test_exact_borders(dev):
