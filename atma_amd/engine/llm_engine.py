@@ -2,7 +2,7 @@
 
 ``generate`` adds every prompt, then steps the scheduler until all requests finish:
 one prefill batch or one decode step per ``step()``.  Inside ``generate`` the decode steps
-of an unchanged greedy batch run as a pipeline (``_decode_run``): step n + 1 is launched
+of an unchanged batch, greedy or sampled from random numbers known in advance, run as a pipeline (``_decode_run``): step n + 1 is launched
 before step n's tokens are read back, so the host's accounting of step n overlaps the
 device's work on step n + 1.  Prefill and decode throughput are measured with HIP events
 around each step (around each pipelined run of decode steps) and kept in

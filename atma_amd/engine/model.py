@@ -20,13 +20,14 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from ..kernel import causal_conv1d_decode_step, packed_causal_conv1d, softcap_argmax, softcap_logits
+from ..kernel import (causal_conv1d_decode_step, packed_causal_conv1d, sample_tokens, softcap_argmax,
+                      softcap_logits)
 from ..kernel.decode_fusions import (PartialSums, lfm2_conv_step, linear_tokens_conv, linear_tokens_conv_supported,
                                      residual_rms_norm_supported)
 from ..kernel.layer_fusions import lfm2_conv_packed
 from ..kernel.train_glue import plain_module
 from ..layers.attention import Attention
-from ..layers.global_attention import (MLP, Fp8MLP, GlobalLayerCache, Linear, PolarAttention, RMSNorm,
+from ..layers.global_attention import (MLP, Fp4Linear, Fp4MLP, Fp8MLP, GlobalLayerCache, Linear, PolarAttention, RMSNorm,
                                        decode_rows)
 from .config import AtmaConfig
 from .context import get_context
@@ -229,6 +230,20 @@ class Atma(nn.Module):
             block.mlp = Fp8MLP(block.mlp)
         return self
 
+    def quantize_weights_fp4(self):
+        """Replace every block's MLP and the LM head by their forms with 4-bit weights (``Fp4MLP``, ``Fp4Linear``), for inference; the
+        weights must be on the GPU.  A module that these do not stand for (changed, or of unsuited widths) is refused before
+        any is replaced."""
+        blocks = [block for block in self.blocks if not isinstance(block.mlp, Fp4MLP)]
+        for block in blocks:
+            Fp4MLP.check(block.mlp)
+        if not isinstance(self.proj, Fp4Linear):
+            Fp4Linear.check(self.proj)
+            self.proj = Fp4Linear(self.proj)
+        for block in blocks:
+            block.mlp = Fp4MLP(block.mlp)
+        return self
+
     def init_weights(self, std=0.02, seed=0):
         """Every parameter N(0, std) from ``seed`` (the random-init convention of the
         reference's tests and of BASELINE configs[4]), drawn on the CPU in registration
@@ -240,12 +255,32 @@ class Atma(nn.Module):
         return self
 
 
+class Picks:
+    """How the requests of a step are sampled, where one of them asks for more than a temperature: per-row tensors on the
+    GPU.  ``race``: rows that ask for a temperature alone (bool), or None where there are none."""
+
+    __slots__ = ("uniform", "temperature", "top_k", "top_p", "min_p", "race")
+
+    def __init__(self, uniform, temperature, top_k, top_p, min_p, race=None):
+        self.uniform, self.temperature, self.top_k, self.top_p, self.min_p = uniform, temperature, top_k, top_p, min_p
+        self.race = race
+
+    def sample(self, logits, ids_out=None):
+        """``sample_tokens`` of every row."""
+        return sample_tokens(logits, self.uniform, self.temperature, top_k=self.top_k, top_p=self.top_p, min_p=self.min_p,
+                             ids_out=ids_out)
+
+
 class Sampler(nn.Module):
     """Next-token sampler (``inference/layers/sampler.py:5-10``) with a greedy mode: rows
     whose temperature is 0 take the argmax; the others sample by the reference's
-    exponential race over ``softmax(logits / t)``."""
+    exponential race over ``softmax(logits / t)``, or, where a request sets ``top_k``, ``top_p``, ``min_p`` or a ``seed``
+    (``picks``), by ``sample_tokens``."""
 
-    def forward(self, logits, temperatures, all_greedy=False):
+    def forward(self, logits, temperatures, all_greedy=False, picks=None):
+        if picks is not None:
+            ids = picks.sample(logits)
+            return ids if picks.race is None else torch.where(picks.race, self(logits, temperatures), ids)
         logits = logits.float()
         greedy = logits.argmax(dim=-1)
         if all_greedy:

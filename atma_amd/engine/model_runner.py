@@ -30,7 +30,7 @@ import torch
 from ..layers.attention import Attention
 from .config import Config
 from .context import get_context, reset_context, set_context
-from .model import Atma, Sampler
+from .model import Atma, Picks, Sampler
 from .sequence import Sequence
 
 POLAR_TILE_ROWS = 128    # query rows per tile of the packed Polar launch
@@ -54,11 +54,17 @@ class ModelRunner:
                 load_model(model, config.model, strict=config.strict_weights)
             else:
                 model.init_weights(config.init_std, config.seed)
+        if config.fp8_mlp and config.fp4_weights:
+            raise ValueError("Config.fp8_mlp and Config.fp4_weights exclude each other: both replace the MLPs")
+        if config.fp4_weights and hf.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"Config.fp4_weights serves 16-bit models (got {hf.dtype})")
         if config.fp8_mlp and hf.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"Config.fp8_mlp serves 16-bit models (got {hf.dtype})")
         self.model = model.to(self.device, hf.dtype).eval()
         if config.fp8_mlp:
             self.model.quantize_mlps()
+        if config.fp4_weights:
+            self.model.quantize_weights_fp4()
         self.sampler = Sampler()
         self.last_logits = None
         self.allocate_conv_state_tables()
@@ -167,9 +173,10 @@ class ModelRunner:
 
     def _decode_stage(self, max_bs, max_blocks):
         """One buffer for every decode-step input the graphs read: token ids and table
-        rows (int64), cache slots, context lengths and block tables (int32).  Each step
+        rows (int64), cache slots, context lengths and block tables (int32); and what the sampler
+        reads behind them: random numbers, temperatures, top_p, min_p (fp32) and top_k (int32).  Each step
         fills a pinned host copy (two, used in turn) and sends it with one H2D copy."""
-        n64, n32 = 2 * max_bs, 2 * max_bs + max_bs * max_blocks
+        n64, n32 = 2 * max_bs, 7 * max_bs + max_bs * max_blocks
         nbytes = 8 * n64 + 4 * n32
         dev = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         hosts = [torch.empty(nbytes, dtype=torch.uint8).pin_memory() for _ in range(2)]
@@ -179,7 +186,9 @@ class ModelRunner:
             i32 = buf[8 * n64:].view(torch.int32)
             return dict(input_ids=i64[:max_bs], seq_slots=i64[max_bs:], slot_mapping=i32[:max_bs],
                         context_lens=i32[max_bs:2 * max_bs],
-                        block_tables=i32[2 * max_bs:].view(max_bs, max_blocks))
+                        block_tables=i32[2 * max_bs:n32 - 5 * max_bs].view(max_bs, max_blocks),
+                        top_k=i32[n32 - 5 * max_bs:n32 - 4 * max_bs],
+                        floats=i32[n32 - 4 * max_bs:].view(torch.float32).view(4, max_bs))
         self._stage_dev, self._stage_hosts = dev, hosts
         self._stage_np = [{k: v.numpy() for k, v in views(h).items()} for h in hosts]
         self._stage_key = [None, None]   # the batch whose table rows and slots each host copy holds
@@ -238,9 +247,10 @@ class ModelRunner:
     def can_pipeline(self, seqs):
         """True when decode steps of this batch can be launched ahead of reading back the
         previous step's tokens: captured graphs that take the greedy ids themselves (16-bit
-        models), every request greedy, the batch within the largest bucket."""
+        models), every request greedy or sampled from random numbers known in advance (``SamplingParams.picks``), the batch
+        within the largest bucket."""
         return (self._uses_graph(len(seqs)) and self.graph_out[self.graph_bs[-1]][0][1] is not None
-                and all(s.temperature == 0 for s in seqs))
+                and all(s.temperature == 0 or s.params.picks for s in seqs))
 
     @torch.inference_mode()
     def launch_decode(self, seqs, ahead):
@@ -259,6 +269,10 @@ class ModelRunner:
         self.graph_flip ^= 1
         self.graphs[bucket][g].replay()
         logits, ids = self.graph_out[bucket][g]
+        if any(s.params.picks for s in seqs):
+            v = self.graph_vars
+            u, t, p, m = v["floats"][:, :bs].unbind(0)
+            ids = Picks(u, t, v["top_k"][:bs], p, m).sample(logits[:bs], v["input_ids"][:bs])
         host, done = self._ids_host[self._ids_flip], self._ids_done[self._ids_flip]
         self._ids_flip ^= 1
         host[:bs].copy_(ids[:bs], non_blocking=True)
@@ -301,9 +315,30 @@ class ModelRunner:
         if not ahead:
             h["input_ids"][:bs] = [s.last_token for s in seqs]
         h["context_lens"][:bs] = lens
+        if any(s.params.picks for s in seqs):
+            h["floats"][:, :bs], h["top_k"][:bs] = self._picks(seqs, ahead)
         pos = lens - 1        # the new token's cache slot: its position's row in its position's page
         h["slot_mapping"][:bs] = bt[np.arange(bs), pos // page] * page + pos % page
         return bucket
+
+    @staticmethod
+    def _picks(seqs, ahead=0):
+        """The sampler's rows: (random numbers, temperatures, top_p, min_p) fp32 and top_k int32."""
+        ps = [s.params for s in seqs]
+        return (np.array([[s.uniform(ahead) for s in seqs], [p.temperature for p in ps], [p.top_p for p in ps],
+                          [p.min_p for p in ps]], dtype=np.float32),
+                np.array([min(p.top_k, 2 ** 31 - 1) for p in ps], dtype=np.int32))
+
+    def _sample(self, logits, seqs):
+        """One id per sequence from its logits, as its parameters ask."""
+        temps = [s.temperature for s in seqs]
+        picks = None
+        if any(s.params.picks for s in seqs):
+            floats, top_k = self._picks(seqs)
+            u, t, p, m = self._to_dev(floats, torch.float32).unbind(0)
+            race = [s.temperature != 0 and not s.params.picks for s in seqs]
+            picks = Picks(u, t, self._to_dev(top_k, torch.int32), p, m, self._to_dev(race, torch.bool) if any(race) else None)
+        return self.sampler(logits, self._to_dev(temps, torch.float32), all_greedy=all(t == 0 for t in temps), picks=picks)
 
     def _run_decode_graph(self, seqs):
         """Replay the smallest captured bucket that fits: the step's inputs go in one H2D
@@ -417,8 +452,7 @@ class ModelRunner:
         for seq in seqs:
             if seq.seq_slot < 0:
                 self.alloc_seq_slot(seq)
-        temps = [s.temperature for s in seqs]
-        greedy = all(t == 0 for t in temps)
+        greedy = all(s.temperature == 0 for s in seqs)
         ids = None
         if not is_prefill and self._uses_graph(len(seqs)):
             logits, ids = self._run_decode_graph(seqs)
@@ -427,6 +461,6 @@ class ModelRunner:
             logits = self.run_model(input_ids, positions, is_prefill)
         self.last_logits = logits
         if ids is None or not greedy:
-            ids = self.sampler(logits, self._to_dev(temps, torch.float32), all_greedy=greedy)
+            ids = self._sample(logits, seqs)
         reset_context()
         return ids.tolist()

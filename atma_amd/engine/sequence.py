@@ -9,12 +9,15 @@ runner reads exactly these attributes, under the names the reference's runner re
 and ``temperature``.  The lifecycle (queued -> active -> done) belongs to the scheduler.
 
 ``temperature == 0`` asks for greedy decoding (the reference's sampler divides by the
-temperature and has no greedy form, ``inference/layers/sampler.py:7-10``).
+temperature and has no greedy form, ``inference/layers/sampler.py:7-10``).  ``top_k`` (0: all), ``top_p`` and ``min_p``
+narrow the choice (``sample_tokens``); with a ``seed`` a request draws the same random numbers in every batch.
 """
 
 from dataclasses import dataclass
 from enum import Enum
 from itertools import count
+from random import getrandbits
+from typing import Optional
 
 
 @dataclass(frozen=True)
@@ -22,6 +25,28 @@ class SamplingParams:
     temperature: float = 1.0
     max_tokens: int = 128
     ignore_eos: bool = False
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: Optional[int] = None
+
+    def __post_init__(self):
+        if self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1:
+            raise ValueError(f"top_k >= 0, 0 < top_p <= 1 and 0 <= min_p <= 1 (got {self.top_k}, {self.top_p}, {self.min_p})")
+
+    @property
+    def picks(self):
+        """Whether the request asks for more than a temperature (and not for the likeliest token)."""
+        return self.temperature != 0 and (self.top_k > 0 or self.top_p < 1 or self.min_p > 0 or self.seed is not None)
+
+
+def uniform(seed, n):
+    """The n-th random number of a seed: a multiple of 2^-24 in [0, 1), from the splitmix64 sequence (Steele, Lea and Flood, 2014)."""
+    mask = (1 << 64) - 1
+    z = (seed + (n + 1) * 0x9E3779B97F4A7C15) & mask
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9 & mask
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EB & mask
+    return ((z ^ (z >> 31)) >> 40) * 2.0 ** -24
 
 
 class Phase(Enum):
@@ -38,7 +63,7 @@ class Sequence:
     ``seq[a:b]`` slices them."""
 
     __slots__ = ("seq_id", "token_ids", "prompt_len", "params", "phase", "block_table", "seq_slot",
-                 "num_cached_tokens", "num_scheduled_tokens")
+                 "num_cached_tokens", "num_scheduled_tokens", "_seed")
 
     def __init__(self, token_ids, sampling_params: SamplingParams = None):
         self.seq_id = next(_ids)
@@ -50,6 +75,7 @@ class Sequence:
         self.seq_slot = -1             # row of the runner's state tables (-1: none held)
         self.num_cached_tokens = 0     # tokens whose K/V, conv tails and memory state are stored
         self.num_scheduled_tokens = 0  # tokens the current step feeds
+        self._seed = getrandbits(64) if self.params.seed is None else self.params.seed
 
     def __len__(self):
         return len(self.token_ids)
@@ -60,6 +86,10 @@ class Sequence:
     @property
     def temperature(self):
         return self.params.temperature
+
+    def uniform(self, ahead=0):
+        """The random number of the token that follows ``ahead`` further ones."""
+        return uniform(self._seed, len(self.token_ids) - self.prompt_len + ahead)
 
     @property
     def last_token(self):

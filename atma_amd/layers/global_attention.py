@@ -50,6 +50,7 @@ from ..kernel.decode_fusions import (PartialSums, chunk_width, global_decode_gat
                                      linear_tokens_chunks, linear_tokens_gated, linear_tokens_multi,
                                      linear_tokens_multi_supported,
                                      residual_rms_norm, residual_rms_norm_supported)
+from ..kernel.fp4 import FP4_SCALE, linear_fp4, linear_gated_fp4, quantize_weight_fp4
 from ..kernel.fp8 import (FP8, FP8_SCALE, linear_fp8, linear_gated_fp8, quantize_fp8, quantize_weight_fp8,
                           residual_rms_norm_fp8)
 from ..kernel.gated_delta import gated_delta_prefill, gated_delta_prefill_supported
@@ -809,6 +810,92 @@ class Fp8MLP(nn.Module):
         h, h_scale = linear_gated_fp8(data, scale, self.fc_weight.view(FP8), self.fc_scale.view(FP8_SCALE), self.fc_bias)
         return linear_fp8(h, h_scale, self.proj_weight.view(FP8), self.proj_scale.view(FP8_SCALE), self.proj_bias,
                           out_dtype=dtype)
+
+
+def _plain_linear(linear):
+    """Whether a module is nothing but a ``Linear`` of this file or torch's: no hooks, parametrisations or forward of its own."""
+    return any(plain_module(linear, cls, every=False) for cls in (Linear, nn.Linear))
+
+
+def _hold_fp4(module, name, linear):
+    """The 4-bit form of a projection as buffers of ``module``: bytes, which ``half()`` and ``to(dtype)`` leave alone."""
+    with torch.no_grad():
+        data, scale = quantize_weight_fp4(linear.weight)
+        module.register_buffer(name + "_weight", data)
+        module.register_buffer(name + "_scale", scale.view(torch.uint8))
+        module.register_buffer(name + "_bias", None if linear.bias is None else linear.bias.detach().clone())
+
+
+def _refuse_16_bit_state(module, state_dict, prefix, keys, errors):
+    """A 16-bit checkpoint is an error also where missing and unexpected names are none (``strict=False``): it would leave the
+    weights as they were."""
+    if any(prefix + k in state_dict for k in keys):
+        errors.append(f"{prefix[:-1] or type(module).__name__} holds its weights in 4 bits: load 16-bit ones before it is "
+                      "replaced")
+
+
+class Fp4Linear(nn.Module):
+    """``Linear`` for inference with its weight in 4 bits (``kernel/fp4``) and 16-bit activations.  Made from a ``Linear`` on the
+    GPU; 0.27 of its 16-bit memory."""
+
+    @staticmethod
+    def check(linear):
+        """Raises where ``linear`` has no 4-bit form: an unsuited width, or more to it than its weight and bias."""
+        if not _plain_linear(linear):
+            raise ValueError("Fp4Linear is made from a plain Linear, without hooks, parametrisations or a forward of its own "
+                             f"(got {type(linear).__name__})")
+        if linear.weight.shape[1] % 32:
+            raise ValueError(f"Fp4Linear: the width must be a multiple of 32 (got {tuple(linear.weight.shape)})")
+
+    def __init__(self, linear):
+        super().__init__()
+        self.check(linear)
+        self.train(linear.training)
+        _hold_fp4(self, "fp4", linear)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        _refuse_16_bit_state(self, state_dict, prefix, ("weight",), args[-1])
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
+    def forward(self, x):
+        """x (..., width) in 16 bits on the GPU."""
+        y = linear_fp4(x.reshape(-1, x.shape[-1]), self.fp4_weight, self.fp4_scale.view(FP4_SCALE), self.fp4_bias)
+        return y.view(*x.shape[:-1], y.shape[1])
+
+
+class Fp4MLP(nn.Module):
+    """``MLP`` for inference with its weights in 4 bits (``kernel/fp4``) and 16-bit activations: two products, the activation
+    formed in the first one's epilogue.  Made from an ``MLP`` on the GPU; 0.27 of its 16-bit memory."""
+
+    @staticmethod
+    def check(mlp):
+        """Raises where ``mlp`` has no 4-bit form: unsuited widths, or more to it than its weights and biases (a subclass,
+        a ``forward``, hook or parametrisation of its own, on the MLP or one of its projections)."""
+        if not plain_module(mlp, MLP, every=False):
+            raise ValueError("Fp4MLP is made from an MLP without hooks, parametrisations or a forward of its own "
+                             f"(got {type(mlp).__name__})")
+        for name, linear in (("fc", mlp.fc), ("proj", mlp.proj)):
+            if not _plain_linear(linear):
+                raise ValueError("Fp4MLP is made from plain Linear projections, without hooks, parametrisations or a forward "
+                                 f"of their own (got {type(linear).__name__} for {name})")
+            if linear.weight.shape[1] % 32:
+                raise ValueError(f"Fp4MLP: widths are multiples of 32 (got {tuple(linear.weight.shape)} for {name})")
+
+    def __init__(self, mlp):
+        super().__init__()
+        self.check(mlp)
+        self.train(mlp.training)
+        _hold_fp4(self, "fc", mlp.fc)
+        _hold_fp4(self, "proj", mlp.proj)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        _refuse_16_bit_state(self, state_dict, prefix, ("fc.weight", "proj.weight"), args[-1])
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
+    def forward(self, x, defer=False):
+        """x (..., dim) in 16 bits on the GPU.  ``defer`` is ``MLP``'s; the output is always summed."""
+        h = linear_gated_fp4(x.reshape(-1, x.shape[-1]), self.fc_weight, self.fc_scale.view(FP4_SCALE), self.fc_bias)
+        return linear_fp4(h, self.proj_weight, self.proj_scale.view(FP4_SCALE), self.proj_bias).view(x.shape)
 
 
 class GlobalBlock(nn.Module):
