@@ -116,6 +116,21 @@ struct SampleRaw {
   }
 };
 
+// 2^43 exp((x - max) / t), rounded, for c = log2(e) / t.  2^y for y = n + j / 256 + r: a table's value times the Taylor
+// polynomial of 2^r, |r| <= 1 / 512, of degree 4 (4e-17 off); the sums with powers of two round to multiples of 1 / 256 and to
+// whole numbers.  (NaN: 0)
+__device__ __forceinline__ uint64_t sample_weight(double x, double xmax, double c, const double* power) {
+  const double y = fmax(fma(x - xmax, c, 43.0), -3.0);
+  const double s = y + 0x1.8p44, r = y - (s - 0x1.8p44);
+  const int j = (int)(uint32_t)__builtin_bit_cast(uint64_t, s);
+  double p = fma(r, 0x1.3b2ab6fba4e77p-7, 0x1.c6b08d704a0bfp-5);
+  p = fma(p, r, 0x1.ebfbdff82c58ep-3);
+  p = fma(p, r, 0x1.62e42fefa39efp-1);
+  const double b = power[j & 255];
+  const double w = __builtin_amdgcn_ldexp(fma(b, p * r, b), j >> 8) + 0x1p52;
+  return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+}
+
 // A token in the order: its key, then the lower index first
 __device__ __forceinline__ uint64_t sample_order(uint32_t key, int i) { return (uint64_t)key << 32 | (uint32_t)~i; }
 
@@ -163,20 +178,10 @@ struct Sampler {
     }
   }
 
-  // 2^43 exp((x - max) / t), rounded; 2^43 for every largest logit, whatever it is.  2^y for y = n + j / 256 + r: a table's value
-  // times the Taylor polynomial of 2^r, |r| <= 1 / 512, of degree 4 (4e-17 off); the sums with powers of two round to
-  // multiples of 1 / 256 and to whole numbers.  (A missing logit's key is that of a NaN: 0)
+  // 2^43 for every largest logit, whatever it is.  (A missing logit's key is that of a NaN: 0)
   __device__ __forceinline__ uint64_t weight(uint32_t k) const {
-    const double y = fmax(fma((double)SampleKey<T>::value(k) - xmax, c, 43.0), -3.0);
-    const double s = y + 0x1.8p44, r = y - (s - 0x1.8p44);
-    const int j = (int)(uint32_t)__builtin_bit_cast(uint64_t, s);
-    double p = fma(r, 0x1.3b2ab6fba4e77p-7, 0x1.c6b08d704a0c0p-5);
-    p = fma(p, r, 0x1.ebfbdff82c58fp-3);
-    p = fma(p, r, 0x1.62e42fefa39efp-1);
-    const double b = sh->power[j & 255];
-    const double w = __builtin_amdgcn_ldexp(fma(b, p * r, b), j >> 8) + 0x1p52;
-    const uint64_t u = __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
-    return k == top ? kSampleOne : u;
+    const uint64_t w = sample_weight((double)SampleKey<T>::value(k), xmax, c, sh->power);
+    return k == top ? kSampleOne : w;
   }
 
   // A logit's bin: equal widths below the largest; what has no weight lies in the last one, which holds nothing else
@@ -455,6 +460,355 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------ 16-bit logits
+// Rows of up to 65,535 16-bit logits hold at most 65,536 different values: one pass over the row counts every value in LDS (two
+// 16-bit counters a word), and the filters are decided on values and counts alone, a weight for each value that occurs.  In
+// falling order the words are 32 strips of 1,024, a word a thread; a strip's wave that holds any leaves its count and
+// weight in a table of 512 entries, and each wave finds a border there, then in the entry's words.  A last pass over the row adds
+// up the kept weights, and counts the tokens of the border's value, of which the first so many are kept; each lane leaves both
+// for each of its chunks in LDS, where the wave in whose part the answer lies finds it.
+//
+// Keys here are the 16 bits in the values' order as they are: NaNs lie at both ends, and -0, 0x7fff, is counted as +0, 0x8000.
+constexpr int kCountedThreads = 1024, kCountedChunks = 8;  // 512 logits a chunk and wave
+
+template <typename T>
+__device__ __forceinline__ uint32_t ordered2(uint32_t x) {  // of two logits
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  return x ^ (__builtin_bit_cast(uint32_t, __builtin_bit_cast(s16x2, x) >> 15) | 0x80008000u);
+}
+template <typename T>
+__device__ __forceinline__ float ordered_value(uint32_t key) {
+  return to_f32(__builtin_bit_cast(T, (uint16_t)(key & 0x8000u ? key ^ 0x8000u : ~key)));
+}
+
+template <typename T>
+struct Counted {
+  static constexpr uint32_t kInf = __is_same(T, bf16) ? 0xff80u : 0xfc00u, kNegInf = 0xffffu - kInf;
+  struct Shared {
+    union {
+      uint32_t table[32768];
+      struct {
+        unsigned long long own[kCountedChunks][kCountedThreads];  // a lane's weight in a chunk
+        uint32_t same[kCountedChunks][kCountedThreads];           // and its tokens of the border's value
+      };
+    };
+    unsigned long long mass[512];
+    uint32_t count[512];
+    double power[256];
+    unsigned long long part[16];
+    uint32_t ties[16];
+    unsigned top, first;
+  };
+  Shared* sh;
+  const uint16_t* row;
+  int V, lane, wave, first, chunks;  // the wave's part of the row: its first chunk and their number
+  uint32_t top;
+  double xmax, c;
+
+  __device__ __forceinline__ int index(int q) const { return (first + q) * kSampleChunk + 8 * lane; }
+  __device__ __forceinline__ uint64_t weight(uint32_t k) const {
+    const uint64_t w = sample_weight((double)ordered_value<T>(k), xmax, c, sh->power);
+    return k == top ? kSampleOne : w;
+  }
+  // The logits of chunk q; what lies behind the row's end reads as 0xffff, key 0
+  __device__ __forceinline__ u32x4 load(int q) const {
+    const int i = index(q);
+    if ((first + q + 1) * kSampleChunk <= V) return *(const u32x4_at2*)(row + i);
+    u32x4 v;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      v[e >> 1] = (i + e < V ? row[i + e] : 0xffffu) | (i + e + 1 < V ? row[i + e + 1] : 0xffffu) << 16;
+    return v;
+  }
+  // f(chunk, its keys, two a word), loads two chunks ahead
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    u32x4 a = {}, b = {};
+    if (chunks > 0) a = load(0);
+    if (chunks > 1) b = load(1);
+#pragma unroll 1
+    for (int q = 0; q < chunks; ++q) {
+      u32x4 now = a;
+      a = b;
+      if (q + 2 < chunks) b = load(q + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) now[e] = ordered2<T>(now[e]);
+      f(q, now);
+    }
+  }
+  static __device__ __forceinline__ uint32_t key(const u32x4& keys, int e) {
+    return e & 1 ? keys[e >> 1] >> 16 : keys[e >> 1] & 0xffffu;
+  }
+
+  __device__ __forceinline__ void count_values() {
+    each([&](int, const u32x4& keys) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t k = key(keys, e);
+        atomicAdd(&sh->table[k >> 1], k & 1 ? 65536u : 1u);
+      }
+    });
+  }
+
+  // The first index whose key is in [lo, hi] or [lo2, hi2]
+  __device__ __forceinline__ int first_of(uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t hi2) {
+    int at = 0x7fffffff;
+    each([&](int q, const u32x4& keys) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t k = key(keys, e);
+        const int i = index(q) + e;
+        if (((k >= lo && k <= hi) || (k >= lo2 && k <= hi2)) && i < V) at = min(at, i);
+      }
+    });
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) at = min(at, __shfl_xor(at, m, 64));
+    if (lane == 0) atomicMin(&sh->first, (unsigned)at);
+    __syncthreads();
+    return (int)sh->first;
+  }
+
+  // Counts and weights of every entry: strip i, wave w of the words in falling order
+  __device__ __forceinline__ void tabulate(bool weights) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      const int at = 1024 * i + threadIdx.x;
+      const uint32_t word = sh->table[32767 - at];
+      uint32_t n = 0;
+      uint64_t m = 0;
+      if (__any(word != 0)) {
+        n = (word >> 16) + (word & 0xffffu);
+        if (weights) {
+          const uint32_t k = 65535u - 2 * at;
+          m = (word >> 16) * weight(k) + (word & 0xffffu) * weight(k - 1);
+          m = wave_sum64(m);
+        }
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1) n += (uint32_t)__shfl_xor((int)n, x, 64);
+      }
+      if (lane == 0) sh->count[16 * i + wave] = n, sh->mass[16 * i + wave] = m;
+    }
+    __syncthreads();
+  }
+
+  // The value at which the tokens in order first hold `target` (>= 1, at most the whole sum): its key, the sum before it and its own
+  // (every wave by itself); before: likewise the weight before it and its count
+  template <bool MASS>
+  __device__ __forceinline__ uint32_t border(uint64_t target, uint64_t& above, uint64_t& held) const {
+    uint64_t v[8], mine = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine += v[j] = MASS ? (uint64_t)sh->mass[8 * lane + j] : (uint64_t)sh->count[8 * lane + j];
+    uint64_t at = wave_scan64(mine, lane) - mine;
+    int entry = 0;
+    const bool here = at < target && at + mine >= target;
+    if (here) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (at + v[j] >= target) {
+          entry = 8 * lane + j;
+          break;
+        }
+        at += v[j];
+      }
+    }
+    const int l = __builtin_ctzll(__ballot(here));
+    entry = __shfl(entry, l, 64);
+    at = (uint64_t)__shfl((unsigned long long)at, l, 64);
+    const int pos = 1024 * (entry >> 4) + 64 * (entry & 15) + lane;
+    const uint32_t word = sh->table[32767 - pos], k = 65535u - 2 * pos;
+    const uint64_t hi = MASS ? (word >> 16) * weight(k) : word >> 16, lo = MASS ? (word & 0xffffu) * weight(k - 1) : word & 0xffffu;
+    at += wave_scan64(hi + lo, lane) - hi - lo;
+    const bool this_one = at < target && at + hi + lo >= target, low = at + hi < target;
+    const int l2 = __builtin_ctzll(__ballot(this_one));
+    above = (uint64_t)__shfl((unsigned long long)(low ? at + hi : at), l2, 64);
+    held = (uint64_t)__shfl((unsigned long long)(low ? lo : hi), l2, 64);
+    return (uint32_t)__shfl((int)(low ? k - 1 : k), l2, 64);
+  }
+
+  // The weight of every value above key k
+  __device__ __forceinline__ uint64_t weight_above(uint32_t k) const {
+    const int pos = (int)(65535u - k) >> 1, entry = 16 * (pos >> 10) + ((pos >> 6) & 15);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += 8 * lane + j < entry ? (uint64_t)sh->mass[8 * lane + j] : 0;
+    const int p = 1024 * (entry >> 4) + 64 * (entry & 15) + lane;
+    const uint32_t word = sh->table[32767 - p], kp = 65535u - 2 * p;
+    if (kp > k) sum += (word >> 16) * weight(kp);
+    if (kp - 1 > k) sum += (word & 0xffffu) * weight(kp - 1);
+    return wave_sum64(sum);
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleArgs a) {
+  using S = Counted<T>;
+  __shared__ typename S::Shared shared;
+  S s;
+  s.sh = &shared;
+  s.V = a.V;
+  s.lane = threadIdx.x & 63;
+  s.wave = threadIdx.x >> 6;
+  const int chunks = (a.V + kSampleChunk - 1) / kSampleChunk, each = (chunks + 15) / 16;
+  s.first = min(s.wave * each, chunks);
+  s.chunks = min(each, chunks - s.first);
+  if (threadIdx.x < 256) shared.power[threadIdx.x] = exp2(threadIdx.x / 256.0);
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ((u32x4*)shared.table)[1024 * i + threadIdx.x] = u32x4{};
+    if (threadIdx.x == 0) shared.top = 0xffffffffu, shared.first = 0x7fffffffu;
+    __syncthreads();
+    s.row = (const uint16_t*)a.logits + r * a.ld;
+    s.count_values();
+    __syncthreads();
+    // ---- the largest value; NaNs at both ends (what lies behind the row's end is counted at key 0)
+    uint32_t top = 0xffffffffu;
+    bool bad = false;
+#pragma unroll
+    for (int i = 31; i >= 0; --i) {
+      const uint32_t at = 1024 * i + threadIdx.x;
+      uint32_t word = shared.table[32767 - at];
+      if (at == 32767) word -= (uint32_t)(chunks * kSampleChunk - a.V);
+      if (word) top = 2 * at + (word >> 16 ? 0 : 1);
+      if (word && (65535u - 2 * at > S::kInf || 65534u - 2 * at < S::kNegInf)) {
+        const uint32_t k = 65535u - 2 * at;
+        bad |= (word >> 16 && (k > S::kInf || k < S::kNegInf)) || (word & 0xffffu && (k - 1 > S::kInf || k - 1 < S::kNegInf));
+      }
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = min(top, (uint32_t)__shfl_xor((int)top, m, 64));
+    if (s.lane == 0) atomicMin(&shared.top, top);
+    const bool nan = __syncthreads_or(bad);
+    s.top = 65535u - shared.top;
+    if (threadIdx.x == 0) {
+      shared.table[0] &= 0xffff0000u;
+      const uint32_t zeros = shared.table[0x3fff] >> 16;  // -0
+      shared.table[0x3fff] &= 0xffffu;
+      shared.table[0x4000] += zeros;
+    }
+    if (s.top == 0x7fffu) s.top = 0x8000u;
+    __syncthreads();
+    const float t = a.temperature ? a.temperature[r] : a.t0;
+    if (nan) {
+      const int i = s.first_of(S::kInf + 1, 0xffffu, 0, S::kNegInf - 1);
+      if (threadIdx.x == 0) a.ids[r] = i;
+    } else if (!(t > 0.f)) {
+      const int i = s.first_of(s.top == 0x8000u ? 0x7fffu : s.top, s.top, 1, 0);
+      if (threadIdx.x == 0) a.ids[r] = i;
+    } else {
+      s.xmax = (double)ordered_value<T>(s.top);
+      s.c = 1.4426950408889634 / (double)t;
+      const int k = a.top_k ? a.top_k[r] : a.k0;
+      const float p = a.top_p ? a.top_p[r] : a.p0, m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
+      const bool by_count = k > 0 && k < a.V, by_mass = p < 1.f;
+      // kept: every value above `at`, and the first n tokens of those from `low` to `at` (none where low > at)
+      uint32_t at = 0, low = 1;
+      uint64_t n = 0, above, held;
+      if (by_count || by_mass) {
+        s.tabulate(by_mass);
+        bool cut = false;
+        if (by_count) {
+          at = s.template border<false>((uint64_t)k, above, held);
+          n = (uint64_t)k - above;
+          cut = n < held;
+        }
+        if (by_mass) {
+          const uint64_t total = s.weight_above(at) + (by_count ? n * s.weight(at) : 0);
+          const double want = (double)p * (double)total;
+          const uint64_t target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
+          const uint32_t pk = s.template border<true>(target, above, held);
+          const uint64_t w = s.weight(pk), take = (target - above + w - 1) / w;
+          if (pk != at || take < n) {
+            cut = (pk == at && cut) || take < held / w;
+            n = take;
+          }
+          at = pk;
+        }
+        low = at == 0x8000u ? 0x7fffu : at;
+        if (!cut) at = low - 1, low = at + 1;
+      }
+      if (m > 0.f) {
+        // the least value with its share of the largest weight, as a key
+        const double x = m >= 1.f ? s.xmax : s.xmax + (double)t * log((double)m);
+        uint32_t least = ordered2<T>(__builtin_bit_cast(uint16_t, from_f32<T>((float)x))) & 0xffffu;
+        if (least == 0x7fffu) least = 0x8000u;
+        // (rounded twice and either way: at most a value off; a NaN, of infinities, keeps all)
+        if (x != x) least = 0;
+        while (least > S::kNegInf && (double)ordered_value<T>(least - 1) >= x) --least;
+        while (least < S::kInf && (double)ordered_value<T>(least) < x) ++least;
+        if (least == 0x8000u) least = 0x7fffu;
+        if (least > at + (low <= at ? 0 : 1)) at = least - 1, low = at + 1;
+      }
+      const bool ties = low <= at;
+      const uint64_t one = ties ? s.weight(at) : 0;
+      // ---- the kept weights, and the border's tokens, of the wave's part
+      uint64_t sum = 0;
+      uint32_t number = 0;
+      __syncthreads();  // the counts are read
+      s.each([&](int q, const u32x4& keys) {
+        uint64_t own = 0;
+        uint32_t same = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t key = S::key(keys, e);
+          if (__any(key > at)) own += key > at ? s.weight(key) : 0;
+          same += key >= low && key <= at;
+        }
+        shared.own[q][threadIdx.x] = own;
+        shared.same[q][threadIdx.x] = same;
+        sum += own;
+        number += same;
+      });
+      sum = wave_sum64(sum);
+#pragma unroll
+      for (int x = 32; x >= 1; x >>= 1) number += (uint32_t)__shfl_xor((int)number, x, 64);
+      if (s.lane == 0) shared.part[s.wave] = sum, shared.ties[s.wave] = number;
+      __syncthreads();
+      uint64_t before = 0, left = n, mine = 0, total = 0, left_here = 0;  // left: tokens of the border still to be kept
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const uint64_t take = min(left, (uint64_t)shared.ties[q]), w = shared.part[q] + take * one;
+        if (q == s.wave) before = total, mine = w, left_here = left;
+        total += w;
+        left -= take;
+      }
+      const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+      const uint64_t aim = (uint64_t)(f * (double)total);
+      if (before <= aim && aim < before + mine) {  // one wave, all of it
+#pragma unroll 1
+        for (int q = 0; q < s.chunks; ++q) {
+          const uint32_t same = shared.same[q][threadIdx.x];
+          uint32_t upto = same;
+#pragma unroll
+          for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t y = (uint32_t)__shfl_up((int)upto, x, 64);
+            if (s.lane >= x) upto += y;
+          }
+          const uint64_t first = upto - same;  // the border's tokens before this lane's
+          uint64_t lane_left = left_here > first ? left_here - first : 0;
+          const uint64_t w = shared.own[q][threadIdx.x] + min(lane_left, (uint64_t)same) * one;
+          const uint64_t scan = wave_scan64(w, s.lane);
+          uint64_t from = before + scan - w;
+          if (from <= aim && aim < from + w) {
+            const u32x4 raw = s.load(q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t pair = ordered2<T>(raw[e >> 1]), key = e & 1 ? pair >> 16 : pair & 0xffffu;
+              uint64_t one_w = key > at ? s.weight(key) : 0;
+              if (key >= low && key <= at && lane_left) one_w = one, --lane_left;
+              if (from <= aim && aim < from + one_w) a.ids[r] = s.index(q) + e;
+              from += one_w;
+            }
+          }
+          before += (uint64_t)__shfl((unsigned long long)scan, 63, 64);
+          left_here -= min(left_here, (uint64_t)(uint32_t)__shfl((int)upto, 63, 64));
+          if (aim < before) break;
+        }
+      }
+    }
+    __syncthreads();  // the table is read before the next row clears it
+  }
+}
+
 }  // namespace atma
 
 extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* uniform, const float* temperature, float t0,
@@ -473,6 +827,12 @@ extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* u
   const unsigned grid = (unsigned)std::min<int64_t>(rows, 1 << 20);
   auto launch = [&](auto zero) {
     using T = decltype(zero);
+    if constexpr (sizeof(T) == 2) {
+      if (V < 65536) {
+        sample_counted_kernel<T><<<grid, kCountedThreads, 0, (hipStream_t)stream>>>(a);
+        return;
+      }
+    }
     if (V <= 8192) sample_tokens_kernel<T, 4><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else sample_tokens_kernel<T, 16><<<grid, 1024, 0, (hipStream_t)stream>>>(a);
   };
