@@ -70,20 +70,34 @@ struct SampleKey<float> {
 __device__ __forceinline__ uint64_t wave_xor64(uint64_t x, int m) {
   return (uint64_t)__shfl_xor((unsigned long long)x, m, 64);
 }
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) x += wave_xor64(x, m);
-  return x;
+// The sum over this lane and the ones below it: lane exchanges inside rows of 16, then the rows' last lanes (no LDS)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_add64(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
+  return x + ((uint64_t)hi << 32 | lo);
 }
-// The sum over this lane and the ones below it
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t x, int lane) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint64_t y = (uint64_t)__shfl_up((unsigned long long)x, m, 64);
-    if (lane >= m) x += y;
-  }
-  return x;
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
+  x = dpp_add64<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8
+  x = dpp_add64<0x112, 0xF>(x);
+  x = dpp_add64<0x114, 0xF>(x);
+  x = dpp_add64<0x118, 0xF>(x);
+  x = dpp_add64<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  return dpp_add64<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
 }
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+}
+__device__ __forceinline__ uint32_t lane32(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
+__device__ __forceinline__ uint64_t lane64(uint64_t x, int l) {
+  return (uint64_t)lane32((uint32_t)(x >> 32), l) << 32 | lane32((uint32_t)x, l);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) { return lane64(wave_scan64(x), 63); }
 
 typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
@@ -116,19 +130,24 @@ struct SampleRaw {
   }
 };
 
-// 2^43 exp((x - max) / t), rounded, for c = log2(e) / t.  2^y for y = n + j / 256 + r: a table's value times the Taylor
-// polynomial of 2^r, |r| <= 1 / 512, of degree 4 (4e-17 off); the sums with powers of two round to multiples of 1 / 256 and to
-// whole numbers.  (NaN: 0)
-__device__ __forceinline__ uint64_t sample_weight(double x, double xmax, double c, const double* power) {
-  const double y = fmax(fma(x - xmax, c, 43.0), -3.0);
+// 2^y for y = n + j / 256 + r: a table's value times the Taylor polynomial of 2^r, |r| <= 1 / 512, of degree 4 (4e-17 off); the sum
+// with a power of two rounds to multiples of 1 / 256
+__device__ __forceinline__ double sample_power(double y, const double* power) {
   const double s = y + 0x1.8p44, r = y - (s - 0x1.8p44);
   const int j = (int)(uint32_t)__builtin_bit_cast(uint64_t, s);
   double p = fma(r, 0x1.3b2ab6fba4e77p-7, 0x1.c6b08d704a0bfp-5);
   p = fma(p, r, 0x1.ebfbdff82c58ep-3);
   p = fma(p, r, 0x1.62e42fefa39efp-1);
   const double b = power[j & 255];
-  const double w = __builtin_amdgcn_ldexp(fma(b, p * r, b), j >> 8) + 0x1p52;
-  return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+  return __builtin_amdgcn_ldexp(fma(b, p * r, b), j >> 8);
+}
+// A number of [0, 2^51] rounded to the nearest integer
+__device__ __forceinline__ uint64_t whole64(double w) {
+  return __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xfffffffffffffull;
+}
+// 2^43 exp((x - max) / t), rounded, for c = log2(e) / t (NaN: 0)
+__device__ __forceinline__ uint64_t sample_weight(double x, double xmax, double c, const double* power) {
+  return whole64(sample_power(fmax(fma(x - xmax, c, 43.0), -3.0), power));
 }
 
 // A token in the order: its key, then the lower index first
@@ -207,7 +226,7 @@ struct Sampler {
     uint64_t v[N], mine = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) mine += v[j] = bins[N * threadIdx.x + j];
-    const uint64_t upto = wave_scan64(mine, lane);
+    const uint64_t upto = wave_scan64(mine);
     if (lane == 63) sh->part[wave] = upto;
     __syncthreads();
     uint64_t at = above + upto - mine;
@@ -321,7 +340,7 @@ struct Sampler {
         uint64_t n[8], own = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) own += n[e] = amount(i + e, i + e < V ? SampleKey<T>::of(now.raw(e)) : 0u);
-        const uint64_t upto = wave_scan64(own, lane);
+        const uint64_t upto = wave_scan64(own);
         uint64_t at = before + upto - own;
         if (at <= aim && aim < at + own) {
 #pragma unroll
@@ -330,7 +349,7 @@ struct Sampler {
             at += n[e];
           }
         }
-        before += (uint64_t)__shfl((unsigned long long)upto, 63, 64);
+        before += lane64(upto, 63);
         if (aim < before) break;
       }
     }
@@ -484,26 +503,33 @@ __device__ __forceinline__ float ordered_value(uint32_t key) {
 template <typename T>
 struct Counted {
   static constexpr uint32_t kInf = __is_same(T, bf16) ? 0xff80u : 0xfc00u, kNegInf = 0xffffu - kInf;
+  // the weights' tables: mantissa bits and the upper ones of them, exponents a sign
+  static constexpr int kMan = __is_same(T, bf16) ? 7 : 10, kBias = __is_same(T, bf16) ? 127 : 15, kHigh = (kMan + 1) / 2,
+                       kLow = kMan - kHigh, kExps = 32;
   struct Shared {
     union {
       uint32_t table[32768];
       struct {
         unsigned long long own[kCountedChunks][kCountedThreads];  // a lane's weight in a chunk
         uint32_t same[kCountedChunks][kCountedThreads];           // and its tokens of the border's value
+        double high[2 * kExps << kHigh], low[2 * kExps << kLow];
       };
     };
     unsigned long long mass[512];
     uint32_t count[512];
     double power[256];
-    unsigned long long part[16];
+    unsigned long long part[16], n, one;
     uint32_t ties[16];
-    unsigned top, first;
+    unsigned top, first, at, low_key;
   };
+  static_assert(sizeof(((Shared*)0)->own) + sizeof(((Shared*)0)->same) + sizeof(((Shared*)0)->high) + sizeof(((Shared*)0)->low) <=
+                    sizeof(((Shared*)0)->table), "they take the counts' place");
   Shared* sh;
   const uint16_t* row;
   int V, lane, wave, first, chunks;  // the wave's part of the row: its first chunk and their number
-  uint32_t top;
+  uint32_t top, strips;              // strips of which the wave's words hold any
   double xmax, c;
+  int least_exp, exps;               // the exponents that the weights' tables hold
 
   __device__ __forceinline__ int index(int q) const { return (first + q) * kSampleChunk + 8 * lane; }
   __device__ __forceinline__ uint64_t weight(uint32_t k) const {
@@ -520,7 +546,7 @@ struct Counted {
       v[e >> 1] = (i + e < V ? row[i + e] : 0xffffu) | (i + e + 1 < V ? row[i + e + 1] : 0xffffu) << 16;
     return v;
   }
-  // f(chunk, its keys, two a word), loads two chunks ahead
+  // f(chunk, its logits, two a word), loads two chunks ahead
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     u32x4 a = {}, b = {};
@@ -528,23 +554,19 @@ struct Counted {
     if (chunks > 1) b = load(1);
 #pragma unroll 1
     for (int q = 0; q < chunks; ++q) {
-      u32x4 now = a;
+      const u32x4 now = a;
       a = b;
       if (q + 2 < chunks) b = load(q + 2);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) now[e] = ordered2<T>(now[e]);
       f(q, now);
     }
   }
-  static __device__ __forceinline__ uint32_t key(const u32x4& keys, int e) {
-    return e & 1 ? keys[e >> 1] >> 16 : keys[e >> 1] & 0xffffu;
-  }
+  static __device__ __forceinline__ uint32_t half(uint32_t pair, int e) { return e & 1 ? pair >> 16 : pair & 0xffffu; }
 
   __device__ __forceinline__ void count_values() {
-    each([&](int, const u32x4& keys) {
+    each([&](int, const u32x4& raw) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t k = key(keys, e);
+        const uint32_t k = half(ordered2<T>(raw[e >> 1]), e);
         atomicAdd(&sh->table[k >> 1], k & 1 ? 65536u : 1u);
       }
     });
@@ -553,10 +575,10 @@ struct Counted {
   // The first index whose key is in [lo, hi] or [lo2, hi2]
   __device__ __forceinline__ int first_of(uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t hi2) {
     int at = 0x7fffffff;
-    each([&](int q, const u32x4& keys) {
+    each([&](int q, const u32x4& raw) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t k = key(keys, e);
+        const uint32_t k = half(ordered2<T>(raw[e >> 1]), e);
         const int i = index(q) + e;
         if (((k >= lo && k <= hi) || (k >= lo2 && k <= hi2)) && i < V) at = min(at, i);
       }
@@ -568,61 +590,50 @@ struct Counted {
     return (int)sh->first;
   }
 
-  // Counts and weights of every entry: strip i, wave w of the words in falling order
+  // Counts and weights of the entries (cleared before): strip i, wave w of the words in falling order
   __device__ __forceinline__ void tabulate(bool weights) {
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i) {
-      const int at = 1024 * i + threadIdx.x;
-      const uint32_t word = sh->table[32767 - at];
-      uint32_t n = 0;
-      uint64_t m = 0;
-      if (__any(word != 0)) {
-        n = (word >> 16) + (word & 0xffffu);
+    for (uint32_t left = strips; left; left &= left - 1) {
+      const int i = __builtin_ctz(left), at = 1024 * i + threadIdx.x;
+      const uint32_t word = sh->table[32767 - at], k = 65535u - 2 * at;
+      if (word) {
+        atomicAdd(&sh->count[16 * i + wave], (word >> 16) + (word & 0xffffu));
         if (weights) {
-          const uint32_t k = 65535u - 2 * at;
-          m = (word >> 16) * weight(k) + (word & 0xffffu) * weight(k - 1);
-          m = wave_sum64(m);
+          const uint64_t m = (word >> 16) * weight(k) + (word & 0xffffu) * weight(k - 1);
+          if (m) atomicAdd(&sh->mass[16 * i + wave], (unsigned long long)m);
         }
-#pragma unroll
-        for (int x = 32; x >= 1; x >>= 1) n += (uint32_t)__shfl_xor((int)n, x, 64);
       }
-      if (lane == 0) sh->count[16 * i + wave] = n, sh->mass[16 * i + wave] = m;
     }
     __syncthreads();
   }
 
   // The value at which the tokens in order first hold `target` (>= 1, at most the whole sum): its key, the sum before it and its own
-  // (every wave by itself); before: likewise the weight before it and its count
   template <bool MASS>
   __device__ __forceinline__ uint32_t border(uint64_t target, uint64_t& above, uint64_t& held) const {
     uint64_t v[8], mine = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) mine += v[j] = MASS ? (uint64_t)sh->mass[8 * lane + j] : (uint64_t)sh->count[8 * lane + j];
-    uint64_t at = wave_scan64(mine, lane) - mine;
-    int entry = 0;
+    uint64_t at = wave_scan64(mine) - mine;
+    int entry = -1;
     const bool here = at < target && at + mine >= target;
-    if (here) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (at + v[j] >= target) {
-          entry = 8 * lane + j;
-          break;
-        }
-        at += v[j];
+    for (int j = 0; j < 8; ++j) {
+      if (here && entry < 0) {
+        if (at + v[j] >= target) entry = 8 * lane + j;
+        else at += v[j];
       }
     }
     const int l = __builtin_ctzll(__ballot(here));
-    entry = __shfl(entry, l, 64);
-    at = (uint64_t)__shfl((unsigned long long)at, l, 64);
+    entry = (int)lane32((uint32_t)entry, l);
+    at = lane64(at, l);
     const int pos = 1024 * (entry >> 4) + 64 * (entry & 15) + lane;
     const uint32_t word = sh->table[32767 - pos], k = 65535u - 2 * pos;
     const uint64_t hi = MASS ? (word >> 16) * weight(k) : word >> 16, lo = MASS ? (word & 0xffffu) * weight(k - 1) : word & 0xffffu;
-    at += wave_scan64(hi + lo, lane) - hi - lo;
+    at += wave_scan64(hi + lo) - hi - lo;
     const bool this_one = at < target && at + hi + lo >= target, low = at + hi < target;
     const int l2 = __builtin_ctzll(__ballot(this_one));
-    above = (uint64_t)__shfl((unsigned long long)(low ? at + hi : at), l2, 64);
-    held = (uint64_t)__shfl((unsigned long long)(low ? lo : hi), l2, 64);
-    return (uint32_t)__shfl((int)(low ? k - 1 : k), l2, 64);
+    above = lane64(low ? at + hi : at, l2);
+    held = lane64(low ? lo : hi, l2);
+    return lane32(low ? k - 1 : k, l2);
   }
 
   // The weight of every value above key k
@@ -636,6 +647,112 @@ struct Counted {
     if (kp > k) sum += (word >> 16) * weight(kp);
     if (kp - 1 > k) sum += (word & 0xffffu) * weight(kp - 1);
     return wave_sum64(sum);
+  }
+
+  // What is kept (one wave finds it): every value above `at`, and the first n tokens of those with keys from `low` to `at` (none where
+  // low > at)
+  __device__ __forceinline__ void filter(int k, float p, float m, float t) {
+    const bool by_count = k > 0 && k < V, by_mass = p < 1.f;
+    uint32_t at = 0, low = 1;
+    uint64_t n = 0, above, held;
+    if (by_count || by_mass) {
+      bool cut = false;
+      if (by_count) {
+        at = border<false>((uint64_t)k, above, held);
+        n = (uint64_t)k - above;
+        cut = n < held;
+      }
+      if (by_mass) {
+        const uint64_t total = weight_above(at) + (by_count ? n * weight(at) : 0);
+        const double want = (double)p * (double)total;
+        const uint64_t target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
+        const uint32_t pk = border<true>(target, above, held);
+        const uint64_t w = weight(pk), take = (target - above + w - 1) / w;
+        if (pk != at || take < n) {
+          cut = (pk == at && cut) || take < held / w;
+          n = take;
+        }
+        at = pk;
+      }
+      low = at == 0x8000u ? 0x7fffu : at;
+      if (!cut) at = low - 1, low = at + 1;
+    }
+    if (m > 0.f) {
+      // the least value with its share of the largest weight, as a key
+      const double x = m >= 1.f ? xmax : xmax + (double)t * log((double)m);
+      uint32_t least = ordered2<T>(__builtin_bit_cast(uint16_t, from_f32<T>((float)x))) & 0xffffu;
+      if (least == 0x7fffu) least = 0x8000u;
+      // (rounded twice and either way: at most a value off; a NaN, of infinities, keeps all)
+      if (x != x) least = 0;
+      while (least > kNegInf && (double)ordered_value<T>(least - 1) >= x) --least;
+      while (least < kInf && (double)ordered_value<T>(least) < x) ++least;
+      if (least == 0x8000u) least = 0x7fffu;
+      if (least > at + (low <= at ? 0 : 1)) at = least - 1, low = at + 1;
+    }
+    if (lane == 0) {
+      sh->at = at;
+      sh->low_key = low;
+      sh->n = n;
+      sh->one = low <= at ? weight(at) : 0;
+    }
+  }
+
+  // Weights by tables, for rows that keep many tokens.  x = s (2^E + f) for each sign and exponent E, its fraction f = f1 + f2 by its
+  // upper and lower bits: 2^43 exp((s (2^E + f1) - max) / t) times exp(s f2 / t), 24 (fp16: 64) values a binade, for the 32 binades up
+  // to the largest magnitude that has a weight.  Returns whether they serve (else a factor might leave fp64's range)
+  __device__ __forceinline__ bool prepare(float t) {
+    const float most = fabsf((float)xmax) + 31.f * t;
+    const uint32_t bits = __builtin_bit_cast(uint16_t, from_f32<T>(most * 1.01f)) & 0x7fffu;
+    const int hi = min((int)(bits >> kMan), (1 << (15 - kMan)) - 2);  // (the last exponent is that of infinities)
+    least_exp = max(hi - kExps + 1, 0);
+    exps = hi - least_exp;
+    const double ulp = __builtin_amdgcn_ldexp(1.0, max(hi, 1) - kBias - kMan);
+    if (!(ulp * c * (1 << kLow) < 500.0) || !(fabs(xmax) < 1e30)) return false;
+    for (int i = threadIdx.x; i < (2 * kExps << kHigh) + (2 * kExps << kLow); i += kCountedThreads) {
+      const bool upper = i < 2 * kExps << kHigh;
+      const int j = upper ? i : i - (2 * kExps << kHigh), shift = upper ? kHigh : kLow;
+      const int E = ((j >> shift) & (kExps - 1)) + least_exp, f = (j & ((1 << shift) - 1)) << (upper ? kLow : 0);
+      double x = __builtin_amdgcn_ldexp((double)(f + (upper && E ? 1 << kMan : 0)), max(E, 1) - kBias - kMan);
+      if (j >> (shift + 5)) x = -x;
+      const double y = upper ? fma(x - xmax, c, 43.0) : x * c;
+      const double w = sample_power(fmin(fmax(y, -1000.0), 1000.0), sh->power);
+      if (upper) sh->high[j] = w;
+      else sh->low[j] = w;
+    }
+    return true;
+  }
+  __device__ __forceinline__ uint64_t table_weight(uint32_t raw, uint32_t k) const {
+    const uint32_t sign = raw >> 15, mag = raw & 0x7fffu;
+    const int e = (int)(mag >> kMan) - least_exp;
+    const uint32_t slot = (uint32_t)min(max(e, 0), exps);
+    const uint32_t hi = (((sign << 5) + slot) << kHigh) + ((mag >> kLow) & ((1 << kHigh) - 1));
+    const uint32_t lo = (((sign << 5) + slot) << kLow) + (mag & ((1 << kLow) - 1));
+    uint64_t w = whole64(sh->high[hi] * sh->low[lo]);
+    if (e > exps) w = 0;  // (negative, and further below the largest than any weight reaches)
+    if (__any(e < 0)) w = e < 0 ? weight(k) : w;
+    return k == top ? kSampleOne : w;
+  }
+
+  // The kept weights, and the border's tokens, of the wave's part
+  template <bool TABLES>
+  __device__ __forceinline__ void add_up(uint32_t at, uint32_t low, uint64_t& sum, uint32_t& number) {
+    each([&](int q, const u32x4& raw) {
+      uint64_t own = 0;
+      uint32_t same = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = half(ordered2<T>(raw[e >> 1]), e);
+        if (__any(key > at)) {
+          const uint64_t w = TABLES ? table_weight(half(raw[e >> 1], e), key) : weight(key);
+          own += key > at ? w : 0;
+        }
+        same += key >= low && key <= at;
+      }
+      sh->own[q][threadIdx.x] = own;
+      sh->same[q][threadIdx.x] = same;
+      sum += own;
+      number += same;
+    });
   }
 };
 
@@ -653,26 +770,27 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
   s.chunks = min(each, chunks - s.first);
   if (threadIdx.x < 256) shared.power[threadIdx.x] = exp2(threadIdx.x / 256.0);
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    s.row = (const uint16_t*)a.logits + r * a.ld;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ((u32x4*)shared.table)[1024 * i + threadIdx.x] = u32x4{};
+    if (threadIdx.x < 512) shared.count[threadIdx.x] = 0, shared.mass[threadIdx.x] = 0;
     if (threadIdx.x == 0) shared.top = 0xffffffffu, shared.first = 0x7fffffffu;
     __syncthreads();
-    s.row = (const uint16_t*)a.logits + r * a.ld;
     s.count_values();
     __syncthreads();
-    // ---- the largest value; NaNs at both ends (what lies behind the row's end is counted at key 0)
+    // ---- the largest value; NaNs lie in the first and the last strip (what lies behind the row's end is counted at key 0)
     uint32_t top = 0xffffffffu;
     bool bad = false;
+    s.strips = 0;
 #pragma unroll
     for (int i = 31; i >= 0; --i) {
       const uint32_t at = 1024 * i + threadIdx.x;
       uint32_t word = shared.table[32767 - at];
-      if (at == 32767) word -= (uint32_t)(chunks * kSampleChunk - a.V);
+      if (i == 31 && at == 32767) word -= (uint32_t)(chunks * kSampleChunk - a.V);
       if (word) top = 2 * at + (word >> 16 ? 0 : 1);
-      if (word && (65535u - 2 * at > S::kInf || 65534u - 2 * at < S::kNegInf)) {
-        const uint32_t k = 65535u - 2 * at;
-        bad |= (word >> 16 && (k > S::kInf || k < S::kNegInf)) || (word & 0xffffu && (k - 1 > S::kInf || k - 1 < S::kNegInf));
-      }
+      if (__any(word != 0)) s.strips |= 1u << i;
+      if (i == 0) bad |= (word >> 16 && 65535u - 2 * at > S::kInf) || (word & 0xffffu && 65534u - 2 * at > S::kInf);
+      if (i == 31) bad |= (word >> 16 && 65535u - 2 * at < S::kNegInf) || (word & 0xffffu && 65534u - 2 * at < S::kNegInf);
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = min(top, (uint32_t)__shfl_xor((int)top, m, 64));
@@ -685,6 +803,7 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
       shared.table[0x3fff] &= 0xffffu;
       shared.table[0x4000] += zeros;
     }
+    s.strips |= 1u << 15;  // (where +0 lies)
     if (s.top == 0x7fffu) s.top = 0x8000u;
     __syncthreads();
     const float t = a.temperature ? a.temperature[r] : a.t0;
@@ -699,68 +818,20 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
       s.c = 1.4426950408889634 / (double)t;
       const int k = a.top_k ? a.top_k[r] : a.k0;
       const float p = a.top_p ? a.top_p[r] : a.p0, m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
-      const bool by_count = k > 0 && k < a.V, by_mass = p < 1.f;
-      // kept: every value above `at`, and the first n tokens of those from `low` to `at` (none where low > at)
-      uint32_t at = 0, low = 1;
-      uint64_t n = 0, above, held;
-      if (by_count || by_mass) {
-        s.tabulate(by_mass);
-        bool cut = false;
-        if (by_count) {
-          at = s.template border<false>((uint64_t)k, above, held);
-          n = (uint64_t)k - above;
-          cut = n < held;
-        }
-        if (by_mass) {
-          const uint64_t total = s.weight_above(at) + (by_count ? n * s.weight(at) : 0);
-          const double want = (double)p * (double)total;
-          const uint64_t target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
-          const uint32_t pk = s.template border<true>(target, above, held);
-          const uint64_t w = s.weight(pk), take = (target - above + w - 1) / w;
-          if (pk != at || take < n) {
-            cut = (pk == at && cut) || take < held / w;
-            n = take;
-          }
-          at = pk;
-        }
-        low = at == 0x8000u ? 0x7fffu : at;
-        if (!cut) at = low - 1, low = at + 1;
-      }
-      if (m > 0.f) {
-        // the least value with its share of the largest weight, as a key
-        const double x = m >= 1.f ? s.xmax : s.xmax + (double)t * log((double)m);
-        uint32_t least = ordered2<T>(__builtin_bit_cast(uint16_t, from_f32<T>((float)x))) & 0xffffu;
-        if (least == 0x7fffu) least = 0x8000u;
-        // (rounded twice and either way: at most a value off; a NaN, of infinities, keeps all)
-        if (x != x) least = 0;
-        while (least > S::kNegInf && (double)ordered_value<T>(least - 1) >= x) --least;
-        while (least < S::kInf && (double)ordered_value<T>(least) < x) ++least;
-        if (least == 0x8000u) least = 0x7fffu;
-        if (least > at + (low <= at ? 0 : 1)) at = least - 1, low = at + 1;
-      }
-      const bool ties = low <= at;
-      const uint64_t one = ties ? s.weight(at) : 0;
-      // ---- the kept weights, and the border's tokens, of the wave's part
+      if ((k > 0 && k < a.V) || p < 1.f) s.tabulate(p < 1.f);
+      if (s.wave == 0) s.filter(k, p, m, t);
+      __syncthreads();  // the counts are read
+      const uint32_t at = shared.at, low = shared.low_key;
+      const uint64_t n = shared.n, one = shared.one;
+      // tables pay where most waves meet a kept token at most of their steps
+      const bool tables = (k <= 0 || k > 512) && s.prepare(t);
+      __syncthreads();
       uint64_t sum = 0;
       uint32_t number = 0;
-      __syncthreads();  // the counts are read
-      s.each([&](int q, const u32x4& keys) {
-        uint64_t own = 0;
-        uint32_t same = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t key = S::key(keys, e);
-          if (__any(key > at)) own += key > at ? s.weight(key) : 0;
-          same += key >= low && key <= at;
-        }
-        shared.own[q][threadIdx.x] = own;
-        shared.same[q][threadIdx.x] = same;
-        sum += own;
-        number += same;
-      });
+      if (tables) s.template add_up<true>(at, low, sum, number);
+      else s.template add_up<false>(at, low, sum, number);
       sum = wave_sum64(sum);
-#pragma unroll
-      for (int x = 32; x >= 1; x >>= 1) number += (uint32_t)__shfl_xor((int)number, x, 64);
+      number = lane32(wave_scan32(number), 63);
       if (s.lane == 0) shared.part[s.wave] = sum, shared.ties[s.wave] = number;
       __syncthreads();
       uint64_t before = 0, left = n, mine = 0, total = 0, left_here = 0;  // left: tokens of the border still to be kept
@@ -776,32 +847,27 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
       if (before <= aim && aim < before + mine) {  // one wave, all of it
 #pragma unroll 1
         for (int q = 0; q < s.chunks; ++q) {
-          const uint32_t same = shared.same[q][threadIdx.x];
-          uint32_t upto = same;
-#pragma unroll
-          for (int x = 1; x < 64; x <<= 1) {
-            const uint32_t y = (uint32_t)__shfl_up((int)upto, x, 64);
-            if (s.lane >= x) upto += y;
-          }
+          const uint32_t same = shared.same[q][threadIdx.x], upto = wave_scan32(same);
           const uint64_t first = upto - same;  // the border's tokens before this lane's
           uint64_t lane_left = left_here > first ? left_here - first : 0;
           const uint64_t w = shared.own[q][threadIdx.x] + min(lane_left, (uint64_t)same) * one;
-          const uint64_t scan = wave_scan64(w, s.lane);
+          const uint64_t scan = wave_scan64(w);
           uint64_t from = before + scan - w;
-          if (from <= aim && aim < from + w) {
+          const bool here = from <= aim && aim < from + w;
+          before += lane64(scan, 63);
+          left_here -= min(left_here, (uint64_t)lane32(upto, 63));
+          if (aim < before) {
             const u32x4 raw = s.load(q);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const uint32_t pair = ordered2<T>(raw[e >> 1]), key = e & 1 ? pair >> 16 : pair & 0xffffu;
-              uint64_t one_w = key > at ? s.weight(key) : 0;
-              if (key >= low && key <= at && lane_left) one_w = one, --lane_left;
-              if (from <= aim && aim < from + one_w) a.ids[r] = s.index(q) + e;
-              from += one_w;
+              const uint32_t bits = S::half(raw[e >> 1], e), key = S::half(ordered2<T>(raw[e >> 1]), e);
+              uint64_t w1 = key > at ? tables ? s.table_weight(bits, key) : s.weight(key) : 0;
+              if (key >= low && key <= at && lane_left) w1 = one, --lane_left;
+              if (here && from <= aim && aim < from + w1) a.ids[r] = s.index(q) + e;
+              from += w1;
             }
+            break;
           }
-          before += (uint64_t)__shfl((unsigned long long)scan, 63, 64);
-          left_here -= min(left_here, (uint64_t)(uint32_t)__shfl((int)upto, 63, 64));
-          if (aim < before) break;
         }
       }
     }

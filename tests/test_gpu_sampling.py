@@ -108,7 +108,10 @@ def test_logits_close_together_and_far_apart(dev, V):
     u = [(r + 0.4) / 12 for r in range(12)]
     for k, p in ((None, None), ([40] * 12, None), (None, [0.9] * 12), ([300] * 12, [0.8] * 12)):
         _check(dev, x, u, [1.0] * 12, k, p, doubtful=1)
+        _check(dev, x.to(BF), u, [1.0] * 12, k, p, doubtful=1)
+        _check(dev, x.to(HF), u, [0.7] * 12, k, p, doubtful=1)
         _check(dev, x.to(HF), u, [0.7] * 12, k, p, [0.05] * 12, doubtful=1)
+        _check(dev, x.to(BF), u, [1e-4, 1e-3, 1e3, 1e-2, 30.0, 1e20, 0.7, 1e-2, 3.0, 1e6, 0.1, 50.0], k, p, doubtful=1)
 
 
 def test_exact_borders(dev):
