@@ -32,7 +32,6 @@ struct SampleArgs {
   float t0, p0, m0;
   int k0;
   int64_t* ids;  // (rows,)
-  int64_t rows;
   int V;
 };
 
@@ -40,13 +39,11 @@ constexpr int kSampleBins = 2048;   // of a level of the exact search
 constexpr int kSampleChunk = 512;   // logits of a wave at a time, 8 a lane
 constexpr uint64_t kSampleOne = 1ull << 43;
 
-// Values as integers in the values' order: -0 as +0, every NaN above +infinity; 0 stands for no logit at all
+// Values as integers in the values' order, -0 as +0
 template <typename T>
 struct SampleKey {
-  static constexpr uint32_t kNan = 0xffffu;
-  static __device__ __forceinline__ uint32_t of(uint32_t raw) {
-    const uint32_t inf = __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
-    if ((raw & 0x7fffu) > inf) return kNan;
+  static __device__ __forceinline__ uint32_t of_value(float x) {
+    uint32_t raw = __builtin_bit_cast(uint16_t, from_f32<T>(x));
     if (raw == 0x8000u) raw = 0;
     return raw & 0x8000u ? raw ^ 0xffffu : raw | 0x8000u;
   }
@@ -56,9 +53,8 @@ struct SampleKey {
 };
 template <>
 struct SampleKey<float> {
-  static constexpr uint32_t kNan = 0xffffffffu;
-  static __device__ __forceinline__ uint32_t of(uint32_t raw) {
-    if ((raw & 0x7fffffffu) > 0x7f800000u) return kNan;
+  static __device__ __forceinline__ uint32_t of_value(float x) {
+    uint32_t raw = __builtin_bit_cast(uint32_t, x);
     if (raw == 0x80000000u) raw = 0;
     return raw & 0x80000000u ? ~raw : raw | 0x80000000u;
   }
@@ -67,9 +63,6 @@ struct SampleKey<float> {
   }
 };
 
-__device__ __forceinline__ uint64_t wave_xor64(uint64_t x, int m) {
-  return (uint64_t)__shfl_xor((unsigned long long)x, m, 64);
-}
 // The sum over this lane and the ones below it: lane exchanges inside rows of 16, then the rows' last lanes (no LDS)
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint64_t dpp_add64(uint64_t x) {
@@ -124,9 +117,13 @@ struct SampleRaw {
       }
     }
   }
-  __device__ __forceinline__ uint32_t raw(int e) const {
-    if constexpr (sizeof(T) == 4) return v[e >> 2][e & 3];
-    else return (v[0][e >> 1] >> (16 * (e & 1))) & 0xffffu;
+  __device__ __forceinline__ float value(int e) const {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t u = v[e >> 2][e & 3];  // (a bit cast of the element itself takes the vector's first)
+      return __builtin_bit_cast(float, u);
+    } else {
+      return elem16<T>(v[0], e);
+    }
   }
 };
 
@@ -153,7 +150,8 @@ __device__ __forceinline__ uint64_t sample_weight(double x, double xmax, double 
 // A token in the order: its key, then the lower index first
 __device__ __forceinline__ uint64_t sample_order(uint32_t key, int i) { return (uint64_t)key << 32 | (uint32_t)~i; }
 
-// A row's workgroup: NW waves, each with a contiguous part of it
+// A row's workgroup: NW waves, each with a contiguous part of it.  Passes work on the values themselves (no row with a NaN comes
+// past the first one): a missing logit, behind the row's end, reads as NaN, which no comparison keeps and which has no weight
 template <typename T, int NW>
 struct Sampler {
   static constexpr int NT = 64 * NW, PER = kSampleBins / NT;
@@ -166,47 +164,45 @@ struct Sampler {
     unsigned long long part[NW];
     uint64_t found[3];
     unsigned long long last, sum;
-    uint32_t n;
+    float top[NW], least[NW];
+    uint32_t n, first;
   };
   Shared* sh;
   const T* row;
   int V, lane, wave, first, last;  // the wave's part in chunks
-  uint32_t top, least;             // the largest and the smallest key
-  float xtop, width;               // the largest logit; bins a unit of logits
-  double xmax, c;                  // the same; log2(e) / temperature
+  float top, least, width;         // the largest and the smallest logit; bins a unit of logits
+  double c;                        // log2(e) / temperature
 
-  // f(index, key) for every logit of the wave's part, loads a chunk ahead
+  // f(index, value) for every logit of the wave's part, loads a chunk ahead
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     SampleRaw<T> next;
     if (first < last) next.load(row, first * kSampleChunk + 8 * lane, V);
+#pragma unroll 1
     for (int q = first; q < last; ++q) {
       const SampleRaw<T> now = next;
       const int i = q * kSampleChunk + 8 * lane;
       if (q + 1 < last) next.load(row, i + kSampleChunk, V);
-      if ((q + 1) * kSampleChunk <= V) {
+      const bool whole = (q + 1) * kSampleChunk <= V;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f(i + e, SampleKey<T>::of(now.raw(e)));
-          if (e & 1) __builtin_amdgcn_sched_barrier(0);  // (eight exponentials side by side take more registers than there are)
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f(i + e, i + e < V ? SampleKey<T>::of(now.raw(e)) : 0u);
+      for (int e = 0; e < 8; ++e) {
+        const float x = now.value(e);
+        f(i + e, whole || i + e < V ? x : __builtin_nanf(""));
+        if (e & 1) __builtin_amdgcn_sched_barrier(0);  // (eight exponentials side by side take more registers than there are)
       }
     }
   }
 
-  // 2^43 for every largest logit, whatever it is.  (A missing logit's key is that of a NaN: 0)
-  __device__ __forceinline__ uint64_t weight(uint32_t k) const {
-    const uint64_t w = sample_weight((double)SampleKey<T>::value(k), xmax, c, sh->power);
-    return k == top ? kSampleOne : w;
+  // 2^43 for every largest logit, whatever it is
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    const uint64_t w = sample_weight((double)x, (double)top, c, sh->power);
+    return x == top ? kSampleOne : w;
   }
 
   // A logit's bin: equal widths below the largest; what has no weight lies in the last one, which holds nothing else
-  __device__ __forceinline__ int bin(uint32_t k) const {
-    const int b = (int)fminf((xtop - SampleKey<T>::value(k)) * width, (float)(B - 1));
-    return k == top ? 0 : b;
+  __device__ __forceinline__ int bin(float x) const {
+    const int b = (int)fminf((top - x) * width, (float)(B - 1));
+    return x == top ? 0 : b;
   }
 
   __device__ __forceinline__ uint64_t block_sum(uint64_t x) {
@@ -254,10 +250,10 @@ struct Sampler {
   __device__ __forceinline__ int gather(int b) {
     if (threadIdx.x == 0) sh->n = 0;
     __syncthreads();
-    each([&](int i, uint32_t k) {
-      if (k && bin(k) == b) {
+    each([&](int i, float x) {
+      if (bin(x) == b && x == x) {
         const uint32_t at = atomicAdd(&sh->n, 1u);
-        if (at < (uint32_t)LIST) sh->key[at] = sample_order(k, i), sh->weight[at] = weight(k);
+        if (at < (uint32_t)LIST) sh->key[at] = sample_order(SampleKey<T>::of_value(x), i), sh->weight[at] = weight(x);
       }
     });
     __syncthreads();
@@ -289,19 +285,20 @@ struct Sampler {
   }
 
   // The exact search: where the tokens in order, those from `from` on left out, first hold `target` (>= 1, at most the whole sum)
-  // of amount(key).  Returns the last token needed
+  // of amount(value).  Returns the last token needed
   template <typename F>
   __device__ __forceinline__ uint64_t search(uint64_t from, uint64_t target, F amount) {
-    uint32_t hi = top, lo = max(least, (uint32_t)(from >> 32));
+    uint32_t hi = SampleKey<T>::of_value(top), lo = max(SampleKey<T>::of_value(least), (uint32_t)(from >> 32));
     uint64_t above = 0, held;
     while (true) {
       const int bits = 32 - __clz((int)(hi - lo));
       const int shift = bits > 11 ? bits - 11 : 0;
       for (int b = threadIdx.x; b < kSampleBins; b += NT) sh->mass[b] = 0;
       __syncthreads();
-      each([&](int, uint32_t k) {
-        if (k >= lo && k <= hi) {
-          const uint64_t n = amount(k);
+      each([&](int, float x) {
+        const uint32_t k = SampleKey<T>::of_value(x);
+        if (k >= lo && k <= hi && x == x) {
+          const uint64_t n = amount(x);
           if (n) atomicAdd(&sh->mass[(hi - k) >> shift], (unsigned long long)n);
         }
       });
@@ -312,16 +309,17 @@ struct Sampler {
       lo = hi - lo > span ? hi - span : lo;
     }
     // of the tokens that hold exactly this value the first so many
-    const uint64_t one = amount(hi), n = (target - above + one - 1) / one;
+    const float at = SampleKey<T>::value(hi);
+    const uint64_t one = amount(at), n = (target - above + one - 1) / one;
     if (n * one >= held) return sample_order(hi, V - 1);
-    return sample_order(hi, find([&](int, uint32_t k) { return (uint64_t)(k == hi); }, [&](uint64_t) { return n - 1; }));
+    return sample_order(hi, find([&](int, float x) { return (uint64_t)(x == at); }, [&](uint64_t) { return n - 1; }));
   }
 
-  // The first index at which the sum of amount(index, key) passes target(the whole sum), which is below it
+  // The first index at which the sum of amount(index, value) passes target(the whole sum), which is below it
   template <typename F, typename G>
   __device__ __forceinline__ int find(F amount, G target) {
     uint64_t mine = 0;
-    each([&](int i, uint32_t k) { mine += amount(i, k); });
+    each([&](int i, float x) { mine += amount(i, x); });
     mine = wave_sum64(mine);
     if (lane == 0) sh->part[wave] = mine;
     __syncthreads();
@@ -333,13 +331,16 @@ struct Sampler {
     }
     const uint64_t aim = target(sum);
     if (before <= aim && aim < before + mine) {  // one wave, all of it
+      SampleRaw<T> next;
+      next.load(row, first * kSampleChunk + 8 * lane, V);
+#pragma unroll 1
       for (int q = first; q < last; ++q) {
         const int i = q * kSampleChunk + 8 * lane;
-        SampleRaw<T> now;
-        now.load(row, i, V);
+        const SampleRaw<T> now = next;
+        if (q + 1 < last) next.load(row, i + kSampleChunk, V);
         uint64_t n[8], own = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) own += n[e] = amount(i + e, i + e < V ? SampleKey<T>::of(now.raw(e)) : 0u);
+        for (int e = 0; e < 8; ++e) own += n[e] = amount(i + e, i + e < V ? now.value(e) : __builtin_nanf(""));
         const uint64_t upto = wave_scan64(own);
         uint64_t at = before + upto - own;
         if (at <= aim && aim < at + own) {
@@ -359,17 +360,25 @@ struct Sampler {
     return i;
   }
 
+  // The tokens up to a last one in order (0: every one)
+  struct Kept {
+    float at;
+    int index;
+    __device__ __forceinline__ explicit Kept(uint64_t last)
+        : at(last ? SampleKey<T>::value((uint32_t)(last >> 32)) : -INFINITY), index(last ? (int)~(uint32_t)last : 0x7fffffff) {}
+    __device__ __forceinline__ bool operator()(int i, float x) const { return x > at || (x == at && i <= index); }
+  };
+
   // The last token that top-k and top-p keep (0: every one)
   __device__ __forceinline__ uint64_t border(int k, float p) {
     const bool by_count = k > 0 && k < V, by_mass = p < 1.f;  // (a NaN is no filter)
     if (!by_count && !by_mass) return 0;
     for (int b = threadIdx.x; b < B; b += NT) sh->mass[b] = 0, sh->count[b] = 0;
     __syncthreads();
-    each([&](int, uint32_t key) {
-      if (!key) return;
-      const int b = bin(key);
+    each([&](int, float x) {  // (a missing one is counted in the last bin, where it changes nothing)
+      const int b = bin(x);
       if (by_count) atomicAdd(&sh->count[b], 1u);
-      if (by_mass) atomicAdd(&sh->mass[b], (unsigned long long)weight(key));
+      if (by_mass) atomicAdd(&sh->mass[b], (unsigned long long)weight(x));
     });
     __syncthreads();
     uint64_t keep = 0, above, held, total = 0;
@@ -384,12 +393,13 @@ struct Sampler {
           keep = cut(gather(b), [&](uint32_t rank, uint64_t) { return above + rank < (uint64_t)k; }, total);
         }
       }
-      if (slow) keep = search(0, (uint64_t)k, [](uint32_t) { return (uint64_t)1; });
+      if (slow) keep = search(0, (uint64_t)k, [](float) { return (uint64_t)1; });
     }
     if (!by_mass) return keep;
     if (slow) {
       uint64_t mine = 0;
-      each([&](int i, uint32_t key) { mine += sample_order(key, i) >= keep ? weight(key) : 0; });
+      const Kept kept(keep);
+      each([&](int i, float x) { mine += kept(i, x) ? weight(x) : 0; });
       total = block_sum(mine);
     } else {
       // the bins above the list's, and what of it is kept
@@ -410,7 +420,7 @@ struct Sampler {
       if (!slow)
         return max(keep, cut((int)min(sh->n, (uint32_t)LIST), [&](uint32_t, uint64_t before) { return above + before < target; }, held));
     }
-    return max(keep, search(keep, target, [&](uint32_t key) { return weight(key); }));
+    return max(keep, search(keep, target, [&](float x) { return weight(x); }));
   }
 };
 
@@ -427,56 +437,51 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
   s.first = min(s.wave * each, chunks);
   s.last = min(s.first + each, chunks);
   for (int j = threadIdx.x; j < 256; j += S::NT) shared.power[j] = exp2(j / 256.0);
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    s.row = (const T*)a.logits + r * a.ld;
-    // the largest logit, at its lowest index, and the smallest
-    uint64_t best = 0;
-    uint32_t least = 0xffffffffu;
-    s.each([&](int i, uint32_t key) {
-      const uint64_t v = sample_order(key, i);
-      best = v > best ? v : best;
-      least = key && key < least ? key : least;
+  const int64_t r = blockIdx.x;
+  s.row = (const T*)a.logits + r * a.ld;
+  // ---- the largest logit and the smallest, and whether there is a NaN
+  float top = -INFINITY, least = INFINITY;
+  bool bad = false;
+  s.each([&](int i, float x) {
+    top = fmaxf(top, x);
+    least = fminf(least, x);
+    bad |= x != x && i < a.V;
+  });
+  top = wave_max(top);
+  least = wave_min(least);
+  if (s.lane == 0) shared.top[s.wave] = top, shared.least[s.wave] = least;
+  if (threadIdx.x == 0) shared.first = 0x7fffffffu;
+  const bool nan = __syncthreads_or(bad);
+#pragma unroll
+  for (int q = 0; q < NW; ++q) top = fmaxf(top, shared.top[q]), least = fminf(least, shared.least[q]);
+  s.top = top;
+  s.least = least;
+  int answer;
+  const float t = a.temperature ? a.temperature[r] : a.t0;
+  if (nan || !(t > 0.f)) {
+    // the first NaN, which is above all as in torch's argmax, or the first of the largest
+    uint32_t at = 0x7fffffffu;
+    s.each([&](int i, float x) {
+      if ((nan ? x != x : x == top) && i < a.V) at = min(at, (uint32_t)i);
     });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      const uint64_t v = wave_xor64(best, m);
-      best = v > best ? v : best;
-      least = min(least, (uint32_t)__shfl_xor((int)least, m, 64));
-    }
-    if (s.lane == 0) shared.mass[2 * s.wave] = best, shared.mass[2 * s.wave + 1] = least;
+    if (at != 0x7fffffffu) atomicMin(&shared.first, at);
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < NW; ++q) {
-      best = max(best, (uint64_t)shared.mass[2 * q]);
-      least = min(least, (uint32_t)shared.mass[2 * q + 1]);
-    }
-    __syncthreads();
-    s.top = (uint32_t)(best >> 32);
-    s.least = least;
-    int answer = (int)~(uint32_t)best;
-    const float t = a.temperature ? a.temperature[r] : a.t0;
-    if (t > 0.f && s.top != SampleKey<T>::kNan) {  // (else the largest logit; a NaN is above all, as in torch's argmax)
-      s.xtop = SampleKey<T>::value(s.top);
-      s.xmax = (double)s.xtop;
-      s.c = 1.4426950408889634 / (double)t;
-      // every logit above the last bin, but what lies 31 temperatures below the largest
-      s.width = (float)(S::B - 1) / fminf((s.xtop - SampleKey<T>::value(least)) * 1.001f, 31.f * t);
-      if (!(s.width > 0.f && s.width < 3e38f)) s.width = 0.f;
-      const uint64_t keep = s.border(a.top_k ? a.top_k[r] : a.k0, a.top_p ? a.top_p[r] : a.p0);
-      const float m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
-      const double least_x = m >= 1.f ? s.xmax : m > 0.f ? s.xmax + (double)t * log((double)m) : -INFINITY;
-      answer = s.find(
-          [&](int i, uint32_t key) {
-            const bool kept = key && sample_order(key, i) >= keep && !((double)SampleKey<T>::value(key) < least_x);
-            return kept ? s.weight(key) : (uint64_t)0;
-          },
-          [&](uint64_t sum) {
-            const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
-            return (uint64_t)(f * (double)sum);
-          });
-    }
-    if (threadIdx.x == 0) a.ids[r] = answer;
+    answer = (int)shared.first;
+  } else {
+    s.c = 1.4426950408889634 / (double)t;
+    // every logit above the last bin, but what lies 31 temperatures below the largest
+    s.width = (float)(S::B - 1) / fminf((top - least) * 1.001f, 31.f * t);
+    if (!(s.width > 0.f && s.width < 3e38f)) s.width = 0.f;
+    const typename S::Kept kept(s.border(a.top_k ? a.top_k[r] : a.k0, a.top_p ? a.top_p[r] : a.p0));
+    const float m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
+    const double least_x = m >= 1.f ? (double)top : m > 0.f ? (double)top + (double)t * log((double)m) : -INFINITY;
+    answer = s.find([&](int i, float x) { return kept(i, x) && !((double)x < least_x) ? s.weight(x) : (uint64_t)0; },
+                    [&](uint64_t sum) {
+                      const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+                      return (uint64_t)(f * (double)sum);
+                    });
   }
+  if (threadIdx.x == 0) a.ids[r] = answer;
 }
 
 // ------------------------------------------------------------------------------------------------ 16-bit logits
@@ -505,14 +510,15 @@ struct Counted {
   static constexpr uint32_t kInf = __is_same(T, bf16) ? 0xff80u : 0xfc00u, kNegInf = 0xffffu - kInf;
   // the weights' tables: mantissa bits and the upper ones of them, exponents a sign
   static constexpr int kMan = __is_same(T, bf16) ? 7 : 10, kBias = __is_same(T, bf16) ? 127 : 15, kHigh = (kMan + 1) / 2,
-                       kLow = kMan - kHigh, kExps = 32;
+                       kLow = kMan - kHigh, kExps = __is_same(T, bf16) ? 32 : 30;
+  static constexpr int kHighs = (kExps << kHigh) + 1, kLows = (kExps + 1) << kLow;  // a sign's, and behind them a weight of 0
   struct Shared {
     union {
       uint32_t table[32768];
       struct {
         unsigned long long own[kCountedChunks][kCountedThreads];  // a lane's weight in a chunk
         uint32_t same[kCountedChunks][kCountedThreads];           // and its tokens of the border's value
-        double high[2 * kExps << kHigh], low[2 * kExps << kLow];
+        double high[2 * kHighs], low[2 * kLows];
       };
     };
     unsigned long long mass[512];
@@ -529,7 +535,7 @@ struct Counted {
   int V, lane, wave, first, chunks;  // the wave's part of the row: its first chunk and their number
   uint32_t top, strips;              // strips of which the wave's words hold any
   double xmax, c;
-  int least_exp, exps;               // the exponents that the weights' tables hold
+  int least_exp;                     // the first exponent that the weights' tables hold
 
   __device__ __forceinline__ int index(int q) const { return (first + q) * kSampleChunk + 8 * lane; }
   __device__ __forceinline__ uint64_t weight(uint32_t k) const {
@@ -546,12 +552,16 @@ struct Counted {
       v[e >> 1] = (i + e < V ? row[i + e] : 0xffffu) | (i + e + 1 < V ? row[i + e + 1] : 0xffffu) << 16;
     return v;
   }
-  // f(chunk, its logits, two a word), loads two chunks ahead
+  // f(chunk, its logits, two a word), loads two chunks ahead (a and b: the first two)
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     u32x4 a = {}, b = {};
     if (chunks > 0) a = load(0);
     if (chunks > 1) b = load(1);
+    each(a, b, f);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(u32x4 a, u32x4 b, F f) const {
 #pragma unroll 1
     for (int q = 0; q < chunks; ++q) {
       const u32x4 now = a;
@@ -562,8 +572,8 @@ struct Counted {
   }
   static __device__ __forceinline__ uint32_t half(uint32_t pair, int e) { return e & 1 ? pair >> 16 : pair & 0xffffu; }
 
-  __device__ __forceinline__ void count_values() {
-    each([&](int, const u32x4& raw) {
+  __device__ __forceinline__ void count_values(const u32x4& a, const u32x4& b) {
+    each(a, b, [&](int, const u32x4& raw) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t k = half(ordered2<T>(raw[e >> 1]), e);
@@ -606,9 +616,10 @@ struct Counted {
     __syncthreads();
   }
 
-  // The value at which the tokens in order first hold `target` (>= 1, at most the whole sum): its key, the sum before it and its own
+  // The value at which the tokens in order first hold `target` (>= 1, at most the whole sum): its key, the sum before it and how
+  // many hold it
   template <bool MASS>
-  __device__ __forceinline__ uint32_t border(uint64_t target, uint64_t& above, uint64_t& held) const {
+  __device__ __forceinline__ uint32_t border(uint64_t target, uint64_t& above, uint64_t& number) const {
     uint64_t v[8], mine = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) mine += v[j] = MASS ? (uint64_t)sh->mass[8 * lane + j] : (uint64_t)sh->count[8 * lane + j];
@@ -632,7 +643,7 @@ struct Counted {
     const bool this_one = at < target && at + hi + lo >= target, low = at + hi < target;
     const int l2 = __builtin_ctzll(__ballot(this_one));
     above = lane64(low ? at + hi : at, l2);
-    held = lane64(low ? lo : hi, l2);
+    number = lane32(low ? word & 0xffffu : word >> 16, l2);
     return lane32(low ? k - 1 : k, l2);
   }
 
@@ -654,22 +665,26 @@ struct Counted {
   __device__ __forceinline__ void filter(int k, float p, float m, float t) {
     const bool by_count = k > 0 && k < V, by_mass = p < 1.f;
     uint32_t at = 0, low = 1;
-    uint64_t n = 0, above, held;
+    uint64_t n = 0, above, number;
     if (by_count || by_mass) {
       bool cut = false;
       if (by_count) {
-        at = border<false>((uint64_t)k, above, held);
+        at = border<false>((uint64_t)k, above, number);
         n = (uint64_t)k - above;
-        cut = n < held;
+        cut = n < number;
       }
       if (by_mass) {
         const uint64_t total = weight_above(at) + (by_count ? n * weight(at) : 0);
         const double want = (double)p * (double)total;
         const uint64_t target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
-        const uint32_t pk = border<true>(target, above, held);
-        const uint64_t w = weight(pk), take = (target - above + w - 1) / w;
+        const uint32_t pk = border<true>(target, above, number);
+        // the least number of them that holds what is missing
+        const uint64_t w = weight(pk), missing = target - above;
+        uint64_t take = (uint64_t)((double)missing / (double)w);
+        while (take * w < missing) ++take;
+        while (take > 1 && (take - 1) * w >= missing) --take;
         if (pk != at || take < n) {
-          cut = (pk == at && cut) || take < held / w;
+          cut = (pk == at && cut) || take < number;
           n = take;
         }
         at = pk;
@@ -698,55 +713,82 @@ struct Counted {
   }
 
   // Weights by tables, for rows that keep many tokens.  x = s (2^E + f) for each sign and exponent E, its fraction f = f1 + f2 by its
-  // upper and lower bits: 2^43 exp((s (2^E + f1) - max) / t) times exp(s f2 / t), 24 (fp16: 64) values a binade, for the 32 binades up
+  // upper and lower bits: 2^43 exp((s (2^E + f1) - max) / t) times exp(s f2 / t), 24 (fp16: 64) values a binade, for the binades up
   // to the largest magnitude that has a weight.  Returns whether they serve (else a factor might leave fp64's range)
   __device__ __forceinline__ bool prepare(float t) {
     const float most = fabsf((float)xmax) + 31.f * t;
     const uint32_t bits = __builtin_bit_cast(uint16_t, from_f32<T>(most * 1.01f)) & 0x7fffu;
     const int hi = min((int)(bits >> kMan), (1 << (15 - kMan)) - 2);  // (the last exponent is that of infinities)
     least_exp = max(hi - kExps + 1, 0);
-    exps = hi - least_exp;
     const double ulp = __builtin_amdgcn_ldexp(1.0, max(hi, 1) - kBias - kMan);
     if (!(ulp * c * (1 << kLow) < 500.0) || !(fabs(xmax) < 1e30)) return false;
-    for (int i = threadIdx.x; i < (2 * kExps << kHigh) + (2 * kExps << kLow); i += kCountedThreads) {
-      const bool upper = i < 2 * kExps << kHigh;
-      const int j = upper ? i : i - (2 * kExps << kHigh), shift = upper ? kHigh : kLow;
-      const int E = ((j >> shift) & (kExps - 1)) + least_exp, f = (j & ((1 << shift) - 1)) << (upper ? kLow : 0);
+    for (int i = threadIdx.x; i < 2 * (kHighs + kLows); i += kCountedThreads) {
+      const bool upper = i < 2 * kHighs;
+      const int size = upper ? kHighs : kLows, shift = upper ? kHigh : kLow;
+      int j = upper ? i : i - 2 * kHighs;
+      const bool negative = j >= size;
+      if (negative) j -= size;
+      const int E = (j >> shift) + least_exp, f = (j & ((1 << shift) - 1)) << (upper ? kLow : 0);
       double x = __builtin_amdgcn_ldexp((double)(f + (upper && E ? 1 << kMan : 0)), max(E, 1) - kBias - kMan);
-      if (j >> (shift + 5)) x = -x;
+      if (negative) x = -x;
       const double y = upper ? fma(x - xmax, c, 43.0) : x * c;
-      const double w = sample_power(fmin(fmax(y, -1000.0), 1000.0), sh->power);
-      if (upper) sh->high[j] = w;
-      else sh->low[j] = w;
+      double w = sample_power(fmin(fmax(y, -1000.0), 1000.0), sh->power);
+      if (j >> shift == kExps) w = 0.0;
+      (upper ? sh->high : sh->low)[i - (upper ? 0 : 2 * kHighs)] = w;
     }
     return true;
   }
-  __device__ __forceinline__ uint64_t table_weight(uint32_t raw, uint32_t k) const {
-    const uint32_t sign = raw >> 15, mag = raw & 0x7fffu;
-    const int e = (int)(mag >> kMan) - least_exp;
-    const uint32_t slot = (uint32_t)min(max(e, 0), exps);
-    const uint32_t hi = (((sign << 5) + slot) << kHigh) + ((mag >> kLow) & ((1 << kHigh) - 1));
-    const uint32_t lo = (((sign << 5) + slot) << kLow) + (mag & ((1 << kLow) - 1));
-    uint64_t w = whole64(sh->high[hi] * sh->low[lo]);
-    if (e > exps) w = 0;  // (negative, and further below the largest than any weight reaches)
-    if (__any(e < 0)) w = e < 0 ? weight(k) : w;
-    return k == top ? kSampleOne : w;
+  // The sum of the weights of chunk elements kept by `keep`, one multiplication and addition each: 2^52 + (a whole number) rounds
+  // every addition to a whole number.  Magnitudes above the tables' belong to negative logits without a weight
+  __device__ __forceinline__ double table_add(double sum, uint32_t raw, bool keep) const {
+    const uint32_t mag = raw & 0x7fffu, sign = raw >> 15;
+    const uint32_t at = min((mag >> kLow) - ((uint32_t)least_exp << kHigh), (uint32_t)(kExps << kHigh));
+    const uint32_t hi = keep ? at + sign * kHighs : (uint32_t)(kExps << kHigh);
+    const uint32_t lo = ((at >> kHigh) << kLow) + (mag & ((1 << kLow) - 1)) + sign * kLows;
+    return fma(sh->high[hi], sh->low[lo], sum);
+  }
+  // The kept weight of eight logits, and up to the e-th
+  __device__ __forceinline__ uint64_t table_weight8(const u32x4& raw, uint32_t at) const {
+    double sum = 0x1p52;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = table_add(sum, half(raw[e >> 1], e), half(ordered2<T>(raw[e >> 1]), e) > at);
+    return __builtin_bit_cast(uint64_t, sum) & 0xfffffffffffffull;
+  }
+  // Whether a chunk's weights are best looked up: three steps and more of its eight meet a kept token, and the tables hold the
+  // magnitudes of all its logits (none lies below them)
+  __device__ __forceinline__ bool held(const u32x4& raw, uint32_t at) const {
+    uint32_t least = 0x7fffu;
+    int steps = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      least = min(least, half(raw[e >> 1], e) & 0x7fffu);
+      steps += __any(half(ordered2<T>(raw[e >> 1]), e) > at) != 0;
+    }
+    return steps >= 3 && !__any((int)(least >> kMan) < least_exp);
   }
 
   // The kept weights, and the border's tokens, of the wave's part
   template <bool TABLES>
   __device__ __forceinline__ void add_up(uint32_t at, uint32_t low, uint64_t& sum, uint32_t& number) {
+    const bool ties = low <= at;
     each([&](int q, const u32x4& raw) {
       uint64_t own = 0;
       uint32_t same = 0;
+      if (TABLES && held(raw, at)) {
+        own = table_weight8(raw, at);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = half(ordered2<T>(raw[e >> 1]), e);
-        if (__any(key > at)) {
-          const uint64_t w = TABLES ? table_weight(half(raw[e >> 1], e), key) : weight(key);
-          own += key > at ? w : 0;
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t key = half(ordered2<T>(raw[e >> 1]), e);
+          if (__any(key > at)) own += key > at ? weight(key) : 0;
         }
-        same += key >= low && key <= at;
+      }
+      if (ties) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t key = half(ordered2<T>(raw[e >> 1]), e);
+          same += key - low <= at - low;
+        }
       }
       sh->own[q][threadIdx.x] = own;
       sh->same[q][threadIdx.x] = same;
@@ -769,109 +811,117 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
   s.first = min(s.wave * each, chunks);
   s.chunks = min(each, chunks - s.first);
   if (threadIdx.x < 256) shared.power[threadIdx.x] = exp2(threadIdx.x / 256.0);
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    s.row = (const uint16_t*)a.logits + r * a.ld;
+  const int64_t r = blockIdx.x;
+  s.row = (const uint16_t*)a.logits + r * a.ld;
+  u32x4 first = {}, second = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ((u32x4*)shared.table)[1024 * i + threadIdx.x] = u32x4{};
-    if (threadIdx.x < 512) shared.count[threadIdx.x] = 0, shared.mass[threadIdx.x] = 0;
-    if (threadIdx.x == 0) shared.top = 0xffffffffu, shared.first = 0x7fffffffu;
+  for (int i = 0; i < 8; ++i) ((u32x4*)shared.table)[1024 * i + threadIdx.x] = u32x4{};
+  if (threadIdx.x < 512) shared.count[threadIdx.x] = 0, shared.mass[threadIdx.x] = 0;
+  if (threadIdx.x == 0) shared.top = 0xffffffffu, shared.first = 0x7fffffffu;
+  __syncthreads();
+  if (s.chunks > 0) first = s.load(0);
+  if (s.chunks > 1) second = s.load(1);
+  s.count_values(first, second);
+  __syncthreads();
+  // ---- the largest value; NaNs lie in the first and the last strip (what lies behind the row's end is counted at key 0)
+  bool bad = false;
+  s.strips = 0;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t at = 1024 * i + threadIdx.x;
+    uint32_t word = shared.table[32767 - at];
+    if (i == 31 && at == 32767) word -= (uint32_t)(chunks * kSampleChunk - a.V);
+    if (__any(word != 0)) s.strips |= 1u << i;
+    if (i == 0) bad |= (word >> 16 && 65535u - 2 * at > S::kInf) || (word & 0xffffu && 65534u - 2 * at > S::kInf);
+    if (i == 31) bad |= (word >> 16 && 65535u - 2 * at < S::kNegInf) || (word & 0xffffu && 65534u - 2 * at < S::kNegInf);
+  }
+  if (s.strips) {
+    const int at = 1024 * __builtin_ctz(s.strips) + threadIdx.x;
+    const uint32_t word = shared.table[32767 - at];
+    const int l = __builtin_ctzll(__ballot(word != 0));
+    if (s.lane == l) atomicMin(&shared.top, 2u * at + (word >> 16 ? 0 : 1));
+  }
+  const bool nan = __syncthreads_or(bad);
+  s.top = 65535u - shared.top;
+  if (threadIdx.x == 0) {
+    shared.table[0] &= 0xffff0000u;
+    const uint32_t zeros = shared.table[0x3fff] >> 16;  // -0
+    shared.table[0x3fff] &= 0xffffu;
+    shared.table[0x4000] += zeros;
+  }
+  s.strips |= 1u << 15;  // (where +0 lies)
+  if (s.top == 0x7fffu) s.top = 0x8000u;
+  __syncthreads();
+  const float t = a.temperature ? a.temperature[r] : a.t0;
+  if (nan) {
+    const int i = s.first_of(S::kInf + 1, 0xffffu, 0, S::kNegInf - 1);
+    if (threadIdx.x == 0) a.ids[r] = i;
+  } else if (!(t > 0.f)) {
+    const int i = s.first_of(s.top == 0x8000u ? 0x7fffu : s.top, s.top, 1, 0);
+    if (threadIdx.x == 0) a.ids[r] = i;
+  } else {
+    s.xmax = (double)ordered_value<T>(s.top);
+    s.c = 1.4426950408889634 / (double)t;
+    const int k = a.top_k ? a.top_k[r] : a.k0;
+    const float p = a.top_p ? a.top_p[r] : a.p0, m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
+    if ((k > 0 && k < a.V) || p < 1.f) s.tabulate(p < 1.f);
+    if (s.wave == 0) s.filter(k, p, m, t);
+    __syncthreads();  // the counts are read
+    const uint32_t at = shared.at, low = shared.low_key;
+    const uint64_t n = shared.n, one = shared.one;
+    // tables pay where most waves meet a kept token at most of their steps
+    const bool tables = (k <= 0 || k > 512) && s.prepare(t);
     __syncthreads();
-    s.count_values();
+    uint64_t sum = 0;
+    uint32_t number = 0;
+    if (tables) s.template add_up<true>(at, low, sum, number);
+    else s.template add_up<false>(at, low, sum, number);
+    sum = wave_sum64(sum);
+    number = lane32(wave_scan32(number), 63);
+    if (s.lane == 0) shared.part[s.wave] = sum, shared.ties[s.wave] = number;
     __syncthreads();
-    // ---- the largest value; NaNs lie in the first and the last strip (what lies behind the row's end is counted at key 0)
-    uint32_t top = 0xffffffffu;
-    bool bad = false;
-    s.strips = 0;
+    uint64_t before = 0, left = n, mine = 0, total = 0, left_here = 0;  // left: tokens of the border still to be kept
 #pragma unroll
-    for (int i = 31; i >= 0; --i) {
-      const uint32_t at = 1024 * i + threadIdx.x;
-      uint32_t word = shared.table[32767 - at];
-      if (i == 31 && at == 32767) word -= (uint32_t)(chunks * kSampleChunk - a.V);
-      if (word) top = 2 * at + (word >> 16 ? 0 : 1);
-      if (__any(word != 0)) s.strips |= 1u << i;
-      if (i == 0) bad |= (word >> 16 && 65535u - 2 * at > S::kInf) || (word & 0xffffu && 65534u - 2 * at > S::kInf);
-      if (i == 31) bad |= (word >> 16 && 65535u - 2 * at < S::kNegInf) || (word & 0xffffu && 65534u - 2 * at < S::kNegInf);
+    for (int q = 0; q < 16; ++q) {
+      const uint64_t take = min(left, (uint64_t)shared.ties[q]), w = shared.part[q] + take * one;
+      if (q == s.wave) before = total, mine = w, left_here = left;
+      total += w;
+      left -= take;
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) top = min(top, (uint32_t)__shfl_xor((int)top, m, 64));
-    if (s.lane == 0) atomicMin(&shared.top, top);
-    const bool nan = __syncthreads_or(bad);
-    s.top = 65535u - shared.top;
-    if (threadIdx.x == 0) {
-      shared.table[0] &= 0xffff0000u;
-      const uint32_t zeros = shared.table[0x3fff] >> 16;  // -0
-      shared.table[0x3fff] &= 0xffffu;
-      shared.table[0x4000] += zeros;
-    }
-    s.strips |= 1u << 15;  // (where +0 lies)
-    if (s.top == 0x7fffu) s.top = 0x8000u;
-    __syncthreads();
-    const float t = a.temperature ? a.temperature[r] : a.t0;
-    if (nan) {
-      const int i = s.first_of(S::kInf + 1, 0xffffu, 0, S::kNegInf - 1);
-      if (threadIdx.x == 0) a.ids[r] = i;
-    } else if (!(t > 0.f)) {
-      const int i = s.first_of(s.top == 0x8000u ? 0x7fffu : s.top, s.top, 1, 0);
-      if (threadIdx.x == 0) a.ids[r] = i;
-    } else {
-      s.xmax = (double)ordered_value<T>(s.top);
-      s.c = 1.4426950408889634 / (double)t;
-      const int k = a.top_k ? a.top_k[r] : a.k0;
-      const float p = a.top_p ? a.top_p[r] : a.p0, m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
-      if ((k > 0 && k < a.V) || p < 1.f) s.tabulate(p < 1.f);
-      if (s.wave == 0) s.filter(k, p, m, t);
-      __syncthreads();  // the counts are read
-      const uint32_t at = shared.at, low = shared.low_key;
-      const uint64_t n = shared.n, one = shared.one;
-      // tables pay where most waves meet a kept token at most of their steps
-      const bool tables = (k <= 0 || k > 512) && s.prepare(t);
-      __syncthreads();
-      uint64_t sum = 0;
-      uint32_t number = 0;
-      if (tables) s.template add_up<true>(at, low, sum, number);
-      else s.template add_up<false>(at, low, sum, number);
-      sum = wave_sum64(sum);
-      number = lane32(wave_scan32(number), 63);
-      if (s.lane == 0) shared.part[s.wave] = sum, shared.ties[s.wave] = number;
-      __syncthreads();
-      uint64_t before = 0, left = n, mine = 0, total = 0, left_here = 0;  // left: tokens of the border still to be kept
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const uint64_t take = min(left, (uint64_t)shared.ties[q]), w = shared.part[q] + take * one;
-        if (q == s.wave) before = total, mine = w, left_here = left;
-        total += w;
-        left -= take;
-      }
-      const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
-      const uint64_t aim = (uint64_t)(f * (double)total);
-      if (before <= aim && aim < before + mine) {  // one wave, all of it
+    const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+    const uint64_t aim = (uint64_t)(f * (double)total);
+    if (before <= aim && aim < before + mine) {  // one wave, all of it
 #pragma unroll 1
-        for (int q = 0; q < s.chunks; ++q) {
-          const uint32_t same = shared.same[q][threadIdx.x], upto = wave_scan32(same);
-          const uint64_t first = upto - same;  // the border's tokens before this lane's
-          uint64_t lane_left = left_here > first ? left_here - first : 0;
-          const uint64_t w = shared.own[q][threadIdx.x] + min(lane_left, (uint64_t)same) * one;
-          const uint64_t scan = wave_scan64(w);
-          uint64_t from = before + scan - w;
-          const bool here = from <= aim && aim < from + w;
-          before += lane64(scan, 63);
-          left_here -= min(left_here, (uint64_t)lane32(upto, 63));
-          if (aim < before) {
-            const u32x4 raw = s.load(q);
+      for (int q = 0; q < s.chunks; ++q) {
+        const uint32_t same = one ? shared.same[q][threadIdx.x] : 0, upto = wave_scan32(same);
+        const uint64_t earlier = upto - same;  // the border's tokens before this lane's
+        uint64_t still = left_here > earlier ? left_here - earlier : 0;
+        const uint64_t w = shared.own[q][threadIdx.x] + min(still, (uint64_t)same) * one;
+        const uint64_t to = before + wave_scan64(w), from = to - w;
+        before = lane64(to, 63);
+        left_here -= min(left_here, (uint64_t)lane32(upto, 63));
+        if (aim >= before) continue;
+        const u32x4 raw = s.load(q);
+        const bool by_table = tables && s.held(raw, at);
+        double part = 0x1p52;
+        uint64_t at_e = from, exact = 0, kept_ties = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t bits = S::half(raw[e >> 1], e), key = S::half(ordered2<T>(raw[e >> 1]), e);
-              uint64_t w1 = key > at ? tables ? s.table_weight(bits, key) : s.weight(key) : 0;
-              if (key >= low && key <= at && lane_left) w1 = one, --lane_left;
-              if (here && from <= aim && aim < from + w1) a.ids[r] = s.index(q) + e;
-              from += w1;
-            }
-            break;
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t bits = S::half(raw[e >> 1], e), key = S::half(ordered2<T>(raw[e >> 1]), e);
+          if (by_table) {
+            part = s.table_add(part, bits, key > at);
+            exact = __builtin_bit_cast(uint64_t, part) & 0xfffffffffffffull;
+          } else if (__any(key > at)) {
+            exact += key > at ? s.weight(key) : 0;
           }
+          if (key >= low && key <= at && still) kept_ties += one, --still;
+          const uint64_t upto_e = from + exact + kept_ties;
+          if (at_e <= aim && aim < upto_e) a.ids[r] = s.index(q) + e;
+          at_e = upto_e;
         }
+        break;
       }
     }
-    __syncthreads();  // the table is read before the next row clears it
   }
 }
 
@@ -889,21 +939,41 @@ extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* u
   if (!logits || !uniform || !ids) return set_error(ATMA_ERR_INVALID, "%s: null pointer", what);
   if ((uintptr_t)logits % dtype_size(dtype)) return set_error(ATMA_ERR_INVALID, "%s: misaligned logits", what);
   if (rows > 1 && ld < V && ld != 0) return set_error(ATMA_ERR_INVALID, "%s: rows overlap", what);
-  SampleArgs a{logits, ld, uniform, temperature, top_k, top_p, min_p, t0, p0, m0, k0, ids, rows, (int)V};
-  const unsigned grid = (unsigned)std::min<int64_t>(rows, 1 << 20);
-  auto launch = [&](auto zero) {
-    using T = decltype(zero);
-    if constexpr (sizeof(T) == 2) {
-      if (V < 65536) {
-        sample_counted_kernel<T><<<grid, kCountedThreads, 0, (hipStream_t)stream>>>(a);
+  SampleArgs a{logits, ld, uniform, temperature, top_k, top_p, min_p, t0, p0, m0, k0, ids, (int)V};
+  // Short rows take workgroups of four waves, of which a CU holds five: us in bf16, four waves / values counted / sixteen waves, 32 rows of
+  // 2,000 logits 12.9 / 14.7 / -, of 8,000 24.4 / 17.0 / 19.4 (eight), of 16,000 - / 19.2 / 25.0; 2,048 rows of 1,000 29 / 109 / -,
+  // of 8,000 63 / 122 / 82 (eight), of 12,000 - / 131 / 155
+  const bool small = V <= (rows > device_cu_count() ? 16384 : 4096);
+  // a workgroup a row; a launch holds fewer than 2^32 threads, so what no one launch holds goes in several
+  constexpr int64_t most = 1 << 20;
+  for (int64_t r = 0; r < rows; r += most) {
+    SampleArgs p = a;
+    p.logits = (const char*)logits + r * ld * dtype_size(dtype);
+    p.uniform += r;
+    if (temperature) p.temperature += r;
+    if (top_k) p.top_k += r;
+    if (top_p) p.top_p += r;
+    if (min_p) p.min_p += r;
+    p.ids += r;
+    const unsigned grid = (unsigned)std::min(rows - r, most);
+    hipStream_t st = (hipStream_t)stream;
+    auto launch = [&](auto zero) {
+      using T = decltype(zero);
+      if (small) {
+        sample_tokens_kernel<T, 4><<<grid, 256, 0, st>>>(p);
         return;
       }
-    }
-    if (V <= 8192) sample_tokens_kernel<T, 4><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-    else sample_tokens_kernel<T, 16><<<grid, 1024, 0, (hipStream_t)stream>>>(a);
-  };
-  if (dtype == ATMA_BF16) launch(bf16{});
-  else if (dtype == ATMA_F16) launch(f16{});
-  else launch(float{});
+      if constexpr (sizeof(T) == 2) {
+        if (V < 65536) {
+          sample_counted_kernel<T><<<grid, kCountedThreads, 0, st>>>(p);
+          return;
+        }
+      }
+      sample_tokens_kernel<T, 16><<<grid, 1024, 0, st>>>(p);
+    };
+    if (dtype == ATMA_BF16) launch(bf16{});
+    else if (dtype == ATMA_F16) launch(f16{});
+    else launch(float{});
+  }
   return check_launch(what);
 }

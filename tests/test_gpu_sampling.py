@@ -65,11 +65,11 @@ def _logits(g, rows, V, spread=3.0):
     return spread * torch.randn(rows, V, generator=g)
 
 
-@pytest.mark.parametrize("V", [1, 2, 7, 8, 63, 500, 511, 512, 513, 2047, 4099, 8192, 8193, 50304])
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 63, 500, 511, 512, 513, 2047, 4097, 8193, 50304, 65535, 65536])
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_all_filters(dev, V, dtype):
     g = torch.Generator().manual_seed(V)
-    rows = 24 if V < 10000 else 10
+    rows = 24 if V < 10000 else 10 if V < 60000 else 4
     rnd = lambda: torch.rand(rows, generator=g)   # noqa: E731
     logits = _logits(g, rows, V).to(dtype)
     u, t = rnd().tolist(), (0.3 + 1.2 * rnd()).tolist()
@@ -81,17 +81,17 @@ def test_all_filters(dev, V, dtype):
         _check(dev, logits, u, t, *sel, doubtful=1)
 
 
-@pytest.mark.parametrize("V", [3000, 20000])
+@pytest.mark.parametrize("V", [3000, 20000, 70000])
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_many_equal_logits(dev, dtype, V):
     """Borders inside runs of equal logits: the lowest indices are kept."""
     g = torch.Generator().manual_seed(1)
-    rows = 16
+    rows = 16 if V < 50000 else 4
     logits = torch.randint(-3, 3, (rows, V), generator=g).to(dtype)
     logits[3] = 1.5
     u = [(r + 0.5) / rows for r in range(rows)]
     k = [1 + 37 * r for r in range(rows)]
-    _check(dev, logits, u, [1.0] * rows, k)
+    _check(dev, logits, u, [1.0] * rows, k, doubtful=1)
     p = [(r + 0.37) / rows for r in range(rows)]
     _check(dev, logits, u, [0.8] * rows, None, p, doubtful=1)
     _check(dev, logits, u, [0.8] * rows, k, p, doubtful=1)
@@ -112,6 +112,26 @@ def test_logits_close_together_and_far_apart(dev, V):
         _check(dev, x.to(HF), u, [0.7] * 12, k, p, doubtful=1)
         _check(dev, x.to(HF), u, [0.7] * 12, k, p, [0.05] * 12, doubtful=1)
         _check(dev, x.to(BF), u, [1e-4, 1e-3, 1e3, 1e-2, 30.0, 1e20, 0.7, 1e-2, 3.0, 1e6, 0.1, 50.0], k, p, doubtful=1)
+
+
+@pytest.mark.parametrize("V", [3000, 5000, 16384, 16385, 50304, 70001])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_many_rows_and_few_agree(dev, V, dtype):
+    """The kernels for many rows and for few, and any number of rows a call, answer the same."""
+    from atma_amd.kernel import sample_tokens
+    g = torch.Generator().manual_seed(9)
+    rows = 600 if V < 20000 else 300
+    x = _logits(g, rows, V).to(dtype).to(dev)
+    u, t = torch.rand(rows, generator=g).to(dev), (torch.rand(rows, generator=g) * 1.5).to(dev)
+    k = torch.randint(0, 400, (rows,), generator=g, dtype=torch.int32).to(dev)
+    p, m = (0.5 + torch.rand(rows, generator=g)).to(dev), (0.2 * torch.rand(rows, generator=g) - 0.1).to(dev)
+    t[3], k[4:8], x[9, 5] = 0, 0, float("nan")
+    for sel in ((None, None, None), (k, None, None), (None, p, None), (k, p, m)):
+        want = sample_tokens(x, u, t, *sel)
+        cut = lambda v, a, b: None if v is None else v[a:b]   # noqa: E731
+        got = torch.cat([sample_tokens(x[a:a + 50], u[a:a + 50], t[a:a + 50], *(cut(v, a, a + 50) for v in sel))
+                         for a in range(0, rows, 50)])
+        assert torch.equal(got, want)
 
 
 def test_exact_borders(dev):
