@@ -94,6 +94,8 @@ SIGNATURES = {
     "atma_dequantize_weight_fp4": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_linear_fp4": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _i32, _p]),
     "atma_linear_gated_fp4": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _i32, _p]),
+    "atma_linear_fp4_form": (_i32, [_i64, _i64, _i64]),
+    "atma_linear_gated_fp4_form": (_i32, [_i64, _i64, _i64]),
     "atma_sample_tokens": (_i32, [_p, _i64, _p, _p, _f32, _p, _i32, _p, _f32, _p, _f32, _p, _i64, _i64, _i32, _p]),
     "atma_partial_sums": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_memory_gate_logits": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),

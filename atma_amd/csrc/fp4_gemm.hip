@@ -512,39 +512,97 @@ static void launch_tiles4(Fp4Args a, hipStream_t s) {
   fp4_tile_kernel<T, TF, TM, WF, WM, NS, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
 }
 
-template <typename T, int MT, int FT, int NW, bool RING, bool GATED>
-static void launch_few4(const Fp4Args& a, hipStream_t s) {
+// How the few rows' kernel is laid over the card
+struct FewPlan {
+  int tiles, groups, log_splits, wgs, steps;  // steps: the blocks of K that a wave goes through
+};
+
+template <int MT, int FT, int NW, bool RING, bool GATED>
+static FewPlan plan_few4(const Fp4Args& a) {
   using C = Fp4Few<MT, FT, NW, RING>;
-  Fp4FewArgs f{a, (int)((a.N + 16 * (GATED ? 1 : FT) - 1) / (16 * (GATED ? 1 : FT))), 0};
-  f.a.nk = (a.K + kFewBlock - 1) / kFewBlock;
-  const int cus = device_cu_count(), groups = (int)((a.M + 16 * MT - 1) / (16 * MT));
+  constexpr int OF = 16 * (GATED ? 1 : FT);
+  FewPlan p{(int)((a.N + OF - 1) / OF), (int)((a.M + 16 * MT - 1) / (16 * MT)), 0, 0, 0};
+  const int cus = device_cu_count(), nk = (a.K + kFewBlock - 1) / kFewBlock;
   // K is split among a workgroup's waves while every workgroup still finds a CU
-  while ((2 << f.log_splits) <= std::min(NW, f.a.nk) && (int64_t)f.tiles * groups * (2 << f.log_splits) <= (int64_t)cus * NW)
-    ++f.log_splits;
-  const int at_once = NW >> f.log_splits;  // tiles of a workgroup
-  const int wgs = std::min((f.tiles + at_once - 1) / at_once, std::max(1, cus * (160 * 1024 / C::LDS) / groups));
-  fp4_few_kernel<T, MT, FT, NW, RING, GATED><<<dim3((unsigned)wgs, (unsigned)groups), dim3(64 * NW), 0, s>>>(f);
+  while ((2 << p.log_splits) <= std::min(NW, nk) && (int64_t)p.tiles * p.groups * (2 << p.log_splits) <= (int64_t)cus * NW)
+    ++p.log_splits;
+  const int at_once = NW >> p.log_splits;  // tiles of a workgroup
+  p.wgs = std::min((p.tiles + at_once - 1) / at_once, std::max(1, cus * (160 * 1024 / C::LDS) / p.groups));
+  p.steps = (p.tiles + at_once * p.wgs - 1) / (at_once * p.wgs) * ((nk + (1 << p.log_splits) - 1) >> p.log_splits);
+  return p;
 }
 
-template <typename T, bool GATED>
-static void launch_rows4(const Fp4Args& a, hipStream_t s) {
-  constexpr int FT = GATED ? 2 : 1, NW = GATED ? 4 : 8;
-  const int64_t per = (a.K + kFewBlock - 1) / kFewBlock * 512;  // LDS for a token
-  if (std::min<int64_t>(a.M, 16) * per > kFewTokens) {
-    if (GATED || a.M <= 16) launch_few4<T, 1, FT, 4, true, GATED>(a, s);
-    else launch_few4<T, 2, 1, 4, true, false>(a, s);
-  } else if (a.M <= 16 || std::min<int64_t>(a.M, 32) * per > kFewTokens) {
-    launch_few4<T, 1, FT, NW, false, GATED>(a, s);
+template <typename T, int MT, int FT, int NW, bool RING, bool GATED>
+static void launch_few4(const Fp4Args& a, hipStream_t s) {
+  const FewPlan p = plan_few4<MT, FT, NW, RING, GATED>(a);
+  Fp4FewArgs f{a, p.tiles, p.log_splits};
+  f.a.nk = (a.K + kFewBlock - 1) / kFewBlock;
+  fp4_few_kernel<T, MT, FT, NW, RING, GATED><<<dim3((unsigned)p.wgs, (unsigned)p.groups), dim3(64 * NW), 0, s>>>(f);
+}
+
+// The kernel for a product: the one with the least time by a cost of its form, us of a graph's launch.  The few rows' kernel:
+// a part that does not depend on the size, the steps of a wave, and all blocks of all waves over the card's SIMDs.  The tiles:
+// TileCost and a part that does not depend on the size.  Fitted to 204 measured shapes of 1 to 16,384 rows, 512 to 50,304 features and K
+// of 256 to 4,096: over them the choice takes 0.7 % longer than the best of all forms in the mean and 19 % at most (gated: 0.6 % and
+// 8 %).  What each form is there for (us, it and the best of the others):
+//   16 rows a workgroup through a ring    16 x 4,096 -> 1,024     5.8 and  7.5    128 x 1,024 -> 1,024    5.0 and  5.4
+//   32 rows a workgroup through a ring   256 x 4,096 -> 1,024    11.1 and 13.4     64 x 4,096 -> 8,192   16.8 and 21.4
+//   16 rows' K kept in LDS                 1 x 1,024 -> 50,304    8.2 and 14.2      8 x 4,096 -> 8,192    7.0 and  8.0
+//   tiles of 128 features x 32 tokens     32 x 1,024 -> 50,304   10.0 and 11.7
+//   tiles of 128 x 64                     64 x 1,024 -> 50,304   12.9 and 17.2
+//   tiles of 128 x 128                   512 x 4,096 -> 8,192    39.1 and 51.6
+//   tiles of 256 x 256                16,384 x 4,096 -> 1,024   107   and 135
+// gated, K of 1,024 -> 4,096: 64 x 64 for 256 rows 10.8 and 12.0, 64 x 128 for 512 12.9 and 14.3, 128 x 256 for 8,192 110 and 132.
+// (codes that atma_linear_fp4_form returns)
+enum Fp4Form { kFp4Ring16, kFp4Ring32, kFp4Kept16, kFp4Tile32, kFp4Tile64, kFp4Tile128, kFp4Tile256 };
+
+static Fp4Form choose_fp4(const Fp4Args& a, bool gated) {
+  Fp4Form best = kFp4Tile256;
+  float least = 0.f;
+  auto offer = [&](Fp4Form form, float us) {
+    if (least == 0.f || us < least) best = form, least = us;
+  };
+  const float simds = 4.f * (float)device_cu_count();
+  const int few_nk = (a.K + kFewBlock - 1) / kFewBlock;
+  auto few = [&](Fp4Form form, const FewPlan& p, float fixed, float step, float block) {
+    offer(form, fixed + step * (float)p.steps + block * (float)p.tiles * (float)p.groups * (float)few_nk / simds);
+  };
+  auto tile = [&](Fp4Form form, float fixed, const TileCost& c) { offer(form, fixed + tile_time(a.M, a.N, a.nk, c)); };
+  const bool some = a.M <= 1024;  // (beyond, tiles are ahead by far)
+  if (gated) {
+    if (some) few(kFp4Ring16, plan_few4<1, 2, 4, true, true>(a), 4.24f, 0.695f, 0.237f);
+    tile(kFp4Tile64, 4.48f, {64, 64, 0.f, 0.334f, 0.346f});
+    tile(kFp4Tile128, 5.01f, {64, 128, 0.f, 0.359f, 0.485f});
+    tile(kFp4Tile256, 5.59f, {128, 256, 1.25f, 0.902f, 1.47f});
   } else {
-    launch_few4<T, 2, FT, NW, false, GATED>(a, s);
+    if (some) few(kFp4Ring16, plan_few4<1, 1, 4, true, false>(a), 3.69f, 0.476f, 0.204f);
+    if (some) few(kFp4Ring32, plan_few4<2, 1, 4, true, false>(a), 4.34f, 0.813f, 0.19f);
+    if (some && std::min<int64_t>(a.M, 16) * few_nk * 2 * kFewBlock <= kFewTokens)
+      few(kFp4Kept16, plan_few4<1, 1, 8, false, false>(a), 4.58f, 0.288f, 0.231f);
+    tile(kFp4Tile32, 4.31f, {128, 32, 0.f, 0.277f, 0.243f});
+    tile(kFp4Tile64, 3.94f, {128, 64, 0.f, 0.319f, 0.34f});
+    tile(kFp4Tile128, 4.87f, {128, 128, 0.19f, 0.388f, 0.482f});
+    tile(kFp4Tile256, 5.5f, {256, 256, 0.88f, 0.994f, 1.5f});
   }
+  return best;
+}
+
+static bool fp4_sizes(int64_t M, int64_t rows, int64_t K) {
+  return M >= 1 && M <= (1 << 30) && rows >= 1 && rows <= (1 << 28) && K >= kFp4Group && K <= (1 << 22) && K % kFp4Group == 0;
+}
+
+static int form_fp4(int64_t M, int64_t N, int64_t K, bool gated) {
+  if (N > (1 << 28) || !fp4_sizes(M, gated ? 2 * N : N, K)) return -1;
+  Fp4Args a{};
+  a.M = M, a.N = N, a.K = (int)K, a.nk = (a.K + kFp4Block - 1) / kFp4Block;
+  return choose_fp4(a, gated);
 }
 
 static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dtype, void* stream) {
-  const int64_t rows = gated ? 2 * a.N : a.N;
+  const int64_t rows = gated && a.N <= (1 << 28) ? 2 * a.N : a.N;
   if (dtype != ATMA_BF16 && dtype != ATMA_F16)
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: 16-bit activations (dtype %d)", what, dtype);
-  if (a.M < 0 || a.N < 1 || K < kFp4Group || K % kFp4Group || K > (1 << 22) || a.M > (1 << 30) || rows > (1 << 28))
+  if (a.M < 0 || !fp4_sizes(std::max<int64_t>(a.M, 1), rows, K))
     return set_error(ATMA_ERR_UNSUPPORTED, "%s: unsupported shape M=%lld N=%lld K=%lld (K a multiple of 32 up to 2^22, M up to "
                      "2^30, weight rows up to 2^28)", what, (long long)a.M, (long long)a.N, (long long)K);
   if (a.M == 0) return ATMA_OK;
@@ -566,22 +624,23 @@ static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dt
   hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto zero) {
     using T = decltype(zero);
-    if (a.M <= 32) {
-      if (gated) launch_rows4<T, true>(a, st);
-      else launch_rows4<T, false>(a, st);
-    } else if (gated) {
-      static constexpr TileCost kTiles[3] = {{128, 256, 5.f, 1.15f, 1.72f}, {64, 128, 1.5f, 0.6f, 0.86f}, {64, 64, 1.f, 0.4f, 0.5f}};
-      switch (cheapest_tile(a.M, a.N, a.nk, kTiles, 3)) {
-        case 0: launch_tiles4<T, 2, 4, 4, 2, 3, true>(a, st); break;
-        case 1: launch_tiles4<T, 2, 2, 2, 2, 3, true>(a, st); break;
-        default: launch_tiles4<T, 2, 1, 2, 2, 4, true>(a, st); break;
+    const Fp4Form form = choose_fp4(a, gated);
+    if (gated) {
+      switch (form) {
+        case kFp4Ring16: launch_few4<T, 1, 2, 4, true, true>(a, st); break;
+        case kFp4Tile64: launch_tiles4<T, 2, 1, 2, 2, 4, true>(a, st); break;
+        case kFp4Tile128: launch_tiles4<T, 2, 2, 2, 2, 3, true>(a, st); break;
+        default: launch_tiles4<T, 2, 4, 4, 2, 3, true>(a, st); break;
       }
     } else {
-      static constexpr TileCost kTiles[3] = {{256, 256, 5.f, 1.15f, 1.72f}, {128, 128, 1.5f, 0.6f, 0.86f}, {128, 64, 1.f, 0.4f, 0.5f}};
-      switch (cheapest_tile(a.M, a.N, a.nk, kTiles, 3)) {
-        case 0: launch_tiles4<T, 2, 4, 4, 2, 3, false>(a, st); break;
-        case 1: launch_tiles4<T, 2, 2, 2, 2, 3, false>(a, st); break;
-        default: launch_tiles4<T, 2, 1, 2, 2, 4, false>(a, st); break;
+      switch (form) {
+        case kFp4Ring16: launch_few4<T, 1, 1, 4, true, false>(a, st); break;
+        case kFp4Ring32: launch_few4<T, 2, 1, 4, true, false>(a, st); break;
+        case kFp4Kept16: launch_few4<T, 1, 1, 8, false, false>(a, st); break;
+        case kFp4Tile32: launch_tiles4<T, 1, 1, 4, 1, 4, false>(a, st); break;
+        case kFp4Tile64: launch_tiles4<T, 1, 2, 4, 1, 4, false>(a, st); break;
+        case kFp4Tile128: launch_tiles4<T, 2, 2, 2, 2, 3, false>(a, st); break;
+        default: launch_tiles4<T, 2, 4, 4, 2, 3, false>(a, st); break;
       }
     }
   };
@@ -605,3 +664,7 @@ extern "C" int atma_linear_gated_fp4(const void* x, int64_t ldx, const void* w, 
   atma::Fp4Args a{x, ldx, (const uint8_t*)w, ldw, (const uint8_t*)ws, ldws, bias, bias_dtype, y, ldy, M, H, 0};
   return atma::linear_fp4("linear_gated_fp4", true, a, K, dtype, stream);
 }
+
+extern "C" int atma_linear_fp4_form(int64_t M, int64_t N, int64_t K) { return atma::form_fp4(M, N, K, false); }
+
+extern "C" int atma_linear_gated_fp4_form(int64_t M, int64_t H, int64_t K) { return atma::form_fp4(M, H, K, true); }

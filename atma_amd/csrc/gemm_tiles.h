@@ -84,16 +84,18 @@ struct TileCost {
   float tile, few, all;
 };
 
+inline float tile_time(int64_t M, int64_t N, int nk, const TileCost& c) {
+  const int64_t tiles = ((M + c.tokens - 1) / c.tokens) * ((N + c.features - 1) / c.features);
+  const float fill = (float)tiles / (float)device_cu_count();
+  if (fill <= 1.f) return c.tile + (float)nk * (c.few + (c.all - c.few) * fill);
+  return ceilf(fill) * (c.tile + (float)nk * c.all);
+}
+
 inline int cheapest_tile(int64_t M, int64_t N, int nk, const TileCost* c, int n) {
-  const float cus = (float)device_cu_count();
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < n; ++i) {
-    const int64_t tiles = ((M + c[i].tokens - 1) / c[i].tokens) * ((N + c[i].features - 1) / c[i].features);
-    const float fill = (float)tiles / cus;
-    float t;
-    if (fill <= 1.f) t = c[i].tile + (float)nk * (c[i].few + (c[i].all - c[i].few) * fill);
-    else t = ceilf(fill) * (c[i].tile + (float)nk * c[i].all);
+    const float t = tile_time(M, N, nk, c[i]);
     if (i == 0 || t < least) best = i, least = t;
   }
   return best;
