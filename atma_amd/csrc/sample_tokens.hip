@@ -70,19 +70,25 @@ __device__ __forceinline__ uint64_t dpp_add64(uint64_t x) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
   return x + ((uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
+__device__ __forceinline__ uint64_t row_scan64(uint64_t x) {
   x = dpp_add64<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8
   x = dpp_add64<0x112, 0xF>(x);
   x = dpp_add64<0x114, 0xF>(x);
-  x = dpp_add64<0x118, 0xF>(x);
+  return dpp_add64<0x118, 0xF>(x);
+}
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
+  x = row_scan64(x);
   x = dpp_add64<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
   return dpp_add64<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
 }
-__device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
+__device__ __forceinline__ uint32_t row_scan32(uint32_t x) {
   x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
   x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
   x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
-  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
+  x = row_scan32(x);
   x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
   return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
 }
@@ -90,6 +96,10 @@ __device__ __forceinline__ uint32_t lane32(uint32_t x, int l) { return (uint32_t
 __device__ __forceinline__ uint64_t lane64(uint64_t x, int l) {
   return (uint64_t)lane32((uint32_t)(x >> 32), l) << 32 | lane32((uint32_t)x, l);
 }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) { return wave_scan32(x); }
+__device__ __forceinline__ uint64_t wave_scan(uint64_t x) { return wave_scan64(x); }
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int l) { return lane32(x, l); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t x, int l) { return lane64(x, l); }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t x) { return lane64(wave_scan64(x), 63); }
 
 typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
@@ -449,11 +459,17 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
   });
   top = wave_max(top);
   least = wave_min(least);
-  if (s.lane == 0) shared.top[s.wave] = top, shared.least[s.wave] = least;
+  bad = __any(bad);
+  if (s.lane == 0) shared.top[s.wave] = bad ? NAN : top, shared.least[s.wave] = least;
   if (threadIdx.x == 0) shared.first = 0x7fffffffu;
-  const bool nan = __syncthreads_or(bad);
+  __syncthreads();
+  bool nan = false;
 #pragma unroll
-  for (int q = 0; q < NW; ++q) top = fmaxf(top, shared.top[q]), least = fminf(least, shared.least[q]);
+  for (int q = 0; q < NW; ++q) {
+    const float its = shared.top[q];
+    nan |= its != its;
+    top = fmaxf(top, its), least = fminf(least, shared.least[q]);
+  }
   s.top = top;
   s.least = least;
   int answer;
@@ -526,7 +542,7 @@ struct Counted {
     double power[256];
     unsigned long long part[16], n, one;
     uint32_t ties[16];
-    unsigned top, first, at, low_key;
+    unsigned top, first, at, low_key, least, nan;
   };
   static_assert(sizeof(((Shared*)0)->own) + sizeof(((Shared*)0)->same) + sizeof(((Shared*)0)->high) + sizeof(((Shared*)0)->low) <=
                     sizeof(((Shared*)0)->table), "they take the counts' place");
@@ -575,9 +591,11 @@ struct Counted {
   __device__ __forceinline__ void count_values(const u32x4& a, const u32x4& b) {
     each(a, b, [&](int, const u32x4& raw) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t k = half(ordered2<T>(raw[e >> 1]), e);
-        atomicAdd(&sh->table[k >> 1], k & 1 ? 65536u : 1u);
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t k = ordered2<T>(raw[e]);
+        uint8_t* t = (uint8_t*)sh->table;
+        atomicAdd((uint32_t*)(t + ((k << 1) & 0x1fffcu)), (k & 1) * 65535u + 1);
+        atomicAdd((uint32_t*)(t + ((k >> 15) & 0x1fffcu)), ((k >> 16) & 1) * 65535u + 1);
       }
     });
   }
@@ -605,12 +623,12 @@ struct Counted {
     for (uint32_t left = strips; left; left &= left - 1) {
       const int i = __builtin_ctz(left), at = 1024 * i + threadIdx.x;
       const uint32_t word = sh->table[32767 - at], k = 65535u - 2 * at;
-      if (word) {
-        atomicAdd(&sh->count[16 * i + wave], (word >> 16) + (word & 0xffffu));
-        if (weights) {
-          const uint64_t m = (word >> 16) * weight(k) + (word & 0xffffu) * weight(k - 1);
-          if (m) atomicAdd(&sh->mass[16 * i + wave], (unsigned long long)m);
-        }
+      if (!__any(word != 0)) continue;
+      const uint32_t n = wave_scan32((word >> 16) + (word & 0xffffu));
+      if (lane == 63) sh->count[16 * i + wave] = n;
+      if (weights) {
+        const uint64_t m = wave_scan64((word >> 16) * weight(k) + (word & 0xffffu) * weight(k - 1));
+        if (lane == 63) sh->mass[16 * i + wave] = m;
       }
     }
     __syncthreads();
@@ -618,12 +636,12 @@ struct Counted {
 
   // The value at which the tokens in order first hold `target` (>= 1, at most the whole sum): its key, the sum before it and how
   // many hold it
-  template <bool MASS>
-  __device__ __forceinline__ uint32_t border(uint64_t target, uint64_t& above, uint64_t& number) const {
-    uint64_t v[8], mine = 0;
+  template <bool MASS, typename A>
+  __device__ __forceinline__ uint32_t border(A target, A& above, uint32_t& number) const {
+    A v[8], mine = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mine += v[j] = MASS ? (uint64_t)sh->mass[8 * lane + j] : (uint64_t)sh->count[8 * lane + j];
-    uint64_t at = wave_scan64(mine) - mine;
+    for (int j = 0; j < 8; ++j) mine += v[j] = MASS ? (A)sh->mass[8 * lane + j] : (A)sh->count[8 * lane + j];
+    A at = wave_scan(mine) - mine;
     int entry = -1;
     const bool here = at < target && at + mine >= target;
 #pragma unroll
@@ -635,14 +653,15 @@ struct Counted {
     }
     const int l = __builtin_ctzll(__ballot(here));
     entry = (int)lane32((uint32_t)entry, l);
-    at = lane64(at, l);
+    at = lane_of(at, l);
     const int pos = 1024 * (entry >> 4) + 64 * (entry & 15) + lane;
     const uint32_t word = sh->table[32767 - pos], k = 65535u - 2 * pos;
-    const uint64_t hi = MASS ? (word >> 16) * weight(k) : word >> 16, lo = MASS ? (word & 0xffffu) * weight(k - 1) : word & 0xffffu;
-    at += wave_scan64(hi + lo) - hi - lo;
+    A hi = word >> 16, lo = word & 0xffffu;
+    if constexpr (MASS) hi *= weight(k), lo *= weight(k - 1);
+    at += wave_scan(hi + lo) - hi - lo;
     const bool this_one = at < target && at + hi + lo >= target, low = at + hi < target;
     const int l2 = __builtin_ctzll(__ballot(this_one));
-    above = lane64(low ? at + hi : at, l2);
+    above = lane_of(low ? at + hi : at, l2);
     number = lane32(low ? word & 0xffffu : word >> 16, l2);
     return lane32(low ? k - 1 : k, l2);
   }
@@ -660,23 +679,39 @@ struct Counted {
     return wave_sum64(sum);
   }
 
+  // The least value with its share m of the largest weight, as a key; every value is above key 0
+  __device__ __forceinline__ uint32_t least_key(float m, float t) const {
+    if (!(m > 0.f)) return 1;
+    const double x = m >= 1.f ? xmax : xmax + (double)t * log((double)m);
+    uint32_t least = ordered2<T>(__builtin_bit_cast(uint16_t, from_f32<T>((float)x))) & 0xffffu;
+    if (least == 0x7fffu) least = 0x8000u;
+    // (rounded twice and either way: at most a value off; a NaN, of infinities, keeps all)
+    if (x != x) return 1;
+    while (least > kNegInf && (double)ordered_value<T>(least - 1) >= x) --least;
+    while (least < kInf && (double)ordered_value<T>(least) < x) ++least;
+    return least == 0x8000u ? 0x7fffu : least;
+  }
+
   // What is kept (one wave finds it): every value above `at`, and the first n tokens of those with keys from `low` to `at` (none where
   // low > at)
-  __device__ __forceinline__ void filter(int k, float p, float m, float t) {
+  __device__ __forceinline__ void filter(int k, float p) {
     const bool by_count = k > 0 && k < V, by_mass = p < 1.f;
     uint32_t at = 0, low = 1;
-    uint64_t n = 0, above, number;
+    uint64_t n = 0;
+    uint32_t number;
     if (by_count || by_mass) {
       bool cut = false;
       if (by_count) {
-        at = border<false>((uint64_t)k, above, number);
-        n = (uint64_t)k - above;
+        uint32_t above;
+        at = border<false>((uint32_t)k, above, number);
+        n = (uint32_t)k - above;
         cut = n < number;
       }
       if (by_mass) {
         const uint64_t total = weight_above(at) + (by_count ? n * weight(at) : 0);
         const double want = (double)p * (double)total;
         const uint64_t target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
+        uint64_t above;
         const uint32_t pk = border<true>(target, above, number);
         // the least number of them that holds what is missing
         const uint64_t w = weight(pk), missing = target - above;
@@ -691,18 +726,6 @@ struct Counted {
       }
       low = at == 0x8000u ? 0x7fffu : at;
       if (!cut) at = low - 1, low = at + 1;
-    }
-    if (m > 0.f) {
-      // the least value with its share of the largest weight, as a key
-      const double x = m >= 1.f ? xmax : xmax + (double)t * log((double)m);
-      uint32_t least = ordered2<T>(__builtin_bit_cast(uint16_t, from_f32<T>((float)x))) & 0xffffu;
-      if (least == 0x7fffu) least = 0x8000u;
-      // (rounded twice and either way: at most a value off; a NaN, of infinities, keeps all)
-      if (x != x) least = 0;
-      while (least > kNegInf && (double)ordered_value<T>(least - 1) >= x) --least;
-      while (least < kInf && (double)ordered_value<T>(least) < x) ++least;
-      if (least == 0x8000u) least = 0x7fffu;
-      if (least > at + (low <= at ? 0 : 1)) at = least - 1, low = at + 1;
     }
     if (lane == 0) {
       sh->at = at;
@@ -770,10 +793,20 @@ struct Counted {
   // The kept weights, and the border's tokens, of the wave's part
   template <bool TABLES>
   __device__ __forceinline__ void add_up(uint32_t at, uint32_t low, uint64_t& sum, uint32_t& number) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     const bool ties = low <= at;
+    const uint32_t least = ties ? low : at + 1;
     each([&](int q, const u32x4& raw) {
       uint64_t own = 0;
       uint32_t same = 0;
+      u16x2 most = {};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, ordered2<T>(raw[e])));
+      if (!__any(max((uint32_t)most[0], (uint32_t)most[1]) >= least)) {  // nothing kept
+        sh->own[q][threadIdx.x] = 0;
+        sh->same[q][threadIdx.x] = 0;
+        return;
+      }
       if (TABLES && held(raw, at)) {
         own = table_weight8(raw, at);
       } else {
@@ -806,7 +839,7 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
   s.sh = &shared;
   s.V = a.V;
   s.lane = threadIdx.x & 63;
-  s.wave = threadIdx.x >> 6;
+  s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunks = (a.V + kSampleChunk - 1) / kSampleChunk, each = (chunks + 15) / 16;
   s.first = min(s.wave * each, chunks);
   s.chunks = min(each, chunks - s.first);
@@ -817,7 +850,7 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
 #pragma unroll
   for (int i = 0; i < 8; ++i) ((u32x4*)shared.table)[1024 * i + threadIdx.x] = u32x4{};
   if (threadIdx.x < 512) shared.count[threadIdx.x] = 0, shared.mass[threadIdx.x] = 0;
-  if (threadIdx.x == 0) shared.top = 0xffffffffu, shared.first = 0x7fffffffu;
+  if (threadIdx.x == 0) shared.top = 0xffffffffu, shared.first = 0x7fffffffu, shared.nan = 0;
   __syncthreads();
   if (s.chunks > 0) first = s.load(0);
   if (s.chunks > 1) second = s.load(1);
@@ -826,14 +859,21 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
   // ---- the largest value; NaNs lie in the first and the last strip (what lies behind the row's end is counted at key 0)
   bool bad = false;
   s.strips = 0;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i) {
-    const uint32_t at = 1024 * i + threadIdx.x;
-    uint32_t word = shared.table[32767 - at];
-    if (i == 31 && at == 32767) word -= (uint32_t)(chunks * kSampleChunk - a.V);
-    if (__any(word != 0)) s.strips |= 1u << i;
-    if (i == 0) bad |= (word >> 16 && 65535u - 2 * at > S::kInf) || (word & 0xffffu && 65534u - 2 * at > S::kInf);
-    if (i == 31) bad |= (word >> 16 && 65535u - 2 * at < S::kNegInf) || (word & 0xffffu && 65534u - 2 * at < S::kNegInf);
+  // four strips at a time, four words a lane: the wave's 64 of each
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t at = 1024 * (4 * i + (s.lane >> 4)) + 64 * s.wave + 4 * (s.lane & 15);
+    u32x4 words = *(const u32x4*)&shared.table[32764 - at];
+    if (i == 7 && at == 32764) words[0] -= (uint32_t)(chunks * kSampleChunk - a.V);
+    const uint64_t any = __ballot((words[0] | words[1] | words[2] | words[3]) != 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.strips |= (any >> (16 * j) & 0xffffu ? 1u : 0u) << (4 * i + j);
+    if (i != 0 && i != 7) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t word = words[3 - e], k = 65535u - 2 * (at + e);
+      bad |= (word >> 16 && (i ? k < S::kNegInf : k > S::kInf)) || (word & 0xffffu && (i ? k - 1 < S::kNegInf : k - 1 > S::kInf));
+    }
   }
   if (s.strips) {
     const int at = 1024 * __builtin_ctz(s.strips) + threadIdx.x;
@@ -841,7 +881,9 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
     const int l = __builtin_ctzll(__ballot(word != 0));
     if (s.lane == l) atomicMin(&shared.top, 2u * at + (word >> 16 ? 0 : 1));
   }
-  const bool nan = __syncthreads_or(bad);
+  if (bad) shared.nan = 1;
+  __syncthreads();
+  const bool nan = shared.nan != 0;
   s.top = 65535u - shared.top;
   if (threadIdx.x == 0) {
     shared.table[0] &= 0xffff0000u;
@@ -865,10 +907,12 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
     const int k = a.top_k ? a.top_k[r] : a.k0;
     const float p = a.top_p ? a.top_p[r] : a.p0, m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
     if ((k > 0 && k < a.V) || p < 1.f) s.tabulate(p < 1.f);
-    if (s.wave == 0) s.filter(k, p, m, t);
+    if (s.wave == 0) s.filter(k, p);
+    if (s.wave == 1 && s.lane == 0) shared.least = s.least_key(m, t);
     __syncthreads();  // the counts are read
-    const uint32_t at = shared.at, low = shared.low_key;
-    const uint64_t n = shared.n, one = shared.one;
+    uint32_t at = shared.at, low = shared.low_key;
+    if (shared.least > at + (low <= at ? 0 : 1)) at = shared.least - 1, low = at + 1;
+    const uint64_t n = shared.n, one = low <= at ? shared.one : 0;
     // tables pay where most waves meet a kept token at most of their steps
     const bool tables = (k <= 0 || k > 512) && s.prepare(t);
     __syncthreads();
@@ -880,45 +924,49 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
     number = lane32(wave_scan32(number), 63);
     if (s.lane == 0) shared.part[s.wave] = sum, shared.ties[s.wave] = number;
     __syncthreads();
-    uint64_t before = 0, left = n, mine = 0, total = 0, left_here = 0;  // left: tokens of the border still to be kept
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const uint64_t take = min(left, (uint64_t)shared.ties[q]), w = shared.part[q] + take * one;
-      if (q == s.wave) before = total, mine = w, left_here = left;
-      total += w;
-      left -= take;
-    }
+    // lane q of 16: wave q's weight, its tokens of the border taken in order
+    const uint32_t most = (uint32_t)min(n, (uint64_t)0xffffffffu), q_ties = shared.ties[s.lane & 15];
+    const uint32_t q_earlier = row_scan32(q_ties) - q_ties;
+    const uint64_t q_mine = shared.part[s.lane & 15] + min(q_ties, most - min(most, q_earlier)) * one;
+    const uint64_t q_upto = row_scan64(q_mine);
+    const uint64_t total = lane64(q_upto, 15), mine = lane64(q_mine, s.wave);
+    uint64_t before = lane64(q_upto, s.wave) - mine;
+    uint32_t left_here = most - min(most, lane32(q_earlier, s.wave));
     const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
     const uint64_t aim = (uint64_t)(f * (double)total);
     if (before <= aim && aim < before + mine) {  // one wave, all of it
 #pragma unroll 1
       for (int q = 0; q < s.chunks; ++q) {
         const uint32_t same = one ? shared.same[q][threadIdx.x] : 0, upto = wave_scan32(same);
-        const uint64_t earlier = upto - same;  // the border's tokens before this lane's
-        uint64_t still = left_here > earlier ? left_here - earlier : 0;
-        const uint64_t w = shared.own[q][threadIdx.x] + min(still, (uint64_t)same) * one;
-        const uint64_t to = before + wave_scan64(w), from = to - w;
+        const uint32_t earlier = upto - same;  // the border's tokens before this lane's
+        const uint32_t still = left_here - min(left_here, earlier);
+        const uint64_t w = shared.own[q][threadIdx.x] + min(still, same) * one;
+        const uint64_t to = before + wave_scan64(w);
         before = lane64(to, 63);
-        left_here -= min(left_here, (uint64_t)lane32(upto, 63));
+        left_here -= min(left_here, lane32(upto, 63));
         if (aim >= before) continue;
         const u32x4 raw = s.load(q);
         const bool by_table = tables && s.held(raw, at);
-        double part = 0x1p52;
-        uint64_t at_e = from, exact = 0, kept_ties = 0;
+        // the lane that has it: its eight logits to eight lanes, lane e with the sum up to the e-th
+        const int l = __builtin_ctzll(__ballot(aim < to));
+        const u32x4 its = {lane32(raw[0], l), lane32(raw[1], l), lane32(raw[2], l), lane32(raw[3], l)};
+        const int e = s.lane & 7;
+        const uint32_t word = e < 4 ? (e < 2 ? its[0] : its[1]) : (e < 6 ? its[2] : its[3]);
+        const uint32_t key = (e & 1 ? ordered2<T>(word) >> 16 : ordered2<T>(word)) & 0xffffu;
+        const uint32_t tie = row_scan32(s.lane < 8 && key - low <= at - low && low <= at);
+        uint64_t sum_e;
+        if (by_table) {
+          double part = 0x1p52;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t bits = S::half(raw[e >> 1], e), key = S::half(ordered2<T>(raw[e >> 1]), e);
-          if (by_table) {
-            part = s.table_add(part, bits, key > at);
-            exact = __builtin_bit_cast(uint64_t, part) & 0xfffffffffffffull;
-          } else if (__any(key > at)) {
-            exact += key > at ? s.weight(key) : 0;
-          }
-          if (key >= low && key <= at && still) kept_ties += one, --still;
-          const uint64_t upto_e = from + exact + kept_ties;
-          if (at_e <= aim && aim < upto_e) a.ids[r] = s.index(q) + e;
-          at_e = upto_e;
+          for (int j = 0; j < 8; ++j)
+            part = s.table_add(part, S::half(its[j >> 1], j), j <= e && S::half(ordered2<T>(its[j >> 1]), j) > at);
+          sum_e = __builtin_bit_cast(uint64_t, part) & 0xfffffffffffffull;
+        } else {
+          sum_e = row_scan64(s.lane < 8 && key > at ? s.weight(key) : 0);
         }
+        sum_e += lane64(to - w, l) + min(tie, lane32(still, l)) * one;
+        const uint64_t past = __ballot(aim < sum_e) & 0xff;
+        if (s.lane == 0) a.ids[r] = s.index(q) + 8 * l + __builtin_ctzll(past);
         break;
       }
     }
