@@ -92,6 +92,15 @@ __device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
   x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
   return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
 }
+__device__ __forceinline__ uint32_t wave_or32(uint32_t x) {
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
+  x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
 __device__ __forceinline__ uint32_t lane32(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
 __device__ __forceinline__ uint64_t lane64(uint64_t x, int l) {
   return (uint64_t)lane32((uint32_t)(x >> 32), l) << 32 | lane32((uint32_t)x, l);
@@ -858,22 +867,25 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
   __syncthreads();
   // ---- the largest value; NaNs lie in the first and the last strip (what lies behind the row's end is counted at key 0)
   bool bad = false;
-  s.strips = 0;
+  const uint32_t behind = (uint32_t)(chunks * kSampleChunk - a.V);
   // four strips at a time, four words a lane: the wave's 64 of each
+  uint32_t strips = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t at = 1024 * (4 * i + (s.lane >> 4)) + 64 * s.wave + 4 * (s.lane & 15);
+    const int at = 1024 * (4 * i + (s.lane >> 4)) + 64 * s.wave + 4 * (s.lane & 15);
     u32x4 words = *(const u32x4*)&shared.table[32764 - at];
-    if (i == 7 && at == 32764) words[0] -= (uint32_t)(chunks * kSampleChunk - a.V);
-    const uint64_t any = __ballot((words[0] | words[1] | words[2] | words[3]) != 0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s.strips |= (any >> (16 * j) & 0xffffu ? 1u : 0u) << (4 * i + j);
-    if (i != 0 && i != 7) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t word = words[3 - e], k = 65535u - 2 * (at + e);
-      bad |= (word >> 16 && (i ? k < S::kNegInf : k > S::kInf)) || (word & 0xffffu && (i ? k - 1 < S::kNegInf : k - 1 > S::kInf));
-    }
+    if (i == 7 && at == 32764) words[0] -= behind;
+    strips |= ((words[0] | words[1] | words[2] | words[3]) != 0 ? 1u : 0u) << (4 * i);
+  }
+  s.strips = wave_or32(strips << (s.lane >> 4));
+  constexpr int nans = (0x10000 - S::kInf) / 2;  // words of either end that hold NaNs
+  if (s.wave < nans / 64) {
+    const uint32_t word = shared.table[32767 - threadIdx.x], k = 65535u - 2 * threadIdx.x;
+    bad = (word >> 16 && k > S::kInf) || (word & 0xffffu && k - 1 > S::kInf);
+  }
+  if (s.wave >= 16 - nans / 64) {
+    const uint32_t word = shared.table[1023 - threadIdx.x] - (threadIdx.x == 1023 ? behind : 0), k = 2047u - 2 * threadIdx.x;
+    bad |= (word >> 16 && k < S::kNegInf) || (word & 0xffffu && k - 1 < S::kNegInf);
   }
   if (s.strips) {
     const int at = 1024 * __builtin_ctz(s.strips) + threadIdx.x;
