@@ -192,9 +192,13 @@ struct Sampler {
   float top, least, width;         // the largest and the smallest logit; bins a unit of logits
   double c;                        // log2(e) / temperature
 
-  // f(index, value) for every logit of the wave's part, loads a chunk ahead
+  // f(index, value) for every logit of the wave's part, done(chunk) behind each chunk; loads a chunk ahead
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
+    each(f, [](int) {});
+  }
+  template <typename F, typename D>
+  __device__ __forceinline__ void each(F f, D done) const {
     SampleRaw<T> next;
     if (first < last) next.load(row, first * kSampleChunk + 8 * lane, V);
 #pragma unroll 1
@@ -209,6 +213,7 @@ struct Sampler {
         f(i + e, whole || i + e < V ? x : __builtin_nanf(""));
         if (e & 1) __builtin_amdgcn_sched_barrier(0);  // (eight exponentials side by side take more registers than there are)
       }
+      done(q);
     }
   }
 
@@ -337,9 +342,15 @@ struct Sampler {
   // The first index at which the sum of amount(index, value) passes target(the whole sum), which is below it
   template <typename F, typename G>
   __device__ __forceinline__ int find(F amount, G target) {
-    uint64_t mine = 0;
-    each([&](int i, float x) { mine += amount(i, x); });
-    mine = wave_sum64(mine);
+    uint64_t mine = 0, own = 0;
+    static_assert(sizeof(Shared::mass) >= 8 * ((1 << 20) / kSampleChunk), "a chunk's sum each: the bins are read");
+    each([&](int i, float x) { own += amount(i, x); },
+         [&](int q) {
+           own = wave_sum64(own);
+           if (lane == 0) sh->mass[q] = own;
+           mine += own;
+           own = 0;
+         });
     if (lane == 0) sh->part[wave] = mine;
     __syncthreads();
     uint64_t sum = 0, before = 0;
@@ -350,27 +361,32 @@ struct Sampler {
     }
     const uint64_t aim = target(sum);
     if (before <= aim && aim < before + mine) {  // one wave, all of it
-      SampleRaw<T> next;
-      next.load(row, first * kSampleChunk + 8 * lane, V);
+      int q = first;
 #pragma unroll 1
-      for (int q = first; q < last; ++q) {
-        const int i = q * kSampleChunk + 8 * lane;
-        const SampleRaw<T> now = next;
-        if (q + 1 < last) next.load(row, i + kSampleChunk, V);
-        uint64_t n[8], own = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) own += n[e] = amount(i + e, i + e < V ? now.value(e) : __builtin_nanf(""));
-        const uint64_t upto = wave_scan64(own);
-        uint64_t at = before + upto - own;
-        if (at <= aim && aim < at + own) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (at <= aim && aim < at + n[e]) sh->found[0] = (uint64_t)(i + e);
-            at += n[e];
-          }
+      for (;; q += 64) {
+        const uint64_t v = q + lane < last ? sh->mass[q + lane] : 0, upto = before + wave_scan64(v);
+        const uint64_t there = __ballot(aim < upto);
+        if (there) {
+          const int l = __builtin_ctzll(there);
+          q += l;
+          before = lane64(upto - v, l);
+          break;
         }
-        before += lane64(upto, 63);
-        if (aim < before) break;
+        before = lane64(upto, 63);
+      }
+      const int i = q * kSampleChunk + 8 * lane;
+      SampleRaw<T> now;
+      now.load(row, i, V);
+      uint64_t n[8], its = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) its += n[e] = amount(i + e, i + e < V ? now.value(e) : __builtin_nanf(""));
+      uint64_t at = before + wave_scan64(its) - its;
+      if (at <= aim && aim < at + its) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (at <= aim && aim < at + n[e]) sh->found[0] = (uint64_t)(i + e);
+          at += n[e];
+        }
       }
     }
     __syncthreads();
@@ -451,7 +467,7 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
   s.sh = &shared;
   s.V = a.V;
   s.lane = threadIdx.x & 63;
-  s.wave = threadIdx.x >> 6;
+  s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunks = (a.V + kSampleChunk - 1) / kSampleChunk, each = (chunks + NW - 1) / NW;
   s.first = min(s.wave * each, chunks);
   s.last = min(s.first + each, chunks);
