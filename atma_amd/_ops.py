@@ -1183,17 +1183,22 @@ def _(data, scale, dtype):
 FP4_PITCH = (1 << 22, 1 << 23)   # elements between rows of x, bytes between rows of the weights: what the products address
 
 
-def fp4_linear(x, data, scale, bias, gated):
-    (M, K), N = x.shape, data.shape[0] // (2 if gated else 1)
+def fp4_linear_at(x, scale, bias, gated, M, rows, K, px, ldx, pd, ldw, lds):
+    N = rows // 2 if gated else rows
     out = x.new_empty((M, N))
     lib = _lib.load()
     rc = (lib.atma_linear_gated_fp4 if gated else lib.atma_linear_fp4)(
-        x.data_ptr(), x.stride(0), data.data_ptr(), data.stride(0), scale.data_ptr(), scale.stride(0),
-        None if bias is None else bias.data_ptr(), 0 if bias is None else _lib.DTYPE_CODE[bias.dtype], out.data_ptr(), N,
-        M, N, K, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(x.device))
+        px, ldx, pd, ldw, scale.data_ptr(), lds, None if bias is None else bias.data_ptr(),
+        0 if bias is None else _lib.DTYPE_CODE[bias.dtype], out.data_ptr(), N, M, N, K, _lib.DTYPE_CODE[x.dtype],
+        _lib.stream_handle(x.device))
     if rc:
         _lib.check(rc, "linear_gated_fp4" if gated else "linear_fp4")
     return out
+
+
+def fp4_linear(x, data, scale, bias, gated):
+    return fp4_linear_at(x, scale, bias, gated, x.shape[0], data.shape[0], x.shape[1], x.data_ptr(), x.stride(0), data.data_ptr(),
+                         data.stride(0), scale.stride(0))
 
 
 def _linear_fp4(x, data, scale, bias, gated):

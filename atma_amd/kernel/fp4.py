@@ -59,29 +59,35 @@ def dequantize_weight_fp4(data, scale, dtype=torch.bfloat16):
 
 
 def _operands(what, x, data, scale, bias):
-    """Checks a product's operands; returns whether it may go straight to its launch (nothing to dispatch or to copy)."""
-    if x.dim() != 2 or x.dtype not in _DT:
-        raise ValueError(f"{what}: x must be a matrix of {_dtypes(_DT)} (got {tuple(x.shape)} {x.dtype})")
-    _pair(what, data, scale)
-    K, N = x.shape[1], data.shape[0]
-    if K != 2 * data.shape[1] or N < 1:
-        raise ValueError(f"{what}: x (M, K) and data (N, K / 2), got {tuple(x.shape)} and {tuple(data.shape)}")
+    """Checks a product's operands; returns its sizes, strides and addresses if it may go straight to its launch (nothing to
+    dispatch or to copy), else None."""
+    xs, ds, ss = x.shape, data.shape, scale.shape
+    if len(xs) != 2 or x.dtype not in _DT:
+        raise ValueError(f"{what}: x must be a matrix of {_dtypes(_DT)} (got {tuple(xs)} {x.dtype})")
+    if len(ds) != 2 or data.dtype != torch.uint8 or ds[1] < 16 or ds[1] % 16 or scale.dtype != FP4_SCALE or ss != (ds[0], ds[1] // 16):
+        _pair(what, data, scale)
+    (M, K), (N, half) = xs, ds
+    if K != 2 * half or N < 1:
+        raise ValueError(f"{what}: x (M, K) and data (N, K / 2), got {tuple(xs)} and {tuple(ds)}")
     if bias is not None and (bias.shape != (N,) or bias.dtype not in _DT32):
         raise ValueError(f"{what}: bias must be ({N},) of {_dtypes(_DT32)}")
     if not _placed(what, x, data, scale, bias):
-        return False
-    (ldx, ix), (ldw, iw) = x.stride(), data.stride()
-    return (ix == iw == scale.stride(1) == 1 and K <= ldx <= _PITCH_X and K <= 2 * ldw and ldw <= _PITCH_W
-            and not (x.data_ptr() | data.data_ptr() | 2 * ldx | ldw) & 15 and scale.stride(0) >= 0
-            and (bias is None or bias.stride(0) == 1))
+        return None
+    (ldx, ix), (ldw, iw), (lds, js) = x.stride(), data.stride(), scale.stride()
+    px, pd = x.data_ptr(), data.data_ptr()
+    if (ix == iw == js == 1 and K <= ldx <= _PITCH_X and half <= ldw <= _PITCH_W and not (px | pd | 2 * ldx | ldw) & 15 and lds >= 0
+            and (bias is None or bias.stride(0) == 1)):
+        return M, N, K, px, ldx, pd, ldw, lds
+    return None
 
 
 def linear_fp4(x, data, scale, bias=None):
     """``F.linear`` with a 4-bit weight: x (M, K) in 16 bits, data (N, K / 2) and scale (N, K / 32), bias (N,) in fp32 or 16 bits
     or None.  The weights are multiplied as ``dequantize_weight_fp4`` gives them in x's type; sums in fp32, one rounding to
     x's type."""
-    if _operands("linear_fp4", x, data, scale, bias):
-        return _ops.fp4_linear(x, data, scale, bias, False)
+    straight = _operands("linear_fp4", x, data, scale, bias)
+    if straight is not None:
+        return _ops.fp4_linear_at(x, scale, bias, False, *straight)
     return _ops.run.linear_fp4(x, data, scale, bias)
 
 
@@ -90,6 +96,7 @@ def linear_gated_fp4(x, data, scale, bias=None):
     ``gate * relu(a)^2`` rounded once to x's type.  data (2H, K / 2): the a rows, then the gate rows.  Returns (M, H)."""
     if data.dim() == 2 and data.shape[0] % 2:
         raise ValueError(f"linear_gated_fp4: data (2H, K / 2), got {tuple(data.shape)}")
-    if _operands("linear_gated_fp4", x, data, scale, bias):
-        return _ops.fp4_linear(x, data, scale, bias, True)
+    straight = _operands("linear_gated_fp4", x, data, scale, bias)
+    if straight is not None:
+        return _ops.fp4_linear_at(x, scale, bias, True, *straight)
     return _ops.run.linear_gated_fp4(x, data, scale, bias)

@@ -47,7 +47,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=None, top_p=None, min_
     top_k, k0 = _per_row(what, "top_k", top_k, rows, torch.int32, 0)
     top_p, p0 = _per_row(what, "top_p", top_p, rows, torch.float32, 1.0)
     min_p, m0 = _per_row(what, "min_p", min_p, rows, torch.float32, 0.0)
-    logits, uniform = logits.detach(), uniform.detach()
+    if logits.requires_grad or uniform.requires_grad:
+        logits, uniform = logits.detach(), uniform.detach()
     straight = _placed(what, logits, uniform, temperature, top_k, top_p, min_p)
     if ids_out is not None:
         if ids_out.shape != (rows,) or ids_out.dtype != torch.int64 or not ids_out.is_contiguous() \
