@@ -58,8 +58,10 @@ __device__ __forceinline__ LateArgs4 late_args4() {
 // A block of 256 x 256 takes 2,760 cycles, 2,048 of them products: two waves share a SIMD, and while one runs its steps
 // at 1.1 to 1.3 times the time of their products, what both lose lies behind the barrier.  Measured without gain: products ahead
 // of the reads in each step, a higher priority for the products, the weights' conversion behind the last step's products,
-// 128 x 64 tiles a wave instead of 64 x 128 (twice the conversions, two thirds of the reads).  65,536 x 4,096 -> 1,024 430 us, where the
-// library's 16-bit product takes 356.
+// 128 x 64 tiles a wave instead of 64 x 128 (twice the conversions, two thirds of the reads), operands read a whole block ahead.
+// 65,536 x 4,096 -> 1,024 takes 430 to 440 us (1.26 PFLOP/s, matrix cores busy 70 % at the 1.7 GHz that power allows), the library's
+// 16-bit product on weights already converted 356 to 460 by the box.  Small tiles, a wave a SIMD, are bound by issue: a block of
+// 128 x 32 is 130 instructions and 128 cycles of products in 700.
 //
 // The weights are the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token
 // (row 8 q + 4 h + e is feature 16 h + 4 q + e).  Their rows are 32 bytes in LDS, chunk c of row r at position
@@ -314,6 +316,10 @@ __device__ __forceinline__ float fp4_bias(const Fp4Args& a, int64_t n) {
 // It has a ring of its own of NS blocks of 256 k, filled by direct copies of whole 128-byte lines of the weights, and waits
 // for nothing but its own copies.  The tokens lie in LDS, all of K, copied once (RING: where they do not fit, a
 // block of them comes with each block of weights).  A workgroup walks over its tiles, and the ring runs on across them.
+//
+// Its time is latency, launch, first copies, join: 1 x 4,096 -> 1,024 5.1 us (2.2 MB), 16 x 1,024 -> 4,096 4.5, gated 5.3; 1 x 1,024 -> 50,304
+// streams 27 MB in 8.2.  Four waves with a ring for the tokens too beat eight with the tokens kept wherever the ring's copies of the tokens
+// (8 KiB a block of 2 KiB of weights, from L2) are few: see choose_fp4.
 //
 // v_mfma_f32_16x16x32: lane (r, g) takes chunks g and g + 4 of a weight row's eight, one group of 32 k each with its scale, and
 // the same k of token r.  Chunk c of a weight row lies at position c ^ (r / 2) % 8, chunk c of a token's row at c ^ r % 16.

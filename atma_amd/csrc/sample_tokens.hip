@@ -15,6 +15,10 @@
 // Weights are formed in fp64 and held as integers, multiples of 2^-43 of the largest: their sums are exact, so neither the
 // order of the additions nor the number of threads changes a result, and a border is decided as in 64-bit arithmetic
 // (with fp32 weights one row in a few thousand would answer its neighbour's token).  V <= 2^20 keeps every sum below 2^63.
+//
+// What bounds it is one CU's work on a row: two passes that form a weight for every logit, some 190 cycles for 64 of them.  One row of 50,304
+// fp32 logits with top-p takes 42 us (without 23), 512 rows 117.  (More CUs a row would need the largest logit, the bins and the
+// sums from each other: five launches of 3 us and a workspace.)
 #include <algorithm>
 
 #include "common.h"
@@ -532,6 +536,9 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
 // weight in a table of 512 entries, and each wave finds a border there, then in the entry's words.  A last pass over the row adds
 // up the kept weights, and counts the tokens of the border's value, of which the first so many are kept; each lane leaves both
 // for each of its chunks in LDS, where the wave in whose part the answer lies finds it.
+//
+// 32 rows of 50,304 with mixed filters take 23 to 26 us (the row with the most kept tokens), 2,048 rows 157, 1.3 TB/s: eight rows a CU one after
+// the other, a third of it the count (LDS atomics, 11 cycles a wave's), a fifth the kept weights.
 //
 // Keys here are the 16 bits in the values' order as they are: NaNs lie at both ends, and -0, 0x7fff, is counted as +0, 0x8000.
 constexpr int kCountedThreads = 1024, kCountedChunks = 8;  // 512 logits a chunk and wave
