@@ -16,6 +16,7 @@ narrow the choice (``sample_tokens``); with a ``seed`` a request draws the same 
 from dataclasses import dataclass
 from enum import Enum
 from itertools import count
+from operator import index
 from random import getrandbits
 from typing import Optional
 
@@ -33,6 +34,10 @@ class SamplingParams:
     def __post_init__(self):
         if self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1:
             raise ValueError(f"top_k >= 0, 0 < top_p <= 1 and 0 <= min_p <= 1 (got {self.top_k}, {self.top_p}, {self.min_p})")
+        for name in ("top_k", "seed"):
+            v = getattr(self, name)
+            if v is not None:
+                object.__setattr__(self, name, index(v))   # a whole number of any integer type, as a Python one
 
     @property
     def picks(self):

@@ -107,6 +107,12 @@ def test_sampling_parameters():
     for bad in (dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=-0.1), dict(min_p=1.5)):
         with pytest.raises(ValueError):
             SamplingParams(**bad)
+    import numpy as np
+    for bad in (dict(seed=0.5), dict(seed="1"), dict(top_k=2.5)):
+        with pytest.raises(TypeError):
+            SamplingParams(**bad)
+    p = SamplingParams(seed=np.int64(3), top_k=np.int32(4))
+    assert type(p.seed) is int and type(p.top_k) is int and Sequence([1], p).uniform() == uniform(3, 0)
     assert not SamplingParams().picks and not SamplingParams(temperature=0.0, top_k=5).picks
     for good in (dict(top_k=1), dict(top_p=0.5), dict(min_p=0.1), dict(seed=0)):
         assert SamplingParams(**good).picks
