@@ -97,6 +97,8 @@ SIGNATURES = {
     "atma_linear_fp4_form": (_i32, [_i64, _i64, _i64]),
     "atma_linear_gated_fp4_form": (_i32, [_i64, _i64, _i64]),
     "atma_sample_tokens": (_i32, [_p, _i64, _p, _p, _f32, _p, _i32, _p, _f32, _p, _f32, _p, _i64, _i64, _i32, _p]),
+    "atma_sample_tokens_workspace": (_i64, [_i64, _i64, _i32]),
+    "atma_sample_tokens_in": (_i32, [_p, _i64, _p, _p, _f32, _p, _i32, _p, _f32, _p, _f32, _p, _i64, _i64, _i32, _p, _i64, _p]),
     "atma_partial_sums": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_memory_gate_logits": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "atma_polar_params_f32": (_i32, [_p] * 6 + [_i64, _i64, _i32, _p]),

@@ -37,6 +37,8 @@ struct SampleArgs {
   int k0;
   int64_t* ids;  // (rows,)
   int V;
+  uint8_t* held;  // of few long rows: their workspace, WideRow's arrays for each
+  int parts;
 };
 
 constexpr int kSampleBins = 2048;   // of a level of the exact search
@@ -175,10 +177,11 @@ __device__ __forceinline__ uint64_t sample_order(uint32_t key, int i) { return (
 
 // A row's workgroup: NW waves, each with a contiguous part of it.  Passes work on the values themselves (no row with a NaN comes
 // past the first one): a missing logit, behind the row's end, reads as NaN, which no comparison keeps and which has no weight
-template <typename T, int NW>
+template <typename T, int NW, int BINS = NW >= 16 ? 4096 : 1024, int LISTED = 64 * NW>
 struct Sampler {
+  typedef T Type;
   static constexpr int NT = 64 * NW, PER = kSampleBins / NT;
-  static constexpr int B = NW >= 8 ? 4096 : 1024, BPER = B / NT, LIST = NT;
+  static constexpr int B = BINS, BPER = B / NT, LIST = LISTED;
   struct Shared {
     unsigned long long mass[B > kSampleBins ? B : kSampleBins];
     uint32_t count[B];
@@ -195,6 +198,17 @@ struct Sampler {
   int V, lane, wave, first, last;  // the wave's part in chunks
   float top, least, width;         // the largest and the smallest logit; bins a unit of logits
   double c;                        // log2(e) / temperature
+
+  // A row's chunks from `from` to before `to`, among the waves
+  __device__ __forceinline__ void start(const SampleArgs& a, int64_t r, int from, int to) {
+    V = a.V;
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int each = (to - from + NW - 1) / NW;
+    first = min(from + wave * each, to);
+    last = min(first + each, to);
+    row = (const T*)a.logits + r * a.ld;
+  }
 
   // f(index, value) for every logit of the wave's part, done(chunk) behind each chunk; loads a chunk ahead
   template <typename F>
@@ -294,15 +308,15 @@ struct Sampler {
   __device__ __forceinline__ uint64_t cut(int n, F keep, uint64_t& sum) {
     if (threadIdx.x == 0) sh->last = ~0ull, sh->sum = 0;
     __syncthreads();
-    if ((int)threadIdx.x < n) {
-      const uint64_t k = sh->key[threadIdx.x];
+    for (int own = threadIdx.x; own < n; own += NT) {
+      const uint64_t k = sh->key[own];
       uint32_t rank = 0;
       uint64_t before = 0;
       for (int j = 0; j < n; ++j)
         if (sh->key[j] > k) ++rank, before += sh->weight[j];
       if (keep(rank, before)) {
         atomicMin(&sh->last, (unsigned long long)k);
-        atomicAdd(&sh->sum, (unsigned long long)sh->weight[threadIdx.x]);
+        atomicAdd(&sh->sum, (unsigned long long)sh->weight[own]);
       }
     }
     __syncthreads();
@@ -346,15 +360,23 @@ struct Sampler {
   // The first index at which the sum of amount(index, value) passes target(the whole sum), which is below it
   template <typename F, typename G>
   __device__ __forceinline__ int find(F amount, G target) {
-    uint64_t mine = 0, own = 0;
+    uint64_t own = 0;
     static_assert(sizeof(Shared::mass) >= 8 * ((1 << 20) / kSampleChunk), "a chunk's sum each: the bins are read");
     each([&](int i, float x) { own += amount(i, x); },
          [&](int q) {
            own = wave_sum64(own);
            if (lane == 0) sh->mass[q] = own;
-           mine += own;
            own = 0;
          });
+    return find_in_chunks(amount, target);
+  }
+  // The same with every chunk's sum in `mass`
+  template <typename F, typename G>
+  __device__ __forceinline__ int find_in_chunks(F amount, G target) {
+    __syncthreads();
+    uint64_t mine = 0;
+#pragma unroll 1
+    for (int q = first; q < last; q += 64) mine += wave_sum64(q + lane < last ? sh->mass[q + lane] : 0);
     if (lane == 0) sh->part[wave] = mine;
     __syncthreads();
     uint64_t sum = 0, before = 0;
@@ -463,21 +485,10 @@ struct Sampler {
   }
 };
 
-template <typename T, int NW>
-__global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
-  using S = Sampler<T, NW>;
-  __shared__ typename S::Shared shared;
-  S s;
-  s.sh = &shared;
-  s.V = a.V;
-  s.lane = threadIdx.x & 63;
-  s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunks = (a.V + kSampleChunk - 1) / kSampleChunk, each = (chunks + NW - 1) / NW;
-  s.first = min(s.wave * each, chunks);
-  s.last = min(s.first + each, chunks);
-  for (int j = threadIdx.x; j < 256; j += S::NT) shared.power[j] = exp2(j / 256.0);
-  const int64_t r = blockIdx.x;
-  s.row = (const T*)a.logits + r * a.ld;
+// The answer of row r, whose parts s has
+template <typename S>
+__device__ __forceinline__ int sample_row(S& s, const SampleArgs& a, int64_t r) {
+  typename S::Shared& sh = *s.sh;
   // ---- the largest logit and the smallest, and whether there is a NaN
   float top = -INFINITY, least = INFINITY;
   bool bad = false;
@@ -489,19 +500,18 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
   top = wave_max(top);
   least = wave_min(least);
   bad = __any(bad);
-  if (s.lane == 0) shared.top[s.wave] = bad ? NAN : top, shared.least[s.wave] = least;
-  if (threadIdx.x == 0) shared.first = 0x7fffffffu;
+  if (s.lane == 0) sh.top[s.wave] = bad ? NAN : top, sh.least[s.wave] = least;
+  if (threadIdx.x == 0) sh.first = 0x7fffffffu;
   __syncthreads();
   bool nan = false;
 #pragma unroll
-  for (int q = 0; q < NW; ++q) {
-    const float its = shared.top[q];
+  for (int q = 0; q < S::NT / 64; ++q) {
+    const float its = sh.top[q];
     nan |= its != its;
-    top = fmaxf(top, its), least = fminf(least, shared.least[q]);
+    top = fmaxf(top, its), least = fminf(least, sh.least[q]);
   }
   s.top = top;
   s.least = least;
-  int answer;
   const float t = a.temperature ? a.temperature[r] : a.t0;
   if (nan || !(t > 0.f)) {
     // the first NaN, which is above all as in torch's argmax, or the first of the largest
@@ -509,9 +519,9 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
     s.each([&](int i, float x) {
       if ((nan ? x != x : x == top) && i < a.V) at = min(at, (uint32_t)i);
     });
-    if (at != 0x7fffffffu) atomicMin(&shared.first, at);
+    if (at != 0x7fffffffu) atomicMin(&sh.first, at);
     __syncthreads();
-    answer = (int)shared.first;
+    return (int)sh.first;
   } else {
     s.c = 1.4426950408889634 / (double)t;
     // every logit above the last bin, but what lies 31 temperatures below the largest
@@ -520,11 +530,317 @@ __global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
     const typename S::Kept kept(s.border(a.top_k ? a.top_k[r] : a.k0, a.top_p ? a.top_p[r] : a.p0));
     const float m = a.min_p ? a.min_p[r] : a.m0, u = a.uniform[r];
     const double least_x = m >= 1.f ? (double)top : m > 0.f ? (double)top + (double)t * log((double)m) : -INFINITY;
-    answer = s.find([&](int i, float x) { return kept(i, x) && !((double)x < least_x) ? s.weight(x) : (uint64_t)0; },
+    return s.find([&](int i, float x) { return kept(i, x) && !((double)x < least_x) ? s.weight(x) : (uint64_t)0; },
                     [&](uint64_t sum) {
                       const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
                       return (uint64_t)(f * (double)sum);
                     });
+  }
+}
+
+template <typename S>
+__device__ __forceinline__ void sample_power_table(S& s) {
+  for (int j = threadIdx.x; j < 256; j += S::NT) s.sh->power[j] = exp2(j / 256.0);
+}
+
+template <typename T, int NW>
+__global__ void __launch_bounds__(64 * NW) sample_tokens_kernel(SampleArgs a) {
+  using S = Sampler<T, NW>;
+  __shared__ typename S::Shared shared;
+  S s;
+  s.sh = &shared;
+  s.start(a, blockIdx.x, 0, (a.V + kSampleChunk - 1) / kSampleChunk);
+  sample_power_table(s);
+  const int answer = sample_row(s, a, blockIdx.x);
+  if (threadIdx.x == 0) a.ids[blockIdx.x] = answer;
+}
+
+// ------------------------------------------------------------------------------------------------ few long rows
+// Rows too few to fill the card are cut into parts of 8 chunks and more, a workgroup each, and the passes above become launches: the
+// parts' largest logits; their bins; where a top-k is asked for, the tokens of its border's bin; the chunks' weights above the
+// last border's bin, and that bin's tokens; and a workgroup a row that orders these, adds what is kept of them to the chunks' sums and finds
+// the token.  What a launch needs of the ones before (the largest logit, the bins' sums, the borders' bins) each workgroup joins for itself, in
+// the same way: nothing is added up in memory, and nothing is waited for.  A row with a NaN, without a temperature, or with more tokens in a border's
+// bin than the list holds is answered by the last launch alone, as a single workgroup does.
+constexpr int kWideParts = 32, kWideBins = 1024, kWideList = 1024;
+
+struct WideRow {
+  float *top, *least;         // of each part; a NaN: one is there
+  unsigned long long* chunk;  // the kept weights of each chunk, but the border's bin
+  unsigned long long* mass;   // the bins of each part
+  uint32_t* count;
+  uint32_t* n;                      // two lists of each part: the tokens of a border's bin
+  unsigned long long *key, *weight;
+  __host__ __device__ static int64_t bytes(int parts, int chunks) {
+    return 2 * 8 * (int64_t)kWideParts + 8 * (int64_t)chunks + parts * (12 * (int64_t)kWideBins + 2 * 16 * (int64_t)kWideList);
+  }
+  __device__ __forceinline__ WideRow(const SampleArgs& a, int64_t r, int chunks) {
+    uint8_t* p = a.held + r * bytes(a.parts, chunks);
+    chunk = (unsigned long long*)p, p += 8 * (int64_t)chunks;
+    mass = (unsigned long long*)p, p += 8 * (int64_t)kWideBins * a.parts;
+    key = (unsigned long long*)p, p += 16 * (int64_t)kWideList * a.parts;
+    weight = (unsigned long long*)p, p += 16 * (int64_t)kWideList * a.parts;
+    count = (uint32_t*)p, p += 4 * (int64_t)kWideBins * a.parts;
+    top = (float*)p, least = top + kWideParts, n = (uint32_t*)(least + kWideParts);  // (n: two for each part)
+  }
+};
+
+// Parts of a row's chunks, or 0: a workgroup a row
+static int wide_parts(int64_t rows, int64_t V, int dtype) {
+  const int chunks = (int)((V + kSampleChunk - 1) / kSampleChunk);
+  if ((dtype_size(dtype) == 2 && V < 65536) || chunks < 32) return 0;
+  const int parts = std::min((chunks + 7) / 8, kWideParts);
+  return rows * parts <= 2 * device_cu_count() ? parts : 0;
+}
+
+template <typename T>
+struct Wide : Sampler<T, 8, kWideBins, kWideList> {
+  using S = Sampler<T, 8, kWideBins, kWideList>;
+  using S::NT, S::sh, S::lane, S::wave, S::top, S::least, S::c, S::width, S::V;
+  static constexpr int B = kWideBins;
+  WideRow w;
+  int parts, part, chunks;
+  float t;
+  double least_x;           // a kept token's least value
+  int border = B;           // the last border's bin; B: none
+  int listed = -1;          // top-k's border's bin, where list 0 has its tokens
+  uint64_t keep = 0;        // the last token that top-k keeps
+  uint64_t above = 0, target = 0;  // top-p's border: the weight above its bin, and where it ends
+
+  __device__ __forceinline__ Wide(const SampleArgs& a, int64_t r, int first_part, int last_part, typename S::Shared* shared)
+      : w(a, r, (a.V + kSampleChunk - 1) / kSampleChunk) {
+    sh = shared;
+    parts = a.parts, part = first_part, chunks = (a.V + kSampleChunk - 1) / kSampleChunk;
+    const int per = (chunks + parts - 1) / parts;
+    S::start(a, r, min(first_part * per, chunks), min(last_part * per, chunks));
+    t = a.temperature ? a.temperature[r] : a.t0;
+  }
+
+  // The row's largest and smallest logit from its parts'; whether the launches share this row
+  __device__ __forceinline__ bool join(const SampleArgs& a, int64_t r) {
+    const float x = lane < parts ? w.top[lane] : -INFINITY, y = lane < parts ? w.least[lane] : INFINITY;
+    const bool nan = __any(x != x);
+    top = wave_max(x);
+    least = wave_min(y);
+    if (nan || !(t > 0.f)) return false;
+    sample_power_table(*this);
+    c = 1.4426950408889634 / (double)t;
+    width = (float)(B - 1) / fminf((top - least) * 1.001f, 31.f * t);
+    if (!(width > 0.f && width < 3e38f)) width = 0.f;
+    const float m = a.min_p ? a.min_p[r] : a.m0;
+    least_x = m >= 1.f ? (double)top : m > 0.f ? (double)top + (double)t * log((double)m) : -INFINITY;
+    __syncthreads();
+    return true;
+  }
+  __device__ __forceinline__ bool by_count(const SampleArgs& a, int64_t r, int& k) const {
+    k = a.top_k ? a.top_k[r] : a.k0;
+    return k > 0 && k < V;
+  }
+  __device__ __forceinline__ bool by_mass(const SampleArgs& a, int64_t r, float& p) const {
+    p = a.top_p ? a.top_p[r] : a.p0;
+    return p < 1.f;
+  }
+
+  // The parts' bins, joined in LDS
+  __device__ __forceinline__ void join_bins(bool masses) {
+    for (int b = threadIdx.x; b < B; b += NT) {
+      uint64_t m = 0;
+      uint32_t n = 0;
+#pragma unroll 8
+      for (int q = 0; q < parts; ++q) {
+        n += w.count[q * B + b];
+        if (masses) m += w.mass[q * B + b];
+      }
+      sh->count[b] = n;
+      sh->mass[b] = m;
+    }
+    __syncthreads();
+  }
+  // A list's tokens, joined in LDS
+  __device__ __forceinline__ int join_list(int which) {
+    const uint32_t its = lane < parts ? min(w.n[2 * lane + which], (uint32_t)kWideList) : 0, upto = wave_scan32(its);
+    const int n = min((int)lane32(upto, 63), kWideList);  // (a row with more is not shared)
+#pragma unroll 1
+    for (int q = wave; q < parts; q += NT / 64) {
+      const int own = (int)lane32(its, q), at = (int)lane32(upto, q) - own;
+      const int64_t from = (int64_t)(2 * q + which) * kWideList;
+      for (int j = lane; j < own && at + j < kWideList; j += 64) sh->key[at + j] = w.key[from + j], sh->weight[at + j] = w.weight[from + j];
+    }
+    __syncthreads();
+    return n;
+  }
+  // Top-k's border's bin, B: none; false where its bin holds too many
+  __device__ __forceinline__ bool count_border(int k, int& b) {
+    uint64_t before, held;
+    b = S::template find_bin<S::BPER>(sh->count, 0, (uint64_t)k, before, held);
+    above = before;
+    if (b == B - 1) b = B;
+    return b == B || held <= kWideList;
+  }
+  // Where the row's filters end; false where a bin holds too many tokens for the list
+  __device__ __forceinline__ bool borders(const SampleArgs& a, int64_t r) {
+    int k;
+    float p;
+    const bool count = by_count(a, r, k), mass = by_mass(a, r, p);
+    if (!count && !mass) return true;
+    join_bins(mass);
+    uint64_t total = 0, held;
+    if (count) {
+      int b;
+      if (!count_border(k, b)) return false;
+      if (b < B) {
+        listed = border = b;
+        const int n = join_list(0);
+        const uint64_t before = above;
+        keep = S::cut(n, [&](uint32_t rank, uint64_t) { return before + rank < (uint64_t)k; }, total);
+      }
+    }
+    if (!mass) return true;
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < S::BPER; ++j)
+      if (listed < 0 || (int)(S::BPER * threadIdx.x + j) < listed) mine += sh->mass[S::BPER * threadIdx.x + j];
+    total += S::block_sum(mine);
+    const double want = (double)p * (double)total;
+    target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
+    border = S::template find_bin<S::BPER>(sh->mass, 0, target, above, held);
+    return sh->count[border] <= (uint32_t)kWideList;
+  }
+  // This part's tokens of bin b into list `which`, and done(chunk) behind each chunk's f(value, bin)
+  template <typename F, typename D>
+  __device__ __forceinline__ void list_tokens(int b, int which, F f, D done) {
+    if (threadIdx.x == 0) sh->n = 0;
+    __syncthreads();
+    const int64_t from = (int64_t)(2 * part + which) * kWideList;
+    S::each(
+        [&](int i, float x) {
+          const int its = S::bin(x);
+          f(x, its);
+          if (its == b && x == x) {
+            const uint32_t at = atomicAdd(&sh->n, 1u);
+            if (at < (uint32_t)kWideList) w.key[from + at] = sample_order(SampleKey<T>::of_value(x), i), w.weight[from + at] = S::weight(x);
+          }
+        },
+        done);
+    __syncthreads();
+    if (threadIdx.x == 0) w.n[2 * part + which] = sh->n;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(512) wide_top_kernel(SampleArgs a) {
+  __shared__ typename Wide<T>::Shared shared;
+  Wide<T> s(a, blockIdx.y, blockIdx.x, blockIdx.x + 1, &shared);
+  float top = -INFINITY, least = INFINITY;
+  bool bad = false;
+  s.each([&](int i, float x) {
+    top = fmaxf(top, x);
+    least = fminf(least, x);
+    bad |= x != x && i < a.V;
+  });
+  top = wave_max(top);
+  least = wave_min(least);
+  if (__any(bad)) top = NAN;
+  if (s.lane == 0) shared.top[s.wave] = top, shared.least[s.wave] = least;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int q = 1; q < 8; ++q) {
+      const float its = shared.top[q];
+      top = its != its || top != top ? NAN : fmaxf(top, its);
+      least = fminf(least, shared.least[q]);
+    }
+    s.w.top[s.part] = top;
+    s.w.least[s.part] = least;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) wide_bins_kernel(SampleArgs a) {
+  using W = Wide<T>;
+  __shared__ typename W::Shared shared;
+  W s(a, blockIdx.y, blockIdx.x, blockIdx.x + 1, &shared);
+  int k;
+  float p;
+  const bool count = s.by_count(a, blockIdx.y, k), mass = s.by_mass(a, blockIdx.y, p);
+  if (!(count || mass) || !s.join(a, blockIdx.y)) return;
+  for (int b = threadIdx.x; b < W::B; b += W::NT) shared.mass[b] = 0, shared.count[b] = 0;
+  __syncthreads();
+  s.each([&](int, float x) {  // (a missing one is counted in the last bin, where it changes nothing)
+    const int b = s.bin(x);
+    atomicAdd(&shared.count[b], 1u);
+    if (mass) atomicAdd(&shared.mass[b], (unsigned long long)s.weight(x));
+  });
+  __syncthreads();
+  for (int b = threadIdx.x; b < W::B; b += W::NT) {
+    s.w.count[s.part * W::B + b] = shared.count[b];
+    if (mass) s.w.mass[s.part * W::B + b] = shared.mass[b];
+  }
+}
+
+// Top-k's border's tokens
+template <typename T>
+__global__ void __launch_bounds__(512) wide_list_kernel(SampleArgs a) {
+  using W = Wide<T>;
+  __shared__ typename W::Shared shared;
+  W s(a, blockIdx.y, blockIdx.x, blockIdx.x + 1, &shared);
+  int k, b;
+  if (!s.by_count(a, blockIdx.y, k) || !s.join(a, blockIdx.y)) return;
+  s.join_bins(false);
+  if (!s.count_border(k, b) || b == W::B) return;
+  s.list_tokens(b, 0, [](float, int) {}, [](int) {});
+}
+
+// The chunks' weights above the last border's bin; top-p's border's tokens
+template <typename T>
+__global__ void __launch_bounds__(512) wide_sums_kernel(SampleArgs a) {
+  using W = Wide<T>;
+  __shared__ typename W::Shared shared;
+  W s(a, blockIdx.y, blockIdx.x, blockIdx.x + 1, &shared);
+  if (!s.join(a, blockIdx.y) || !s.borders(a, blockIdx.y)) return;
+  uint64_t own = 0;
+  s.list_tokens(s.border == s.listed ? -1 : s.border, 1,
+                [&](float x, int b) { own += b < s.border && !((double)x < s.least_x) ? s.weight(x) : 0; },
+                [&](int q) {
+                  own = wave_sum64(own);
+                  if (s.lane == 0) s.w.chunk[q] = own;
+                  own = 0;
+                });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) wide_pick_kernel(SampleArgs a) {
+  using W = Wide<T>;
+  __shared__ typename W::Shared shared;
+  const int64_t r = blockIdx.x;
+  W s(a, r, 0, a.parts, &shared);
+  int answer;
+  if (!s.join(a, r) || !s.borders(a, r)) {
+    __syncthreads();
+    sample_power_table(s);
+    answer = sample_row((typename W::S&)s, a, r);
+  } else {
+    uint64_t last = s.keep;
+    int n = 0;
+    if (s.border < W::B) {
+      __syncthreads();  // the bins and list 0 are read
+      n = s.join_list(s.border == s.listed ? 0 : 1);
+      uint64_t sum;
+      if (s.target) last = max(last, s.cut(n, [&](uint32_t, uint64_t before) { return s.above + before < s.target; }, sum));
+    }
+    for (int q = threadIdx.x; q < s.chunks; q += W::NT) shared.mass[q] = s.w.chunk[q];
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += W::NT) {
+      const uint64_t k = shared.key[j];
+      if (k >= last && !((double)SampleKey<T>::value((uint32_t)(k >> 32)) < s.least_x))
+        atomicAdd(&shared.mass[(int)~(uint32_t)k / kSampleChunk], (unsigned long long)shared.weight[j]);
+    }
+    const typename W::Kept kept(last);
+    const float u = a.uniform[r];
+    answer = s.find_in_chunks([&](int i, float x) { return kept(i, x) && !((double)x < s.least_x) ? s.weight(x) : (uint64_t)0; },
+                              [&](uint64_t sum) {
+                                const double f = u > 0.f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+                                return (uint64_t)(f * (double)sum);
+                              });
   }
   if (threadIdx.x == 0) a.ids[r] = answer;
 }
@@ -1010,9 +1326,17 @@ __global__ void __launch_bounds__(kCountedThreads) sample_counted_kernel(SampleA
 
 }  // namespace atma
 
-extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* uniform, const float* temperature, float t0,
-                                  const int32_t* top_k, int k0, const float* top_p, float p0, const float* min_p, float m0,
-                                  int64_t* ids, int64_t rows, int64_t V, int dtype, void* stream) {
+extern "C" int64_t atma_sample_tokens_workspace(int64_t rows, int64_t V, int dtype) {
+  using namespace atma;
+  if (rows < 1 || V < 1 || V > (1 << 20) || !dtype_size(dtype)) return 0;
+  const int parts = wide_parts(rows, V, dtype);
+  return parts ? rows * WideRow::bytes(parts, (int)((V + kSampleChunk - 1) / kSampleChunk)) : 0;
+}
+
+extern "C" int atma_sample_tokens_in(const void* logits, int64_t ld, const float* uniform, const float* temperature, float t0,
+                                     const int32_t* top_k, int k0, const float* top_p, float p0, const float* min_p, float m0,
+                                     int64_t* ids, int64_t rows, int64_t V, int dtype, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
   using namespace atma;
   const char* what = "sample_tokens";
   if (!dtype_size(dtype)) return set_error(ATMA_ERR_UNSUPPORTED, "%s: fp32 or 16-bit logits (dtype %d)", what, dtype);
@@ -1022,7 +1346,29 @@ extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* u
   if (!logits || !uniform || !ids) return set_error(ATMA_ERR_INVALID, "%s: null pointer", what);
   if ((uintptr_t)logits % dtype_size(dtype)) return set_error(ATMA_ERR_INVALID, "%s: misaligned logits", what);
   if (rows > 1 && ld < V && ld != 0) return set_error(ATMA_ERR_INVALID, "%s: rows overlap", what);
-  SampleArgs a{logits, ld, uniform, temperature, top_k, top_p, min_p, t0, p0, m0, k0, ids, (int)V};
+  SampleArgs a{logits, ld, uniform, temperature, top_k, top_p, min_p, t0, p0, m0, k0, ids, (int)V, nullptr, 0};
+  const int64_t need = atma_sample_tokens_workspace(rows, V, dtype);
+  if (need && workspace) {
+    if (workspace_bytes < need || (uintptr_t)workspace % 8)
+      return set_error(ATMA_ERR_INVALID, "%s: a workspace of %lld bytes, 8-byte aligned", what, (long long)need);
+    a.held = (uint8_t*)workspace;
+    a.parts = wide_parts(rows, V, dtype);
+    const dim3 grid((unsigned)a.parts, (unsigned)rows);
+    hipStream_t st = (hipStream_t)stream;
+    auto launch = [&](auto zero) {
+      using T = decltype(zero);
+      wide_top_kernel<T><<<grid, 512, 0, st>>>(a);
+      const bool count = top_k || (k0 > 0 && k0 < V);
+      if (count || top_p || p0 < 1.f) wide_bins_kernel<T><<<grid, 512, 0, st>>>(a);
+      if (count) wide_list_kernel<T><<<grid, 512, 0, st>>>(a);
+      wide_sums_kernel<T><<<grid, 512, 0, st>>>(a);
+      wide_pick_kernel<T><<<dim3((unsigned)rows), 512, 0, st>>>(a);
+    };
+    if (dtype == ATMA_F32) launch(0.f);
+    else if (dtype == ATMA_BF16) launch(bf16{});
+    else launch(f16{});
+    return check_launch(what);
+  }
   // Short rows take workgroups of four waves, of which a CU holds five: us in bf16, four waves / values counted / sixteen waves, 32 rows of
   // 2,000 logits 12.9 / 14.7 / -, of 8,000 24.4 / 17.0 / 19.4 (eight), of 16,000 - / 19.2 / 25.0; 2,048 rows of 1,000 29 / 109 / -,
   // of 8,000 63 / 122 / 82 (eight), of 12,000 - / 131 / 155
@@ -1059,4 +1405,11 @@ extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* u
     else launch(float{});
   }
   return check_launch(what);
+}
+
+extern "C" int atma_sample_tokens(const void* logits, int64_t ld, const float* uniform, const float* temperature, float t0,
+                                  const int32_t* top_k, int k0, const float* top_p, float p0, const float* min_p, float m0,
+                                  int64_t* ids, int64_t rows, int64_t V, int dtype, void* stream) {
+  return atma_sample_tokens_in(logits, ld, uniform, temperature, t0, top_k, k0, top_p, p0, min_p, m0, ids, rows, V, dtype, nullptr,
+                               0, stream);
 }

@@ -726,6 +726,18 @@ int atma_sample_tokens(const void* logits, int64_t ld, const float* uniform, con
                        int64_t* ids, int64_t rows, int64_t V, int dtype, void* stream);
 
 /*
+ * atma_sample_tokens has a workgroup answer a row, in one launch.  For few long rows atma_sample_tokens_workspace gives a number of
+ * bytes above 0: with a workspace of as many (8-byte aligned, in any state, the call's own until its launches are done) many
+ * workgroups share each row, in three to five launches.  Without one (NULL), and where the number is 0, it is
+ * atma_sample_tokens.  The answers are the same.
+ */
+int64_t atma_sample_tokens_workspace(int64_t rows, int64_t V, int dtype);
+int atma_sample_tokens_in(const void* logits, int64_t ld, const float* uniform, const float* temperature, float t0,
+                          const int32_t* top_k, int k0, const float* top_p, float p0, const float* min_p, float m0,
+                          int64_t* ids, int64_t rows, int64_t V, int dtype, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/*
  * The LFM2 block's decode mixer (model/reference.py:31-48, inference/models/atma.py:
  * 625-673) as one call: with b, c, x the three D-wide thirds of each bcx row (in_proj's
  * output), out = c * conv(b * x), the depthwise conv of K taps (weight (D, K)) over the

@@ -53,3 +53,19 @@ def test_oracle_rules():
     assert O.draw([0.0] * 4, 0.5, 1.0) == 2 and O.draw([0.0] * 4, 0.49, 1.0) == 1 and O.draw(x, 0.99, 0.0) == 1
     assert O.draw([1.0, math.nan, math.inf], 0.0, 1.0) == 1 and O.draw([-math.inf] * 3, 0.5, 1.0) == 1
     assert O.draw([0.0, math.inf, math.inf], 0.7, 1.0) == 2 and O.draw(x, 1.0, 1.0) == 3 and O.draw(x, math.nan, 1.0) == 0
+
+
+def test_workspace_of_shared_rows():
+    """Asked without a launch; a workspace that is too small, or misaligned, is refused before one."""
+    from atma_amd import _lib
+    lib = _lib.load()
+    size = lib.atma_sample_tokens_workspace
+    assert size(1, 50304, _lib.ATMA_F32) > 0 and size(1, 50304, _lib.ATMA_BF16) == 0 and size(1, 65536, _lib.ATMA_BF16) > 0
+    assert size(2048, 50304, _lib.ATMA_F32) == 0 and size(1, 1000, _lib.ATMA_F32) == 0
+    assert size(4, 50304, _lib.ATMA_F32) == 4 * size(1, 50304, _lib.ATMA_F32)
+    for bad in ((0, 50304, 0), (-1, 50304, 0), (1, 0, 0), (1, (1 << 20) + 1, 0), (1, 50304, 77)):
+        assert size(*bad) == 0
+    need = size(1, 50304, _lib.ATMA_F32)
+    call = lambda at, n: lib.atma_sample_tokens_in(64, 50304, 64, None, 1.0, None, 0, None, 1.0, None, 0.0, 64, 1, 50304,   # noqa: E731
+                                                   _lib.ATMA_F32, at, n, None)
+    assert call(64, need - 1) == call(60, need) == 1   # invalid
