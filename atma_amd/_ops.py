@@ -1231,7 +1231,7 @@ def _(x, data, scale, bias):
 def sample_into(ids, logits, uniform, temperature, t0, top_k, k0, top_p, p0, min_p, m0):
     (rows, V), code, lib = logits.shape, _lib.DTYPE_CODE[logits.dtype], _lib.load()
     # few long rows are shared by many workgroups (V of 16 bits below 65,536: never)
-    need = lib.atma_sample_tokens_workspace(rows, V, code) if V > 16000 and rows < 256 and (V >= 65536 or code == _lib.ATMA_F32) else 0
+    need = lib.atma_sample_tokens_workspace(rows, V, code) if V > 32000 and rows < 256 and (V >= 65536 or code == _lib.ATMA_F32) else 0
     work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     rc = lib.atma_sample_tokens_in(
         logits.data_ptr(), logits.stride(0), uniform.data_ptr(), _lib.ptr(temperature), t0, _lib.ptr(top_k), k0,

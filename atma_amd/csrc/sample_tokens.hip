@@ -16,9 +16,8 @@
 // order of the additions nor the number of threads changes a result, and a border is decided as in 64-bit arithmetic
 // (with fp32 weights one row in a few thousand would answer its neighbour's token).  V <= 2^20 keeps every sum below 2^63.
 //
-// What bounds it is one CU's work on a row: two passes that form a weight for every logit, some 190 cycles for 64 of them.  One row of 50,304
-// fp32 logits with top-p takes 42 us (without 23), 512 rows 117.  (More CUs a row would need the largest logit, the bins and the
-// sums from each other: five launches of 3 us and a workspace.)
+// What bounds it is a CU's work on a row: two passes that form a weight for every logit, some 190 cycles for 64 of them.  512 rows of 50,304
+// fp32 logits with top-p take 117 us, one in one workgroup 43, shared by 13 of them 23.
 #include <algorithm>
 
 #include "common.h"
@@ -312,8 +311,12 @@ struct Sampler {
       const uint64_t k = sh->key[own];
       uint32_t rank = 0;
       uint64_t before = 0;
-      for (int j = 0; j < n; ++j)
-        if (sh->key[j] > k) ++rank, before += sh->weight[j];
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const bool above = sh->key[j] > k;
+        rank += above;
+        before += above ? sh->weight[j] : 0;
+      }
       if (keep(rank, before)) {
         atomicMin(&sh->last, (unsigned long long)k);
         atomicAdd(&sh->sum, (unsigned long long)sh->weight[own]);
@@ -566,16 +569,18 @@ constexpr int kWideParts = 32, kWideBins = 1024, kWideList = 1024;
 
 struct WideRow {
   float *top, *least;         // of each part; a NaN: one is there
+  unsigned long long* ends;   // where the filters end: Wide's members behind borders(), and whether it found them
   unsigned long long* chunk;  // the kept weights of each chunk, but the border's bin
   unsigned long long* mass;   // the bins of each part
   uint32_t* count;
   uint32_t* n;                      // two lists of each part: the tokens of a border's bin
   unsigned long long *key, *weight;
   __host__ __device__ static int64_t bytes(int parts, int chunks) {
-    return 2 * 8 * (int64_t)kWideParts + 8 * (int64_t)chunks + parts * (12 * (int64_t)kWideBins + 2 * 16 * (int64_t)kWideList);
+    return 64 + 2 * 8 * (int64_t)kWideParts + 8 * (int64_t)chunks + parts * (12 * (int64_t)kWideBins + 2 * 16 * (int64_t)kWideList);
   }
   __device__ __forceinline__ WideRow(const SampleArgs& a, int64_t r, int chunks) {
     uint8_t* p = a.held + r * bytes(a.parts, chunks);
+    ends = (unsigned long long*)p, p += 64;
     chunk = (unsigned long long*)p, p += 8 * (int64_t)chunks;
     mass = (unsigned long long*)p, p += 8 * (int64_t)kWideBins * a.parts;
     key = (unsigned long long*)p, p += 16 * (int64_t)kWideList * a.parts;
@@ -585,10 +590,16 @@ struct WideRow {
   }
 };
 
-// Parts of a row's chunks, or 0: a workgroup a row
+// Parts of a row's chunks, or 0: a workgroup a row.  us, a workgroup a row / shared, fp32 without a filter, with top-p, top-k, both:
+//   16,001 logits,  1 row  12.2 / 12.5   20.7 / 21.3   16.2 / 23.1   23.5 / 27.3
+//   30,000          1      18.1 / 13.0   31.7 / 22.8   21.7 / 25.1   33.2 / 29.3
+//   50,304          1      27.0 / 13.1   43.1 / 22.9   30.7 / 26.9   48.1 / 31.7
+//   50,304         32      28.0 / 15.6   48.4 / 34.0   31.4 / 33.1   49.5 / 44.0
+//   2^20            1       396 / 30      648 / 59      397 / 49      679 / 62
+//   2^20           16       398 / 49      661 / 93      398 / 77      681 / 98
 static int wide_parts(int64_t rows, int64_t V, int dtype) {
   const int chunks = (int)((V + kSampleChunk - 1) / kSampleChunk);
-  if ((dtype_size(dtype) == 2 && V < 65536) || chunks < 32) return 0;
+  if ((dtype_size(dtype) == 2 && V < 65536) || chunks < 64) return 0;
   const int parts = std::min((chunks + 7) / 8, kWideParts);
   return rows * parts <= 2 * device_cu_count() ? parts : 0;
 }
@@ -641,20 +652,21 @@ struct Wide : Sampler<T, 8, kWideBins, kWideList> {
     return p < 1.f;
   }
 
-  // The parts' bins, joined in LDS
-  __device__ __forceinline__ void join_bins(bool masses) {
+  // The sum over the parts of each bin's count or mass, in LDS; eight parts' loads at once
+  template <typename A>
+  __device__ __forceinline__ void join_bins(const A* from, A* to) {
     for (int b = threadIdx.x; b < B; b += NT) {
-      uint64_t m = 0;
-      uint32_t n = 0;
-#pragma unroll 8
-      for (int q = 0; q < parts; ++q) {
-        n += w.count[q * B + b];
-        if (masses) m += w.mass[q * B + b];
+      A sum = 0;
+#pragma unroll 1
+      for (int q = 0; q < parts; q += 8) {
+        A v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = q + i < parts ? from[(q + i) * B + b] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += v[i];
       }
-      sh->count[b] = n;
-      sh->mass[b] = m;
+      to[b] = sum;
     }
-    __syncthreads();
   }
   // A list's tokens, joined in LDS
   __device__ __forceinline__ int join_list(int which) {
@@ -683,7 +695,9 @@ struct Wide : Sampler<T, 8, kWideBins, kWideList> {
     float p;
     const bool count = by_count(a, r, k), mass = by_mass(a, r, p);
     if (!count && !mass) return true;
-    join_bins(mass);
+    if (count) join_bins(w.count, sh->count);
+    if (mass) join_bins(w.mass, sh->mass);
+    __syncthreads();
     uint64_t total = 0, held;
     if (count) {
       int b;
@@ -704,7 +718,14 @@ struct Wide : Sampler<T, 8, kWideBins, kWideList> {
     const double want = (double)p * (double)total;
     target = min(max((uint64_t)(want > 0.0 ? ceil(want) : 1.0), (uint64_t)1), total);
     border = S::template find_bin<S::BPER>(sh->mass, 0, target, above, held);
-    return sh->count[border] <= (uint32_t)kWideList;
+    return lane32(wave_scan32(lane < parts ? w.count[lane * B + border] : 0), 63) <= (uint32_t)kWideList;
+  }
+  __device__ __forceinline__ void store_ends(bool found) const {
+    w.ends[0] = found, w.ends[1] = (unsigned)border, w.ends[2] = (unsigned)listed, w.ends[3] = keep, w.ends[4] = above, w.ends[5] = target;
+  }
+  __device__ __forceinline__ bool load_ends() {
+    border = (int)w.ends[1], listed = (int)(unsigned)w.ends[2], keep = w.ends[3], above = w.ends[4], target = w.ends[5];
+    return w.ends[0] != 0;
   }
   // This part's tokens of bin b into list `which`, and done(chunk) behind each chunk's f(value, bin)
   template <typename F, typename D>
@@ -785,7 +806,8 @@ __global__ void __launch_bounds__(512) wide_list_kernel(SampleArgs a) {
   W s(a, blockIdx.y, blockIdx.x, blockIdx.x + 1, &shared);
   int k, b;
   if (!s.by_count(a, blockIdx.y, k) || !s.join(a, blockIdx.y)) return;
-  s.join_bins(false);
+  s.join_bins(s.w.count, shared.count);
+  __syncthreads();
   if (!s.count_border(k, b) || b == W::B) return;
   s.list_tokens(b, 0, [](float, int) {}, [](int) {});
 }
@@ -796,7 +818,10 @@ __global__ void __launch_bounds__(512) wide_sums_kernel(SampleArgs a) {
   using W = Wide<T>;
   __shared__ typename W::Shared shared;
   W s(a, blockIdx.y, blockIdx.x, blockIdx.x + 1, &shared);
-  if (!s.join(a, blockIdx.y) || !s.borders(a, blockIdx.y)) return;
+  if (!s.join(a, blockIdx.y)) return;
+  const bool found = s.borders(a, blockIdx.y);
+  if (s.part == 0 && threadIdx.x == 0) s.store_ends(found);
+  if (!found) return;
   uint64_t own = 0;
   s.list_tokens(s.border == s.listed ? -1 : s.border, 1,
                 [&](float x, int b) { own += b < s.border && !((double)x < s.least_x) ? s.weight(x) : 0; },
@@ -814,7 +839,7 @@ __global__ void __launch_bounds__(512) wide_pick_kernel(SampleArgs a) {
   const int64_t r = blockIdx.x;
   W s(a, r, 0, a.parts, &shared);
   int answer;
-  if (!s.join(a, r) || !s.borders(a, r)) {
+  if (!s.join(a, r) || !s.load_ends()) {
     __syncthreads();
     sample_power_table(s);
     answer = sample_row((typename W::S&)s, a, r);
@@ -822,7 +847,6 @@ __global__ void __launch_bounds__(512) wide_pick_kernel(SampleArgs a) {
     uint64_t last = s.keep;
     int n = 0;
     if (s.border < W::B) {
-      __syncthreads();  // the bins and list 0 are read
       n = s.join_list(s.border == s.listed ? 0 : 1);
       uint64_t sum;
       if (s.target) last = max(last, s.cut(n, [&](uint32_t, uint64_t before) { return s.above + before < s.target; }, sum));

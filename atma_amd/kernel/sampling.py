@@ -1,6 +1,6 @@
 """Next-token sampling: temperature, top-k, top-p and min-p from one given random number a row (C ABI
-``atma_sample_tokens``), in one launch.  The reference samples by temperature alone, with random numbers of its own
-(``inference/layers/sampler.py:5-10``)."""
+``atma_sample_tokens``, ``atma_sample_tokens_in``), in one launch, few long rows in three to five.  The reference samples by
+temperature alone, with random numbers of its own (``inference/layers/sampler.py:5-10``)."""
 
 import torch
 

@@ -77,7 +77,7 @@ def _rows(g, kind, rows, V):
 
 
 @pytest.mark.parametrize("kind", ["plain", "quarters", "whole", "constant", "few", "infinite", "nan", "close", "far", "zeros"])
-@pytest.mark.parametrize("V,dtype", [(16001, F32), (50304, F32), (65536, BF), (70001, HF), (100003, F32)])
+@pytest.mark.parametrize("V,dtype", [(32769, F32), (50304, F32), (65536, BF), (70001, HF), (100003, F32)])
 def test_shared_rows(dev, V, dtype, kind):
     g = torch.Generator().manual_seed(V + len(kind))
     for rows in (1, 12):
@@ -108,7 +108,7 @@ def test_the_most_rows(dev):
     from atma_amd import _lib
     lib = _lib.load()
     g = torch.Generator().manual_seed(2)
-    V = 30000
+    V = 33333
     most = max(r for r in range(1, 600) if lib.atma_sample_tokens_workspace(r, V, _lib.ATMA_F32))
     wide = _rows(g, "plain", most + 1, V + 5).to(dev)
     for rows in (most, most + 1):
