@@ -66,7 +66,10 @@ __device__ __forceinline__ LateArgs4 late_args4() {
 // The weights are the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token
 // (row 8 q + 4 h + e is feature 16 h + 4 q + e).  Their rows are 32 bytes in LDS, chunk c of row r at position
 // c ^ (r / 16) % 2: the 16 lanes that read one chunk of 16 such rows cover all banks.
-template <int TF, int TM, int WF, int WM, int NS_, bool GATED>
+//
+// KS = 2: two such sets of waves, each with a ring of its own, take half of K each, and the first adds the second's sums, which come
+// through LDS.  For tiles that are few: their time is the chain of blocks, and two waves a SIMD issue beside each other.
+template <int TF, int TM, int WF, int WM, int NS_, bool GATED, int KS = 1>
 struct Fp4Tile {
   static constexpr int NW = WF * WM, NS = NS_;
   static constexpr int BF = 32 * TF * WF, BM = 32 * TM * WM;
@@ -77,22 +80,25 @@ struct Fp4Tile {
   static constexpr int FIRST = COPIES / 4;        // of them in the last step of a block
   static constexpr int RING = NS + 2;    // blocks and tiles under way: copies run NS blocks ahead
   static constexpr int SLOT = NW * 256;  // a block's scales, in words: two a weight row
-  static constexpr int AUX = NS * STAGE, BIAS = AUX + RING * SLOT, TURN = BIAS + RING * 1024, LDS = TURN + 2048 * NW;
+  static constexpr int AUX = NS * STAGE, BIAS = AUX + RING * SLOT, TURN = BIAS + RING * 1024, SET = TURN + 2048 * NW;
+  static constexpr int JOIN = KS * SET, LDS = JOIN + (KS - 1) * NW * TF * TM * 4096;
   static_assert(BF == 32 * NW && BM % (8 * NW) == 0 && BF <= 256 && NW > 2, "whole copies, a bias of 1 KiB, copied by wave 2");
   static_assert(!GATED || TF % 2 == 0, "a gated wave has its features' a and gate rows");
   static_assert(NS >= 3 && (NS - 1) * COPIES < 63, "vmcnt counts to 63");
 };
 
-template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
-__global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
-  using C = Fp4Tile<TF, TM, WF, WM, NS, GATED>;
+template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED, int KS>
+__global__ void __launch_bounds__(64 * WF * WM * KS, 2) fp4_tile_kernel(Fp4Args a) {
+  using C = Fp4Tile<TF, TM, WF, WM, NS, GATED, KS>;
   constexpr int TO = C::TO;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
+  __shared__ __attribute__((aligned(1024))) uint8_t all_lds[C::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int any_wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int set = KS == 1 ? 0 : any_wave / C::NW, wave = any_wave - set * C::NW;
+  uint8_t* lds = all_lds + set * C::SET;
   const int wf = wave % WF, wm = wave / WF;
   const int r = lane & 31, h = lane >> 5;
-  const int nk = a.nk;
+  const int nk = (a.nk + KS - 1) / KS, pk0 = set * nk;  // the set's blocks of K
   int64_t m0, f0;
   int u = blockIdx.x >> 3;
   if (!gemm_tile_at<C>(a, blockIdx.x & 7, u, m0, f0)) return;
@@ -111,7 +117,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
   const uint32_t wv0 = (uint32_t)(wbase + (lane >> 1)) * (uint32_t)a.ldw + (uint32_t)wk;
   __amdgpu_buffer_rsrc_t xr, wr;
   const uint8_t* scales;  // the first code of a lane's weight row
-  int pu = u, pk = 0, plimit = 0, ptile = 0, pslot = 0, pstage = 0;
+  int pu = u, pk = pk0, plimit = 0, ptile = 0, pslot = 0, pstage = 0;
   auto aim = [&](int64_t tm0, int64_t tf0) {
     LateArgs4 p = late_args4();
     const int64_t rows = min((int64_t)C::BM, p->M - tm0);
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
     const int64_t last = (GATED && wave >= half ? 2 : 1) * p->N - 1;
     scales = p->ws + min(n0 + wbase + (lane >> 1), last) * p->ldws;
     plimit = p->K;
-    if (p->bias && wave == 2) {
+    if (p->bias && wave == 2 && set == 0) {
       // the tile's biases (gated: those of a, then of gate), a word each, to its slot
       const bool wide = p->bias_dtype == ATMA_F32;
       for (int i = 0; i < C::BF / 64; ++i) {
@@ -136,7 +142,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
   };
   auto next_tile = [&]() {
     int64_t nm0, nf0;
-    pk = 0;
+    pk = pk0;
     pu += gridDim.x >> 3;
     if (gemm_tile_at<C>(*late_args4(), blockIdx.x & 7, pu, nm0, nf0)) aim(nm0, nf0);
     else plimit = 0;
@@ -145,7 +151,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
   uint32_t ps;
   const uint8_t* pscale;
   auto copies_begin = [&]() {
-    if (pk == nk) next_tile();
+    if (pk == pk0 + nk) next_tile();
     pscale = scales + max(0, min(2 * pk + (lane & 1), plimit / kFp4Group - 1));
     ps = lds0 + C::AUX + C::SLOT * pslot + 256 * wave;
     pslot = pslot + 1 == C::RING ? 0 : pslot + 1;
@@ -210,7 +216,7 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
       float b[16] = {};
       const int f = wrow0 + 16 * h + (GATED ? t / TO * C::OF + 32 * (t % TO) : 32 * t);
       LateArgs4 p = late_args4();
-      if (p->bias) {
+      if (p->bias && set == 0) {
         const uint8_t* at = lds + C::BIAS + 1024 * tile;
         const int dtype = p->bias_dtype;
 #pragma unroll
@@ -270,12 +276,37 @@ __global__ void __launch_bounds__(64 * WF * WM, 2) fp4_tile_kernel(Fp4Args a) {
     // ---- epilogue of tile (m0, f0): token 32 (TM wm + j) + r, 16 consecutive features a tile.  Through LDS, a wave its own 2 KiB:
     // 32 tokens x 32 features at a time turn from a token a lane to 64-byte pieces, four lanes each (chunk c of row r at position
     // c ^ (r / 4) % 4)
+    if constexpr (KS > 1) {
+      // (the buffer is written again behind the barriers of the next tile's blocks)
+      f32x4* join = (f32x4*)(all_lds + C::JOIN) + wave * TF * TM * 256 + lane;
+      if (set) {
+#pragma unroll
+        for (int i = 0; i < TF * TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const f32x16& v = acc[i / TM][i % TM];
+            join[256 * i + 16 * e] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+          }
+      }
+      lds_barrier();
+      if (!set) {
+#pragma unroll
+        for (int i = 0; i < TF * TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const f32x4 v = join[256 * i + 16 * e];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i / TM][i % TM][e + q] += v[q];
+          }
+      }
+    }
     LateArgs4 p = late_args4();
     const bool whole = f0 + C::OF <= p->N;  // every feature of the tile
     uint8_t* turn = lds + C::TURN + 2048 * wave;
     const int64_t ldy = p->ldy, N = p->N, M = p->M;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
+      if (set) break;
 #pragma unroll
       for (int t = 0; t < TO; ++t) {
         f32x16 v = acc[t][j];
@@ -506,16 +537,16 @@ __global__ void __launch_bounds__(64 * NW) fp4_few_kernel(Fp4FewArgs f) {
   wait_vmcnt<0>();  // no copy outlives its workgroup's LDS
 }
 
-template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED>
+template <typename T, int TF, int TM, int WF, int WM, int NS, bool GATED, int KS = 1>
 static void launch_tiles4(Fp4Args a, hipStream_t s) {
-  using C = Fp4Tile<TF, TM, WF, WM, NS, GATED>;
+  using C = Fp4Tile<TF, TM, WF, WM, NS, GATED, KS>;
   a.m_tiles = (int)((a.M + C::BM - 1) / C::BM);
   a.f_tiles = (int)((a.N + C::OF - 1) / C::OF);
   const int64_t tiles = (int64_t)a.m_tiles * a.f_tiles;
   a.per_xcd = (int)((tiles + 7) / 8);
   constexpr int per_cu = 160 * 1024 / C::LDS;
   const int64_t wgs = std::min<int64_t>((int64_t)device_cu_count() / 8 * 8 * per_cu, 8 * (int64_t)a.per_xcd);
-  fp4_tile_kernel<T, TF, TM, WF, WM, NS, GATED><<<dim3((unsigned)wgs), dim3(64 * C::NW), 0, s>>>(a);
+  fp4_tile_kernel<T, TF, TM, WF, WM, NS, GATED, KS><<<dim3((unsigned)wgs), dim3(64 * C::NW * KS), 0, s>>>(a);
 }
 
 // How the few rows' kernel is laid over the card
@@ -548,19 +579,21 @@ static void launch_few4(const Fp4Args& a, hipStream_t s) {
 
 // The kernel for a product: the one with the least time by a cost of its form, us of a graph's launch.  The few rows' kernel:
 // a part that does not depend on the size, the steps of a wave, and all blocks of all waves over the card's SIMDs.  The tiles:
-// TileCost and a part that does not depend on the size.  Fitted to 204 measured shapes of 1 to 16,384 rows, 512 to 50,304 features and K
-// of 256 to 4,096: over them the choice takes 0.7 % longer than the best of all forms in the mean and 19 % at most (gated: 0.6 % and
-// 8 %).  What each form is there for (us, it and the best of the others):
-//   16 rows a workgroup through a ring    16 x 4,096 -> 1,024     5.8 and  7.5    128 x 1,024 -> 1,024    5.0 and  5.4
-//   32 rows a workgroup through a ring   256 x 4,096 -> 1,024    11.1 and 13.4     64 x 4,096 -> 8,192   16.8 and 21.4
+// TileCost and a part that does not depend on the size.  Fitted to 221 measured shapes of 1 to 16,384 rows, 512 to 50,304 features and K
+// of 256 to 4,096: over them the choice takes 1.0 % longer than the best of all forms in the mean and 15 % at most (gated: 0.6 % and
+// 12 %).  What each form is there for (us, it and the best of the others):
+//   16 rows a workgroup through a ring    16 x 4,096 -> 1,024     5.8 and  7.5    128 x 1,024 -> 1,024    4.9 and  5.3
+//   32 rows a workgroup through a ring   192 x 4,096 -> 1,024    11.0 and 13.2     32 x 4,096 -> 8,192   10.6 and 12.6
 //   16 rows' K kept in LDS                 1 x 1,024 -> 50,304    8.2 and 14.2      8 x 4,096 -> 8,192    7.0 and  8.0
-//   tiles of 128 features x 32 tokens     32 x 1,024 -> 50,304   10.0 and 11.7
-//   tiles of 128 x 64                     64 x 1,024 -> 50,304   12.9 and 17.2
-//   tiles of 128 x 128                   512 x 4,096 -> 8,192    39.1 and 51.6
+//   tiles of 128 features x 32 tokens     32 x 1,024 -> 50,304   10.4 and 12.0
+//   tiles of 128 x 64                     64 x 1,024 -> 50,304   13.1 and 16.3
+//   tiles of 128 x 128                   512 x 4,096 -> 8,192    39.1 and 50.7
 //   tiles of 256 x 256                16,384 x 4,096 -> 1,024   107   and 135
-// gated, K of 1,024 -> 4,096: 64 x 64 for 256 rows 10.8 and 12.0, 64 x 128 for 512 12.9 and 14.3, 128 x 256 for 8,192 110 and 132.
+//   tiles of 128 x 32, K in halves       512 x 4,096 -> 1,024    16.8 and 18.8    777 x 1,024 -> 1,024    7.2 and  8.1
+//   tiles of 128 x 64, K in halves       192 x 4,096 -> 8,192    21.9 and 27.1    512 x 1,024 -> 4,096    8.8 and  9.9
+// gated: 64 x 64 with K in halves for 256 x 1,024 -> 4,096 9.3 and 11.5 (all K 10.2), 64 x 128 for 512 12.8 and 16.6, 128 x 256 for 8,192 110 and 132.
 // (codes that atma_linear_fp4_form returns)
-enum Fp4Form { kFp4Ring16, kFp4Ring32, kFp4Kept16, kFp4Tile32, kFp4Tile64, kFp4Tile128, kFp4Tile256 };
+enum Fp4Form { kFp4Ring16, kFp4Ring32, kFp4Kept16, kFp4Tile32, kFp4Tile64, kFp4Tile128, kFp4Tile256, kFp4Halves32, kFp4Halves64 };
 
 static Fp4Form choose_fp4(const Fp4Args& a, bool gated) {
   Fp4Form best = kFp4Tile256;
@@ -573,21 +606,25 @@ static Fp4Form choose_fp4(const Fp4Args& a, bool gated) {
   auto few = [&](Fp4Form form, const FewPlan& p, float fixed, float step, float block) {
     offer(form, fixed + step * (float)p.steps + block * (float)p.tiles * (float)p.groups * (float)few_nk / simds);
   };
-  auto tile = [&](Fp4Form form, float fixed, const TileCost& c) { offer(form, fixed + tile_time(a.M, a.N, a.nk, c)); };
+  auto tile = [&](Fp4Form form, float fixed, const TileCost& c) {
+    offer(form, fixed + tile_time(a.M, a.N, form >= kFp4Halves32 ? (a.nk + 1) / 2 : a.nk, c));
+  };
   const bool some = a.M <= 1024;  // (beyond, tiles are ahead by far)
   if (gated) {
-    if (some) few(kFp4Ring16, plan_few4<1, 2, 4, true, true>(a), 4.24f, 0.695f, 0.237f);
-    tile(kFp4Tile64, 4.48f, {64, 64, 0.f, 0.334f, 0.346f});
-    tile(kFp4Tile128, 5.01f, {64, 128, 0.f, 0.359f, 0.485f});
+    if (some) few(kFp4Ring16, plan_few4<1, 2, 4, true, true>(a), 4.25f, 0.673f, 0.245f);
+    tile(kFp4Halves64, 3.08f, {64, 64, 1.59f, 0.456f, 0.693f});
+    tile(kFp4Tile128, 4.75f, {64, 128, 0.01f, 0.38f, 0.495f});
     tile(kFp4Tile256, 5.59f, {128, 256, 1.25f, 0.902f, 1.47f});
   } else {
-    if (some) few(kFp4Ring16, plan_few4<1, 1, 4, true, false>(a), 3.69f, 0.476f, 0.204f);
-    if (some) few(kFp4Ring32, plan_few4<2, 1, 4, true, false>(a), 4.34f, 0.813f, 0.19f);
+    if (some) few(kFp4Ring16, plan_few4<1, 1, 4, true, false>(a), 3.68f, 0.483f, 0.198f);
+    if (some) few(kFp4Ring32, plan_few4<2, 1, 4, true, false>(a), 4.34f, 0.818f, 0.189f);
     if (some && std::min<int64_t>(a.M, 16) * few_nk * 2 * kFewBlock <= kFewTokens)
-      few(kFp4Kept16, plan_few4<1, 1, 8, false, false>(a), 4.58f, 0.288f, 0.231f);
-    tile(kFp4Tile32, 4.31f, {128, 32, 0.f, 0.277f, 0.243f});
-    tile(kFp4Tile64, 3.94f, {128, 64, 0.f, 0.319f, 0.34f});
-    tile(kFp4Tile128, 4.87f, {128, 128, 0.19f, 0.388f, 0.482f});
+      few(kFp4Kept16, plan_few4<1, 1, 8, false, false>(a), 4.57f, 0.297f, 0.225f);
+    tile(kFp4Tile32, 4.15f, {128, 32, 0.f, 0.281f, 0.245f});
+    tile(kFp4Tile64, 3.76f, {128, 64, 0.11f, 0.32f, 0.341f});
+    tile(kFp4Halves32, 2.39f, {128, 32, 1.5f, 0.37f, 0.484f});
+    tile(kFp4Halves64, 2.32f, {128, 64, 1.93f, 0.43f, 0.618f});
+    tile(kFp4Tile128, 4.62f, {128, 128, 0.37f, 0.386f, 0.477f});
     tile(kFp4Tile256, 5.5f, {256, 256, 0.88f, 0.994f, 1.5f});
   }
   return best;
@@ -634,7 +671,7 @@ static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dt
     if (gated) {
       switch (form) {
         case kFp4Ring16: launch_few4<T, 1, 2, 4, true, true>(a, st); break;
-        case kFp4Tile64: launch_tiles4<T, 2, 1, 2, 2, 4, true>(a, st); break;
+        case kFp4Halves64: launch_tiles4<T, 2, 1, 2, 2, 3, true, 2>(a, st); break;
         case kFp4Tile128: launch_tiles4<T, 2, 2, 2, 2, 3, true>(a, st); break;
         default: launch_tiles4<T, 2, 4, 4, 2, 3, true>(a, st); break;
       }
@@ -645,6 +682,8 @@ static int linear_fp4(const char* what, bool gated, Fp4Args a, int64_t K, int dt
         case kFp4Kept16: launch_few4<T, 1, 1, 8, false, false>(a, st); break;
         case kFp4Tile32: launch_tiles4<T, 1, 1, 4, 1, 4, false>(a, st); break;
         case kFp4Tile64: launch_tiles4<T, 1, 2, 4, 1, 4, false>(a, st); break;
+        case kFp4Halves32: launch_tiles4<T, 1, 1, 4, 1, 3, false, 2>(a, st); break;
+        case kFp4Halves64: launch_tiles4<T, 1, 2, 4, 1, 3, false, 2>(a, st); break;
         case kFp4Tile128: launch_tiles4<T, 2, 2, 2, 2, 3, false>(a, st); break;
         default: launch_tiles4<T, 2, 4, 4, 2, 3, false>(a, st); break;
       }

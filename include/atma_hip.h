@@ -706,7 +706,7 @@ int atma_linear_gated_fp4(const void* x, int64_t ldx, const void* w, int64_t ldw
 /*
  * Which kernel a call of these sizes takes on the current device, -1 where they are not served.  The kernel of few rows with
  * 0: 16 rows a workgroup, 1: 32 rows, 2: 16 rows kept in LDS; tiles of 3: 128 features x 32 tokens, 4: 128 x 64, 5: 128 x 128,
- * 6: 256 x 256.  Gated: 0, and tiles of 4: 64 x 64, 5: 64 x 128, 6: 128 x 256.
+ * 6: 256 x 256; with K in halves 7: 128 x 32, 8: 128 x 64.  Gated: 0, and tiles of 5: 64 x 128, 6: 128 x 256, 8: 64 x 64 with K in halves.
  */
 int atma_linear_fp4_form(int64_t M, int64_t N, int64_t K);
 int atma_linear_gated_fp4_form(int64_t M, int64_t H, int64_t K);

@@ -14,17 +14,21 @@ BF, HF = torch.bfloat16, torch.float16
 E8 = torch.float8_e8m0fnu
 
 # form, rows, features, K
-FORMS = [(0, 5, 100, 544), (0, 17, 1, 4128), (0, 777, 100, 1056), (0, 300, 530, 96),
-         (1, 50, 2300, 2080), (1, 130, 520, 4128), (1, 1000, 300, 2080),
-         (2, 1, 8200, 4128), (2, 7, 16500, 2080), (2, 1000, 300, 544),
-         (3, 3, 50304, 96), (3, 2001, 1, 1056), (3, 31, 16500, 1056), (3, 300, 2300, 1056),
-         (4, 1025, 9, 32), (4, 100, 8200, 1056), (4, 257, 4100, 1056), (4, 1041, 1100, 288), (4, 4097, 4100, 96),
-         (5, 100, 16500, 288), (5, 500, 4100, 288), (5, 4097, 520, 288),
-         (6, 200, 50304, 288), (6, 1000, 8200, 544), (6, 2001, 4100, 1056)]
+FORMS = [(0, 5, 100, 544), (0, 17, 1, 4128), (0, 777, 100, 1056),
+         (1, 50, 2300, 2080), (1, 130, 520, 4128), (1, 1000, 100, 4128),
+         (2, 1, 8200, 4128), (2, 7, 16500, 2080), (2, 1000, 300, 1056),
+         (3, 3, 50304, 96), (3, 17, 50304, 32), (3, 31, 50304, 1056), (3, 200, 16500, 2080),
+         (4, 777, 2300, 1056), (4, 1025, 9, 32), (4, 1041, 1100, 288), (4, 4097, 4100, 96),
+         (5, 100, 16500, 288), (5, 257, 8200, 1056), (5, 500, 4100, 288), (5, 4097, 520, 288),
+         (6, 200, 50304, 288), (6, 1000, 8200, 544), (6, 2001, 4100, 1056),
+         (7, 31, 16500, 1056), (7, 300, 530, 96), (7, 300, 2300, 1056), (7, 1000, 300, 544), (7, 1025, 1, 96),
+          (7, 2001, 1, 1056), (7, 4097, 100, 4128),
+         (8, 33, 16500, 4128), (8, 100, 8200, 1056), (8, 257, 4100, 1056), (8, 4097, 300, 4128)]
 GATED = [(0, 5, 100, 544), (0, 16, 1, 4128), (0, 1000, 100, 2080),
-         (4, 1, 1, 32), (4, 63, 4100, 1056), (4, 2001, 1, 1056), (4, 300, 1001, 544),
          (5, 70, 8200, 96), (5, 300, 4100, 1056), (5, 1041, 1001, 288),
-         (6, 500, 8200, 544), (6, 1000, 4100, 544), (6, 2049, 2300, 1056)]
+         (6, 500, 8200, 544), (6, 1000, 4100, 544), (6, 2049, 2300, 1056),
+         (8, 63, 4100, 1056), (8, 300, 1001, 544), (8, 1025, 1, 32), (8, 1030, 70, 96), (8, 2001, 1, 1056),
+          (8, 4097, 100, 4128)]
 
 
 def _run(dev, form, rows, n, k, dtype, gated):
