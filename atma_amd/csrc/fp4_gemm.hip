@@ -59,7 +59,7 @@ __device__ __forceinline__ LateArgs4 late_args4() {
 // at 1.1 to 1.3 times the time of their products, what both lose lies behind the barrier.  Measured without gain: products ahead
 // of the reads in each step, a higher priority for the products, the weights' conversion behind the last step's products,
 // 128 x 64 tiles a wave instead of 64 x 128 (twice the conversions, two thirds of the reads), operands read a whole block ahead.
-// 65,536 x 4,096 -> 1,024 takes 430 to 458 us by the box (1.2 PFLOP/s, matrix cores busy 70 % at the 1.7 GHz that power allows), the
+// 65,536 x 4,096 -> 1,024 takes 430 to 458 us by the card (1.2 PFLOP/s, matrix cores busy 70 % at the 1.7 GHz that power allows), the
 // library's 16-bit product on weights already converted 356 to 376.  Small tiles, a wave a SIMD, are bound by issue: a block of
 // 128 x 32 is 130 instructions and 128 cycles of products in 700.
 //
