@@ -10,15 +10,18 @@ and ``temperature``.  The lifecycle (queued -> active -> done) belongs to the sc
 
 ``temperature == 0`` asks for greedy decoding (the reference's sampler divides by the
 temperature and has no greedy form, ``inference/layers/sampler.py:7-10``).  ``top_k`` (0: all), ``top_p`` and ``min_p``
-narrow the choice (``sample_tokens``); with a ``seed`` a request draws the same random numbers in every batch.
+narrow the choice (``sample_tokens``); with a ``seed`` a request draws the same random numbers in every batch.  One that
+narrows it without a seed takes its seed from torch's CPU generator when it is first sampled, so ``torch.manual_seed`` repeats it, as it does
+the requests that ask for a temperature alone; Python's ``random`` is left as it is.
 """
 
 from dataclasses import dataclass
 from enum import Enum
 from itertools import count
 from operator import index
-from random import getrandbits
 from typing import Optional
+
+import torch
 
 
 @dataclass(frozen=True)
@@ -80,7 +83,7 @@ class Sequence:
         self.seq_slot = -1             # row of the runner's state tables (-1: none held)
         self.num_cached_tokens = 0     # tokens whose K/V, conv tails and memory state are stored
         self.num_scheduled_tokens = 0  # tokens the current step feeds
-        self._seed = getrandbits(64) if self.params.seed is None else self.params.seed
+        self._seed = self.params.seed  # None: drawn when the first random number is asked for
 
     def __len__(self):
         return len(self.token_ids)
@@ -93,7 +96,12 @@ class Sequence:
         return self.params.temperature
 
     def uniform(self, ahead=0):
-        """The random number of the token that follows ``ahead`` further ones."""
+        """The random number of the token that follows ``ahead`` further ones (0 for a request that ``sample_tokens`` draws
+        nothing for)."""
+        if self._seed is None:
+            if not self.params.picks:
+                return 0.0
+            self._seed = int(torch.randint(2 ** 63 - 1, (), device="cpu"))
         return uniform(self._seed, len(self.token_ids) - self.prompt_len + ahead)
 
     @property
