@@ -60,7 +60,7 @@ class LLMEngine:
 
     def _decode_run(self, batch):
         """Decode steps of one batch, each launched before the previous one's tokens are read
-        back (the graph leaves its greedy ids in place as the next step's inputs), while the
+        back (the graph, or the sampler behind it, leaves its ids in place as the next step's inputs), while the
         batch stays the same: the run ends when a request finishes (its token limit, known in
         advance, or the end-of-sequence id, seen one step late: the step already launched
         still comes back, and its token for the finished request is dropped).  Returns what

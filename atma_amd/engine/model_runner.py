@@ -193,6 +193,7 @@ class ModelRunner:
         self._stage_np = [{k: v.numpy() for k, v in views(h).items()} for h in hosts]
         self._stage_key = [None, None]   # the batch whose table rows and slots each host copy holds
         self._stage_flip = 0
+        self._run_picks = False          # whether a request of the launched run is sampled (launch_decode)
         self._stage_ids_bytes = 8 * max_bs  # the token ids lead the buffer
         # greedy ids of a launched step come back through these (pinned, used in turn)
         self._ids_host = [torch.empty(max_bs, dtype=torch.int64).pin_memory() for _ in range(2)]
@@ -257,19 +258,22 @@ class ModelRunner:
         """Enqueue one decode step of ``seqs`` without waiting for it; ``collect`` returns its
         tokens.  ahead 0: every request's newest token is known on the host.  ahead 1: the
         step right after a launched, not yet collected step of the same batch in the same
-        order -- its input tokens are that step's greedy ids, already in place on the device
-        (the graph writes them over its input ids), and each request is one token longer
+        order -- its input tokens are that step's ids, already in place on the device
+        (the graph writes its greedy ids over its input ids, and the sampler, where a request
+        asks for it, its own over those), and each request is one token longer
         than its host record.  The step's ids are copied back into pinned memory behind the
         graph."""
         bs = len(seqs)
-        bucket = self._stage(seqs, ahead)
+        if not ahead:
+            self._run_picks = any(s.params.picks for s in seqs)
+        bucket = self._stage(seqs, ahead, self._run_picks)
         off = self._stage_ids_bytes if ahead else 0
         self._stage_dev[off:].copy_(self._stage_hosts[self._stage_flip ^ 1][off:], non_blocking=True)
         g = self.graph_flip
         self.graph_flip ^= 1
         self.graphs[bucket][g].replay()
         logits, ids = self.graph_out[bucket][g]
-        if any(s.params.picks for s in seqs):
+        if self._run_picks:
             v = self.graph_vars
             u, t, p, m = v["floats"][:, :bs].unbind(0)
             ids = Picks(u, t, v["top_k"][:bs], p, m).sample(logits[:bs], v["input_ids"][:bs])
@@ -287,10 +291,10 @@ class ModelRunner:
         done.synchronize()
         return host[:bs].tolist()
 
-    def _stage(self, seqs, ahead=0):
+    def _stage(self, seqs, ahead=0, picks=False):
         """Fill the next pinned staging copy for a decode step of ``seqs`` whose requests are
         ``ahead`` tokens longer than their host records (rows past the batch: token 0, slot
-        -1, length 0, the padding table row); returns the graph bucket."""
+        -1, length 0, the padding table row), with what the sampler reads if ``picks``; returns the graph bucket."""
         bs = len(seqs)
         bucket = next(b for b in self.graph_bs if b >= bs)
         k = self._stage_flip
@@ -315,7 +319,7 @@ class ModelRunner:
         if not ahead:
             h["input_ids"][:bs] = [s.last_token for s in seqs]
         h["context_lens"][:bs] = lens
-        if any(s.params.picks for s in seqs):
+        if picks:
             h["floats"][:, :bs], h["top_k"][:bs] = self._picks(seqs, ahead)
         pos = lens - 1        # the new token's cache slot: its position's row in its position's page
         h["slot_mapping"][:bs] = bt[np.arange(bs), pos // page] * page + pos % page
@@ -332,13 +336,13 @@ class ModelRunner:
     def _sample(self, logits, seqs):
         """One id per sequence from its logits, as its parameters ask."""
         temps = [s.temperature for s in seqs]
-        picks = None
-        if any(s.params.picks for s in seqs):
+        greedy, picks = all(t == 0 for t in temps), None
+        if not greedy and any(s.params.picks for s in seqs):
             floats, top_k = self._picks(seqs)
             u, t, p, m = self._to_dev(floats, torch.float32).unbind(0)
             race = [s.temperature != 0 and not s.params.picks for s in seqs]
             picks = Picks(u, t, self._to_dev(top_k, torch.int32), p, m, self._to_dev(race, torch.bool) if any(race) else None)
-        return self.sampler(logits, self._to_dev(temps, torch.float32), all_greedy=all(t == 0 for t in temps), picks=picks)
+        return self.sampler(logits, self._to_dev(temps, torch.float32), all_greedy=greedy, picks=picks)
 
     def _run_decode_graph(self, seqs):
         """Replay the smallest captured bucket that fits: the step's inputs go in one H2D
