@@ -52,10 +52,10 @@ class Config:
     max_model_len: int = 4096
     enforce_eager: bool = False
     fp8_mlp: bool = False                   # serve the MLPs in 8 bits (e4m3, block scales); 16-bit models only
-    fp4_weights: bool = False               # serve the MLPs and the LM head with 4-bit weights (e2m1, group scales); 16-bit models only
     strict_weights: bool = False
     eos: int = 50256
     num_kvcache_blocks: int = -1            # -1: enough for max_num_seqs x max_model_len, within memory
     init_std: float = 0.02                  # random init N(0, init_std) of every parameter
     seed: int = 0
     hf_config: AtmaConfig = field(default_factory=AtmaConfig)
+    fp4_weights: bool = False               # serve the MLPs and the LM head with 4-bit weights (e2m1, group scales); 16-bit models only
