@@ -175,7 +175,8 @@ class ModelRunner:
         """One buffer for every decode-step input the graphs read: token ids and table
         rows (int64), cache slots, context lengths and block tables (int32); and what the sampler
         reads behind them: random numbers, temperatures, top_p, min_p (fp32) and top_k (int32).  Each step
-        fills a pinned host copy (two, used in turn) and sends it with one H2D copy."""
+        fills a pinned host copy (two, used in turn) and sends it with one H2D copy, the sampler's rows
+        with the steps that it reads them in."""
         n64, n32 = 2 * max_bs, 7 * max_bs + max_bs * max_blocks
         nbytes = 8 * n64 + 4 * n32
         dev = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -195,6 +196,7 @@ class ModelRunner:
         self._stage_flip = 0
         self._run_picks = False          # whether a request of the launched run is sampled (launch_decode)
         self._stage_ids_bytes = 8 * max_bs  # the token ids lead the buffer
+        self._stage_graph_bytes = nbytes - 4 * 5 * max_bs  # the sampler's rows end it
         # greedy ids of a launched step come back through these (pinned, used in turn)
         self._ids_host = [torch.empty(max_bs, dtype=torch.int64).pin_memory() for _ in range(2)]
         self._ids_done = [torch.cuda.Event(), torch.cuda.Event()]
@@ -267,8 +269,8 @@ class ModelRunner:
         if not ahead:
             self._run_picks = any(s.params.picks for s in seqs)
         bucket = self._stage(seqs, ahead, self._run_picks)
-        off = self._stage_ids_bytes if ahead else 0
-        self._stage_dev[off:].copy_(self._stage_hosts[self._stage_flip ^ 1][off:], non_blocking=True)
+        part = slice(self._stage_ids_bytes if ahead else 0, None if self._run_picks else self._stage_graph_bytes)
+        self._stage_dev[part].copy_(self._stage_hosts[self._stage_flip ^ 1][part], non_blocking=True)
         g = self.graph_flip
         self.graph_flip ^= 1
         self.graphs[bucket][g].replay()
@@ -351,7 +353,8 @@ class ModelRunner:
         (bs, V), greedy ids (bs,) or None)."""
         bs = len(seqs)
         bucket = self._stage(seqs)
-        self._stage_dev.copy_(self._stage_hosts[self._stage_flip ^ 1], non_blocking=True)
+        part = slice(self._stage_graph_bytes)
+        self._stage_dev[part].copy_(self._stage_hosts[self._stage_flip ^ 1][part], non_blocking=True)
         g = self.graph_flip
         self.graph_flip ^= 1
         self.graphs[bucket][g].replay()

@@ -102,3 +102,21 @@ def test_what_a_run_hands_the_sampler(monkeypatch, later):
         assert ids == [1100, 1101, 1102] and drawn[0][2].tolist() == [6, 0, 0] and drawn[0][4].tolist() == [0.25, 0.0, 0.0]
     else:
         assert ids == [100, 101, 102] and not drawn
+
+
+def test_greedy_steps_send_no_sampler_rows(monkeypatch):
+    """What the sampler reads lies behind what the graphs read, and is sent with the steps that it is filled for."""
+    r, drawn = _runner(monkeypatch)
+    v = r.graph_vars
+    greedy, sampled = _seqs([dict(temperature=0.0)] * 3), _seqs([dict(temperature=0.7, top_k=5, seed=3)] * 2)
+    v["floats"].fill_(-1.0)
+    v["top_k"].fill_(-1)
+    for step in (lambda: r.launch_decode(greedy, ahead=0), lambda: r.launch_decode(greedy, ahead=1), lambda: r._run_decode_graph(greedy)):
+        v["context_lens"].fill_(-1)
+        step()
+        assert v["context_lens"][:3].min() > 0 and v["slot_mapping"][:3].tolist()[0] >= 0
+        assert (v["floats"] == -1).all() and (v["top_k"] == -1).all()
+    r.launch_decode(sampled, ahead=0)
+    assert v["top_k"][:2].tolist() == [5, 5] and v["block_tables"][:2, 0].tolist() == [0, 1]
+    r.launch_decode(sampled, ahead=1)
+    assert drawn[1][0].tolist() == [s.uniform(1) for s in sampled]
