@@ -60,8 +60,8 @@ __device__ __forceinline__ LateArgs4 late_args4() {
 // of the reads in each step, a higher priority for the products, the weights' conversion behind the last step's products,
 // 128 x 64 tiles a wave instead of 64 x 128 (twice the conversions, two thirds of the reads), operands read a whole block ahead.
 // 65,536 x 4,096 -> 1,024 takes 430 to 458 us by the card (1.2 PFLOP/s, matrix cores busy 70 % at the 1.7 GHz that power allows), the
-// library's 16-bit product on weights already converted 356 to 376.  Small tiles, a wave a SIMD, are bound by issue: a block of
-// 128 x 32 is 130 instructions and 128 cycles of products in 700.
+// library's 16-bit product on weights already converted 356 to 376, converted in the call 368 to 370.
+// Small tiles, a wave a SIMD, are bound by issue: a block of 128 x 32 is 130 instructions and 128 cycles of products in 700.
 //
 // The weights are the MFMA's rows, in an order such that a lane's accumulators are 16 consecutive features of one token
 // (row 8 q + 4 h + e is feature 16 h + 4 q + e).  Their rows are 32 bytes in LDS, chunk c of row r at position

@@ -14,10 +14,11 @@
 //
 // Weights are formed in fp64 and held as integers, multiples of 2^-43 of the largest: their sums are exact, so neither the
 // order of the additions nor the number of threads changes a result, and a border is decided as in 64-bit arithmetic
-// (with fp32 weights one row in a few thousand would answer its neighbour's token).  V <= 2^20 keeps every sum below 2^63.
+// (with fp32 weights one row in a few thousand would answer its neighbour's token).  V <= 2^20 keeps every sum at 2^63 or
+// below, in unsigned 64-bit integers.
 //
 // What bounds it is a CU's work on a row: two passes that form a weight for every logit, some 190 cycles for 64 of them.  512 rows of 50,304
-// fp32 logits with top-p take 117 us, one in one workgroup 43, shared by 13 of them 23.
+// fp32 logits with top-p take 117 us, one in one workgroup 43, shared by 13 of them 23 to 24.
 #include <algorithm>
 
 #include "common.h"
