@@ -96,11 +96,8 @@ class Sequence:
         return self.params.temperature
 
     def uniform(self, ahead=0):
-        """The random number of the token that follows ``ahead`` further ones (0 for a request that ``sample_tokens`` draws
-        nothing for)."""
+        """The random number of the token that follows ``ahead`` further ones."""
         if self._seed is None:
-            if not self.params.picks:
-                return 0.0
             self._seed = int(torch.randint(2 ** 63 - 1, (), device="cpu"))
         return uniform(self._seed, len(self.token_ids) - self.prompt_len + ahead)
 

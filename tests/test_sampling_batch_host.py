@@ -91,7 +91,7 @@ def test_what_a_run_hands_the_sampler(monkeypatch, later):
         assert got == [1100, 1101, 1102]
     assert len(drawn) == 3
     for n, (u, t, k, p, m) in enumerate(drawn):
-        assert u.tolist() == [s.uniform(int(n > 0)) for s in seqs]
+        assert u.tolist() == [s.uniform(int(n > 0)) if s.params.picks else 0.0 for s in seqs]
         assert k.tolist() == [5, 0, 0]
         for v, want in ((t, (0.7, 0.0, 1.5)), (p, (1.0, 1.0, 0.5)), (m, (0.0, 0.0, 0.0))):
             assert np.array_equal(v.numpy(), np.float32(want))

@@ -5,7 +5,7 @@ import random
 import pytest
 import torch
 
-from atma_amd.engine import Sequence
+from atma_amd.engine import ModelRunner, Sequence
 from atma_amd.engine.sequence import SamplingParams, uniform
 
 ASKS = [dict(), dict(temperature=0.0), dict(temperature=0.7), dict(top_k=5), dict(top_p=0.9, min_p=0.1), dict(seed=3),
@@ -20,8 +20,8 @@ def test_the_callers_random_numbers_stay(ask):
     before, torch_before = random.getstate(), torch.get_rng_state()
     s = Sequence([1, 2, 3], SamplingParams(**ask))
     assert torch.equal(torch.get_rng_state(), torch_before)
-    first = s.uniform()
-    assert s.uniform() == first and s.uniform(1) == s.uniform(1)
+    first = ModelRunner._picks([s])[0][0, 0]
+    assert ModelRunner._picks([s])[0][0, 0] == first
     assert random.getstate() == before
     draws = s.params.picks and s.params.seed is None
     assert torch.equal(torch.get_rng_state(), torch_before) == (not draws)
