@@ -330,9 +330,9 @@ class ModelRunner:
     @staticmethod
     def _picks(seqs, ahead=0):
         """The sampler's rows: (random numbers, temperatures, top_p, min_p) fp32 and top_k int32.  Requests that it draws nothing
-        for have no random number."""
+        for take no seed."""
         ps = [s.params for s in seqs]
-        return (np.array([[s.uniform(ahead) if s.params.picks else 0.0 for s in seqs], [p.temperature for p in ps], [p.top_p for p in ps],
+        return (np.array([[s.uniform(ahead) if s.seed is not None or p.picks else 0.0 for s, p in zip(seqs, ps)], [p.temperature for p in ps], [p.top_p for p in ps],
                           [p.min_p for p in ps]], dtype=np.float32),
                 np.array([min(p.top_k, 2 ** 31 - 1) for p in ps], dtype=np.int32))
 

@@ -71,7 +71,7 @@ class Sequence:
     ``seq[a:b]`` slices them."""
 
     __slots__ = ("seq_id", "token_ids", "prompt_len", "params", "phase", "block_table", "seq_slot",
-                 "num_cached_tokens", "num_scheduled_tokens", "_seed")
+                 "num_cached_tokens", "num_scheduled_tokens", "seed")
 
     def __init__(self, token_ids, sampling_params: SamplingParams = None):
         self.seq_id = next(_ids)
@@ -83,7 +83,7 @@ class Sequence:
         self.seq_slot = -1             # row of the runner's state tables (-1: none held)
         self.num_cached_tokens = 0     # tokens whose K/V, conv tails and memory state are stored
         self.num_scheduled_tokens = 0  # tokens the current step feeds
-        self._seed = self.params.seed  # None: drawn when the first random number is asked for
+        self.seed = self.params.seed  # None: drawn when the first random number is asked for
 
     def __len__(self):
         return len(self.token_ids)
@@ -97,9 +97,9 @@ class Sequence:
 
     def uniform(self, ahead=0):
         """The random number of the token that follows ``ahead`` further ones."""
-        if self._seed is None:
-            self._seed = int(torch.randint(2 ** 63 - 1, (), device="cpu"))
-        return uniform(self._seed, len(self.token_ids) - self.prompt_len + ahead)
+        if self.seed is None:
+            self.seed = int(torch.randint(2 ** 63 - 1, (), device="cpu"))
+        return uniform(self.seed, len(self.token_ids) - self.prompt_len + ahead)
 
     @property
     def last_token(self):
