@@ -332,8 +332,8 @@ class ModelRunner:
         """The sampler's rows: (random numbers, temperatures, top_p, min_p) fp32 and top_k int32.  Requests that it draws nothing
         for take no seed."""
         ps = [s.params for s in seqs]
-        return (np.array([[s.uniform(ahead) if s.seed is not None or p.picks else 0.0 for s, p in zip(seqs, ps)], [p.temperature for p in ps], [p.top_p for p in ps],
-                          [p.min_p for p in ps]], dtype=np.float32),
+        return (np.array([[s.uniform(ahead) if s.seed is not None or p.picks else 0.0 for s, p in zip(seqs, ps)],
+                          [p.temperature for p in ps], [p.top_p for p in ps], [p.min_p for p in ps]], dtype=np.float32),
                 np.array([min(p.top_k, 2 ** 31 - 1) for p in ps], dtype=np.int32))
 
     def _sample(self, logits, seqs):
